@@ -248,6 +248,58 @@ int ygg_float_take_errors(const ygg_fmodel *m, void *stream, uint32_t *errors);
 
 void ygg_float_free(ygg_fmodel *m);
 
+/* ---- Operators of an output head (no counterpart in the reference, whose step holds them inside): the products of
+   routed experts, an int8 projection of float rows, and the log-probabilities of given tokens, with the gradients a
+   training step takes. They run on the caller's current device and stream, wait for nothing and allocate nothing.
+   type: 0 f32, 1 bf16, 2 f16. Sums, maxima and softmax statistics are held in 32 bits; an output is rounded once. ---- */
+enum {
+    YGG_MOST_TOP = 64,             /* alternatives of a row */
+    YGG_MOST_VOCAB = 1 << 24,
+    YGG_MOST_ROWS = 1 << 24,       /* rows of a product */
+    YGG_MOST_EXPERTS = 1 << 20,
+    YGG_MOST_INNER = 1 << 17       /* a product's inner and outer sizes (int8 sums of that many products fit 32 bits) */
+};
+
+/* For each of `rows` rows of V logits, `stride` values apart: d_entropy (rows), the entropy of softmax(row) in nats; with
+   targets (target_bytes 4 or 8: int32 or int64, 0: none) d_logp (rows), the target's log-probability, 0 for a target of
+   -1 (no token) and NaN for others outside [0, V); with top > 0 d_top_ids and d_top_logp (rows, top), the most likely
+   tokens in falling order, equal ones by rising id, filled up with -1 and -inf (entries of -inf are never among them).
+   d_stats (rows, 2) or NULL: what ygg_logprobs_grad wants. A row of -inf alone has log-probability -inf and entropy 0; a
+   row that holds a NaN or +inf has NaN outputs and ids of -1. d_scratch: device memory of ygg_logprobs_scratch bytes (0:
+   none wanted), 256-byte aligned, that no other call uses until this one has run. */
+int64_t ygg_logprobs_scratch(int type, int64_t rows, int V, int top);
+int ygg_logprobs(const void *d_logits, int type, int64_t rows, int V, int64_t stride, const void *d_targets,
+                 int target_bytes, int top, float *d_logp, float *d_entropy, float *d_top_logp, int32_t *d_top_ids,
+                 float *d_stats, void *d_scratch, int64_t scratch_bytes, void *stream);
+
+/* The logits' gradient (rows, V), contiguous, in the logits' type, from the gradients of ygg_logprobs' outputs (NULL: none
+   comes from that output) and its d_entropy, d_top_ids and d_stats. Zero for a row of -inf alone; a target of -1 takes no
+   part, a bad one makes its row NaN. */
+int ygg_logprobs_grad(const void *d_logits, int type, int64_t rows, int V, int64_t stride, const void *d_targets,
+                      int target_bytes, int top, const float *d_entropy, const int32_t *d_top_ids, const float *d_stats,
+                      const float *d_g_logp, const float *d_g_entropy, const float *d_g_top, void *d_out, void *stream);
+
+/* M rows, each times the matrix of the expert it takes: y (M, N) = W[expert] x, with x (M, K) and W (E, N, K), contiguous.
+   d_offsets (E + 1) int32, rising: expert e takes the places d_offsets[e] .. d_offsets[e + 1] - 1 (d_offsets[0] counts as
+   0) of d_order (M) int32, a permutation of the rows, or NULL: place p is row p. Rows that no expert takes get 0. The
+   offsets are clamped to [0, M] and entries of d_order outside [0, M) skipped, so that bad ones give wrong sums and no
+   access out of bounds. The gradients: dx (M, K) = W[expert]^T dy, dW (E, N, K) = the sum over an expert's rows of
+   dy x^T, zero for an expert without rows. */
+int ygg_grouped_matmul(const void *d_x, const void *d_w, int type, const int32_t *d_offsets, const int32_t *d_order, int M,
+                       int E, int N, int K, void *d_y, void *stream);
+int ygg_grouped_grad_x(const void *d_dy, const void *d_w, int type, const int32_t *d_offsets, const int32_t *d_order, int M,
+                       int E, int N, int K, void *d_dx, void *stream);
+int ygg_grouped_grad_w(const void *d_dy, const void *d_x, int type, const int32_t *d_offsets, const int32_t *d_order, int M,
+                       int E, int N, int K, void *d_dw, void *stream);
+
+/* y (M, N) in x's type: x (M, K) quantised to int8 row by row, s_i = max(max |x_i| / 127, 2^-126) and q = x / s_i in f32,
+   rounded to nearest even, times w (N, K) int8 with a scale for each of its rows: (q . w) s_i d_w_scale. A row that holds a
+   NaN or an infinity is NaN. d_scratch: device memory of ygg_int8_scratch bytes, 256-byte aligned, that no other call uses
+   until this one has run. */
+int64_t ygg_int8_scratch(int M, int N, int K);
+int ygg_int8_linear(const void *d_x, int type, const int8_t *d_w, const float *d_w_scale, int M, int N, int K, void *d_y,
+                    void *d_scratch, int64_t scratch_bytes, void *stream);
+
 /* Message of the last failed call on this thread ("" if none). */
 const char *ygg_last_error(void);
 

@@ -1,0 +1,309 @@
+"""grouped_matmul and its gradients against products in 64 bits: every type, expert loads from none to all rows, sizes that
+end inside a tile or off an alignment, rows in their own order, bad offsets.
+
+Tolerance: an output is a sum of I products, each exact to a rounding in f32 and added in f32, so it is off by at most
+2^-24 (I + 1) sum |a b|, and by far less in the mean: sqrt(I) roundings of random sign, each of a partial sum that is about
+the root of the sum of squares of the products. Held here to 2^-22 (8 + 2 sqrt(I)) times that root, then half a step of the
+output's type."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def loads(kind, M, E, g):
+    """Rows of each expert."""
+    if kind == "even":
+        leaves = torch.arange(M) % E
+    elif kind == "one":
+        leaves = torch.full((M,), E // 2)
+    elif kind == "ends":
+        leaves = torch.where(torch.arange(M) % 2 == 0, 0, E - 1)
+    else:
+        p = 1.0 / (1 + torch.arange(E, dtype=torch.double))
+        leaves = torch.multinomial(p[torch.randperm(E, generator=g)], M, replacement=True, generator=g) if M else torch.zeros(0)
+    return leaves.long()
+
+
+def make(M, E, N, K, dtype, kind="ragged", ordered=False, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    leaves = loads(kind, M, E, g)
+    if ordered:
+        leaves = leaves[torch.randperm(M, generator=g)]
+    else:
+        leaves = leaves.sort().values
+    x = torch.randn(M, K, generator=g).to(dtype)
+    w = (torch.randn(E, N, K, generator=g) / math.sqrt(K)).to(dtype)
+    dy = torch.randn(M, N, generator=g).to(dtype)
+    return leaves, x, w, dy
+
+
+def near(got, ref, a2, terms):
+    """a2: sum of squares of the products of each output."""
+    half = torch.finfo(got.dtype).eps / 2
+    least = {torch.float32: 2.0 ** -126, torch.bfloat16: 2.0 ** -126, torch.float16: 2.0 ** -25}[got.dtype]
+    tol = 2.0 ** -23 * (8 + 2 * math.sqrt(terms)) * 2 * a2.sqrt()
+    err = (got.detach().double().cpu() - ref).abs()
+    assert (err <= tol + half * (ref.abs() + tol) + least).all(), float((err - tol - half * ref.abs()).max())
+
+
+def check(leaves, x, w, dy, ordered, train=True):
+    from yggdrasil_amd import ops
+    E, N, K = w.shape
+    M = len(x)
+    dev = [v.cuda() for v in (x, w, dy)]
+    xg, wg, dyg = dev
+    if train:
+        xg.requires_grad_()
+        wg.requires_grad_()
+    offsets, order = ops.group_rows(leaves.cuda(), E)
+    y = ops.grouped_matmul(xg, wg, offsets, order if ordered else None)
+    x64, w64, dy64 = x.double(), w.double(), dy.double()
+    ref, sq = torch.zeros(M, N, dtype=torch.double), torch.zeros(M, N, dtype=torch.double)
+    rx, sx = torch.zeros(M, K, dtype=torch.double), torch.zeros(M, K, dtype=torch.double)
+    rw, sw = torch.zeros(E, N, K, dtype=torch.double), torch.zeros(E, N, K, dtype=torch.double)
+    most = 1
+    for e in torch.unique(leaves).tolist():
+        if not 0 <= e < E:
+            continue
+        i = (leaves == e).nonzero()[:, 0]
+        most = max(most, len(i))
+        ref[i] = x64[i] @ w64[e].t()
+        sq[i] = x64[i] ** 2 @ (w64[e] ** 2).t()
+        if train:
+            rx[i] = dy64[i] @ w64[e]
+            sx[i] = dy64[i] ** 2 @ w64[e] ** 2
+            rw[e] = dy64[i].t() @ x64[i]
+            sw[e] = (dy64[i] ** 2).t() @ x64[i] ** 2
+    assert y.dtype == x.dtype
+    near(y, ref, sq, K)
+    if train:
+        dx, dw = torch.autograd.grad(y, (xg, wg), dyg)
+        assert dx.dtype == x.dtype and dw.dtype == x.dtype
+        near(dx, rx, sx, N)
+        near(dw, rw, sw, most)
+    return y
+
+
+SHAPES = [(1, 1, 1, 1), (1, 4, 8, 16), (7, 3, 5, 3), (40, 16, 8, 64), (100, 300, 8, 128), (64, 5, 17, 33), (200, 4, 64, 256),
+          (130, 9, 100, 72), (300, 2, 129, 200), (513, 3, 256, 136), (700, 2, 264, 520), (33, 2, 300, 1000), (1000, 8, 40, 24)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("M, E, N, K", SHAPES)
+def test_shapes(M, E, N, K, dtype):
+    for ordered in (False, True):
+        leaves, x, w, dy = make(M, E, N, K, dtype, ordered=ordered, seed=M + N)
+        check(leaves, x, w, dy, ordered)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("kind", ["even", "one", "ends"])
+@pytest.mark.parametrize("M, E, N, K", [(96, 32, 16, 64), (520, 6, 144, 96), (257, 3, 256, 512)])
+def test_loads(M, E, N, K, kind, dtype):
+    """Even loads, one expert that takes all rows, experts without a row between the first and the last."""
+    leaves, x, w, dy = make(M, E, N, K, dtype, kind, True)
+    check(leaves, x, w, dy, True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_more_experts_than_rows(dtype):
+    leaves, x, w, dy = make(50, 5000, 8, 32, dtype, ordered=True)
+    check(leaves, x, w, dy, True)
+    leaves, x, w, dy = make(3, 70, 96, 160, dtype)
+    check(leaves, x, w, dy, False)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("M", [2000, 4500])
+def test_tall(M, dtype):
+    """Long groups: sums over thousands of rows in the weights' gradient, several tiles an expert."""
+    leaves, x, w, dy = make(M, 3, 200, 264, dtype, ordered=True)
+    check(leaves, x, w, dy, True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_rows_of_no_expert_are_zero(dtype):
+    from yggdrasil_amd import ops
+    leaves, x, w, dy = make(90, 4, 24, 40, dtype, ordered=True)
+    leaves[::3] = -1
+    leaves[1::9] = 4
+    y = check(leaves, x, w, dy, True)
+    assert (y[::3] == 0).all()
+    # offsets that end before the rows do: rows past the end
+    offsets = torch.tensor([0, 10, 10, 20, 30], dtype=torch.int32, device="cuda")
+    z = ops.grouped_matmul(x.cuda(), w.cuda(), offsets)
+    assert (z[30:] == 0).all() and (z[:30] != 0).any()
+    xg, wg = x.cuda().requires_grad_(), w.cuda().requires_grad_()
+    dx, dw = torch.autograd.grad(ops.grouped_matmul(xg, wg, offsets), (xg, wg), dy.cuda())
+    assert (dx[30:] == 0).all() and (dw[1] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("N, K", [(16, 64), (200, 328)])
+def test_values_that_are_not_finite_stay_in_their_rows(N, K, dtype):
+    """A NaN or an infinity in one row reaches that row's outputs and its expert's gradient alone."""
+    from yggdrasil_amd import ops
+    leaves, x, w, dy = make(150, 3, N, K, dtype, "even")
+    x[10, 3] = math.nan
+    x[70, 0] = math.inf
+    e = {int(leaves[10]), int(leaves[70])}
+    xg, wg = x.cuda().requires_grad_(), w.cuda().requires_grad_()
+    offsets, _ = ops.group_rows(leaves.cuda(), 3)
+    y = ops.grouped_matmul(xg, wg, offsets)
+    rows = [i for i in range(150) if i not in (10, 70)]
+    assert torch.isfinite(y[rows]).all() and not torch.isfinite(y[10]).any() and not torch.isfinite(y[70]).any()
+    dx, dw = torch.autograd.grad(y, (xg, wg), dy.cuda())
+    assert torch.isfinite(dx).all()
+    for k in range(3):
+        assert torch.isfinite(dw[k]).all() == (k not in e)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("M, N, K", [(60, 8, 32), (400, 160, 192)])
+def test_bad_offsets_and_orders_stay_in_bounds(M, N, K, dtype):
+    """Offsets past the rows, falling or negative ones, an order with entries that are no rows: no access out of bounds (the
+    kernels clamp the offsets and skip such entries), and the call ends."""
+    from yggdrasil_amd import ops
+    leaves, x, w, dy = make(M, 4, N, K, dtype)
+    bad = [[0, M + 50, 2 * M, 1 << 30, (1 << 31) - 1], [0, -5, M // 2, -(1 << 31), M], [5, 4, 3, 2, 1], [M, M, M, M, M]]
+    order = torch.randperm(M, dtype=torch.int32)
+    order[::7] = M + 3
+    order[3::11] = -1
+    for o in bad:
+        for r in (None, order.cuda()):
+            xg, wg = x.cuda().requires_grad_(), w.cuda().requires_grad_()
+            y = ops.grouped_matmul(xg, wg, torch.tensor(o, dtype=torch.int32, device="cuda"), r)
+            torch.autograd.grad(y, (xg, wg), dy.cuda())
+            torch.cuda.synchronize()
+
+
+def test_strided_and_shared_inputs():
+    from yggdrasil_amd import ops
+    leaves, x, w, dy = make(60, 4, 24, 40, torch.float32)
+    offsets, _ = ops.group_rows(leaves.cuda(), 4)
+    want = ops.grouped_matmul(x.cuda(), w.cuda(), offsets)
+    wide = torch.zeros(60, 80, device="cuda")
+    wide[:, ::2] = x.cuda()
+    assert torch.equal(ops.grouped_matmul(wide[:, ::2], w.cuda(), offsets), want)
+    wt = w.transpose(1, 2).contiguous().cuda()
+    assert torch.equal(ops.grouped_matmul(x.cuda(), wt.transpose(1, 2), offsets), want)
+    # one matrix for every expert, one row for all: their gradients are sums
+    shared = w[:1].cuda().requires_grad_()
+    one = x[:1].cuda().requires_grad_()
+    y = ops.grouped_matmul(one.expand(60, 40), shared.expand(4, 24, 40), offsets)
+    y.sum().backward()
+    ref = torch.ones(24, 1, dtype=torch.double) * 60 * x[0].double()
+    assert ((shared.grad[0].double().cpu() - ref).abs() <= 2.0 ** -20 * ref.abs() + 1e-30).all()
+    ref = 60 * w[0].double().sum(0)
+    assert ((one.grad[0].double().cpu() - ref).abs() <= 2.0 ** -19 * 60 * w[0].double().abs().sum(0)).all()
+    e = ops.grouped_matmul(torch.empty(0, 40, device="cuda"), w.cuda(), torch.zeros(5, dtype=torch.int32, device="cuda"))
+    assert e.shape == (0, 24)
+    xe, we = torch.empty(0, 40, device="cuda", requires_grad=True), w.cuda().requires_grad_()
+    ops.grouped_matmul(xe, we, torch.zeros(5, dtype=torch.int32, device="cuda")).sum().backward()
+    assert (we.grad == 0).all()
+
+
+def test_only_the_gradients_asked_for():
+    from yggdrasil_amd import ops
+    leaves, x, w, dy = make(30, 4, 8, 16, torch.float32)
+    offsets, _ = ops.group_rows(leaves.cuda(), 4)
+    wg = w.cuda().requires_grad_()
+    y = ops.grouped_matmul(x.cuda(), wg, offsets)
+    y.backward(dy.cuda())
+    assert wg.grad.shape == w.shape
+    xg = x.cuda().requires_grad_()
+    ops.grouped_matmul(xg, w.cuda(), offsets).backward(dy.cuda())
+    assert xg.grad.shape == x.shape
+
+
+def test_gradient_against_differences():
+    """Central differences of the product in 64 bits: the function is linear in x and in w, so they are exact but for
+    rounding; the kernel's own error is that of the sums above."""
+    from yggdrasil_amd import ops
+    leaves, x, w, dy = make(40, 5, 12, 20, torch.float32, ordered=True)
+    offsets, order = ops.group_rows(leaves.cuda(), 5)
+    xg, wg = x.cuda().requires_grad_(), w.cuda().requires_grad_()
+    dx, dw = torch.autograd.grad(ops.grouped_matmul(xg, wg, offsets, order), (xg, wg), dy.cuda())
+
+    def f(a, b):
+        return float((torch.einsum("mk,mnk->mn", a, b[leaves]) * dy.double()).sum())
+    for s in range(4):
+        g = torch.Generator().manual_seed(s)
+        vx, vw = torch.randn(x.shape, generator=g).double(), torch.randn(w.shape, generator=g).double()
+        for v, d, at in ((vx, dx, lambda h: f(x.double() + h * vx, w.double())),
+                         (vw, dw, lambda h: f(x.double(), w.double() + h * vw))):
+            want, got = (at(1e-3) - at(-1e-3)) / 2e-3, float((d.double().cpu() * v).sum())
+            assert abs(got - want) <= 1e-4 * (1 + abs(want))
+
+
+def test_same_result_every_time():
+    from yggdrasil_amd import ops
+    leaves, x, w, dy = make(3000, 6, 72, 136, torch.bfloat16, ordered=True)
+    offsets, order = ops.group_rows(leaves.cuda(), 6)
+    runs = []
+    for _ in range(3):
+        xg, wg = x.cuda().requires_grad_(), w.cuda().requires_grad_()
+        y = ops.grouped_matmul(xg, wg, offsets, order)
+        runs.append((y.detach(), *torch.autograd.grad(y, (xg, wg), dy.cuda())))
+    for r in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(r, runs[0]))
+
+
+@pytest.mark.parametrize("M, E, N, K", [(24, 40, 8, 32), (500, 4, 160, 192)])
+def test_streams_and_graphs(M, E, N, K):
+    from yggdrasil_amd import ops
+    leaves, x, w, dy = make(M, E, N, K, torch.bfloat16)
+    xg, wg = x.cuda(), w.cuda()
+    offsets, order = ops.group_rows(leaves.cuda(), E)
+    want = ops.grouped_matmul(xg, wg, offsets, order)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = ops.grouped_matmul(xg, wg, offsets, order)
+    s.synchronize()
+    assert torch.equal(got, want)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = ops.grouped_matmul(xg, wg, offsets, order)
+    for k in range(4):
+        l2, x2, w2, _ = make(M, E, N, K, torch.bfloat16, seed=k + 5)
+        o2, r2 = ops.group_rows(l2.cuda(), E)
+        for a, b in ((xg, x2), (wg, w2), (offsets, o2), (order, r2)):
+            a.copy_(b)
+        g.replay()
+        torch.cuda.synchronize()
+        want = ops.grouped_matmul(x2.cuda(), w2.cuda(), o2, r2)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), k
+
+
+def test_group_rows():
+    from yggdrasil_amd import ops
+    leaves = torch.tensor([3, 0, 3, -1, 1, 9, 0], device="cuda")
+    offsets, order = ops.group_rows(leaves, 5)
+    assert offsets.tolist() == [0, 2, 3, 3, 5, 5] and order.tolist() == [1, 6, 4, 0, 2, 3, 5]
+    assert offsets.dtype == order.dtype == torch.int32
+    offsets, order = ops.group_rows(torch.empty(0, dtype=torch.int64, device="cuda"), 2)
+    assert offsets.tolist() == [0, 0, 0] and order.numel() == 0
+
+
+def test_refusals():
+    from yggdrasil_amd import ops
+    x, w = torch.zeros(6, 8, device="cuda"), torch.zeros(3, 4, 8, device="cuda")
+    off = torch.zeros(4, dtype=torch.int32, device="cuda")
+    ops.grouped_matmul(x, w, off)
+    for a in ((x[0], w, off), (x, w[0], off), (x, w.half(), off), (x, w[:, :, :7], off), (x, w, off[:3]), (x, w, off.long()),
+              (x, w, off.cpu()), (x, w, off, torch.zeros(5, dtype=torch.int32, device="cuda")),
+              (x, w, off, torch.zeros(6, dtype=torch.int64, device="cuda")), (x.double(), w.double(), off), (x, w.cpu(), off),
+              (x, w[:, :0], off), (x, w[:0], off[:1])):
+        with pytest.raises(ValueError):
+            ops.grouped_matmul(*a)
+    with pytest.raises(ValueError):
+        ops.group_rows(torch.zeros(3, device="cuda"), 2)
+    with pytest.raises(ValueError):
+        ops.group_rows(torch.zeros(3, dtype=torch.int32, device="cuda"), 0)

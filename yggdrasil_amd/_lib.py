@@ -19,10 +19,11 @@ SYMBOLS = ("ygg_load", "ygg_load_blob", "ygg_model_info", "ygg_free", "ygg_step"
            "ygg_score_scratch",
            "ygg_generate", "ygg_take_errors", "ygg_float_load", "ygg_float_run", "ygg_float_scratch",
            "ygg_float_run_scratch", "ygg_float_nll", "ygg_float_take_errors",
-           "ygg_float_free", "ygg_kernel_name", "ygg_spec_stats", "ygg_last_error", "ygg_version")
+           "ygg_float_free", "ygg_logprobs_scratch", "ygg_logprobs", "ygg_logprobs_grad", "ygg_grouped_matmul",
+           "ygg_grouped_grad_x", "ygg_grouped_grad_w", "ygg_int8_scratch", "ygg_int8_linear", "ygg_kernel_name", "ygg_spec_stats", "ygg_last_error", "ygg_version")
 
 ERRORS = {1: "io", 2: "format", 3: "limits", 4: "nomem", 5: "arg", 6: "token", 7: "device"}
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 
 class FloatLayer(ctypes.Structure):
@@ -96,6 +97,16 @@ def lib() -> ctypes.CDLL:
     L.ygg_float_take_errors.argtypes = [vp, vp, ctypes.POINTER(ctypes.c_uint32)]
     L.ygg_float_free.argtypes = [vp]
     L.ygg_float_free.restype = None
+    i64 = ctypes.c_int64
+    L.ygg_logprobs_scratch.argtypes = [i32, i64, i32, i32]
+    L.ygg_logprobs_scratch.restype = i64
+    L.ygg_logprobs.argtypes = [vp, i32, i64, i32, i64, vp, i32, i32, vp, vp, vp, vp, vp, vp, i64, vp]
+    L.ygg_logprobs_grad.argtypes = [vp, i32, i64, i32, i64, vp, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]
+    for f in (L.ygg_grouped_matmul, L.ygg_grouped_grad_x, L.ygg_grouped_grad_w):
+        f.argtypes = [vp, vp, i32, vp, vp, i32, i32, i32, i32, vp, vp]
+    L.ygg_int8_scratch.argtypes = [i32, i32, i32]
+    L.ygg_int8_scratch.restype = i64
+    L.ygg_int8_linear.argtypes = [vp, i32, vp, vp, i32, i32, i32, vp, vp, i64, vp]
     L.ygg_last_error.argtypes = []
     L.ygg_last_error.restype = ctypes.c_char_p
     L.ygg_version.argtypes = []

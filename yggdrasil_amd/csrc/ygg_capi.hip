@@ -18,6 +18,7 @@
 
 #include "../../include/ygg_hip.h"
 #include "ygg_launch.h"
+#include "ygg_ops.h"
 #include "ygg_scan.h"
 #include "ygg_layout.h"
 
@@ -932,7 +933,7 @@ int set_error(int code, const char *msg) { return fail(code, "%s", msg); }
 
 extern "C" {
 
-int ygg_version(void) { return 11; }
+int ygg_version(void) { return 12; }
 
 const char *ygg_last_error(void) { return g_err.c_str(); }
 
@@ -1204,6 +1205,113 @@ int ygg_step(const ygg_model *m, const int32_t *d_tokens, const int8_t *d_state_
     io.logits = d_logits;
     io.leaves = d_leaves;
     HIP_TRY(k.fn(m->dev, d_tokens, B, 1, d_state_out, io, (hipStream_t)stream));
+    return YGG_OK;
+}
+
+// ---- the output head's operators, on the caller's current device and stream
+
+static const char *const kTypeHelp = "type %d: 0 f32, 1 bf16, 2 f16";
+static const char *const kOpLimits = "%s %lld outside [%d, %d]";
+
+int64_t ygg_logprobs_scratch(int type, int64_t rows, int V, int top) {
+    if (type < 0 || type > 2 || rows < 1 || V < 1 || top < 0 || top > YGG_MOST_TOP) return 0;
+    return ygg::logprobs_scratch(type, rows, V, top);
+}
+
+int ygg_logprobs(const void *d_logits, int type, int64_t rows, int V, int64_t stride, const void *d_targets,
+                 int target_bytes, int top, float *d_logp, float *d_entropy, float *d_top_logp, int32_t *d_top_ids,
+                 float *d_stats, void *d_scratch, int64_t scratch_bytes, void *stream) {
+    if (type < 0 || type > 2) return fail(YGG_ERR_ARG, kTypeHelp, type);
+    if (rows < 0) return fail(YGG_ERR_ARG, "negative rows (%lld)", (long long)rows);
+    if (V < 1 || V > YGG_MOST_VOCAB) return fail(YGG_ERR_ARG, kOpLimits, "V", (long long)V, 1, YGG_MOST_VOCAB);
+    if (stride < V && rows > 1) return fail(YGG_ERR_ARG, "rows of %d values %lld apart", V, (long long)stride);
+    if (top < 0 || top > YGG_MOST_TOP) return fail(YGG_ERR_ARG, kOpLimits, "top", (long long)top, 0, YGG_MOST_TOP);
+    if (target_bytes != 0 && target_bytes != 4 && target_bytes != 8)
+        return fail(YGG_ERR_ARG, "target_bytes %d: 4, 8 or 0", target_bytes);
+    if (rows == 0) return YGG_OK;
+    if (!d_logits || !d_entropy || (target_bytes && (!d_targets || !d_logp)) || (top && (!d_top_logp || !d_top_ids)))
+        return fail(YGG_ERR_ARG, "NULL buffer");
+    const int64_t need = ygg::logprobs_scratch(type, rows, V, top);
+    if (need && (!d_scratch || scratch_bytes < need))
+        return fail(YGG_ERR_ARG, "scratch of %lld bytes, %lld wanted", (long long)scratch_bytes, (long long)need);
+    const ygg::LogprobsArgs a = {d_logits, rows, stride, V, top, target_bytes, d_targets, d_logp, d_entropy, d_top_logp,
+                                 d_top_ids, (float2 *)d_stats};
+    HIP_TRY(ygg::launch_logprobs(type, a, d_scratch, (hipStream_t)stream));
+    return YGG_OK;
+}
+
+int ygg_logprobs_grad(const void *d_logits, int type, int64_t rows, int V, int64_t stride, const void *d_targets,
+                      int target_bytes, int top, const float *d_entropy, const int32_t *d_top_ids, const float *d_stats,
+                      const float *d_g_logp, const float *d_g_entropy, const float *d_g_top, void *d_out, void *stream) {
+    if (type < 0 || type > 2) return fail(YGG_ERR_ARG, kTypeHelp, type);
+    if (rows < 0) return fail(YGG_ERR_ARG, "negative rows (%lld)", (long long)rows);
+    if (V < 1 || V > YGG_MOST_VOCAB) return fail(YGG_ERR_ARG, kOpLimits, "V", (long long)V, 1, YGG_MOST_VOCAB);
+    if (stride < V && rows > 1) return fail(YGG_ERR_ARG, "rows of %d values %lld apart", V, (long long)stride);
+    if (top < 0 || top > YGG_MOST_TOP) return fail(YGG_ERR_ARG, kOpLimits, "top", (long long)top, 0, YGG_MOST_TOP);
+    if (d_g_logp && target_bytes != 4 && target_bytes != 8) return fail(YGG_ERR_ARG, "target_bytes %d: 4 or 8", target_bytes);
+    if (rows == 0) return YGG_OK;
+    if (!d_logits || !d_entropy || !d_stats || !d_out || (d_g_logp && !d_targets) || (d_g_top && top && !d_top_ids))
+        return fail(YGG_ERR_ARG, "NULL buffer");
+    const ygg::LogprobsGradArgs a = {d_logits, rows, stride, V, top, target_bytes, d_targets, d_entropy, d_top_ids,
+                                     (const float2 *)d_stats, d_g_logp, d_g_entropy, top ? d_g_top : nullptr, d_out};
+    HIP_TRY(ygg::launch_logprobs_grad(type, a, (hipStream_t)stream));
+    return YGG_OK;
+}
+
+// sizes of a product over experts: an error code, or 0 (done: there is nothing to compute)
+static int check_grouped(int type, const void *d_offsets, int M, int E, int N, int K) {
+    if (type < 0 || type > 2) return fail(YGG_ERR_ARG, kTypeHelp, type);
+    if (M < 0 || M > YGG_MOST_ROWS) return fail(YGG_ERR_ARG, kOpLimits, "M", (long long)M, 0, YGG_MOST_ROWS);
+    if (E < 1 || E > YGG_MOST_EXPERTS) return fail(YGG_ERR_ARG, kOpLimits, "E", (long long)E, 1, YGG_MOST_EXPERTS);
+    if (N < 1 || N > YGG_MOST_INNER) return fail(YGG_ERR_ARG, kOpLimits, "N", (long long)N, 1, YGG_MOST_INNER);
+    if (K < 1 || K > YGG_MOST_INNER) return fail(YGG_ERR_ARG, kOpLimits, "K", (long long)K, 1, YGG_MOST_INNER);
+    if (!d_offsets) return fail(YGG_ERR_ARG, "NULL buffer");
+    return YGG_OK;
+}
+
+int ygg_grouped_matmul(const void *d_x, const void *d_w, int type, const int32_t *d_offsets, const int32_t *d_order, int M,
+                       int E, int N, int K, void *d_y, void *stream) {
+    if (int rc = check_grouped(type, d_offsets, M, E, N, K)) return rc;
+    if (M == 0) return YGG_OK;
+    if (!d_x || !d_w || !d_y) return fail(YGG_ERR_ARG, "NULL buffer");
+    HIP_TRY(ygg::launch_grouped_matmul(type, d_x, d_w, {d_offsets, d_order, M, E}, N, K, d_y, (hipStream_t)stream));
+    return YGG_OK;
+}
+
+int ygg_grouped_grad_x(const void *d_dy, const void *d_w, int type, const int32_t *d_offsets, const int32_t *d_order, int M,
+                       int E, int N, int K, void *d_dx, void *stream) {
+    if (int rc = check_grouped(type, d_offsets, M, E, N, K)) return rc;
+    if (M == 0) return YGG_OK;
+    if (!d_dy || !d_w || !d_dx) return fail(YGG_ERR_ARG, "NULL buffer");
+    HIP_TRY(ygg::launch_grouped_grad_x(type, d_dy, d_w, {d_offsets, d_order, M, E}, N, K, d_dx, (hipStream_t)stream));
+    return YGG_OK;
+}
+
+int ygg_grouped_grad_w(const void *d_dy, const void *d_x, int type, const int32_t *d_offsets, const int32_t *d_order, int M,
+                       int E, int N, int K, void *d_dw, void *stream) {
+    if (int rc = check_grouped(type, d_offsets, M, E, N, K)) return rc;
+    if (!d_dw || (M > 0 && (!d_dy || !d_x))) return fail(YGG_ERR_ARG, "NULL buffer");
+    HIP_TRY(ygg::launch_grouped_grad_w(type, d_dy, d_x, {d_offsets, d_order, M, E}, N, K, d_dw, (hipStream_t)stream));
+    return YGG_OK;
+}
+
+int64_t ygg_int8_scratch(int M, int N, int K) {
+    if (M < 1 || M > YGG_MOST_ROWS || N < 1 || K < 1 || K > YGG_MOST_INNER) return 0;
+    return ygg::int8_scratch(M, N, K);
+}
+
+int ygg_int8_linear(const void *d_x, int type, const int8_t *d_w, const float *d_w_scale, int M, int N, int K, void *d_y,
+                    void *d_scratch, int64_t scratch_bytes, void *stream) {
+    if (type < 0 || type > 2) return fail(YGG_ERR_ARG, kTypeHelp, type);
+    if (M < 0 || M > YGG_MOST_ROWS) return fail(YGG_ERR_ARG, kOpLimits, "M", (long long)M, 0, YGG_MOST_ROWS);
+    if (N < 1 || N > YGG_MOST_VOCAB) return fail(YGG_ERR_ARG, kOpLimits, "N", (long long)N, 1, YGG_MOST_VOCAB);
+    if (K < 1 || K > YGG_MOST_INNER) return fail(YGG_ERR_ARG, kOpLimits, "K", (long long)K, 1, YGG_MOST_INNER);
+    if (M == 0) return YGG_OK;
+    if (!d_x || !d_w || !d_w_scale || !d_y) return fail(YGG_ERR_ARG, "NULL buffer");
+    const int64_t need = ygg::int8_scratch(M, N, K);
+    if (need && (!d_scratch || scratch_bytes < need))
+        return fail(YGG_ERR_ARG, "scratch of %lld bytes, %lld wanted", (long long)scratch_bytes, (long long)need);
+    HIP_TRY(ygg::launch_int8_linear(type, d_x, d_w, d_w_scale, M, N, K, d_y, d_scratch, (hipStream_t)stream));
     return YGG_OK;
 }
 
