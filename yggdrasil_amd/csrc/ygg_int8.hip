@@ -1,9 +1,9 @@
 // The int8 projection of float rows: row i is quantised with its own scale, s_i = max(max |x_i| / 127, 2^-126),
 // q = x / s_i rounded to nearest with ties to even, and multiplied by an int8 matrix with a scale for each of its rows,
-// y_in = (sum_k q_ik w_nk) ws_n s_i (multiplied in this order: a row's scale may be near the ends of f32's range). The integer sums are exact in 32 bits (K <= 131072). A row with a NaN or an infinity
-// has a NaN scale, so it is NaN throughout.
+// y_in = (sum_k q_ik w_nk) ws_n s_i (multiplied in this order: a row's scale may be near the ends of f32's range). The
+// integer sums are exact in 32 bits (K <= 131072). A row with a NaN or an infinity has a NaN scale, so it is NaN throughout.
+#include "ygg_gemm.h"
 #include "ygg_ops.h"
-#include "ygg_optype.h"
 
 namespace ygg {
 namespace {
@@ -31,15 +31,35 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T *x, int K, int Kp
         q[k] = k < K && !bad ? (int8_t)(int)__builtin_rintf(to_f32(x[k]) / s) : (int8_t)0;
 }
 
-template <class T>
-__global__ __launch_bounds__(256) void int8_kernel(const int8_t *q, const float *scale, const int8_t *w, const float *ws,
-                                                   int N, int K, int Kp, T *y) {
-    const int64_t row = blockIdx.x;
-    const int n = blockIdx.y * 256 + threadIdx.x;
-    if (n >= N) return;
-    int acc = 0;
-    for (int k = 0; k < K; k++) acc += (int)q[row * Kp + k] * (int)w[(int64_t)n * K + k];
-    y[row * N + n] = from_f32<T>((float)acc * ws[n] * scale[row]);
+// A tile of rows and w's rows: the integers' products on the matrix cores, then a row's and a column's scale
+template <class T, int FI, int FO, int WI, int WO, int kBufs>
+__global__ __launch_bounds__(64 * WI * WO) void int8_kernel(const int8_t *q, const float *scale, const int8_t *w, const float *ws,
+                                                            int M, int N, int K, int Kp, T *y, int cols) {
+    constexpr int kThreads = 64 * WI * WO, kI = 16 * FI * WI, kO = 16 * FO * WO;
+    typedef Along<int8_t, kI, kThreads, FI, true> A;
+    typedef Along<int8_t, kO, kThreads, FO, false> B;
+    typedef Tile<int8_t, FI, FO, WI, WO, kBufs, A, B> Tl;
+    __shared__ __align__(128) char lds[Tl::kLds];
+    const int t = tile_of(blockIdx.x, gridDim.x), i0 = t / cols * kI, o0 = t % cols * kO;
+    Tl tile;
+    A a;
+    B b;
+    a.begin([&](int i) { return q + (int64_t)min(i0 + i, M - 1) * Kp; });
+    b.begin([&](int o) { return w + (int64_t)min(o0 + o, N - 1) * K; });
+    tile.run(a, b, lds, (K + 127) / 128, [&](int s) {
+        a.load(s * 128, Kp);
+        b.load(s * 128, K);
+    });
+    tile.template each<true>([&](int i, int o, const i32x4 *v, auto n) {
+        constexpr int kN = decltype(n)::value;
+        const int row = i0 + i, col = o0 + o;
+        if (row >= M || col >= N) return;
+        const float s = scale[row];
+        float f[kN];
+#pragma unroll
+        for (int j = 0; j < kN; j++) f[j] = (float)v[j / 4][j % 4] * ws[min(col + j, N - 1)] * s;
+        store_run<T, kN>(y + (int64_t)row * N + col, f, N - col);
+    });
 }
 
 int padded(int K) { return (K + 127) / 128 * 128; }
@@ -49,7 +69,12 @@ hipError_t go(const void *x, const int8_t *w, const float *ws, int M, int N, int
     float *scale = (float *)scratch;
     int8_t *q = (int8_t *)scratch + ((int64_t)M * 4 + 255) / 256 * 256;
     hipLaunchKernelGGL(quantize_kernel<T>, dim3(M), dim3(256), 0, st, (const T *)x, K, padded(K), q, scale);
-    hipLaunchKernelGGL(int8_kernel<T>, dim3(M, (N + 255) / 256), dim3(256), 0, st, q, scale, w, ws, N, K, padded(K), (T *)y);
+    constexpr int FI = 4, FO = 4, WI = 2, WO = 2, kBufs = 1, kI = 16 * FI * WI, kO = 16 * FO * WO;
+    const int cols = (N + kO - 1) / kO;
+    const int64_t tiles = (int64_t)((M + kI - 1) / kI) * cols;
+    if (tiles > INT32_MAX) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((int8_kernel<T, FI, FO, WI, WO, kBufs>), dim3((unsigned)tiles), dim3(64 * WI * WO), 0, st, q, scale, w,
+                       ws, M, N, K, padded(K), (T *)y, cols);
     return hipGetLastError();
 }
 
