@@ -307,3 +307,36 @@ def test_refusals():
         ops.group_rows(torch.zeros(3, device="cuda"), 2)
     with pytest.raises(ValueError):
         ops.group_rows(torch.zeros(3, dtype=torch.int32, device="cuda"), 0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("M, E, N, K, ordered", [
+    (8192, 8, 2048, 2056, True), (5000, 16, 1528, 2040, False), (9000, 2, 4096, 264, True), (16384, 1, 2048, 1000, True),
+    (3000, 16, 1000, 1000, True), (2500, 9, 1027, 2049, True)])
+def test_large_tiles(M, E, N, K, ordered, dtype):
+    """Products large enough for the largest tiles, with rows of no expert, ends inside a tile and a step, more rows of one
+    expert than a workgroup holds numbers of; against products in 64 bits on the GPU, to the tolerances above."""
+    from yggdrasil_amd import ops
+    g = torch.Generator("cuda").manual_seed(M + N)
+    leaves = torch.randint(E, (M,), device="cuda", generator=g)
+    leaves[torch.rand(M, device="cuda", generator=g) < 0.3] = E // 2
+    leaves[:5] = -1
+    if not ordered:
+        leaves = torch.where(leaves < 0, E, leaves).sort().values
+    offsets, order = ops.group_rows(leaves, E)
+    x = torch.randn(M, K, device="cuda", generator=g).to(dtype).requires_grad_()
+    w = (torch.randn(E, N, K, device="cuda", generator=g) / math.sqrt(K)).to(dtype).requires_grad_()
+    dy = torch.randn(M, N, device="cuda", generator=g).to(dtype)
+    y = ops.grouped_matmul(x, w, offsets, order if ordered else None)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    x, w = x.detach(), w.detach()
+    for e in range(-1, E):
+        i = ((leaves < 0) | (leaves >= E) if e < 0 else leaves == e).nonzero()[:, 0]
+        if e < 0:
+            assert (y[i] == 0).all() and (dx[i] == 0).all()
+            continue
+        a, b, c = x[i].double(), w[e].double(), dy[i].double()
+        bt, ct = b.t().contiguous(), c.t().contiguous()
+        near(y[i], (a @ bt).cpu(), (a ** 2 @ bt ** 2).cpu(), K)
+        near(dx[i], (c @ b).cpu(), (c ** 2 @ b ** 2).cpu(), N)
+        near(dw[e], (ct @ a).cpu(), (ct ** 2 @ a ** 2).cpu(), max(len(i), 1))

@@ -164,3 +164,14 @@ def test_refusals():
         ops.int8_linear(x.requires_grad_(), w, ws)
     with torch.no_grad():
         ops.int8_linear(x, w, ws)
+
+
+@pytest.mark.parametrize("M, N, K", [(4100, 4100, 1008), (4096, 4096, 2048), (5000, 3000, 1040), (4111, 4099, 333)])
+def test_large_tiles(M, N, K):
+    """Enough tiles for the largest ones, ends inside a tile and a step; the integers' products in 64 bits on the GPU."""
+    from yggdrasil_amd import ops
+    x, w, ws = make(M, N, K, torch.float32)
+    s = (x.double().abs().amax(1) / 127).float().double()[:, None]
+    ref = (torch.round((x.double() / s).float()).double() @ w.double().t().contiguous()) * s * ws.double()
+    err = (ops.int8_linear(x, w, ws).double() - ref).abs()
+    assert (err <= 4 * 2.0 ** -24 * ref.abs() * (1 + 2.0 ** -20) + 2.0 ** -126).all()

@@ -198,6 +198,43 @@ template <class T, int kB, int kThreads> struct Across {
     }
 };
 
+// The 64 lanes' u[k] as four groups of 16 lanes: group g gets u[g] of group k in the place of u[k]
+template <class V> __device__ __forceinline__ void transpose_groups(V (&u)[4]) {
+    auto swap = [](V &a, V &b, bool far) {
+        const uint32_t x = __builtin_bit_cast(uint32_t, a), y = __builtin_bit_cast(uint32_t, b);
+        const u32x2 r = far ? __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(x, y, false, false))
+                            : __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(x, y, false, false));
+        a = __builtin_bit_cast(V, (uint32_t)r[0]);
+        b = __builtin_bit_cast(V, (uint32_t)r[1]);
+    };
+    swap(u[0], u[2], true);
+    swap(u[1], u[3], true);
+    swap(u[0], u[1], false);
+    swap(u[2], u[3], false);
+}
+
+// The lane's results: of tile row row0 + 16 i + lane % 16, 16 consecutive columns. put(row, column, values, count) for each;
+// dealt: the columns' operand is Along. Otherwise a lane has 4 of each fragment's 16, and the four groups of lanes trade them:
+// stores of 8 bytes to 16 rows each took 5 us a workgroup of 256 x 256 bf16, these 2.
+template <bool kDealt, int FI, int FO, class Acc, class F>
+__device__ __forceinline__ void each_run(Acc (&acc)[FI][FO], int row0, int col0, F put) {
+    static_assert(FO == 4, "");
+    const int l = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < FI; i++) {
+        if constexpr (!kDealt) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                decltype(acc[0][0][0] + 0) u[4] = {acc[i][0][j], acc[i][1][j], acc[i][2][j], acc[i][3][j]};
+                transpose_groups(u);
+#pragma unroll
+                for (int o = 0; o < 4; o++) acc[i][o][j] = u[o];
+            }
+        }
+        put(row0 + 16 * i + (l & 15), col0 + 16 * (l >> 4), &acc[i][0], std::integral_constant<int, 16>());
+    }
+}
+
 // A workgroup's tile: WI x WO waves, each 16 FI rows by 16 FO columns. a.load and b.load are called by load(step); kBufs 2:
 // a step is stored while the one before it is read, one barrier a step and twice the LDS; 1: two barriers, and other
 // workgroups of the CU work meanwhile.
@@ -258,21 +295,212 @@ template <class T, int FI, int FO, int WI, int WO, int kBufs, class A, class B> 
             }
         }
     }
-    // The lane's results: of tile row row0() + 16 i + lane % 16, runs of consecutive columns. put(row, column, values, count)
-    // for each; dealt: the columns' operand is Along.
-    template <bool kDealt, class F> __device__ __forceinline__ void each(F put) const {
-        const int l = threadIdx.x & 63;
+    template <bool kDealt, class F> __device__ __forceinline__ void each(F put) { each_run<kDealt>(acc, row0(), col0(), put); }
+};
+
+// The same product for operands whose rows are 16-byte aligned, straight from memory into LDS (no registers, no stores).
+//
+// 8 waves, two a SIMD, in two groups that take turns: while one reads fragments and issues loads, the other's matrix
+// instructions run; a barrier after every turn. A step of 128 bytes is two turns, half the wave's rows each, so that half the
+// rows' fragments are held. Of the two LDS buffers each half operand (a region) is filled anew as soon as both groups have
+// read it, two steps ahead of its use: three turns pass between a load and its first use, and no wait drains the queue.
+//
+//   turn 0 reads a0, b0, b1, loads a1 of the step before's place;  products a0 b0, a0 b1
+//   turn 1 reads a1, loads a0, b0, b1;                             products a1 b0, a1 b1
+//
+// A buffer load whose lane lies past the descriptor's size brings zeros: what the reduction's end leaves of a step.
+typedef uint32_t Rsrc __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ Rsrc rsrc_of(const void *p, uint32_t bytes) {
+    const uint64_t a = (uint64_t)p;
+    return Rsrc{(uint32_t)__builtin_amdgcn_readfirstlane((int)a), (uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)) & 0xffffu,
+                (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
+}
+constexpr uint32_t kFar = 0x80000000u;   // past every descriptor's size
+// 16 bytes a lane to LDS from `lds` on (a wave's number: the same for all its lanes), lane after lane. The load has no output
+// registers; the caller waits for it.
+__device__ __forceinline__ void load_lds(Rsrc r, uint32_t offset, uint32_t lds) {
+    lds = __builtin_amdgcn_readfirstlane((int)lds);
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(r), "s"(lds) : "memory", "m0");
+}
+template <int kCount> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kCount) : "memory"); }
+__device__ __forceinline__ void turn_over() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// An operand whose reduction index is contiguous, kW wave parts of 16 kF rows each: two regions of kW * 8 kF rows of 128
+// bytes, in the order of the fragments. kRow as for Along.
+template <class T, int kF, int kW, bool kRow> struct AlongLds {
+    static constexpr int kRows = kW * 8 * kF, kBytes = kRows * 128, kN = kRows / 64;   // loads of a region a thread
+    static_assert(kF % 2 == 0 && kN * 64 == kRows, "");
+    Rsrc src;
+    uint32_t at[2][kN];
+    int end;       // bytes of the reduction from the lane's piece on
+    // offset(i): where tile row i begins, in bytes from base; bytes: of the whole operand, bytes_r: of a row
+    template <class F> __device__ __forceinline__ void begin(const void *base, uint32_t bytes, int bytes_r, F offset) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, piece = ((lane & 7) ^ (lane >> 3)) * 16;
+        src = rsrc_of(base, bytes);
+        end = bytes_r - piece;
 #pragma unroll
-        for (int i = 0; i < FI; i++) {
-            const int row = row0() + 16 * i + (l & 15);
-            if constexpr (kDealt) {
-                put(row, col0() + 4 * FO * (l >> 4), &acc[i][0], std::integral_constant<int, 4 * FO>());
-            } else {
+        for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int o = 0; o < FO; o++) put(row, col0() + 16 * o + 4 * (l >> 4), &acc[i][o], std::integral_constant<int, 4>());
+            for (int i = 0; i < kN; i++) {
+                const int row = (i * 8 + wave) * 8 + (lane >> 3);
+                const int part = row / (8 * kF), f = row / 16 % (kF / 2) + h * (kF / 2), d = row & 15;
+                at[h][i] = offset(part * 16 * kF + (kRow ? 16 * f + d : 4 * kF * (d >> 2) + 4 * f + (d & 3))) + piece;
             }
+    }
+    template <int h> __device__ __forceinline__ void load(int step, uint32_t lds) const {
+        const uint32_t add = step * 128 < end ? step * 128 : kFar;
+#pragma unroll
+        for (int i = 0; i < kN; i++) load_lds(src, at[h][i] + add, lds + (i * 8 + (threadIdx.x >> 6)) * 1024);
+    }
+    // fragment f (of kF / 2) of wave part `part`
+    static __device__ __forceinline__ u32x4 frag(const char *lds, int part, int f, int half) {
+        const int d = threadIdx.x & 15, q = threadIdx.x >> 4 & 3;
+        return *(const u32x4 *)(lds + part * (8 * kF * 128) + f * 2048 + d * 128 + (((half * 4 + q) ^ (d & 7)) << 4));
+    }
+};
+
+// An operand whose reduction index is strided: two regions of kStep r's of kW parts of 8 kF elements each
+template <class T, int kF, int kW> struct AcrossLds {
+    static constexpr int kWide = kW * 8 * kF * sizeof(T), kStep = 128 / sizeof(T), kBytes = kStep * kWide, kN = kBytes / 8192;
+    static constexpr int kPer = 1024 / kWide;        // r's of one load of a wave
+    static_assert(kN * 8192 == kBytes && kWide == (sizeof(T) == 2 ? 256 : 512), "");
+    Rsrc src;
+    uint32_t at[2];
+    static __device__ __forceinline__ int turn(int r) { return Across<T, 256, 512>::turn(r); }
+    // the r in the step of the thread's i th load
+    static __device__ __forceinline__ int r_of(int i) {
+        return (i * 8 + (int)(threadIdx.x >> 6)) * kPer + (int)(threadIdx.x & 63) / (kWide / 16);
+    }
+    // the tile's elements begin `left` bytes before a row's end, `first` bytes from base
+    __device__ __forceinline__ void begin(const void *base, uint32_t bytes, uint32_t first, int left) {
+        const int c = (((int)threadIdx.x * 16) & (kWide - 1)) ^ turn(r_of(0));    // the same for every load
+        constexpr int kPart = 8 * kF * sizeof(T);
+        src = rsrc_of(base, bytes);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int col = c / kPart * 2 * kPart + h * kPart + c % kPart;
+            at[h] = col < left ? first + col : kFar;
         }
     }
+    // row(i): bytes from base to the row of the thread's i th r, or kFar
+    template <int h, class F> __device__ __forceinline__ void load(uint32_t lds, F row) const {
+#pragma unroll
+        for (int i = 0; i < kN; i++) {
+            const uint32_t r = row(i);
+            load_lds(src, max(at[h], r) >= kFar ? kFar : at[h] + r, lds + (i * 8 + (threadIdx.x >> 6)) * 1024);
+        }
+    }
+    static __device__ __forceinline__ u32x4 frag(const char *lds, int part, int f, int half) {
+        const int l = threadIdx.x & 63, d = l & 15, q = l >> 4, base = part * 8 * kF + 16 * f;
+        u32x4 v;
+        if constexpr (sizeof(T) == 2) {
+            typedef __attribute__((address_space(3))) s16x4 *Shared;
+            const int c = (base + 4 * (d & 3)) * 2;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int r = half * 32 + 8 * q + 4 * h + (d >> 2);
+                const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Shared)(lds + r * kWide + (c ^ turn(r)))));
+                v[2 * h] = x[0];
+                v[2 * h + 1] = x[1];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int r = half * 16 + 4 * q + j;
+                v[j] = *(const uint32_t *)(lds + r * kWide + (((base + d) * 4) ^ turn(r)));
+            }
+        }
+        return v;
+    }
+};
+
+template <class T, int FI, int FO, int WI, int WO, class A, class B> struct TurnTile {
+    static constexpr int kI = 16 * FI * WI, kO = 16 * FO * WO, kThreads = 64 * WI * WO;
+    static constexpr int kBuf = 2 * (A::kBytes + B::kBytes), kLds = 2 * kBuf;
+    static constexpr int kA = A::kN, kB = B::kN, kStep = 2 * (kA + kB);
+    static_assert(WI * WO == 8, "");
+    typedef typename Mma<T>::Acc Acc;
+    Acc acc[FI][FO];
+    static __device__ __forceinline__ int wave() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
+    static __device__ __forceinline__ int row0() { return wave() / WO * 16 * FI; }
+    static __device__ __forceinline__ int col0() { return wave() % WO * 16 * FO; }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < FI; i++)
+#pragma unroll
+            for (int o = 0; o < FO; o++) acc[i][o] = Acc{0, 0, 0, 0};
+    }
+    template <int i0> __device__ __forceinline__ void products(const u32x4 (&x)[2][FI / 2], const u32x4 (&y)[2][FO]) {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int half = 0; half < 2; half++)
+#pragma unroll
+            for (int i = 0; i < FI / 2; i++)
+#pragma unroll
+                for (int o = 0; o < FO; o++) acc[i0 + i][o] = Mma<T>::run(y[half][o], x[half][i], acc[i0 + i][o]);
+        __builtin_amdgcn_s_setprio(0);
+    }
+    // lds: the workgroup's kLds bytes, at an LDS address of its own
+    // load_a(half, step, LDS address) and load_b issue a region's loads, half an integral_constant; fetch(step) comes a turn
+    // or more before a step's first loads, so that what they need from LDS is there
+    template <class LA, class LB, class F>
+    __device__ __forceinline__ void run(char *lds, int steps, LA load_a, LB load_b, F fetch) {
+        typedef __attribute__((address_space(3))) char *Shared;
+        const uint32_t base = __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(Shared)lds);
+        constexpr int kA0 = 0, kA1 = A::kBytes, kB0 = 2 * A::kBytes, kB1 = kB0 + B::kBytes;
+        const int w = wave(), wi = w / WO, wo = w % WO;
+        constexpr std::integral_constant<int, 0> k0{};
+        constexpr std::integral_constant<int, 1> k1{};
+        if (steps <= 0) return;
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const uint32_t buf = base + t * kBuf;
+            fetch(t);
+            load_a(k0, t, buf + kA0);
+            load_b(k0, t, buf + kB0);
+            load_b(k1, t, buf + kB1);
+            load_a(k1, t, buf + kA1);
+        }
+        wait_loads<kA + kStep>();
+        turn_over();
+        if (w >= 4) turn_over();
+        for (int t = 0; t < steps; t++) {
+            const char *now = lds + (t & 1) * kBuf;
+            const uint32_t buf = base + (t & 1) * kBuf;
+            u32x4 x[2][FI / 2], y[2][FO];
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+#pragma unroll
+                for (int o = 0; o < FO; o++) y[half][o] = B::frag(now + (o < FO / 2 ? kB0 : kB1), wo, o % (FO / 2), half);
+#pragma unroll
+                for (int i = 0; i < FI / 2; i++) x[half][i] = A::frag(now + kA0, wi, i, half);
+            }
+            if (t > 0) load_a(k1, t + 1, base + (~t & 1) * kBuf + kA1);
+            fetch(t + 2);
+            wait_loads<kStep>();
+            turn_over();
+            products<0>(x, y);
+            turn_over();
+#pragma unroll
+            for (int half = 0; half < 2; half++)
+#pragma unroll
+                for (int i = 0; i < FI / 2; i++) x[half][i] = A::frag(now + kA1, wi, i, half);
+            load_a(k0, t + 2, buf + kA0);
+            load_b(k0, t + 2, buf + kB0);
+            load_b(k1, t + 2, buf + kB1);
+            wait_loads<kStep>();
+            turn_over();
+            products<FI / 2>(x, y);
+            turn_over();
+        }
+        if (w < 4) turn_over();
+        wait_loads<0>();    // those of the steps past the last write LDS too
+    }
+    template <bool kDealt, class F> __device__ __forceinline__ void each(F put) { each_run<kDealt>(acc, row0(), col0(), put); }
 };
 
 // kN consecutive values rounded to T at an address of T's alignment, of which the first `left` exist
@@ -301,6 +529,15 @@ __device__ __forceinline__ int tile_of(int id, int tiles) {
     const int most = (tiles + 7) / 8, full = tiles - (most - 1) * 8;   // the first `full` XCDs have `most`
     const int x = id & 7;
     return (x < full ? x * most : full * most + (x - full) * (most - 1)) + (id >> 3);
+}
+
+// Tile t of rows x cols of them, by bands of `band` rows, down each column of a band: neighbours share both operands
+struct Place {
+    int row, col;
+};
+__device__ __forceinline__ Place place_of(int t, int rows, int cols, int band) {
+    const int b = t / (band * cols), in = t - b * band * cols, high = min(band, rows - b * band);
+    return {b * band + in % high, in / high};
 }
 
 }  // namespace ygg

@@ -34,13 +34,14 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T *x, int K, int Kp
 // A tile of rows and w's rows: the integers' products on the matrix cores, then a row's and a column's scale
 template <class T, int FI, int FO, int WI, int WO, int kBufs>
 __global__ __launch_bounds__(64 * WI * WO) void int8_kernel(const int8_t *q, const float *scale, const int8_t *w, const float *ws,
-                                                            int M, int N, int K, int Kp, T *y, int cols) {
+                                                            int M, int N, int K, int Kp, T *y, int cols, int band) {
     constexpr int kThreads = 64 * WI * WO, kI = 16 * FI * WI, kO = 16 * FO * WO;
     typedef Along<int8_t, kI, kThreads, FI, true> A;
     typedef Along<int8_t, kO, kThreads, FO, false> B;
     typedef Tile<int8_t, FI, FO, WI, WO, kBufs, A, B> Tl;
     __shared__ __align__(128) char lds[Tl::kLds];
-    const int t = tile_of(blockIdx.x, gridDim.x), i0 = t / cols * kI, o0 = t % cols * kO;
+    const Place t = place_of(tile_of(blockIdx.x, gridDim.x), gridDim.x / cols, cols, band);
+    const int i0 = t.row * kI, o0 = t.col * kO;
     Tl tile;
     A a;
     B b;
@@ -62,6 +63,37 @@ __global__ __launch_bounds__(64 * WI * WO) void int8_kernel(const int8_t *q, con
     });
 }
 
+// The same where K is a multiple of 16 and the integers of x and of w have less than 2 GiB
+template <class T, int FI, int FO, int WI, int WO>
+__global__ __launch_bounds__(512) void int8_turn_kernel(const int8_t *q, const float *scale, const int8_t *w, const float *ws, int M,
+                                                        int N, int K, int Kp, T *y, int cols, int band) {
+    constexpr int kI = 16 * FI * WI, kO = 16 * FO * WO;
+    typedef AlongLds<int8_t, FI, WI, true> A;
+    typedef AlongLds<int8_t, FO, WO, false> B;
+    typedef TurnTile<int8_t, FI, FO, WI, WO, A, B> Tl;
+    __shared__ __align__(1024) char lds[Tl::kLds];
+    const Place t = place_of(tile_of(blockIdx.x, gridDim.x), gridDim.x / cols, cols, band);
+    const int i0 = t.row * kI, o0 = t.col * kO;
+    Tl tile;
+    A a;
+    B b;
+    a.begin(q, (uint32_t)M * Kp, Kp, [&](int i) { return (uint32_t)min(i0 + i, M - 1) * Kp; });
+    b.begin(w, (uint32_t)N * K, K, [&](int o) { return (uint32_t)min(o0 + o, N - 1) * K; });
+    tile.clear();
+    tile.run(lds, (K + 127) / 128, [&](auto h, int s, uint32_t to) { a.template load<decltype(h)::value>(s, to); },
+             [&](auto h, int s, uint32_t to) { b.template load<decltype(h)::value>(s, to); }, [](int) {});
+    tile.template each<true>([&](int i, int o, const i32x4 *v, auto n) {
+        constexpr int kN = decltype(n)::value;
+        const int row = i0 + i, col = o0 + o;
+        if (row >= M || col >= N) return;
+        const float s = scale[row];
+        float f[kN];
+#pragma unroll
+        for (int j = 0; j < kN; j++) f[j] = (float)v[j / 4][j % 4] * ws[min(col + j, N - 1)] * s;
+        store_run<T, kN>(y + (int64_t)row * N + col, f, N - col);
+    });
+}
+
 int padded(int K) { return (K + 127) / 128 * 128; }
 
 template <class T>
@@ -69,12 +101,20 @@ hipError_t go(const void *x, const int8_t *w, const float *ws, int M, int N, int
     float *scale = (float *)scratch;
     int8_t *q = (int8_t *)scratch + ((int64_t)M * 4 + 255) / 256 * 256;
     hipLaunchKernelGGL(quantize_kernel<T>, dim3(M), dim3(256), 0, st, (const T *)x, K, padded(K), q, scale);
+    // tiles of 256 x 256 straight to LDS where there are enough of them: 8192 x 4096 x 8192 228 us against 424
+    const int64_t big = (int64_t)((M + 255) / 256) * ((N + 255) / 256);
+    if (K % 16 == 0 && (uintptr_t)w % 16 == 0 && (int64_t)M * padded(K) < 0x78000000 && (int64_t)N * K < 0x78000000 && big >= 256 &&
+        big <= INT32_MAX) {
+        hipLaunchKernelGGL((int8_turn_kernel<T, 8, 4, 2, 4>), dim3((unsigned)big), dim3(512), 0, st, q, scale, w, ws, M, N, K,
+                           padded(K), (T *)y, (N + 255) / 256, 16);
+        return hipGetLastError();
+    }
     constexpr int FI = 4, FO = 4, WI = 2, WO = 2, kBufs = 1, kI = 16 * FI * WI, kO = 16 * FO * WO;
     const int cols = (N + kO - 1) / kO;
     const int64_t tiles = (int64_t)((M + kI - 1) / kI) * cols;
     if (tiles > INT32_MAX) return hipErrorInvalidValue;
     hipLaunchKernelGGL((int8_kernel<T, FI, FO, WI, WO, kBufs>), dim3((unsigned)tiles), dim3(64 * WI * WO), 0, st, q, scale, w,
-                       ws, M, N, K, padded(K), (T *)y, cols);
+                       ws, M, N, K, padded(K), (T *)y, cols, 8);
     return hipGetLastError();
 }
 
