@@ -32,8 +32,6 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 // D += A B^T of 16 rows each: lane l's results are D's rows 4 (l / 16) + j (A's row), column l % 16 (B's row)
 template <class T> struct Mma;
@@ -64,33 +62,6 @@ template <> struct Mma<int8_t> {
         return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
     }
 };
-
-// 16 bytes from an address of T's alignment
-template <class T> __device__ __forceinline__ u32x4 load16(const T *p) {
-    typedef uint32_t any __attribute__((ext_vector_type(4), aligned(1)));
-    return *(const any *)p;
-}
-// of which the first n elements exist; the others come as zero
-template <class T> __device__ __forceinline__ u32x4 load16(const T *p, int n) {
-    constexpr int kE = 16 / sizeof(T);
-    if (n >= kE) return load16(p);
-    u32x4 v = {0, 0, 0, 0};
-    if (n <= 0) return v;
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int j = 0; j < 3; j++)
-            if (j < n) v[j] = ((const uint32_t *)p)[j];
-    } else if constexpr (sizeof(T) == 2) {
-#pragma unroll
-        for (int j = 0; j < 7; j++)
-            if (j < n) v[j / 2] |= (uint32_t)((const uint16_t *)p)[j] << 16 * (j % 2);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 15; j++)
-            if (j < n) v[j / 4] |= (uint32_t)((const uint8_t *)p)[j] << 8 * (j % 4);
-    }
-    return v;
-}
 
 // An operand whose reduction index is contiguous: kB rows of 128 bytes a step. kRow: its fragments are 16 rows in order (the
 // rows' operand), else 4 kF columns are dealt to kF fragments (the columns' operand).
@@ -320,7 +291,7 @@ constexpr uint32_t kFar = 0x80000000u;   // past every descriptor's size
 // registers; the caller waits for it.
 __device__ __forceinline__ void load_lds(Rsrc r, uint32_t offset, uint32_t lds) {
     lds = __builtin_amdgcn_readfirstlane((int)lds);
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(r), "s"(lds) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(r), "s"(lds) : "memory");
 }
 template <int kCount> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kCount) : "memory"); }
 __device__ __forceinline__ void turn_over() {
@@ -502,27 +473,6 @@ template <class T, int FI, int FO, int WI, int WO, class A, class B> struct Turn
     }
     template <bool kDealt, class F> __device__ __forceinline__ void each(F put) { each_run<kDealt>(acc, row0(), col0(), put); }
 };
-
-// kN consecutive values rounded to T at an address of T's alignment, of which the first `left` exist
-template <class T, int kN, class V> __device__ __forceinline__ void store_run(T *p, const V *v, int left) {
-    constexpr int kE = kN * sizeof(T) < 16 ? kN : 16 / sizeof(T);
-    typedef uint32_t any __attribute__((ext_vector_type(kE * sizeof(T) / 4), aligned(1)));
-    if (left >= kN) {
-#pragma unroll
-        for (int k = 0; k < kN; k += kE) {
-            T t[kE];
-#pragma unroll
-            for (int j = 0; j < kE; j++) t[j] = from_f32<T>(v[k + j]);
-            any a;
-            __builtin_memcpy(&a, t, sizeof(a));
-            *(any *)(p + k) = a;
-        }
-    } else {
-#pragma unroll
-        for (int k = 0; k < kN; k++)
-            if (k < left) p[k] = from_f32<T>(v[k]);
-    }
-}
 
 // Workgroups go round the 8 XCDs in turn, each with an L2 of its own: a run of neighbouring tiles to each
 __device__ __forceinline__ int tile_of(int id, int tiles) {
