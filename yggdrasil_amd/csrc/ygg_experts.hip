@@ -1,6 +1,8 @@
 // Products of routed experts: rows x_i times the (N, K) matrix of the expert that row i takes, y_i = W[e_i] x_i, and the
 // gradients dx_i = W[e_i]^T dy_i and dW[e] = sum over e's rows of dy_i x_i^T. Sums are held in f32, each output is rounded
 // once.
+#include <algorithm>
+
 #include "ygg_gemm.h"
 #include "ygg_ops.h"
 
@@ -42,6 +44,22 @@ template <int kI> __device__ __forceinline__ Piece piece_at(const Groups &g, int
     return {lo, (int)at, left};
 }
 
+// The tiles by place, for fewer rows than experts: the tile that begins at this place, if one does
+template <int kI> __device__ __forceinline__ Piece piece_from(const Groups &g, int place) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = g.E + 1;
+    while (n > 1) {
+        const int step = (n + 63) / 64, e = lane * step;
+        const bool before = e < n && (e == 0 || first_of(g, lo + e) <= place);
+        const int at = (63 - __builtin_clzll(__ballot(before))) * step;
+        lo += at;
+        n = min(step, n - at);
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    const int first = first_of(g, lo);
+    return {lo, place, place >= first && (place - first) % kI == 0 ? min(end_of(g, lo) - place, kI) : 0};
+}
+
 // out[row][o] = sum over r of in[row][r] * (TR ? w[e][r][o] : w[e][o][r]): dimensions O and R
 template <class T, int FI, int FO, int WI, int WO, int kBufs, bool TR> struct RowsTile {
     static constexpr int kThreads = 64 * WI * WO, kI = 16 * FI * WI, kO = 16 * FO * WO;
@@ -49,9 +67,7 @@ template <class T, int FI, int FO, int WI, int WO, int kBufs, bool TR> struct Ro
     typedef std::conditional_t<TR, Across<T, kO, kThreads>, Along<T, kO, kThreads, FO, false>> B;
     typedef Tile<T, FI, FO, WI, WO, kBufs, A, B> Tl;
     static __device__ __forceinline__ void run(char *lds, const T *in, const T *w, const Groups &g, int O, int R, T *out,
-                                               int slot, int o0) {
-        const Piece pc = piece_at<kI>(g, slot);
-        if (pc.count <= 0) return;
+                                               const Piece &pc, int o0) {
         Tl tile;
         A a;
         B b;
@@ -61,7 +77,7 @@ template <class T, int FI, int FO, int WI, int WO, int kBufs, bool TR> struct Ro
                 const int row = row_of(g, pc.first + min(i, pc.count - 1));
                 return in + (int64_t)max(row, 0) * R;
             });
-            if constexpr (TR) b.begin(we + o0, O - o0);
+            if constexpr (TR) b.begin(we, o0, O);
             else b.begin([&](int o) { return we + (int64_t)min(o0 + o, O - 1) * R; });
         }
         const int steps = pc.e < g.E ? (R + A::kStep - 1) / A::kStep : 0;
@@ -82,11 +98,13 @@ template <class T, int FI, int FO, int WI, int WO, int kBufs, bool TR> struct Ro
     }
 };
 template <class T, int FI, int FO, int WI, int WO, int kBufs, bool TR>
-__global__ __launch_bounds__(64 * WI * WO) void rows_kernel(const T *in, const T *w, Groups g, int O, int R, T *out, int cols, int band) {
+__global__ __launch_bounds__(64 * WI * WO) void rows_kernel(const T *in, const T *w, Groups g, int O, int R, T *out, int cols, int band,
+                                                            bool by_place) {
     typedef RowsTile<T, FI, FO, WI, WO, kBufs, TR> K;
     __shared__ __align__(128) char lds[K::Tl::kLds];
     const Place t = place_of(tile_of(blockIdx.x, gridDim.x), gridDim.x / cols, cols, band);
-    K::run(lds, in, w, g, O, R, out, t.row, t.col * K::kO);
+    const Piece pc = by_place ? piece_from<K::kI>(g, t.row) : piece_at<K::kI>(g, t.row);
+    if (pc.count > 0) K::run(lds, in, w, g, O, R, out, pc, t.col * K::kO);
 }
 
 // dw[e][n][k] = sum over e's rows of dy[row][n] x[row][k], a tile of (n, k)
@@ -104,8 +122,8 @@ __global__ __launch_bounds__(64 * WI * WO) void grad_w_kernel(const T *dy, const
     Tl tile;
     A a;
     B b;
-    a.begin(dy + n0, N - n0);
-    b.begin(x + k0, K - k0);
+    a.begin(dy, n0, N);
+    b.begin(x, k0, K);
     const int steps = (count + A::kStep - 1) / A::kStep;
     tile.run(a, b, lds, steps, [&](int s) {
         a.load([&](int i) {
@@ -122,6 +140,200 @@ __global__ __launch_bounds__(64 * WI * WO) void grad_w_kernel(const T *dy, const
         if (n0 + i >= N || k0 + o >= K) return;
         store_run<T, decltype(n)::value>(out + (int64_t)(n0 + i) * K + k0 + o, (const float *)v, K - k0 - o);
     });
+}
+
+// Few rows an expert: y (not its transpose) of 16 rows by 16 columns a workgroup, whose kW waves take a part of r each; the
+// fragments come straight from memory, 8 of each operand in flight a lane. A row that there is not is row 0: it reaches only
+// results that are not stored.
+template <class T, int kW>
+__global__ __launch_bounds__(64 * kW) void few_rows_kernel(const T *in, const T *w, Groups g, int O, int R, T *out, int cols,
+                                                           bool by_place) {
+    constexpr int kE = 16 / sizeof(T), kStep = 4 * kE, kU = 8;
+    __shared__ f32x4 parts[kW][64];
+    const int t = tile_of(blockIdx.x, gridDim.x), o0 = t % cols * 16;
+    const Piece pc = by_place ? piece_from<16>(g, t / cols) : piece_at<16>(g, t / cols);
+    if (pc.count <= 0) return;
+    const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, d = l & 15, q = l >> 4;
+    const int row = d < pc.count ? row_of(g, pc.first + d) : -1;
+    f32x4 acc = {0, 0, 0, 0};
+    if (pc.e < g.E) {
+        const int steps = (R + kStep - 1) / kStep, per = (steps + kW - 1) / kW, end = min(per * (wave + 1), steps);
+        const T *wp = w + ((int64_t)pc.e * O + min(o0 + d, O - 1)) * R + q * kE, *xp = in + (int64_t)max(row, 0) * R + q * kE;
+        const int last = R - q * kE;
+        int s = per * wave;
+        for (; s + kU <= end && (s + kU) * kStep <= R; s += kU) {
+            u32x4 a[kU], b[kU];
+#pragma unroll
+            for (int u = 0; u < kU; u++) a[u] = load16(wp + (s + u) * kStep);
+#pragma unroll
+            for (int u = 0; u < kU; u++) b[u] = load16(xp + (s + u) * kStep);
+#pragma unroll
+            for (int u = 0; u < kU; u++) acc = Mma<T>::run(a[u], b[u], acc);
+        }
+        for (; s < end && R >= kE; s += 4) {
+            u32x4 a[4], b[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) a[u] = load16_end(wp + (s + u) * kStep, last - (s + u) * kStep);
+#pragma unroll
+            for (int u = 0; u < 4; u++) b[u] = load16_end(xp + (s + u) * kStep, last - (s + u) * kStep);
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (s + u >= end) a[u] = b[u] = u32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int u = 0; u < 4; u++) acc = Mma<T>::run(a[u], b[u], acc);
+        }
+        for (; s < end; s++) {
+            const int n = last - s * kStep;
+            const u32x4 a = load16(wp + s * kStep, n), b = load16(xp + s * kStep, row >= 0 ? n : 0);
+            acc = Mma<T>::run(a, b, acc);
+        }
+    }
+    if constexpr (kW > 1) {
+        parts[wave][l] = acc;
+        __syncthreads();
+        if (wave) return;
+#pragma unroll
+        for (int i = 1; i < kW; i++) acc += parts[i][l];
+    }
+    const int o = o0 + 4 * q;
+    if (row >= 0 && o < O) store_run<T, 4>(out + (int64_t)row * O + o, (const float *)&acc, O - o);
+}
+
+// kF consecutive values, p being n before its row's end; those past it come as zero. Rows of kF or more (inner: n >= kF).
+template <class T, int kF> __device__ __forceinline__ void load_few(const T *p, int n, bool inner, float *f) {
+    T t[kF];
+    if (inner) {
+        __builtin_memcpy(t, p, sizeof(t));
+#pragma unroll
+        for (int j = 0; j < kF; j++) f[j] = to_f32(t[j]);
+    } else {
+        __builtin_memcpy(t, p + min(n - kF, 0), sizeof(t));
+        const int by = max(kF - n, 0);
+#pragma unroll
+        for (int j = 0; j < kF; j++) {
+            f[j] = 0.0f;
+#pragma unroll
+            for (int i = j; i < kF; i++) f[j] = i - j == by ? to_f32(t[i]) : f[j];
+        }
+    }
+}
+
+// dw of small matrices, in f32 products whatever the type (they are few; 16-bit values are exact in f32): a workgroup of kW
+// waves takes 16 FN x 16 FK of one expert's (n, k), a wave every kW th 16 rows, straight from memory: lane (q, d) holds values
+// FN d .. of dy and FK d .. of x at the rows 4 j + q, so instruction j multiplies row 4 j + q's, and fragment f's d th n is
+// FN d + f. The waves' sums are joined in their order.
+//
+// An expert of kLong rows or more takes a multiple of a tile's time, so the grid's first `early` workgroups are for such
+// experts: one holds a place that kLong divides, and the first of those names it. With half of 65536 rows at 16 of 1024
+// experts (256 x 64 f32) that is 60 us for 104.
+constexpr int kLong = 256;
+template <class T, int FN, int FK, int kW>
+__global__ __launch_bounds__(64 * kW) void grad_w_small_kernel(const T *dy, const T *x, Groups g, int N, int K, T *dw, int tn, int tk,
+                                                               int early) {
+    typedef float Run __attribute__((ext_vector_type(FK)));
+    __shared__ Run parts[kW][4][64];
+    constexpr int kHop = 16 * kW;
+    const int l = threadIdx.x & 63, d = l & 15, q = l >> 4, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const bool is_early = (int)blockIdx.x < early;
+    const int t = is_early ? tile_of(blockIdx.x, early) : tile_of(blockIdx.x - early, gridDim.x - early);
+    const int n0 = t / tk % tn * 16 * FN, k0 = t % tk * 16 * FK;
+    int e = t / (tn * tk);
+    if (is_early) {
+        const int place = e * kLong;
+        const Piece pc = piece_from<1>(g, place);
+        if (pc.count <= 0 || pc.e >= g.E || (place > 0 && first_of(g, pc.e) <= place - kLong)) return;
+        e = pc.e;
+    }
+    const int first = first_of(g, e), count = end_of(g, e) - first;
+    if (is_early != (count >= kLong)) return;
+    T *out = dw + (int64_t)e * N * K;
+    auto put = [&](int n, const float *v) {
+        const int k = k0 + FK * d;
+        if (n < N && k < K) store_run<T, FK>(out + (int64_t)n * K + k, v, K - k);
+    };
+    if (count <= 0) {
+        const float zero[FK] = {};
+        for (int n = n0 + (threadIdx.x >> 4); n < n0 + 16 * FN; n += 4 * kW) put(n, zero);
+        return;
+    }
+    if (count <= 16 * wave && count <= 16) return;
+    const int nn = N - n0 - FN * d, nk = K - k0 - FK * d;
+    const T *dyp = dy + n0 + FN * d, *xp = x + k0 + FK * d;
+    const bool in_n = n0 + 16 * FN <= N, in_k = k0 + 16 * FK <= K;
+    f32x4 acc[FN][FK];
+#pragma unroll
+    for (int i = 0; i < FN; i++)
+#pragma unroll
+        for (int o = 0; o < FK; o++) acc[i][o] = f32x4{0, 0, 0, 0};
+    // a block of rows is in flight while the one before it is multiplied, with the rows' numbers of the one after it
+    int row[4];
+    auto rows = [&](int b) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) row[j] = b + 4 * j + q < count ? row_of(g, first + b + 4 * j + q) : -1;
+    };
+    float a[4][FN], b[4][FK];
+    bool none[4];
+    auto load = [&] {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            none[j] = row[j] < 0;
+            load_few<T, FN>(dyp + (int64_t)max(row[j], 0) * N, nn, in_n, a[j]);
+            load_few<T, FK>(xp + (int64_t)max(row[j], 0) * K, nk, in_k, b[j]);
+        }
+    };
+    rows(16 * wave);
+    load();
+    rows(16 * wave + kHop);
+    for (int at = 16 * wave; at < count; at += kHop) {
+        float a1[4][FN], b1[4][FK];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+#pragma unroll
+            for (int i = 0; i < FN; i++) a1[j][i] = none[j] ? 0.0f : a[j][i];
+#pragma unroll
+            for (int o = 0; o < FK; o++) b1[j][o] = none[j] ? 0.0f : b[j][o];
+        }
+        if (at + kHop < count) {
+            load();
+            rows(at + 2 * kHop);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int i = 0; i < FN; i++)
+#pragma unroll
+                for (int o = 0; o < FK; o++) acc[i][o] = __builtin_amdgcn_mfma_f32_16x16x4f32(a1[j][i], b1[j][o], acc[i][o], 0, 0, 0);
+    }
+    if (count <= 16) {
+#pragma unroll
+        for (int i = 0; i < FN; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                float v[FK];
+#pragma unroll
+                for (int o = 0; o < FK; o++) v[o] = acc[i][o][j];
+                put(n0 + FN * (4 * q + j) + i, v);
+            }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < FN; i++) {
+        if (i) __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            Run v;
+#pragma unroll
+            for (int o = 0; o < FK; o++) v[o] = acc[i][o][j];
+            parts[wave][j][l] = v;
+        }
+        __syncthreads();
+        if (wave < 4) {
+            Run v = parts[0][wave][l];
+#pragma unroll
+            for (int p = 1; p < kW; p++) v += parts[p][wave][l];
+            put(n0 + FN * (4 * q + wave) + i, (const float *)&v);
+        }
+    }
 }
 
 // The same where rows are 16-byte aligned and the operands (of w one expert's matrix) small enough for 32-bit offsets
@@ -228,13 +440,58 @@ hipError_t go_rows(const void *in, const void *w, const Groups &g, int O, int R,
             return hipGetLastError();
         }
     }
-    constexpr int FI = 4, FO = 4, WI = 2, WO = 2, kBufs = 1, kI = 16 * FI * WI, kO = 16 * FO * WO;
-    const int cols = (O + kO - 1) / kO;
-    const int64_t tiles = ((int64_t)g.M / kI + g.E + 2) * cols;
-    if (tiles > INT32_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((rows_kernel<T, FI, FO, WI, WO, kBufs, TR>), dim3((unsigned)tiles), dim3(64 * WI * WO), 0, st,
-                       (const T *)in, (const T *)w, g, O, R, (T *)out, cols, 16);
-    return hipGetLastError();
+    auto tiles = [&](auto fi, auto wi, auto wo) {
+        constexpr int FI = decltype(fi)::value, WI = decltype(wi)::value, WO = decltype(wo)::value, kI = 16 * FI * WI, kO = 64 * WO;
+        const int cols = (O + kO - 1) / kO;
+        const int64_t slots = (int64_t)g.M / kI + g.E + 2, rows = std::min<int64_t>(slots, g.M);
+        if (rows * cols > INT32_MAX) return hipErrorInvalidValue;
+        hipLaunchKernelGGL((rows_kernel<T, FI, 4, WI, WO, 1, TR>), dim3((unsigned)(rows * cols)), dim3(64 * WI * WO), 0, st,
+                           (const T *)in, (const T *)w, g, O, R, (T *)out, cols, 16, slots > g.M);
+        return hipGetLastError();
+    };
+    constexpr std::integral_constant<int, 1> one{};
+    constexpr std::integral_constant<int, 2> two{};
+    constexpr std::integral_constant<int, 4> four{};
+    // Measured with 64 experts of 1528 x 2040 and M / 64 rows each, bf16 / f32, us:
+    //   rows of each                           1          7         31         62        125        250
+    //   y   few_rows                      75/148    111/212    216/461    920/812
+    //       16 x 64, 1 wave               75/144    118/224    177/366    288/600    400/893
+    //       32 x 64, 1                    75/179    101/207    146/319    224/526    297/805
+    //       64 x 64, 2                    77/315     96/329    143/452    174/437    227/812    434/1341
+    //       64 x 128, 4                   86/301     99/312    133/385    158/452    183/683    331/1147
+    //       128 x 128, 4                 101/559    115/564    136/719    186/740    167/750    290/1276
+    //   dx  16 x 64, 1                   121/297    156/331    213/454    316/615    407/919
+    //       64 x 64, 2                   115/372    131/432    146/510    201/541    246/848    404/1342
+    //       64 x 128, 4                   94/354    138/437    149/487    169/544    212/842    343/1298
+    // f32's matrix instructions are 1/16 of bf16's rate, so rows that a tile lacks cost it more. Matrices of 64 values along a
+    // side keep to the 16-row tiles: with loads as uneven as a router's most experts have fewer rows than the mean.
+    const int64_t mean = g.M / g.E;
+    const bool f32 = sizeof(T) == 4, small = O <= 64 || R <= 64;
+    if constexpr (!TR) {
+        if (mean < 4 || g.M < 64 || (small && mean < 16)) {
+            const int cols = (O + 15) / 16;
+            const int64_t slots = (int64_t)g.M / 16 + g.E + 2, rows = std::min<int64_t>(slots, g.M);
+            if (rows * cols > INT32_MAX) return hipErrorInvalidValue;
+            if (in_row <= 1024)
+                hipLaunchKernelGGL((few_rows_kernel<T, 1>), dim3((unsigned)(rows * cols)), dim3(64), 0, st, (const T *)in,
+                                   (const T *)w, g, O, R, (T *)out, cols, slots > g.M);
+            else
+                hipLaunchKernelGGL((few_rows_kernel<T, 4>), dim3((unsigned)(rows * cols)), dim3(256), 0, st, (const T *)in,
+                                   (const T *)w, g, O, R, (T *)out, cols, slots > g.M);
+            return hipGetLastError();
+        }
+        if constexpr (sizeof(T) == 4) {
+            if (small && mean <= 128) return tiles(one, one, one);
+            if (mean < 48) return tiles(two, one, one);
+        } else if (mean >= 96 && O > 64) {
+            return tiles(four, two, two);
+        }
+        return mean < 48 || O <= 64 ? tiles(two, two, one) : tiles(two, two, two);
+    } else {
+        if (small && mean <= (f32 ? 128 : 16)) return tiles(one, one, one);
+        if (f32 && mean < 48) return tiles(one, one, one);
+        return O <= 64 ? tiles(two, two, one) : tiles(two, two, two);
+    }
 }
 template <class T>
 hipError_t go_grad_w(const void *dy, const void *x, const Groups &g, int N, int K, void *dw, hipStream_t st) {
@@ -248,13 +505,31 @@ hipError_t go_grad_w(const void *dy, const void *x, const Groups &g, int N, int 
             return hipGetLastError();
         }
     }
-    constexpr int FI = 4, FO = 4, WI = 2, WO = 2, kBufs = 1, kI = 16 * FI * WI, kO = 16 * FO * WO;
-    const int tn = (N + kI - 1) / kI, tk = (K + kO - 1) / kO;
-    const int64_t tiles = (int64_t)g.E * tn * tk;
-    if (tiles > INT32_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((grad_w_kernel<T, FI, FO, WI, WO, kBufs>), dim3((unsigned)tiles), dim3(64 * WI * WO), 0, st,
-                       (const T *)dy, (const T *)x, g, N, K, (T *)dw, tn, tk);
-    return hipGetLastError();
+    // us of 64 experts of 1528 x 2040 as above: f32 1 row of each 210 (64 x 128 tiles 262), 7 rows 247 (276), 31 rows 419 (315)
+    if (N >= 4 && K >= 4 && (N <= 64 || (sizeof(T) == 4 && g.M < 16 * (int64_t)g.E))) {
+        auto small = [&](auto fn) {
+            constexpr int FN = decltype(fn)::value;
+            const int tn = (N + 16 * FN - 1) / (16 * FN), tk = (K + 63) / 64;
+            const int64_t early = ((int64_t)g.M / kLong + 1) * tn * tk, tiles = (int64_t)g.E * tn * tk + early;
+            if (tiles > INT32_MAX) return hipErrorInvalidValue;
+            hipLaunchKernelGGL((grad_w_small_kernel<T, FN, 4, 4>), dim3((unsigned)tiles), dim3(256), 0, st, (const T *)dy, (const T *)x, g,
+                               N, K, (T *)dw, tn, tk, (int)early);
+            return hipGetLastError();
+        };
+        return N <= 16 ? small(std::integral_constant<int, 1>()) : small(std::integral_constant<int, 2>());
+    }
+    auto tiles = [&](auto fi) {
+        constexpr int FI = decltype(fi)::value, kI = 32 * FI;
+        const int tn = (N + kI - 1) / kI, tk = (K + 127) / 128;
+        const int64_t tiles = (int64_t)g.E * tn * tk;
+        if (tiles > INT32_MAX) return hipErrorInvalidValue;
+        hipLaunchKernelGGL((grad_w_kernel<T, FI, 4, 2, 2, 1>), dim3((unsigned)tiles), dim3(256), 0, st, (const T *)dy, (const T *)x, g, N,
+                           K, (T *)dw, tn, tk);
+        return hipGetLastError();
+    };
+    // 128 x 128 where there are enough (bf16, 250 rows of each: 381 us for 411), else 64 x 128 (4 experts of 1000 x 1000: 74 for 81)
+    if (sizeof(T) == 2 && (int64_t)g.E * ((N + 127) / 128) * ((K + 127) / 128) >= 512) return tiles(std::integral_constant<int, 4>());
+    return tiles(std::integral_constant<int, 2>());
 }
 
 }  // namespace

@@ -5,8 +5,8 @@
 // dy and x in the weights' gradient, an expert's matrix in the rows' gradient). Both are staged through registers into LDS,
 // 16 bytes a thread, a step of 128 bytes of r ("along") or as many r's ("across") at a time; the loads of a step are issued
 // before the products of the step before it. Rows may begin at any address of their element's alignment (a 16-byte load of
-// global memory needs no more here), and what a row's end or the reduction's end leaves of 16 bytes is loaded element by
-// element, so nothing outside the operands is read.
+// global memory needs no more here), and where fewer than 16 bytes are left of a row its last 16 are loaded and moved down,
+// so nothing outside the operands is read.
 //
 // A fragment of the 16-row matrix instructions is 16 bytes a lane: lane l holds row l % 16 and the l / 16 th quarter of 64
 // bytes of r. bf16 and f16 take 32 r's in one instruction, int8 64, f32 16 in four (instruction j takes the j th element of
@@ -87,8 +87,13 @@ template <class T, int kB, int kThreads, int kF, bool kRow> struct Along {
             for (int i = 0; i < kN; i++) v[i] = load16(p[i] + r0);
         } else {
             const int n = R - r0 - (threadIdx.x & 7) * kE;
+            if (R >= kE) {
 #pragma unroll
-            for (int i = 0; i < kN; i++) v[i] = load16(p[i] + r0, n);
+                for (int i = 0; i < kN; i++) v[i] = load16_end(p[i] + r0, n);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kN; i++) v[i] = load16(p[i] + r0, n);
+            }
         }
     }
     __device__ __forceinline__ void store(char *lds) const {
@@ -111,36 +116,50 @@ template <class T, int kB, int kThreads> struct Across {
     static constexpr int kE = 16 / sizeof(T), kStep = 128 / sizeof(T), kBytes = kB * 128, kWide = kB * sizeof(T);
     static constexpr int kPer = kB / kE;             // 16-byte pieces of one r
     static constexpr int kN = kB * 8 / kThreads, kHop = kThreads / kPer;
-    static_assert(kN * kThreads == kB * 8 && kHop * kPer == kThreads && kWide >= 256, "");
+    static_assert(kN * kThreads == kB * 8 && kHop * kPer == kThreads && kWide >= (sizeof(T) == 2 ? 128 : 256), "");
     const T *p;
     int n;              // how many elements of the thread's pieces exist
+    bool inner, tiny;   // all the tile's elements exist; rows shorter than 16 bytes
     u32x4 v[kN];
-    // base: the address of the tile's first element at r = 0; left: elements from there to the row's end
-    __device__ __forceinline__ void begin(const T *base, int left) {
-        const int c = (int)threadIdx.x % kPer * kE;
+    bool none[kN];
+    // rows from base on, the tile's elements from `first` on of `width`
+    __device__ __forceinline__ void begin(const T *base, int first, int width) {
+        const int c = first + (int)threadIdx.x % kPer * kE;
         p = base + c;
-        n = left - c;
+        n = width - c;
+        inner = first + kB <= width;
+        tiny = width < kE;
     }
     // the r in the step of the thread's i th piece
     static __device__ __forceinline__ int r_of(int i) { return (int)threadIdx.x / kPer + i * kHop; }
     // offset(i): how far from r = 0 the i th piece's r lies, in elements, or -1: it counts as zero
     template <class F> __device__ __forceinline__ void load(F offset) {
+        int64_t o[kN];
 #pragma unroll
-        for (int i = 0; i < kN; i++) {
-            const int64_t o = offset(i);
-            v[i] = load16(p + (o < 0 ? 0 : o), o < 0 ? 0 : n);
+        for (int i = 0; i < kN; i++) o[i] = offset(i);
+        if (inner) {
+#pragma unroll
+            for (int i = 0; i < kN; i++) v[i] = load16(p + max(o[i], (int64_t)0));
+        } else if (!tiny) {
+#pragma unroll
+            for (int i = 0; i < kN; i++) v[i] = load16_end(p + max(o[i], (int64_t)0), n);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kN; i++) v[i] = load16(p + max(o[i], (int64_t)0), n);
         }
+#pragma unroll
+        for (int i = 0; i < kN; i++) none[i] = o[i] < 0;
     }
     // exchanges pieces of 32 bytes (16-bit types) or 64 (f32): the r's that one read takes together differ
     static __device__ __forceinline__ int turn(int r) {
-        if constexpr (sizeof(T) == 2) return ((r & 3) | (r >> 3 & 1) << 2) << 5;
+        if constexpr (sizeof(T) == 2) return ((r & 3) | (kWide >= 256 ? (r >> 3 & 1) << 2 : 0)) << 5;
         else return (r >> 2 & 3) << 6;
     }
     __device__ __forceinline__ void store(char *lds) const {
 #pragma unroll
         for (int i = 0; i < kN; i++) {
             const int r = r_of(i);
-            *(u32x4 *)(lds + r * kWide + (((int)threadIdx.x % kPer * 16) ^ turn(r))) = v[i];
+            *(u32x4 *)(lds + r * kWide + (((int)threadIdx.x % kPer * 16) ^ turn(r))) = none[i] ? u32x4{0, 0, 0, 0} : v[i];
         }
     }
     static __device__ __forceinline__ u32x4 frag(const char *lds, int base, int f, int half) {

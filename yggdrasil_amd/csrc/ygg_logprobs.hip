@@ -159,7 +159,7 @@ template <class T, int kG, int kU> __global__ __launch_bounds__(256) void narrow
 #pragma unroll
         for (int u = 0; u < kU; u++) {
             const int first = (u * kG + l) * kC, n = a.V - first;
-            unpack(load16(x + min(first, a.V - 1), n), v + u * kC, T{});
+            unpack(a.V >= kC ? load16_end(x + first, n) : load16(x + min(first, a.V - 1), n), v + u * kC, T{});
 #pragma unroll
             for (int j = 0; j < kC; j++) v[u * kC + j] = j < n ? v[u * kC + j] : -INFINITY;
         }
@@ -291,7 +291,7 @@ template <class T, int kU, class F> __device__ __forceinline__ void for_pieces(c
 #pragma unroll
         for (int u = 0; u < kU; u++) {
             const int first = c + (u * 256 + l) * kC, n = c1 - first;
-            unpack(load16(x + min(first, c1 - 1), n), v + u * kC, T{});
+            unpack(load16_end(x + first, n), v + u * kC, T{});      // c1 is past a whole piece of the row
 #pragma unroll
             for (int j = 0; j < kC; j++) v[u * kC + j] = j < n ? v[u * kC + j] : -INFINITY;
         }
@@ -508,10 +508,15 @@ template <class T, int kU> __global__ __launch_bounds__(256) void grad_kernel(Lo
             if (a.top_ids[row * a.top + k] >= 0) all += a.g_top[row * a.top + k];
     const bool none = st.x == -INFINITY;
     u32x4 p[kU];
+    if (blocks > 1 && (int)(blockIdx.x % blocks + 1) * kU * 256 * kC <= a.V) {
 #pragma unroll
-    for (int u = 0; u < kU; u++) {
-        const int c = c0 + (u * kC << shift);
-        p[u] = load16(x + min(c, a.V - 1), a.V - c);
+        for (int u = 0; u < kU; u++) p[u] = load16(x + c0 + (u * kC << shift));
+    } else {
+#pragma unroll
+        for (int u = 0; u < kU; u++) {
+            const int c = c0 + (u * kC << shift);
+            p[u] = a.V >= kC ? load16_end(x + c, a.V - c) : load16(x + min(c, a.V - 1), a.V - c);
+        }
     }
 #pragma unroll
     for (int u = 0; u < kU; u++) {

@@ -50,6 +50,17 @@ template <class T> __device__ __forceinline__ u32x4 load16(const T *p, int n) {
     return v;
 }
 
+// The same without a branch, so that loads that follow are not held up, for rows of 16 bytes or more: p is n elements (any
+// number, also none or less) before its row's end. The row's last 16 bytes are loaded where fewer are left, and moved down.
+template <class T> __device__ __forceinline__ u32x4 load16_end(const T *p, int n) {
+    constexpr int kE = 16 / sizeof(T);
+    const u32x4 v = load16(p + min(n - kE, 0));
+    const int bits = max(kE - n, 0) * 8 * (int)sizeof(T);
+    const uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
+    uint64_t a = bits < 64 ? lo >> (bits & 63) | (hi << 1) << (~bits & 63) : hi >> (bits & 63), b = bits < 64 ? hi >> (bits & 63) : 0;
+    if (bits >= 128) a = 0;
+    return u32x4{(uint32_t)a, (uint32_t)(a >> 32), (uint32_t)b, (uint32_t)(b >> 32)};
+}
 // the values of 16 bytes
 __device__ __forceinline__ void unpack(u32x4 v, float *f, float) {
 #pragma unroll
