@@ -125,15 +125,25 @@ __global__ __launch_bounds__(64 * WI * WO) void grad_w_kernel(const T *dy, const
     a.begin(dy, n0, N);
     b.begin(x, k0, K);
     const int steps = (count + A::kStep - 1) / A::kStep;
+    // the rows of the step to be loaded next: their numbers come a step ahead
+    int ra[A::kN], rb[B::kN];
+    auto fetch = [&](int s) {
+#pragma unroll
+        for (int i = 0; i < A::kN; i++) {
+            const int r = s * A::kStep + A::r_of(i);
+            ra[i] = r < count ? row_of(g, first + r) : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < B::kN; i++) {
+            const int r = s * B::kStep + B::r_of(i);
+            rb[i] = r < count ? row_of(g, first + r) : -1;
+        }
+    };
+    fetch(0);
     tile.run(a, b, lds, steps, [&](int s) {
-        a.load([&](int i) {
-            const int r = s * A::kStep + A::r_of(i), row = r < count ? row_of(g, first + r) : -1;
-            return row < 0 ? -1 : (int64_t)row * N;
-        });
-        b.load([&](int i) {
-            const int r = s * B::kStep + B::r_of(i), row = r < count ? row_of(g, first + r) : -1;
-            return row < 0 ? -1 : (int64_t)row * K;
-        });
+        a.load([&](int i) { return ra[i] < 0 ? -1 : (int64_t)ra[i] * N; });
+        b.load([&](int i) { return rb[i] < 0 ? -1 : (int64_t)rb[i] * K; });
+        fetch(s + 1);
     });
     T *out = dw + (int64_t)e * N * K;
     tile.template each<false>([&](int i, int o, const typename Tl::Acc *v, auto n) {
@@ -218,100 +228,86 @@ template <class T, int kF> __device__ __forceinline__ void load_few(const T *p, 
     }
 }
 
-// dw of small matrices, in f32 products whatever the type (they are few; 16-bit values are exact in f32): a workgroup of kW
-// waves takes 16 FN x 16 FK of one expert's (n, k), a wave every kW th 16 rows, straight from memory: lane (q, d) holds values
-// FN d .. of dy and FK d .. of x at the rows 4 j + q, so instruction j multiplies row 4 j + q's, and fragment f's d th n is
-// FN d + f. The waves' sums are joined in their order.
-//
-// An expert of kLong rows or more takes a multiple of a tile's time, so the grid's first `early` workgroups are for such
-// experts: one holds a place that kLong divides, and the first of those names it. With half of 65536 rows at 16 of 1024
-// experts (256 x 64 f32) that is 60 us for 104.
-constexpr int kLong = 256;
-template <class T, int FN, int FK, int kW>
-__global__ __launch_bounds__(64 * kW) void grad_w_small_kernel(const T *dy, const T *x, Groups g, int N, int K, T *dw, int tn, int tk,
-                                                               int early) {
-    typedef float Run __attribute__((ext_vector_type(FK)));
-    __shared__ Run parts[kW][4][64];
-    constexpr int kHop = 16 * kW;
+// dw of small matrices, in f32 products whatever the type (they are few; 16-bit values are exact in f32): a workgroup of 4
+// waves takes 16 FN x 64 of one expert's (n, k), a wave every fourth 16 rows, straight from memory: lane (q, d) holds values
+// FN d .. of dy and 4 d .. of x at the rows 4 j + q, so instruction j multiplies row 4 j + q's, and fragment f's d th n is
+// FN d + f. kDepth blocks of 16 rows are in flight a wave. The waves' sums are joined in their order.
+template <class T, int FN, int kDepth>
+__device__ __forceinline__ void grad_w_small(f32x4 (*parts)[4][64], const T *dy, const T *x, const Groups &g, int N, int K, T *out,
+                                             int first, int count, int n0, int k0) {
     const int l = threadIdx.x & 63, d = l & 15, q = l >> 4, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const bool is_early = (int)blockIdx.x < early;
-    const int t = is_early ? tile_of(blockIdx.x, early) : tile_of(blockIdx.x - early, gridDim.x - early);
-    const int n0 = t / tk % tn * 16 * FN, k0 = t % tk * 16 * FK;
-    int e = t / (tn * tk);
-    if (is_early) {
-        const int place = e * kLong;
-        const Piece pc = piece_from<1>(g, place);
-        if (pc.count <= 0 || pc.e >= g.E || (place > 0 && first_of(g, pc.e) <= place - kLong)) return;
-        e = pc.e;
-    }
-    const int first = first_of(g, e), count = end_of(g, e) - first;
-    if (is_early != (count >= kLong)) return;
-    T *out = dw + (int64_t)e * N * K;
     auto put = [&](int n, const float *v) {
-        const int k = k0 + FK * d;
-        if (n < N && k < K) store_run<T, FK>(out + (int64_t)n * K + k, v, K - k);
+        const int k = k0 + 4 * d;
+        if (n < N && k < K) store_run<T, 4>(out + (int64_t)n * K + k, v, K - k);
     };
     if (count <= 0) {
-        const float zero[FK] = {};
-        for (int n = n0 + (threadIdx.x >> 4); n < n0 + 16 * FN; n += 4 * kW) put(n, zero);
+        const float zero[4] = {};
+        for (int n = n0 + (threadIdx.x >> 4); n < n0 + 16 * FN; n += 16) put(n, zero);
         return;
     }
-    if (count <= 16 * wave && count <= 16) return;
-    const int nn = N - n0 - FN * d, nk = K - k0 - FK * d;
-    const T *dyp = dy + n0 + FN * d, *xp = x + k0 + FK * d;
-    const bool in_n = n0 + 16 * FN <= N, in_k = k0 + 16 * FK <= K;
-    f32x4 acc[FN][FK];
+    if (count <= 16 && wave) return;
+    const int nn = N - n0 - FN * d, nk = K - k0 - 4 * d;
+    const T *dyp = dy + n0 + FN * d, *xp = x + k0 + 4 * d;
+    const bool in_n = n0 + 16 * FN <= N, in_k = k0 + 64 <= K;
+    f32x4 acc[FN][4];
 #pragma unroll
     for (int i = 0; i < FN; i++)
 #pragma unroll
-        for (int o = 0; o < FK; o++) acc[i][o] = f32x4{0, 0, 0, 0};
-    // a block of rows is in flight while the one before it is multiplied, with the rows' numbers of the one after it
-    int row[4];
-    auto rows = [&](int b) {
+        for (int o = 0; o < 4; o++) acc[i][o] = f32x4{0, 0, 0, 0};
+    // blocks in flight, and the rows' numbers of those to be loaded in their place
+    struct {
+        int row[4];
+        bool none[4];
+        float a[4][FN], b[4][4];
+    } in[kDepth];
+    auto rows = [&](int h, int at) {
 #pragma unroll
-        for (int j = 0; j < 4; j++) row[j] = b + 4 * j + q < count ? row_of(g, first + b + 4 * j + q) : -1;
+        for (int j = 0; j < 4; j++) in[h].row[j] = at + 4 * j + q < count ? row_of(g, first + at + 4 * j + q) : -1;
     };
-    float a[4][FN], b[4][FK];
-    bool none[4];
-    auto load = [&] {
+    auto load = [&](int h) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            none[j] = row[j] < 0;
-            load_few<T, FN>(dyp + (int64_t)max(row[j], 0) * N, nn, in_n, a[j]);
-            load_few<T, FK>(xp + (int64_t)max(row[j], 0) * K, nk, in_k, b[j]);
+            const int row = in[h].row[j];
+            in[h].none[j] = row < 0;
+            load_few<T, FN>(dyp + (int64_t)max(row, 0) * N, nn, in_n, in[h].a[j]);
+            load_few<T, 4>(xp + (int64_t)max(row, 0) * K, nk, in_k, in[h].b[j]);
         }
     };
-    rows(16 * wave);
-    load();
-    rows(16 * wave + kHop);
-    for (int at = 16 * wave; at < count; at += kHop) {
-        float a1[4][FN], b1[4][FK];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+    for (int h = 0; h < kDepth; h++) rows(h, 16 * wave + 64 * h);
 #pragma unroll
-            for (int i = 0; i < FN; i++) a1[j][i] = none[j] ? 0.0f : a[j][i];
+    for (int h = 0; h < kDepth; h++) load(h);
 #pragma unroll
-            for (int o = 0; o < FK; o++) b1[j][o] = none[j] ? 0.0f : b[j][o];
+    for (int h = 0; h < kDepth; h++) rows(h, 16 * wave + 64 * (h + kDepth));
+    for (int at = 16 * wave; at < count; at += 64 * kDepth) {
+#pragma unroll
+        for (int h = 0; h < kDepth; h++) {
+            float a[4][FN], b[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+#pragma unroll
+                for (int i = 0; i < FN; i++) a[j][i] = in[h].none[j] ? 0.0f : in[h].a[j][i];
+#pragma unroll
+                for (int o = 0; o < 4; o++) b[j][o] = in[h].none[j] ? 0.0f : in[h].b[j][o];
+            }
+            if (kDepth > 1 || at + 64 < count) {
+                load(h);
+                rows(h, at + 64 * (h + 2 * kDepth));
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int i = 0; i < FN; i++)
+#pragma unroll
+                    for (int o = 0; o < 4; o++) acc[i][o] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j][i], b[j][o], acc[i][o], 0, 0, 0);
         }
-        if (at + kHop < count) {
-            load();
-            rows(at + 2 * kHop);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-#pragma unroll
-            for (int i = 0; i < FN; i++)
-#pragma unroll
-                for (int o = 0; o < FK; o++) acc[i][o] = __builtin_amdgcn_mfma_f32_16x16x4f32(a1[j][i], b1[j][o], acc[i][o], 0, 0, 0);
     }
     if (count <= 16) {
 #pragma unroll
         for (int i = 0; i < FN; i++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                float v[FK];
-#pragma unroll
-                for (int o = 0; o < FK; o++) v[o] = acc[i][o][j];
+                const float v[4] = {acc[i][0][j], acc[i][1][j], acc[i][2][j], acc[i][3][j]};
                 put(n0 + FN * (4 * q + j) + i, v);
             }
         return;
@@ -320,19 +316,32 @@ __global__ __launch_bounds__(64 * kW) void grad_w_small_kernel(const T *dy, cons
     for (int i = 0; i < FN; i++) {
         if (i) __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            Run v;
-#pragma unroll
-            for (int o = 0; o < FK; o++) v[o] = acc[i][o][j];
-            parts[wave][j][l] = v;
-        }
+        for (int j = 0; j < 4; j++) parts[wave][j][l] = f32x4{acc[i][0][j], acc[i][1][j], acc[i][2][j], acc[i][3][j]};
         __syncthreads();
-        if (wave < 4) {
-            Run v = parts[0][wave][l];
-#pragma unroll
-            for (int p = 1; p < kW; p++) v += parts[p][wave][l];
-            put(n0 + FN * (4 * q + wave) + i, (const float *)&v);
-        }
+        const f32x4 v = ((parts[0][wave][l] + parts[1][wave][l]) + parts[2][wave][l]) + parts[3][wave][l];
+        put(n0 + FN * (4 * q + wave) + i, (const float *)&v);
+    }
+}
+// An expert of kLong rows or more takes a multiple of a tile's time, most of it memory's latency, so the grid's first `early`
+// workgroups are for such experts (one holds a place that kLong divides, and the first of those names it), in tiles of 16 x 64
+// with two blocks in flight: with half of 65536 rows at 16 of 1024 experts (256 x 64 f32) 75 us for 104 (even loads 47 for 42).
+constexpr int kLong = 256;
+template <class T, int FN>
+__global__ __launch_bounds__(256) void grad_w_small_kernel(const T *dy, const T *x, Groups g, int N, int K, T *dw, int tk, int early) {
+    __shared__ f32x4 parts[4][4][64];
+    const int b = blockIdx.x;
+    if (b < early) {
+        const int tn = (N + 15) / 16, t = tile_of(b, early), place = t / (tn * tk) * kLong;
+        const Piece pc = piece_from<1>(g, place);
+        if (pc.count <= 0 || pc.e >= g.E) return;
+        const int first = first_of(g, pc.e), count = end_of(g, pc.e) - first;
+        if (count < kLong || (place > 0 && first <= place - kLong)) return;
+        grad_w_small<T, 1, 2>(parts, dy, x, g, N, K, dw + (int64_t)pc.e * N * K, first, count, t / tk % tn * 16, t % tk * 64);
+    } else {
+        const int tn = (N + 16 * FN - 1) / (16 * FN), t = tile_of(b - early, gridDim.x - early), e = t / (tn * tk);
+        const int first = first_of(g, e), count = end_of(g, e) - first;
+        if (count >= kLong) return;
+        grad_w_small<T, FN, 1>(parts, dy, x, g, N, K, dw + (int64_t)e * N * K, first, count, t / tk % tn * 16 * FN, t % tk * 64);
     }
 }
 
@@ -354,7 +363,8 @@ __global__ __launch_bounds__(512) void rows_turn_kernel(const T *in, const T *w,
     const int bytes_r = R * (int)sizeof(T), e = min(pc.e, g.E - 1);
     const T *we = w + (int64_t)e * O * R;
     a.begin(in, (uint32_t)g.M * bytes_r, bytes_r, [&](int i) {
-        return (uint32_t)max(row_of(g, pc.first + min(i, pc.count - 1)), 0) * bytes_r;
+        const int row = i < pc.count ? row_of(g, pc.first + i) : -1;
+        return row < 0 ? kFar : (uint32_t)row * bytes_r;     // brings zeros
     });
     if constexpr (TR) b.begin(we, (uint32_t)O * bytes_r, o0 * (int)sizeof(T), (O - o0) * (int)sizeof(T));
     else b.begin(we, (uint32_t)O * bytes_r, bytes_r, [&](int o) { return (uint32_t)min(o0 + o, O - 1) * bytes_r; });
@@ -368,7 +378,7 @@ __global__ __launch_bounds__(512) void rows_turn_kernel(const T *in, const T *w,
                  });
                  else b.template load<decltype(h)::value>(s, to);
              },
-             [](int) {});
+             [](int) {}, pc.count);
     tile.template each<!TR>([&](int i, int o, const typename Tl::Acc *v, auto n) {
         if (i >= pc.count || o0 + o >= O) return;
         const int row = row_of(g, pc.first + i);
@@ -422,6 +432,10 @@ __global__ __launch_bounds__(512) void grad_w_turn_kernel(const T *dy, const T *
     });
 }
 
+constexpr std::integral_constant<int, 1> one{};
+constexpr std::integral_constant<int, 2> two{};
+constexpr std::integral_constant<int, 4> four{};
+
 bool aligned16(const void *p, int64_t row_bytes) { return (uintptr_t)p % 16 == 0 && row_bytes % 16 == 0; }
 constexpr int64_t kMostBytes = 0x78000000;   // of an operand with 32-bit offsets: kFar and a few steps stay past it
 
@@ -449,9 +463,6 @@ hipError_t go_rows(const void *in, const void *w, const Groups &g, int O, int R,
                            (const T *)in, (const T *)w, g, O, R, (T *)out, cols, 16, slots > g.M);
         return hipGetLastError();
     };
-    constexpr std::integral_constant<int, 1> one{};
-    constexpr std::integral_constant<int, 2> two{};
-    constexpr std::integral_constant<int, 4> four{};
     // Measured with 64 experts of 1528 x 2040 and M / 64 rows each, bf16 / f32, us:
     //   rows of each                           1          7         31         62        125        250
     //   y   few_rows                      75/148    111/212    216/461    920/812
@@ -469,6 +480,9 @@ hipError_t go_rows(const void *in, const void *w, const Groups &g, int O, int R,
     const bool f32 = sizeof(T) == 4, small = O <= 64 || R <= 64;
     if constexpr (!TR) {
         if (mean < 4 || g.M < 64 || (small && mean < 16)) {
+            // off 16 bytes a row's 64 take two or three lines each, which tiles' whole 128 bytes feel less: 22 rows through 27
+            // experts of 1702 x 1543 bf16 24 us for 57 (1704 x 1544: 23 and 27; 16 through 64 of 1536 x 2048: 23 and 18)
+            if (!small && !(aligned16(in, in_row) && aligned16(w, w_row))) return tiles(one, one, one);
             const int cols = (O + 15) / 16;
             const int64_t slots = (int64_t)g.M / 16 + g.E + 2, rows = std::min<int64_t>(slots, g.M);
             if (rows * cols > INT32_MAX) return hipErrorInvalidValue;
@@ -510,13 +524,14 @@ hipError_t go_grad_w(const void *dy, const void *x, const Groups &g, int N, int 
         auto small = [&](auto fn) {
             constexpr int FN = decltype(fn)::value;
             const int tn = (N + 16 * FN - 1) / (16 * FN), tk = (K + 63) / 64;
-            const int64_t early = ((int64_t)g.M / kLong + 1) * tn * tk, tiles = (int64_t)g.E * tn * tk + early;
+            const int64_t early = g.M >= kLong ? ((int64_t)g.M / kLong + 1) * ((N + 15) / 16) * tk : 0;
+            const int64_t tiles = (int64_t)g.E * tn * tk + early;
             if (tiles > INT32_MAX) return hipErrorInvalidValue;
-            hipLaunchKernelGGL((grad_w_small_kernel<T, FN, 4, 4>), dim3((unsigned)tiles), dim3(256), 0, st, (const T *)dy, (const T *)x, g,
-                               N, K, (T *)dw, tn, tk, (int)early);
+            hipLaunchKernelGGL((grad_w_small_kernel<T, FN>), dim3((unsigned)tiles), dim3(256), 0, st, (const T *)dy, (const T *)x, g, N,
+                               K, (T *)dw, tk, (int)early);
             return hipGetLastError();
         };
-        return N <= 16 ? small(std::integral_constant<int, 1>()) : small(std::integral_constant<int, 2>());
+        return N <= 16 ? small(one) : N <= 32 ? small(two) : small(four);
     }
     auto tiles = [&](auto fi) {
         constexpr int FI = decltype(fi)::value, kI = 32 * FI;
@@ -527,9 +542,9 @@ hipError_t go_grad_w(const void *dy, const void *x, const Groups &g, int N, int 
                            K, (T *)dw, tn, tk);
         return hipGetLastError();
     };
-    // 128 x 128 where there are enough (bf16, 250 rows of each: 381 us for 411), else 64 x 128 (4 experts of 1000 x 1000: 74 for 81)
-    if (sizeof(T) == 2 && (int64_t)g.E * ((N + 127) / 128) * ((K + 127) / 128) >= 512) return tiles(std::integral_constant<int, 4>());
-    return tiles(std::integral_constant<int, 2>());
+    // 128 x 128 where there are enough (250 rows of each, bf16 494 us for 538, f32 1250 for 1345), else 64 x 128 (4 experts of
+    // 1000 x 1000: 74 for 81)
+    return (int64_t)g.E * ((N + 127) / 128) * ((K + 127) / 128) >= 512 ? tiles(four) : tiles(two);
 }
 
 }  // namespace

@@ -11,8 +11,8 @@
 // A fragment of the 16-row matrix instructions is 16 bytes a lane: lane l holds row l % 16 and the l / 16 th quarter of 64
 // bytes of r. bf16 and f16 take 32 r's in one instruction, int8 64, f32 16 in four (instruction j takes the j th element of
 // every quarter). The columns' operand is the instruction's first, so that a lane's results are of one row i; the columns
-// of an "along" operand are dealt to the fragments so that a lane has 4 FO consecutive ones: column 4 FO (l / 16) + 4 f + j
-// for fragment f's j th.
+// of an "along" operand are dealt to pairs of fragments so that a lane has 8 consecutive ones: fragment f's j th is column
+// 32 (f / 2) + 8 (l / 16) + 4 (f % 2) + j.
 //
 // LDS: "along" rows of 128 bytes whose 16-byte pieces are exchanged by the row's number, so that the 16 rows that a fragment
 // reads at one r lie in different banks; "across" rows of all the tile's i or o at one r, 32-byte pieces exchanged likewise,
@@ -63,8 +63,11 @@ template <> struct Mma<int8_t> {
     }
 };
 
+// the column of fragment f's row d
+__device__ __forceinline__ int dealt(int f, int d) { return 32 * (f >> 1) + 8 * (d >> 2) + 4 * (f & 1) + (d & 3); }
+
 // An operand whose reduction index is contiguous: kB rows of 128 bytes a step. kRow: its fragments are 16 rows in order (the
-// rows' operand), else 4 kF columns are dealt to kF fragments (the columns' operand).
+// rows' operand), else its columns are dealt to the fragments (the columns' operand).
 template <class T, int kB, int kThreads, int kF, bool kRow> struct Along {
     static constexpr int kN = kB * 8 / kThreads, kE = 16 / sizeof(T), kStep = 128 / sizeof(T), kBytes = kB * 128;
     static_assert(kN * kThreads == kB * 8, "");
@@ -72,8 +75,7 @@ template <class T, int kB, int kThreads, int kF, bool kRow> struct Along {
     u32x4 v[kN];
     // the row's part of a piece's place: the 8 rows that 8 lanes read at once differ in it
     static __device__ __forceinline__ int turn(int row) {
-        if constexpr (kRow || kF == 1) return row & 7;
-        else return (row & 3) | (row / (4 * kF) & 1) << 2;
+        return kRow ? row & 7 : (row & 3) | (row >> 3 & 1) << 2;
     }
     // at(i): the address of tile row i's values
     template <class F> __device__ __forceinline__ void begin(F at) {
@@ -106,7 +108,7 @@ template <class T, int kB, int kThreads, int kF, bool kRow> struct Along {
     // fragment f of the wave's part that begins at tile row `base`; half: which 64 bytes
     static __device__ __forceinline__ u32x4 frag(const char *lds, int base, int f, int half) {
         const int l = threadIdx.x & 63, d = l & 15;
-        const int row = base + (kRow ? 16 * f + d : 4 * kF * (d >> 2) + 4 * f + (d & 3));
+        const int row = base + (kRow ? 16 * f + d : dealt(f, d));
         return *(const u32x4 *)(lds + row * 128 + (((half * 4 + (l >> 4)) ^ turn(row)) << 4));
     }
 };
@@ -188,40 +190,44 @@ template <class T, int kB, int kThreads> struct Across {
     }
 };
 
-// The 64 lanes' u[k] as four groups of 16 lanes: group g gets u[g] of group k in the place of u[k]
-template <class V> __device__ __forceinline__ void transpose_groups(V (&u)[4]) {
-    auto swap = [](V &a, V &b, bool far) {
-        const uint32_t x = __builtin_bit_cast(uint32_t, a), y = __builtin_bit_cast(uint32_t, b);
-        const u32x2 r = far ? __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(x, y, false, false))
-                            : __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(x, y, false, false));
-        a = __builtin_bit_cast(V, (uint32_t)r[0]);
-        b = __builtin_bit_cast(V, (uint32_t)r[1]);
-    };
-    swap(u[0], u[2], true);
-    swap(u[1], u[3], true);
-    swap(u[0], u[1], false);
-    swap(u[2], u[3], false);
+// Two fragments' results, a and b, of 4 columns a group of 16 lanes each: group q gets 8 of the pair's 32 in order, 8 q .. 8 q + 7
+__device__ __forceinline__ void trade(float &a, float &b) {
+    u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b),
+                                                                         false, false));
+    r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(r[0], r[1], false, false));
+    a = __builtin_bit_cast(float, (uint32_t)r[0]);
+    b = __builtin_bit_cast(float, (uint32_t)r[1]);
 }
 
-// The lane's results: of tile row row0 + 16 i + lane % 16, 16 consecutive columns. put(row, column, values, count) for each;
-// dealt: the columns' operand is Along. Otherwise a lane has 4 of each fragment's 16, and the four groups of lanes trade them:
-// stores of 8 bytes to 16 rows each took 5 us a workgroup of 256 x 256 bf16, these 2.
-template <bool kDealt, int FI, int FO, class Acc, class F>
+// The lane's results, of tile row row0 + 16 i + lane % 16: put(row, column, values, count) for runs of consecutive columns.
+// dealt: the columns' operand is Along, runs of 8. Otherwise a lane has 4 of a fragment's 16; stores of 4 16-bit values were
+// 5 us a workgroup of 256 x 256, so there the groups of lanes trade for runs of 8.
+template <class T, bool kDealt, int FI, int FO, class Acc, class F>
 __device__ __forceinline__ void each_run(Acc (&acc)[FI][FO], int row0, int col0, F put) {
-    static_assert(FO == 4, "");
-    const int l = threadIdx.x & 63;
+    static_assert(FO % 2 == 0, "");
+    const int l = threadIdx.x & 63, q = l >> 4;
 #pragma unroll
     for (int i = 0; i < FI; i++) {
-        if constexpr (!kDealt) {
+        const int row = row0 + 16 * i + (l & 15);
+        if constexpr (kDealt) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                decltype(acc[0][0][0] + 0) u[4] = {acc[i][0][j], acc[i][1][j], acc[i][2][j], acc[i][3][j]};
-                transpose_groups(u);
+            for (int o = 0; o < FO; o += 2) put(row, col0 + 16 * o + 8 * q, &acc[i][o], std::integral_constant<int, 8>());
+        } else if constexpr (sizeof(T) == 2) {
 #pragma unroll
-                for (int o = 0; o < 4; o++) acc[i][o][j] = u[o];
+            for (int o = 0; o < FO; o += 2) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    float a = acc[i][o][j], b = acc[i][o + 1][j];
+                    trade(a, b);
+                    acc[i][o][j] = a;
+                    acc[i][o + 1][j] = b;
+                }
+                put(row, col0 + 16 * o + 8 * q, &acc[i][o], std::integral_constant<int, 8>());
             }
+        } else {
+#pragma unroll
+            for (int o = 0; o < FO; o++) put(row, col0 + 16 * o + 4 * q, &acc[i][o], std::integral_constant<int, 4>());
         }
-        put(row0 + 16 * i + (l & 15), col0 + 16 * (l >> 4), &acc[i][0], std::integral_constant<int, 16>());
     }
 }
 
@@ -285,7 +291,7 @@ template <class T, int FI, int FO, int WI, int WO, int kBufs, class A, class B> 
             }
         }
     }
-    template <bool kDealt, class F> __device__ __forceinline__ void each(F put) { each_run<kDealt>(acc, row0(), col0(), put); }
+    template <bool kDealt, class F> __device__ __forceinline__ void each(F put) { each_run<T, kDealt>(acc, row0(), col0(), put); }
 };
 
 // The same product for operands whose rows are 16-byte aligned, straight from memory into LDS (no registers, no stores).
@@ -338,7 +344,7 @@ template <class T, int kF, int kW, bool kRow> struct AlongLds {
             for (int i = 0; i < kN; i++) {
                 const int row = (i * 8 + wave) * 8 + (lane >> 3);
                 const int part = row / (8 * kF), f = row / 16 % (kF / 2) + h * (kF / 2), d = row & 15;
-                at[h][i] = offset(part * 16 * kF + (kRow ? 16 * f + d : 4 * kF * (d >> 2) + 4 * f + (d & 3))) + piece;
+                at[h][i] = offset(part * 16 * kF + (kRow ? 16 * f + d : dealt(f, d))) + piece;
             }
     }
     template <int h> __device__ __forceinline__ void load(int step, uint32_t lds) const {
@@ -436,9 +442,10 @@ template <class T, int FI, int FO, int WI, int WO, class A, class B> struct Turn
     }
     // lds: the workgroup's kLds bytes, at an LDS address of its own
     // load_a(half, step, LDS address) and load_b issue a region's loads, half an integral_constant; fetch(step) comes a turn
-    // or more before a step's first loads, so that what they need from LDS is there
+    // or more before a step's first loads, so that what they need from LDS is there. count: rows that there are, of the wave's
+    // 64-row halves without any no products are taken
     template <class LA, class LB, class F>
-    __device__ __forceinline__ void run(char *lds, int steps, LA load_a, LB load_b, F fetch) {
+    __device__ __forceinline__ void run(char *lds, int steps, LA load_a, LB load_b, F fetch, int count = kI) {
         typedef __attribute__((address_space(3))) char *Shared;
         const uint32_t base = __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(Shared)lds);
         constexpr int kA0 = 0, kA1 = A::kBytes, kB0 = 2 * A::kBytes, kB1 = kB0 + B::kBytes;
@@ -458,39 +465,45 @@ template <class T, int FI, int FO, int WI, int WO, class A, class B> struct Turn
         wait_loads<kA + kStep>();
         turn_over();
         if (w >= 4) turn_over();
-        for (int t = 0; t < steps; t++) {
-            const char *now = lds + (t & 1) * kBuf;
-            const uint32_t buf = base + (t & 1) * kBuf;
-            u32x4 x[2][FI / 2], y[2][FO];
+        const bool some = wi * 16 * FI < count, more = wi * 16 * FI + 8 * FI < count;
+        auto turns = [&](auto all) {
+            for (int t = 0; t < steps; t++) {
+                const char *now = lds + (t & 1) * kBuf;
+                const uint32_t buf = base + (t & 1) * kBuf;
+                u32x4 x[2][FI / 2], y[2][FO];
 #pragma unroll
-            for (int half = 0; half < 2; half++) {
+                for (int half = 0; half < 2; half++) {
 #pragma unroll
-                for (int o = 0; o < FO; o++) y[half][o] = B::frag(now + (o < FO / 2 ? kB0 : kB1), wo, o % (FO / 2), half);
+                    for (int o = 0; o < FO; o++) y[half][o] = B::frag(now + (o < FO / 2 ? kB0 : kB1), wo, o % (FO / 2), half);
 #pragma unroll
-                for (int i = 0; i < FI / 2; i++) x[half][i] = A::frag(now + kA0, wi, i, half);
+                    for (int i = 0; i < FI / 2; i++) x[half][i] = A::frag(now + kA0, wi, i, half);
+                }
+                if (t > 0) load_a(k1, t + 1, base + (~t & 1) * kBuf + kA1);
+                fetch(t + 2);
+                wait_loads<kStep>();
+                turn_over();
+                if (decltype(all)::value || some) products<0>(x, y);
+                turn_over();
+#pragma unroll
+                for (int half = 0; half < 2; half++)
+#pragma unroll
+                    for (int i = 0; i < FI / 2; i++) x[half][i] = A::frag(now + kA1, wi, i, half);
+                load_a(k0, t + 2, buf + kA0);
+                load_b(k0, t + 2, buf + kB0);
+                load_b(k1, t + 2, buf + kB1);
+                wait_loads<kStep>();
+                turn_over();
+                if (decltype(all)::value || more) products<FI / 2>(x, y);
+                turn_over();
             }
-            if (t > 0) load_a(k1, t + 1, base + (~t & 1) * kBuf + kA1);
-            fetch(t + 2);
-            wait_loads<kStep>();
-            turn_over();
-            products<0>(x, y);
-            turn_over();
-#pragma unroll
-            for (int half = 0; half < 2; half++)
-#pragma unroll
-                for (int i = 0; i < FI / 2; i++) x[half][i] = A::frag(now + kA1, wi, i, half);
-            load_a(k0, t + 2, buf + kA0);
-            load_b(k0, t + 2, buf + kB0);
-            load_b(k1, t + 2, buf + kB1);
-            wait_loads<kStep>();
-            turn_over();
-            products<FI / 2>(x, y);
-            turn_over();
-        }
+        };
+        // a loop of its own for whole tiles: the branches cost it 3%
+        if (count >= kI) turns(std::true_type());
+        else turns(std::false_type());
         if (w < 4) turn_over();
         wait_loads<0>();    // those of the steps past the last write LDS too
     }
-    template <bool kDealt, class F> __device__ __forceinline__ void each(F put) { each_run<kDealt>(acc, row0(), col0(), put); }
+    template <bool kDealt, class F> __device__ __forceinline__ void each(F put) { each_run<T, kDealt>(acc, row0(), col0(), put); }
 };
 
 // Workgroups go round the 8 XCDs in turn, each with an L2 of its own: a run of neighbouring tiles to each

@@ -77,7 +77,7 @@ int padded(int K) { return (K + 127) / 128 * 128; }
 template <class T> bool fits_fused(int M, int K) {
     int rows = 1;
     while (rows < M) rows *= 2;
-    return rows <= 16 && M * (padded(K) + 16) <= kFusedBytes && padded(K) / (int)(16 / sizeof(T)) <= kFusedPieces * (256 / rows);
+    return rows <= 8 && M * (padded(K) + 16) <= kFusedBytes && padded(K) / (int)(16 / sizeof(T)) <= kFusedPieces * (256 / rows);
 }
 template <class T, int FI, bool kFused>
 __global__ __launch_bounds__(256) void few_int8_kernel(const T *x, const int8_t *q, const float *scale, const int8_t *w, const float *ws,
@@ -247,7 +247,7 @@ hipError_t go(const void *x, const int8_t *w, const float *ws, int M, int N, int
         return hipGetLastError();
     };
     using std::integral_constant;
-    if (K >= 16 && M <= 16 && fits_fused<T>(M, K)) return few(integral_constant<int, 1>(), std::true_type());
+    if (K >= 16 && fits_fused<T>(M, K)) return few(integral_constant<int, 1>(), std::true_type());
     hipLaunchKernelGGL(quantize_kernel<T>, dim3(M), dim3(256), 0, st, (const T *)x, K, padded(K), q, scale);
     // w is read once for 16 or 32 rows, by four waves a workgroup; more rows, or a short K, go by tiles (8192 x 4096: 16 rows
     // 10 us for 20, 32 rows 14 for 20, 64 rows 25 for 21), but where there are few of those (77 rows, 1000 x 4096: 8 for 17)
@@ -279,7 +279,10 @@ hipError_t go(const void *x, const int8_t *w, const float *ws, int M, int N, int
 
 }  // namespace
 
-int64_t int8_scratch(int M, int, int K) { return ((int64_t)M * 4 + 255) / 256 * 256 + (int64_t)M * padded(K); }
+int64_t int8_scratch(int M, int, int K) {
+    if (K >= 16 && fits_fused<float>(M, K)) return 0;    // then every type does
+    return ((int64_t)M * 4 + 255) / 256 * 256 + (int64_t)M * padded(K);
+}
 
 hipError_t launch_int8_linear(int type, const void *x, const int8_t *w, const float *w_scale, int M, int N, int K, void *y,
                               void *scratch, hipStream_t st) {

@@ -137,6 +137,42 @@ __device__ __forceinline__ uint64_t max_key(uint64_t v, int lanes) {
     return v;
 }
 
+// The top-th largest of 16 lanes' values, ties by lane (-inf: there are fewer), the same in each of them
+__device__ __forceinline__ float bound_of_16(float most, int top) {
+    const int l = threadIdx.x & 15;
+    int above = 0;
+    auto turn = [&](uint32_t u, int by) {
+        const float w = __builtin_bit_cast(float, u);
+        above += w > most || (w == most && (l - by & 15) < l);     // row_ror by `by`: lane l has lane l - by's
+    };
+    const uint32_t u = __builtin_bit_cast(uint32_t, most);
+    turn(rotated<0x121>(u), 1), turn(rotated<0x122>(u), 2), turn(rotated<0x123>(u), 3), turn(rotated<0x124>(u), 4);
+    turn(rotated<0x125>(u), 5), turn(rotated<0x126>(u), 6), turn(rotated<0x127>(u), 7), turn(rotated<0x128>(u), 8);
+    turn(rotated<0x129>(u), 9), turn(rotated<0x12a>(u), 10), turn(rotated<0x12b>(u), 11), turn(rotated<0x12c>(u), 12);
+    turn(rotated<0x12d>(u), 13), turn(rotated<0x12e>(u), 14), turn(rotated<0x12f>(u), 15);
+    return max_of<16>(above == top - 1 ? most : -INFINITY);
+}
+// of a wave's 64
+__device__ __forceinline__ float bound_of_64(float most, int top) {
+    const int l = threadIdx.x & 63;
+    int above = 0;
+#pragma unroll
+    for (int i = 0; i < 64; i++) {
+        const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, most), i));
+        above += w > most || (w == most && i < l);
+    }
+    return max_of<64>(above == top - 1 ? most : -INFINITY);
+}
+// the largest of lanes l, l + 16, l + 32, l + 48
+__device__ __forceinline__ float max_of_rows(float v) {
+    uint32_t u = __builtin_bit_cast(uint32_t, v);
+    u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(u, u, false, false));
+    v = __builtin_fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+    u = __builtin_bit_cast(uint32_t, v);
+    r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(u, u, false, false));
+    return __builtin_fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+
 // Rows of up to kG kC kU entries, kG lanes a row with the row in their registers. 64 rows of 256 bytes by 16 lanes each keep
 // 2 to 3 us of arithmetic a wave against the loads of the others: 262144 rows of 256 f32 are bound by both.
 template <class T, int kG, int kU> __global__ __launch_bounds__(256) void narrow_kernel(LogprobsArgs a) {
@@ -179,26 +215,7 @@ template <class T, int kG, int kU> __global__ __launch_bounds__(256) void narrow
     o.of(z);
     if (live && l == 0) put_row(a, row, o, t, vt);
     if (!a.top) return;
-    // the top-th largest of the lanes' maxima, ties by lane
-    int above = 0;
-    if constexpr (kG == 16) {
-        auto turn = [&](uint32_t u, int by) {
-            const float w = __builtin_bit_cast(float, u);
-            above += w > most || (w == most && (l - by & 15) < l);     // row_ror by `by`: lane l has lane l - by's
-        };
-        const uint32_t u = __builtin_bit_cast(uint32_t, most);
-        turn(rotated<0x121>(u), 1), turn(rotated<0x122>(u), 2), turn(rotated<0x123>(u), 3), turn(rotated<0x124>(u), 4);
-        turn(rotated<0x125>(u), 5), turn(rotated<0x126>(u), 6), turn(rotated<0x127>(u), 7), turn(rotated<0x128>(u), 8);
-        turn(rotated<0x129>(u), 9), turn(rotated<0x12a>(u), 10), turn(rotated<0x12b>(u), 11), turn(rotated<0x12c>(u), 12);
-        turn(rotated<0x12d>(u), 13), turn(rotated<0x12e>(u), 14), turn(rotated<0x12f>(u), 15);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 64; i++) {
-            const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, most), i));
-            above += w > most || (w == most && i < l);
-        }
-    }
-    const float bound = max_of<kG>(above == a.top - 1 ? most : -INFINITY);
+    const float bound = kG == 16 || a.top <= 8 ? bound_of_16(kG == 16 ? most : max_of_rows(most), a.top) : bound_of_64(most, a.top);
     uint32_t reach = 0;
 #pragma unroll
     for (int j = 0; j < kN; j++) reach |= (v[j] >= bound && v[j] > -INFINITY ? 1u : 0u) << j;
@@ -246,7 +263,8 @@ template <class T, int kG, int kU> __global__ __launch_bounds__(256) void narrow
         for (int i = 0; i < longest; i++) rank += keys[at + i] > key;
         if (live) {
             if (l < all && rank < a.top) put_top(a, row, rank, key, o);
-            if (l >= all && l < a.top) put_top(a, row, l, 0, o);
+            for (int i = l; i < a.top; i += kG)
+                if (i >= all) put_top(a, row, i, 0, o);
         }
         return;
     }
@@ -374,14 +392,8 @@ template <class T, int kU> __global__ __launch_bounds__(256) void wide_kernel(Lo
     // the top-th largest of 64 maxima, those of the threads tid, tid + 64, ...
     const int l = tid & 63;
     const float mine = __builtin_fmaxf(__builtin_fmaxf(sh.most[l], sh.most[l + 64]), __builtin_fmaxf(sh.most[l + 128], sh.most[l + 192]));
-    int above = 0;
-#pragma unroll
-    for (int i = 0; i < 64; i++) {
-        const float v = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), i));
-        above += v > mine || (v == mine && i < l);
-    }
-    const float bound = max_of<64>(above == a.top - 1 ? mine : -INFINITY);
-    if (!o.bad) {
+    const float bound = a.top <= 8 ? bound_of_16(max_of_rows(mine), a.top) : bound_of_64(mine, a.top);
+    if (!o.bad && most >= bound) {      // few threads have an entry that reaches it
         for_pieces<T, kU>(x, c0, c1, [&](const float *v, int c) {
 #pragma unroll
             for (int j = 0; j < kN; j++) {
@@ -571,8 +583,8 @@ template <class T> hipError_t go(const LogprobsArgs &a, void *scratch, hipStream
         return hipGetLastError();
     };
     using std::integral_constant;
-    // 16 lanes hold 8 alternatives with room for as many more that reach the bound
-    if (a.V <= 256 && a.top <= 8) {
+    // 16 lanes hold 8 alternatives with room for as many more that reach the bound, or all of 16 classes
+    if ((a.V <= 256 && a.top <= 8) || a.V <= 16) {
         if (a.V <= 16 * kC) return narrow(integral_constant<int, 16>(), integral_constant<int, 1>());
         return narrow(integral_constant<int, 16>(), integral_constant<int, 16 / kC>());
     }

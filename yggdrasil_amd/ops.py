@@ -12,6 +12,7 @@ values, never an access out of bounds. Types: float32, bfloat16 and float16.
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -47,11 +48,24 @@ def _ptr(t: Optional[torch.Tensor]):
 
 def _call(fn, device, *args) -> None:
     """fn(*args, stream) on device's current stream."""
-    if torch.cuda.current_device() == device.index:
-        check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)))
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        if rc:
+            check(rc)
     else:
         with torch.cuda.device(device):
-            check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)))
+            check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+
+
+@functools.lru_cache(maxsize=256)
+def _logprobs_scratch(type: int, rows: int, V: int, top: int) -> int:
+    return _lib.lib().ygg_logprobs_scratch(type, rows, V, top) if rows else 0
+
+
+@functools.lru_cache(maxsize=256)
+def _int8_scratch(M: int, N: int, K: int) -> int:
+    return _lib.lib().ygg_int8_scratch(M, N, K) if M else 0
 
 
 # ---------------------------------------------------------------------------------------------- log-probabilities
@@ -64,6 +78,8 @@ class LogProbs(NamedTuple):
 
 def _rows(logits: torch.Tensor) -> torch.Tensor:
     """logits as (rows, V), values next to each other, rows at any distance of at least V; a copy where they are not."""
+    if logits.is_contiguous() and logits.dim() == 2:
+        return logits
     V = logits.shape[-1]
     x = logits if logits.dim() == 2 else logits.reshape(-1, V)
     if x.shape[0] <= 1:
@@ -73,17 +89,16 @@ def _rows(logits: torch.Tensor) -> torch.Tensor:
 
 def _logprobs(x, targets, top: int, keep: bool):
     rows, V = x.shape
-    dev = x.device
-    f32 = dict(dtype=torch.float32, device=dev)
-    lib = _lib.lib()
-    logp = torch.empty(rows, **f32) if targets is not None else None
-    entropy = torch.empty(rows, **f32)
-    top_logp = torch.empty(rows, top, **f32) if top else None
-    top_ids = torch.empty(rows, top, dtype=torch.int32, device=dev) if top else None
-    stats = torch.empty(rows, 2, **f32) if keep else None
-    need = lib.ygg_logprobs_scratch(_TYPES[x.dtype], rows, V, top) if rows else 0
+    dev, type = x.device, _TYPES[x.dtype]
+    f32 = torch.float32
+    logp = torch.empty(rows, dtype=f32, device=dev) if targets is not None else None
+    entropy = torch.empty(rows, dtype=f32, device=dev)
+    top_logp = torch.empty((rows, top), dtype=f32, device=dev) if top else None
+    top_ids = torch.empty((rows, top), dtype=torch.int32, device=dev) if top else None
+    stats = torch.empty((rows, 2), dtype=f32, device=dev) if keep else None
+    need = _logprobs_scratch(type, rows, V, top)
     scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _call(lib.ygg_logprobs, dev, x.data_ptr(), _TYPES[x.dtype], rows, V, x.stride(0) if rows > 1 else V, _ptr(targets),
+    _call(_lib.lib().ygg_logprobs, dev, x.data_ptr(), type, rows, V, x.stride(0) if rows > 1 else V, _ptr(targets),
           targets.element_size() if targets is not None else 0, top, _ptr(logp), entropy.data_ptr(), _ptr(top_logp),
           _ptr(top_ids), _ptr(stats), _ptr(scratch), need)
     return logp, entropy, top_logp, top_ids, stats
@@ -131,7 +146,8 @@ def token_logprobs(logits, targets=None, top: int = 0) -> LogProbs:
     lead = logits.shape[:-1]
     if targets is not None:
         _on(targets, logits.device, "targets", (torch.int32, torch.int64), lead)
-        targets = targets.reshape(-1).contiguous()
+        if len(lead) != 1 or not targets.is_contiguous():
+            targets = targets.reshape(-1).contiguous()
     x = _rows(logits)
     if x.requires_grad and torch.is_grad_enabled():
         r = _TokenLogprobs.apply(x, targets, top)
@@ -179,9 +195,9 @@ class _GroupedMatmul(torch.autograd.Function):
 
 
 def _grouped(fn, a, b, offsets, order, M, shape, out_shape):
-    out = torch.empty(out_shape, dtype=a.dtype, device=a.device)
-    _call(fn, a.device, a.data_ptr(), b.data_ptr(), _TYPES[a.dtype], offsets.data_ptr(), _ptr(order), M, *shape,
-          out.data_ptr())
+    dtype, dev = a.dtype, a.device
+    out = torch.empty(out_shape, dtype=dtype, device=dev)
+    _call(fn, dev, a.data_ptr(), b.data_ptr(), _TYPES[dtype], offsets.data_ptr(), _ptr(order), M, *shape, out.data_ptr())
     return out
 
 
@@ -203,8 +219,10 @@ def grouped_matmul(x, w, offsets, order=None) -> torch.Tensor:
     _on(offsets, x.device, "offsets", (torch.int32,), (E + 1,))
     if order is not None:
         _on(order, x.device, "order", (torch.int32,), (M,))
-        order = order.contiguous()
-    x, w, offsets = x.contiguous(), w.contiguous(), offsets.contiguous()
+        if not order.is_contiguous():
+            order = order.contiguous()
+    if not (x.is_contiguous() and w.is_contiguous() and offsets.is_contiguous()):
+        x, w, offsets = x.contiguous(), w.contiguous(), offsets.contiguous()
     if (x.requires_grad or w.requires_grad) and torch.is_grad_enabled():
         return _GroupedMatmul.apply(x, w, offsets, order)
     return _grouped(_lib.lib().ygg_grouped_matmul, x, w, offsets, order, M, w.shape, (M, N))
@@ -241,13 +259,14 @@ def int8_linear(x, w, w_scale) -> torch.Tensor:
     M = x2.shape[0]
     if M > MOST_ROWS or not 1 <= N <= MOST_VOCAB or not 1 <= K <= MOST_INNER:
         raise ValueError(f"{M} rows, N = {N}, K = {K}: at most {MOST_ROWS} rows, N 1 to {MOST_VOCAB}, K 1 to {MOST_INNER}")
-    x2, w, w_scale = x2.contiguous(), w.contiguous(), w_scale.contiguous()
-    y = torch.empty(M, N, dtype=x.dtype, device=x.device)
-    lib = _lib.lib()
-    need = lib.ygg_int8_scratch(M, N, K) if M else 0
-    scratch = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    _call(lib.ygg_int8_linear, x.device, x2.data_ptr(), _TYPES[x.dtype], w.data_ptr(), w_scale.data_ptr(), M, N, K,
-          y.data_ptr(), _ptr(scratch), need)
+    if not (x2.is_contiguous() and w.is_contiguous() and w_scale.is_contiguous()):
+        x2, w, w_scale = x2.contiguous(), w.contiguous(), w_scale.contiguous()
+    dtype, dev = x.dtype, x.device
+    y = torch.empty((M, N), dtype=dtype, device=dev)
+    need = _int8_scratch(M, N, K)
+    scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _call(_lib.lib().ygg_int8_linear, dev, x2.data_ptr(), _TYPES[dtype], w.data_ptr(), w_scale.data_ptr(), M, N, K, y.data_ptr(),
+          _ptr(scratch), need)
     return y if x.dim() == 2 else y.reshape(x.shape[:-1] + (N,))
 
 
