@@ -78,14 +78,16 @@ struct Sums {
     }
     // values none of which is above m; -inf ones add nothing
     template <int kN> __device__ __forceinline__ void add(const float *v) {
+        int count = 0;
 #pragma unroll
         for (int j = 0; j < kN; j++) {
             const float d = v[j] - m, e = exp_of(d);
             const bool at = d == 0.0f;
-            n += at ? 1.0f : 0.0f;
+            count += at;
             r += at ? 0.0f : e;
             s = __builtin_fmaf(e, __builtin_fmaxf(d, kLowest), s);
         }
+        n += (float)count;
     }
     template <int kG> __device__ __forceinline__ void join_lanes() {
         move(max_of<kG>(m));
@@ -290,7 +292,8 @@ struct Wide {
     uint64_t *keys;     // (rows, parts, top), falling, then zeros
 };
 
-// calls f(values, index of the first) for the row's entries from c0 to c1, kU pieces of 16 bytes a thread at a time
+// calls f(values, index of the first, count) for the row's entries from c0 to c1, kU pieces of 16 bytes a thread at a time, and
+// what is left by one
 template <class T, int kU, class F> __device__ __forceinline__ void for_pieces(const T *x, int c0, int c1, F f) {
     constexpr int kC = 16 / sizeof(T), kN = kU * kC, kSpan = 256 * kN;
     const int l = threadIdx.x;
@@ -302,18 +305,15 @@ template <class T, int kU, class F> __device__ __forceinline__ void for_pieces(c
         for (int u = 0; u < kU; u++) p[u] = load16(x + c + (u * 256 + l) * kC);
 #pragma unroll
         for (int u = 0; u < kU; u++) unpack(p[u], v + u * kC, T{});
-        f(v, c + l * kC);
+        f(v, c + l * kC, std::integral_constant<int, kN>());
     }
-    if (c < c1) {
-        float v[kN];
+    for (; c < c1; c += 256 * kC) {
+        float v[kC];
+        const int first = c + l * kC, n = c1 - first;
+        unpack(load16_end(x + first, n), v, T{});      // c1 is past a whole piece of the row
 #pragma unroll
-        for (int u = 0; u < kU; u++) {
-            const int first = c + (u * 256 + l) * kC, n = c1 - first;
-            unpack(load16_end(x + first, n), v + u * kC, T{});      // c1 is past a whole piece of the row
-#pragma unroll
-            for (int j = 0; j < kC; j++) v[u * kC + j] = j < n ? v[u * kC + j] : -INFINITY;
-        }
-        f(v, c + l * kC);
+        for (int j = 0; j < kC; j++) v[j] = j < n ? v[j] : -INFINITY;
+        f(v, first, std::integral_constant<int, kC>());
     }
 }
 
@@ -335,7 +335,7 @@ template <class F> __device__ __forceinline__ void put_ranked(const TopShared &s
 }
 
 template <class T, int kU> __global__ __launch_bounds__(256) void wide_kernel(LogprobsArgs a, Wide w) {
-    constexpr int kC = 16 / sizeof(T), kN = kU * kC;
+    constexpr int kC = 16 / sizeof(T);
     __shared__ Sums waves[4];
     __shared__ TopShared sh;
     const int64_t row = blockIdx.x / w.parts;
@@ -344,7 +344,8 @@ template <class T, int kU> __global__ __launch_bounds__(256) void wide_kernel(Lo
     const int c0 = min((int64_t)part * w.width, (int64_t)a.V), c1 = (int)min((int64_t)c0 + w.width, (int64_t)a.V);
     Sums z;
     z.clear();
-    for_pieces<T, kU>(x, c0, c1, [&](const float *v, int) {
+    for_pieces<T, kU>(x, c0, c1, [&](const float *v, int, auto count) {
+        constexpr int kN = decltype(count)::value;
         float most = v[0];
 #pragma unroll
         for (int j = 1; j < kN; j++) most = __builtin_fmaxf(most, v[j]);
@@ -394,7 +395,8 @@ template <class T, int kU> __global__ __launch_bounds__(256) void wide_kernel(Lo
     const float mine = __builtin_fmaxf(__builtin_fmaxf(sh.most[l], sh.most[l + 64]), __builtin_fmaxf(sh.most[l + 128], sh.most[l + 192]));
     const float bound = a.top <= 8 ? bound_of_16(max_of_rows(mine), a.top) : bound_of_64(mine, a.top);
     if (!o.bad && most >= bound) {      // few threads have an entry that reaches it
-        for_pieces<T, kU>(x, c0, c1, [&](const float *v, int c) {
+        for_pieces<T, kU>(x, c0, c1, [&](const float *v, int c, auto count) {
+            constexpr int kN = decltype(count)::value;
 #pragma unroll
             for (int j = 0; j < kN; j++) {
                 if (v[j] >= bound && v[j] > -INFINITY) {
@@ -413,7 +415,7 @@ template <class T, int kU> __global__ __launch_bounds__(256) void wide_kernel(Lo
     uint64_t last = ~0ull;
     for (int k = 0; k < a.top; k++) {
         uint64_t best = 0;
-        for_pieces<T, 1>(x, c0, c1, [&](const float *v, int c) {
+        for_pieces<T, 1>(x, c0, c1, [&](const float *v, int c, auto) {
 #pragma unroll
             for (int j = 0; j < kC; j++) {
                 const uint64_t key = key_of(v[j], c + j);
