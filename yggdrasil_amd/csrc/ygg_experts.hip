@@ -481,8 +481,9 @@ hipError_t go_rows(const void *in, const void *w, const Groups &g, int O, int R,
     if constexpr (!TR) {
         if (mean < 4 || g.M < 64 || (small && mean < 16)) {
             // off 16 bytes a row's 64 take two or three lines each, which tiles' whole 128 bytes feel less: 22 rows through 27
-            // experts of 1702 x 1543 bf16 24 us for 57 (1704 x 1544: 23 and 27; 16 through 64 of 1536 x 2048: 23 and 18)
-            if (!small && !(aligned16(in, in_row) && aligned16(w, w_row))) return tiles(one, one, one);
+            // experts of 1702 x 1543 bf16 24 us for 57 (1704 x 1544: 23 and 27; 16 through 64 of 1536 x 2048: 23 and 18).
+            // They do not split r, so there have to be enough of them.
+            if (!small && !(aligned16(in, in_row) && aligned16(w, w_row)) && (int64_t)g.M * ((O + 63) / 64) >= 256) return tiles(one, one, one);
             const int cols = (O + 15) / 16;
             const int64_t slots = (int64_t)g.M / 16 + g.E + 2, rows = std::min<int64_t>(slots, g.M);
             if (rows * cols > INT32_MAX) return hipErrorInvalidValue;
@@ -533,18 +534,22 @@ hipError_t go_grad_w(const void *dy, const void *x, const Groups &g, int N, int 
         };
         return N <= 16 ? small(one) : N <= 32 ? small(two) : small(four);
     }
-    auto tiles = [&](auto fi) {
-        constexpr int FI = decltype(fi)::value, kI = 32 * FI;
-        const int tn = (N + kI - 1) / kI, tk = (K + 127) / 128;
+    auto tiles = [&](auto fi, auto wi, auto wo) {
+        constexpr int FI = decltype(fi)::value, WI = decltype(wi)::value, WO = decltype(wo)::value, kI = 16 * FI * WI, kO = 64 * WO;
+        const int tn = (N + kI - 1) / kI, tk = (K + kO - 1) / kO;
         const int64_t tiles = (int64_t)g.E * tn * tk;
         if (tiles > INT32_MAX) return hipErrorInvalidValue;
-        hipLaunchKernelGGL((grad_w_kernel<T, FI, 4, 2, 2, 1>), dim3((unsigned)tiles), dim3(256), 0, st, (const T *)dy, (const T *)x, g, N,
-                           K, (T *)dw, tn, tk);
+        hipLaunchKernelGGL((grad_w_kernel<T, FI, 4, WI, WO, 1>), dim3((unsigned)tiles), dim3(64 * WI * WO), 0, st, (const T *)dy,
+                           (const T *)x, g, N, K, (T *)dw, tn, tk);
         return hipGetLastError();
     };
-    // 128 x 128 where there are enough (250 rows of each, bf16 494 us for 538, f32 1250 for 1345), else 64 x 128 (4 experts of
-    // 1000 x 1000: 74 for 81)
-    return (int64_t)g.E * ((N + 127) / 128) * ((K + 127) / 128) >= 512 ? tiles(four) : tiles(two);
+    // 64 x 128, 128 x 128 and (16 waves) 256 x 256: 4 experts of 1000 x 1000 bf16 74, 81 and 120 us; 64 of 1527 x 2041, 250 rows of
+    // each, bf16 413, 372 and 349, f32 1345 and 1250; 8 of 3001 x 2999 bf16 1379, 1157 and 936
+    const int64_t tiles128 = (int64_t)g.E * ((N + 127) / 128) * ((K + 127) / 128);
+    if constexpr (sizeof(T) == 2) {
+        if (tiles128 >= 2048) return tiles(four, four, four);
+    }
+    return tiles128 >= 512 ? tiles(four, two, two) : tiles(two, two, two);
 }
 
 }  // namespace

@@ -222,24 +222,22 @@ template <class T, int kG, int kU> __global__ __launch_bounds__(256) void narrow
 #pragma unroll
     for (int j = 0; j < kN; j++) reach |= (v[j] >= bound && v[j] > -INFINITY ? 1u : 0u) << j;
     if (o.bad) reach = 0;
-    int count = __popc(reach), place = 0, all = 0;
+    // how many reach it in the lanes before mine, and in all: sums over the lanes to the left, row_shr of 1, 2, 4, 8 (zeros come
+    // in) and, past 16 lanes, the rows' last ones to the rows after (row_bcast 15 and 31)
+    const int count = __popc(reach);
+    int place = count, all;
+    place += (int)__builtin_amdgcn_update_dpp(0, place, 0x111, 0xf, 0xf, true);
+    place += (int)__builtin_amdgcn_update_dpp(0, place, 0x112, 0xf, 0xf, true);
+    place += (int)__builtin_amdgcn_update_dpp(0, place, 0x114, 0xf, 0xf, true);
+    place += (int)__builtin_amdgcn_update_dpp(0, place, 0x118, 0xf, 0xf, true);
     if constexpr (kG == 16) {
-        // lanes before mine, by row_shr of 1, 2, 4, 8 (zeros come in)
-        place = count;
-        place += (int)__builtin_amdgcn_update_dpp(0, place, 0x111, 0xf, 0xf, true);
-        place += (int)__builtin_amdgcn_update_dpp(0, place, 0x112, 0xf, 0xf, true);
-        place += (int)__builtin_amdgcn_update_dpp(0, place, 0x114, 0xf, 0xf, true);
-        place += (int)__builtin_amdgcn_update_dpp(0, place, 0x118, 0xf, 0xf, true);
-        all = __builtin_bit_cast(int, join<16>(place, [](int p, int q) { return max(p, q); }));
-        place -= count;
+        all = join<16>(place, [](int p, int q) { return max(p, q); });
     } else {
-#pragma unroll
-        for (int j = 0; j < kN; j++) {
-            const uint64_t who = __ballot(reach >> j & 1);
-            place += __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
-            all += __popcll(who);
-        }
+        place += (int)__builtin_amdgcn_update_dpp(0, place, 0x142, 0xa, 0xf, false);
+        place += (int)__builtin_amdgcn_update_dpp(0, place, 0x143, 0xc, 0xf, false);
+        all = __builtin_amdgcn_readlane(place, 63);
     }
+    place -= count;
     if (__all(all <= kG)) {
         while (__any(reach != 0)) {
             if (reach) {
@@ -565,12 +563,13 @@ template <class T, int kU> __global__ __launch_bounds__(256) void grad_kernel(Lo
     }
 }
 
-constexpr int kNarrow = 1024;    // most entries of a row held in registers
+constexpr int kNarrow = 2048;    // most entries of a row held in registers
 constexpr int kWideU = 4;
 
-// Parts of a wide row: enough workgroups for 4 a CU, each of at least 4096 entries (a piece of 16 bytes, twice, a thread)
+// Parts of a wide row: enough workgroups for 4 a CU, each of at least 4096 entries. Rows of up to 32768 are not worth the second
+// launch (16 rows of 10426: 15 us in parts, 10 whole).
 int parts_of(int64_t rows, int V) {
-    if (V <= kNarrow) return 1;
+    if (V <= 32768) return 1;
     const int64_t want = (1024 + rows - 1) / rows, most = (V + 4095) / 4096;
     return (int)(want < most ? want < 64 ? want : 64 : most < 64 ? most : 64);
 }
@@ -591,7 +590,9 @@ template <class T> hipError_t go(const LogprobsArgs &a, void *scratch, hipStream
         return narrow(integral_constant<int, 16>(), integral_constant<int, 16 / kC>());
     }
     if (a.V <= 64 * kC) return narrow(integral_constant<int, 64>(), integral_constant<int, 1>());
-    if (a.V <= kNarrow) return narrow(integral_constant<int, 64>(), integral_constant<int, 16 / kC>());
+    if (kC == 4 && a.V <= 512) return narrow(integral_constant<int, 64>(), integral_constant<int, 2>());
+    if (a.V <= 1024) return narrow(integral_constant<int, 64>(), integral_constant<int, 16 / kC>());
+    if (a.V <= kNarrow) return narrow(integral_constant<int, 64>(), integral_constant<int, 32 / kC>());
     Wide w;
     w.parts = parts_of(a.rows, a.V);
     w.width = ((a.V + w.parts - 1) / w.parts + kC - 1) / kC * kC;
