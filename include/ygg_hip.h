@@ -294,8 +294,8 @@ int ygg_grouped_grad_w(const void *d_dy, const void *d_x, int type, const int32_
 
 /* y (M, N) in x's type: x (M, K) quantised to int8 row by row, s_i = max(max |x_i| / 127, 2^-126) and q = x / s_i in f32,
    rounded to nearest even, times w (N, K) int8 with a scale for each of its rows: (q . w) s_i d_w_scale. A row that holds a
-   NaN or an infinity is NaN. d_scratch: device memory of ygg_int8_scratch bytes, 256-byte aligned, that no other call uses
-   until this one has run. */
+   NaN or an infinity is NaN. d_scratch: device memory of ygg_int8_scratch bytes (0: none wanted), 256-byte aligned, that no
+   other call uses until this one has run. */
 int64_t ygg_int8_scratch(int M, int N, int K);
 int ygg_int8_linear(const void *d_x, int type, const int8_t *d_w, const float *d_w_scale, int M, int N, int K, void *d_y,
                     void *d_scratch, int64_t scratch_bytes, void *stream);

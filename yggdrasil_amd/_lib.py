@@ -20,7 +20,8 @@ SYMBOLS = ("ygg_load", "ygg_load_blob", "ygg_model_info", "ygg_free", "ygg_step"
            "ygg_generate", "ygg_take_errors", "ygg_float_load", "ygg_float_run", "ygg_float_scratch",
            "ygg_float_run_scratch", "ygg_float_nll", "ygg_float_take_errors",
            "ygg_float_free", "ygg_logprobs_scratch", "ygg_logprobs", "ygg_logprobs_grad", "ygg_grouped_matmul",
-           "ygg_grouped_grad_x", "ygg_grouped_grad_w", "ygg_int8_scratch", "ygg_int8_linear", "ygg_kernel_name", "ygg_spec_stats", "ygg_last_error", "ygg_version")
+           "ygg_grouped_grad_x", "ygg_grouped_grad_w", "ygg_int8_scratch", "ygg_int8_linear", "ygg_kernel_name",
+           "ygg_spec_stats", "ygg_last_error", "ygg_version")
 
 ERRORS = {1: "io", 2: "format", 3: "limits", 4: "nomem", 5: "arg", 6: "token", 7: "device"}
 ABI_VERSION = 12

@@ -61,11 +61,11 @@ template <int kI> __device__ __forceinline__ Piece piece_from(const Groups &g, i
 }
 
 // out[row][o] = sum over r of in[row][r] * (TR ? w[e][r][o] : w[e][o][r]): dimensions O and R
-template <class T, int FI, int FO, int WI, int WO, int kBufs, bool TR> struct RowsTile {
+template <class T, int FI, int FO, int WI, int WO, bool TR> struct RowsTile {
     static constexpr int kThreads = 64 * WI * WO, kI = 16 * FI * WI, kO = 16 * FO * WO;
     typedef Along<T, kI, kThreads, FI, true> A;
     typedef std::conditional_t<TR, Across<T, kO, kThreads>, Along<T, kO, kThreads, FO, false>> B;
-    typedef Tile<T, FI, FO, WI, WO, kBufs, A, B> Tl;
+    typedef Tile<T, FI, FO, WI, WO, A, B> Tl;
     static __device__ __forceinline__ void run(char *lds, const T *in, const T *w, const Groups &g, int O, int R, T *out,
                                                const Piece &pc, int o0) {
         Tl tile;
@@ -97,10 +97,10 @@ template <class T, int FI, int FO, int WI, int WO, int kBufs, bool TR> struct Ro
         });
     }
 };
-template <class T, int FI, int FO, int WI, int WO, int kBufs, bool TR>
+template <class T, int FI, int FO, int WI, int WO, bool TR>
 __global__ __launch_bounds__(64 * WI * WO) void rows_kernel(const T *in, const T *w, Groups g, int O, int R, T *out, int cols, int band,
                                                             bool by_place) {
-    typedef RowsTile<T, FI, FO, WI, WO, kBufs, TR> K;
+    typedef RowsTile<T, FI, FO, WI, WO, TR> K;
     __shared__ __align__(128) char lds[K::Tl::kLds];
     const Place t = place_of(tile_of(blockIdx.x, gridDim.x), gridDim.x / cols, cols, band);
     const Piece pc = by_place ? piece_from<K::kI>(g, t.row) : piece_at<K::kI>(g, t.row);
@@ -108,13 +108,13 @@ __global__ __launch_bounds__(64 * WI * WO) void rows_kernel(const T *in, const T
 }
 
 // dw[e][n][k] = sum over e's rows of dy[row][n] x[row][k], a tile of (n, k)
-template <class T, int FI, int FO, int WI, int WO, int kBufs>
+template <class T, int FI, int FO, int WI, int WO>
 __global__ __launch_bounds__(64 * WI * WO) void grad_w_kernel(const T *dy, const T *x, Groups g, int N, int K, T *dw, int tn,
                                                               int tk) {
     constexpr int kThreads = 64 * WI * WO, kI = 16 * FI * WI, kO = 16 * FO * WO;
     typedef Across<T, kI, kThreads> A;
     typedef Across<T, kO, kThreads> B;
-    typedef Tile<T, FI, FO, WI, WO, kBufs, A, B> Tl;
+    typedef Tile<T, FI, FO, WI, WO, A, B> Tl;
     __shared__ __align__(128) char lds[Tl::kLds];
     const int t = tile_of(blockIdx.x, gridDim.x);
     const int e = t / (tn * tk), n0 = t / tk % tn * kI, k0 = t % tk * kO;
@@ -459,7 +459,7 @@ hipError_t go_rows(const void *in, const void *w, const Groups &g, int O, int R,
         const int cols = (O + kO - 1) / kO;
         const int64_t slots = (int64_t)g.M / kI + g.E + 2, rows = std::min<int64_t>(slots, g.M);
         if (rows * cols > INT32_MAX) return hipErrorInvalidValue;
-        hipLaunchKernelGGL((rows_kernel<T, FI, 4, WI, WO, 1, TR>), dim3((unsigned)(rows * cols)), dim3(64 * WI * WO), 0, st,
+        hipLaunchKernelGGL((rows_kernel<T, FI, 4, WI, WO, TR>), dim3((unsigned)(rows * cols)), dim3(64 * WI * WO), 0, st,
                            (const T *)in, (const T *)w, g, O, R, (T *)out, cols, 16, slots > g.M);
         return hipGetLastError();
     };
@@ -539,7 +539,7 @@ hipError_t go_grad_w(const void *dy, const void *x, const Groups &g, int N, int 
         const int tn = (N + kI - 1) / kI, tk = (K + kO - 1) / kO;
         const int64_t tiles = (int64_t)g.E * tn * tk;
         if (tiles > INT32_MAX) return hipErrorInvalidValue;
-        hipLaunchKernelGGL((grad_w_kernel<T, FI, 4, WI, WO, 1>), dim3((unsigned)tiles), dim3(64 * WI * WO), 0, st, (const T *)dy,
+        hipLaunchKernelGGL((grad_w_kernel<T, FI, 4, WI, WO>), dim3((unsigned)tiles), dim3(64 * WI * WO), 0, st, (const T *)dy,
                            (const T *)x, g, N, K, (T *)dw, tn, tk);
         return hipGetLastError();
     };

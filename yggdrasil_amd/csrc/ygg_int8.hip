@@ -171,13 +171,13 @@ __global__ __launch_bounds__(256) void few_int8_kernel(const T *x, const int8_t 
 }
 
 // A tile of rows and w's rows: the integers' products on the matrix cores, then a row's and a column's scale
-template <class T, int FI, int FO, int WI, int WO, int kBufs>
+template <class T, int FI, int FO, int WI, int WO>
 __global__ __launch_bounds__(64 * WI * WO) void int8_kernel(const int8_t *q, const float *scale, const int8_t *w, const float *ws,
                                                             int M, int N, int K, int Kp, T *y, int cols, int band) {
     constexpr int kThreads = 64 * WI * WO, kI = 16 * FI * WI, kO = 16 * FO * WO;
     typedef Along<int8_t, kI, kThreads, FI, true> A;
     typedef Along<int8_t, kO, kThreads, FO, false> B;
-    typedef Tile<int8_t, FI, FO, WI, WO, kBufs, A, B> Tl;
+    typedef Tile<int8_t, FI, FO, WI, WO, A, B> Tl;
     __shared__ __align__(128) char lds[Tl::kLds];
     const Place t = place_of(tile_of(blockIdx.x, gridDim.x), gridDim.x / cols, cols, band);
     const int i0 = t.row * kI, o0 = t.col * kO;
@@ -267,7 +267,7 @@ hipError_t go(const void *x, const int8_t *w, const float *ws, int M, int N, int
         const int cols = (N + kO - 1) / kO;
         const int64_t tiles = (int64_t)((M + kI - 1) / kI) * cols;
         if (tiles > INT32_MAX) return hipErrorInvalidValue;
-        hipLaunchKernelGGL((int8_kernel<T, FI, 4, 2, WO, 1>), dim3((unsigned)tiles), dim3(128 * WO), 0, st, q, scale, w, ws, M, N, K,
+        hipLaunchKernelGGL((int8_kernel<T, FI, 4, 2, WO>), dim3((unsigned)tiles), dim3(128 * WO), 0, st, q, scale, w, ws, M, N, K,
                            padded(K), (T *)y, cols, 16);
         return hipGetLastError();
     };
