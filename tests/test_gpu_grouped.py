@@ -312,7 +312,7 @@ def test_refusals():
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("M, E, N, K, ordered", [
     (8192, 8, 2048, 2056, True), (5000, 16, 1528, 2040, False), (9000, 2, 4096, 264, True), (16384, 1, 2048, 1000, True),
-    (3000, 16, 1000, 1000, True), (2500, 9, 1027, 2049, True)])
+    (3000, 16, 1000, 1000, True), (2500, 9, 1027, 2049, True), (1200, 8, 2101, 2051, True)])
 def test_large_tiles(M, E, N, K, ordered, dtype):
     """Products large enough for the largest tiles, with rows of no expert, ends inside a tile and a step, more rows of one
     expert than a workgroup holds numbers of; against products in 64 bits on the GPU, to the tolerances above."""
@@ -340,3 +340,47 @@ def test_large_tiles(M, E, N, K, ordered, dtype):
         near(y[i], (a @ bt).cpu(), (a ** 2 @ bt ** 2).cpu(), K)
         near(dx[i], (c @ b).cpu(), (c ** 2 @ b ** 2).cpu(), N)
         near(dw[e], (ct @ a).cpu(), (ct ** 2 @ a ** 2).cpu(), max(len(i), 1))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("N, K", [(8, 64), (20, 48), (64, 200), (33, 70)])
+def test_long_experts_of_small_matrices(N, K, dtype):
+    """Experts of 256 rows and more beside short ones, their first places on, before and after multiples of 256."""
+    sizes = [256, 255, 1, 0, 257, 511, 0, 30, 1024, 16, 17, 700, 0]
+    leaves = torch.repeat_interleave(torch.arange(len(sizes)), torch.tensor(sizes))
+    g = torch.Generator().manual_seed(N)
+    for ordered in (False, True):
+        M = len(leaves)
+        mine = leaves[torch.randperm(M, generator=g)] if ordered else leaves
+        x, dy = torch.randn(M, K, generator=g).to(dtype), torch.randn(M, N, generator=g).to(dtype)
+        w = (torch.randn(len(sizes), N, K, generator=g) / math.sqrt(K)).to(dtype)
+        check(mine, x, w, dy, ordered)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("M, E, N, K", [(1, 3, 70, 1300), (7, 45, 200, 2111), (20, 9, 150, 1024), (63, 2, 90, 2056), (200, 100, 300, 513)])
+def test_few_rows(M, E, N, K, dtype):
+    """Few rows an expert and long reductions, at and off an alignment of 16 bytes."""
+    leaves, x, w, dy = make(M, E, N, K, dtype, ordered=True, seed=M)
+    check(leaves, x, w, dy, True)
+
+
+@pytest.mark.parametrize("at", [1, 2, 4])
+def test_operands_off_their_alignment(at):
+    """x, w and dy that begin `at` elements into their storage, at sizes whose rows would be aligned."""
+    from yggdrasil_amd import ops
+    M, E, N, K = 2100, 4, 520, 2048
+    leaves, x, w, dy = make(M, E, N, K, torch.bfloat16, "even", True)
+    offsets, order = ops.group_rows(leaves.cuda(), E)
+
+    def off(t):
+        flat = torch.zeros(t.numel() + at, dtype=t.dtype, device="cuda")
+        flat[at:] = t.reshape(-1).cuda()
+        return flat[at:].view(t.shape)
+    runs = []
+    for f in (lambda t: t.cuda(), off):
+        a, b = f(x).requires_grad_(), f(w).requires_grad_()
+        y = ops.grouped_matmul(a, b, offsets, order)
+        runs.append((y.detach(), *torch.autograd.grad(y, (a, b), f(dy))))
+    for p, q in zip(*runs):      # another order of the same sums in f32, then the type's rounding
+        assert ((p.double() - q.double()).abs() <= 2.0 ** -7 * q.double().abs() + 2.0 ** -10).all()

@@ -175,3 +175,10 @@ def test_large_tiles(M, N, K):
     ref = (torch.round((x.double() / s).float()).double() @ w.double().t().contiguous()) * s * ws.double()
     err = (ops.int8_linear(x, w, ws).double() - ref).abs()
     assert (err <= 4 * 2.0 ** -24 * ref.abs() * (1 + 2.0 ** -20) + 2.0 ** -126).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("M, N, K", [(1, 50, 15), (1, 50, 16), (1, 50, 17), (8, 40, 1000), (8, 40, 8192), (9, 40, 1000), (7, 33, 2047),
+                                     (32, 70, 1024), (33, 70, 1024), (77, 100, 2049), (1, 20, 33000), (600, 700, 64)])
+def test_borders_between_the_kernels(M, N, K, dtype):
+    check(*make(M, N, K, dtype, M + N + K))

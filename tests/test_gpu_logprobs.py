@@ -361,3 +361,14 @@ def test_streams_and_graphs(n, V, top):
         want = ops.token_logprobs(x2, t2, top=top)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("V", [15, 16, 17, 64, 65, 128, 129, 511, 512, 513, 1023, 1537, 2047, 2049, 32767, 32769])
+@pytest.mark.parametrize("top", [8, 9, 40])
+def test_borders_between_the_kernels(V, top, dtype):
+    x, t = rows_of(5, V, dtype, V + top)
+    x[1, ::2] = -INF
+    x[2] = 1.0
+    x[3, V // 2] = math.nan
+    check(x, t.int(), top)
