@@ -271,10 +271,10 @@ template <class T, int kG, int kU> __global__ __launch_bounds__(256) void narrow
     uint64_t last = ~0ull;
     for (int k = 0; k < a.top; k++) {
         uint64_t best = 0;
-#pragma unroll
-        for (int j = 0; j < kN; j++) {
-            const uint64_t key = key_of(v[j], (j / kC * kG + l) * kC + j % kC);
-            if (v[j] > -INFINITY && key < last && key > best) best = key;
+        for (int c = l; c < a.V; c += kG) {      // from the cache: the registers are not held for this
+            const float u = to_f32(x[c]);
+            const uint64_t key = key_of(u, c);
+            if (u > -INFINITY && key < last && key > best) best = key;
         }
         last = max_key(o.bad ? 0 : best, kG);
         if (live && l == 0) put_top(a, row, k, last, o);
