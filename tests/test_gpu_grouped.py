@@ -384,3 +384,15 @@ def test_operands_off_their_alignment(at):
         runs.append((y.detach(), *torch.autograd.grad(y, (a, b), f(dy))))
     for p, q in zip(*runs):      # another order of the same sums in f32, then the type's rounding
         assert ((p.double() - q.double()).abs() <= 2.0 ** -7 * q.double().abs() + 2.0 ** -10).all()
+
+
+def test_second_derivatives_are_refused():
+    from yggdrasil_amd import ops
+    leaves, x, w, dy = make(12, 3, 8, 16, torch.float32)
+    offsets, _ = ops.group_rows(leaves.cuda(), 3)
+    xg, wg = x.cuda().requires_grad_(), w.cuda().requires_grad_()
+    y = ops.grouped_matmul(xg, wg, offsets)
+    gx, gw = torch.autograd.grad(y, (xg, wg), dy.cuda(), create_graph=True)
+    for g in (gx, gw):
+        with pytest.raises(RuntimeError, match="second derivative"):
+            g.sum().backward(retain_graph=True)

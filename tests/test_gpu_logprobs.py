@@ -372,3 +372,32 @@ def test_borders_between_the_kernels(V, top, dtype):
     x[2] = 1.0
     x[3, V // 2] = math.nan
     check(x, t.int(), top)
+
+
+def test_second_derivatives_are_refused():
+    from yggdrasil_amd import ops
+    x, t = rows_of(3, 20, torch.float32, 0)
+    x.requires_grad_()
+    g, = torch.autograd.grad(ops.token_logprobs(x, t).logp.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        g.sum().backward()
+
+
+def test_outputs_alone_and_kept_graphs():
+    """Each output's gradient by itself, a graph used twice, and logits that are used twice."""
+    from yggdrasil_amd import ops
+    x, t = rows_of(5, 300, torch.float32, 4)
+    x.requires_grad_()
+    r = ops.token_logprobs(x, t, top=3)
+    assert not r.top_ids.requires_grad and r.logp.requires_grad and r.entropy.requires_grad and r.top_logp.requires_grad
+    gl, gh, gt = _weights(5, 3, 9)
+    parts = [(r.logp, gl), (r.entropy, gh), (r.top_logp, gt[:, :3])]
+    one = [torch.autograd.grad(o, x, w.cuda(), retain_graph=True)[0] for o, w in parts]
+    whole, = torch.autograd.grad([o for o, _ in parts], x, [w.cuda() for _, w in parts], retain_graph=True)
+    again, = torch.autograd.grad([o for o, _ in parts], x, [w.cuda() for _, w in parts])
+    assert torch.equal(whole, again)
+    # each part's own roundings: a few steps of the largest of them
+    size = sum(o.abs() for o in one)
+    assert ((sum(one) - whole).abs() <= 2.0 ** -20 * size + 1e-30).all()
+    with torch.no_grad():
+        assert not ops.token_logprobs(x, t).logp.requires_grad

@@ -107,3 +107,10 @@ def test_int8_refuses(kw, word):
     assert word in L.ygg_last_error()
     assert L.ygg_int8_scratch(0, 8, 8) == 0 and L.ygg_int8_scratch(1, 8, 1 << 18) == 0
     assert L.ygg_int8_linear(None, 0, None, None, 0, 8, 8, None, None, 0, None) == 0
+
+
+def test_native_errors_are_raised():
+    """The torch part raises the library's message (sizes the library refuses, on host tensors that it never reads)."""
+    with pytest.raises(RuntimeError, match="NULL|type|outside"):
+        ops._native()
+        _lib.check(_lib.lib().ygg_int8_linear(None, 7, None, None, 1, 1, 1, None, None, 0, None))

@@ -1,6 +1,7 @@
-"""Build the gfx950 library (libygg_hip.so, in this package directory) and, for the tests, the CPU oracle.
+"""Build the gfx950 library (libygg_hip.so, in this package directory), the operators on torch tensors and, for the tests, the
+CPU oracle.
 
-    python -m yggdrasil_amd.build            # the HIP library
+    python -m yggdrasil_amd.build            # the HIP library and the operators' torch part
     python -m yggdrasil_amd.build --oracle   # also oracle/libygg_oracle.so and, where /root/reference exists,
                                              # the reference kernel in oracle/_ref/
 
@@ -69,6 +70,23 @@ def build_library(verbose: bool = False) -> Path:
     return LIB
 
 
+def build_torch(verbose: bool = False) -> Path:
+    """The operators on torch tensors (csrc/ygg_torch.cpp, host code): _ygg_torch in this package directory."""
+    import sysconfig
+
+    from torch.utils import cpp_extension as ext
+    out = PKG / ("_ygg_torch" + sysconfig.get_config_var("EXT_SUFFIX"))
+    include = [f"-isystem{p}" for p in [*ext.include_paths("cuda"), sysconfig.get_paths()["include"]]]
+    tmp = out.with_name(out.name + ".tmp")
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", *include,
+          str(CSRC / "ygg_torch.cpp"), "-o", str(tmp), *[f"-L{p}" for p in ext.library_paths("cuda")],
+          "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python"])
+    os.replace(tmp, out)
+    if verbose:
+        print(f"built {out}")
+    return out
+
+
 def build_oracle(verbose: bool = False) -> None:
     """The C oracle, and the reference kernel where its source is present (test infrastructure)."""
     _run(["make", "-s", "-C", str(ORACLE), "-B", "libygg_oracle.so"])
@@ -83,6 +101,7 @@ def main():
     ap.add_argument("--oracle", action="store_true")
     a = ap.parse_args()
     build_library(verbose=True)
+    build_torch(verbose=True)
     if a.oracle:
         build_oracle(verbose=True)
 

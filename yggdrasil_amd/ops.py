@@ -6,20 +6,19 @@
     y = int8_linear(x, w_int8, w_scale)             # rows quantised to int8, an int8 matrix with scales
 
 The kernels are those of csrc/ygg_logprobs.hip, csrc/ygg_experts.hip and csrc/ygg_int8.hip, through the C-ABI of
-include/ygg_hip.h, on the current torch stream of the tensors' device. Nothing waits for the GPU, so a call can be captured
-into a graph; values that only the GPU holds (tokens, offsets, an order) are not checked here, and bad ones give wrong or NaN
-values, never an access out of bounds. Types: float32, bfloat16 and float16.
+include/ygg_hip.h, on the current torch stream of the tensors' device (csrc/ygg_torch.cpp: allocation, the call, autograd).
+Nothing waits for the GPU, so a call can be captured into a graph; values that only the GPU holds (tokens, offsets, an order)
+are not checked here, and bad ones give wrong or NaN values, never an access out of bounds. Types: float32, bfloat16 and
+float16.
 """
 from __future__ import annotations
 
-import functools
+import ctypes
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import check
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MOST_TOP = 64
@@ -42,30 +41,23 @@ def _on(t, device, name: str, dtypes, shape=None) -> None:
         raise ValueError(f"{name} of shape {tuple(t.shape)}, expected {tuple(shape)}")
 
 
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+_ENTRIES = ("ygg_logprobs_scratch", "ygg_logprobs", "ygg_logprobs_grad", "ygg_grouped_matmul", "ygg_grouped_grad_x",
+            "ygg_grouped_grad_w", "ygg_int8_scratch", "ygg_int8_linear", "ygg_last_error")
+_module = None
 
 
-def _call(fn, device, *args) -> None:
-    """fn(*args, stream) on device's current stream."""
-    index = device.index
-    if torch._C._cuda_getDevice() == index:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-        if rc:
-            check(rc)
-    else:
-        with torch.cuda.device(device):
-            check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
-
-
-@functools.lru_cache(maxsize=256)
-def _logprobs_scratch(type: int, rows: int, V: int, top: int) -> int:
-    return _lib.lib().ygg_logprobs_scratch(type, rows, V, top) if rows else 0
-
-
-@functools.lru_cache(maxsize=256)
-def _int8_scratch(M: int, N: int, K: int) -> int:
-    return _lib.lib().ygg_int8_scratch(M, N, K) if M else 0
+def _native():
+    """csrc/ygg_torch.cpp, bound to the library's entries."""
+    global _module
+    if _module is None:
+        try:
+            from . import _ygg_torch
+        except ImportError as e:
+            raise ImportError(f"the torch part of yggdrasil_amd is not built ({e}): run `python -m yggdrasil_amd.build`") from e
+        lib = _lib.lib()
+        _ygg_torch.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _ENTRIES})
+        _module = _ygg_torch
+    return _module
 
 
 # ---------------------------------------------------------------------------------------------- log-probabilities
@@ -85,47 +77,6 @@ def _rows(logits: torch.Tensor) -> torch.Tensor:
     if x.shape[0] <= 1:
         return x if x.stride(1) == 1 or V == 1 else x.contiguous()
     return x if (x.stride(1) == 1 or V == 1) and x.stride(0) >= V else x.contiguous()
-
-
-def _logprobs(x, targets, top: int, keep: bool):
-    rows, V = x.shape
-    dev, type = x.device, _TYPES[x.dtype]
-    f32 = torch.float32
-    logp = torch.empty(rows, dtype=f32, device=dev) if targets is not None else None
-    entropy = torch.empty(rows, dtype=f32, device=dev)
-    top_logp = torch.empty((rows, top), dtype=f32, device=dev) if top else None
-    top_ids = torch.empty((rows, top), dtype=torch.int32, device=dev) if top else None
-    stats = torch.empty((rows, 2), dtype=f32, device=dev) if keep else None
-    need = _logprobs_scratch(type, rows, V, top)
-    scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _call(_lib.lib().ygg_logprobs, dev, x.data_ptr(), type, rows, V, x.stride(0) if rows > 1 else V, _ptr(targets),
-          targets.element_size() if targets is not None else 0, top, _ptr(logp), entropy.data_ptr(), _ptr(top_logp),
-          _ptr(top_ids), _ptr(stats), _ptr(scratch), need)
-    return logp, entropy, top_logp, top_ids, stats
-
-
-class _TokenLogprobs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, targets, top):
-        logp, entropy, top_logp, top_ids, stats = _logprobs(x, targets, top, True)
-        ctx.save_for_backward(x, targets, entropy, top_ids, stats)
-        ctx.set_materialize_grads(False)
-        if top_ids is not None:
-            ctx.mark_non_differentiable(top_ids)
-        return logp, entropy, top_logp, top_ids
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_logp, g_entropy, g_top, _):
-        x, targets, entropy, top_ids, stats = ctx.saved_tensors
-        rows, V = x.shape
-        dx = torch.empty(rows, V, dtype=x.dtype, device=x.device)
-        g = [None if v is None else v.float().contiguous() for v in (g_logp, g_entropy, g_top)]
-        _call(_lib.lib().ygg_logprobs_grad, x.device, x.data_ptr(), _TYPES[x.dtype], rows, V,
-              x.stride(0) if rows > 1 else V, _ptr(targets), targets.element_size() if targets is not None else 0,
-              0 if top_ids is None else top_ids.shape[1], entropy.data_ptr(), _ptr(top_ids), stats.data_ptr(), _ptr(g[0]),
-              _ptr(g[1]), _ptr(g[2]), dx.data_ptr())
-        return dx, None, None
 
 
 def token_logprobs(logits, targets=None, top: int = 0) -> LogProbs:
@@ -148,11 +99,7 @@ def token_logprobs(logits, targets=None, top: int = 0) -> LogProbs:
         _on(targets, logits.device, "targets", (torch.int32, torch.int64), lead)
         if len(lead) != 1 or not targets.is_contiguous():
             targets = targets.reshape(-1).contiguous()
-    x = _rows(logits)
-    if x.requires_grad and torch.is_grad_enabled():
-        r = _TokenLogprobs.apply(x, targets, top)
-    else:
-        r = _logprobs(x, targets, top, False)[:4]
+    r = _native().token_logprobs(_rows(logits), targets, top)
     if len(lead) == 1:
         return LogProbs(*r)
     return LogProbs(*(None if v is None else v.reshape(lead + v.shape[1:]) for v in r))
@@ -172,33 +119,6 @@ def group_rows(leaves, n_experts: int):
     by, order = torch.sort(x, stable=True)
     ends = torch.arange(n_experts + 1, dtype=torch.int32, device=x.device)
     return torch.searchsorted(by, ends, out_int32=True), order.to(torch.int32)
-
-
-class _GroupedMatmul(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w, offsets, order):
-        ctx.save_for_backward(x, w, offsets, order)
-        return _grouped(_lib.lib().ygg_grouped_matmul, x, w, offsets, order, x.shape[0], w.shape, (x.shape[0], w.shape[1]))
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, w, offsets, order = ctx.saved_tensors
-        M, lib = x.shape[0], _lib.lib()
-        dy = dy.contiguous()
-        dx = dw = None
-        if ctx.needs_input_grad[0]:
-            dx = _grouped(lib.ygg_grouped_grad_x, dy, w, offsets, order, M, w.shape, x.shape)
-        if ctx.needs_input_grad[1]:
-            dw = _grouped(lib.ygg_grouped_grad_w, dy, x, offsets, order, M, w.shape, w.shape)
-        return dx, dw, None, None
-
-
-def _grouped(fn, a, b, offsets, order, M, shape, out_shape):
-    dtype, dev = a.dtype, a.device
-    out = torch.empty(out_shape, dtype=dtype, device=dev)
-    _call(fn, dev, a.data_ptr(), b.data_ptr(), _TYPES[dtype], offsets.data_ptr(), _ptr(order), M, *shape, out.data_ptr())
-    return out
 
 
 def grouped_matmul(x, w, offsets, order=None) -> torch.Tensor:
@@ -223,9 +143,7 @@ def grouped_matmul(x, w, offsets, order=None) -> torch.Tensor:
             order = order.contiguous()
     if not (x.is_contiguous() and w.is_contiguous() and offsets.is_contiguous()):
         x, w, offsets = x.contiguous(), w.contiguous(), offsets.contiguous()
-    if (x.requires_grad or w.requires_grad) and torch.is_grad_enabled():
-        return _GroupedMatmul.apply(x, w, offsets, order)
-    return _grouped(_lib.lib().ygg_grouped_matmul, x, w, offsets, order, M, w.shape, (M, N))
+    return _native().grouped_matmul(x, w, offsets, order)
 
 
 # ---------------------------------------------------------------------------------------------- the int8 projection
@@ -261,12 +179,7 @@ def int8_linear(x, w, w_scale) -> torch.Tensor:
         raise ValueError(f"{M} rows, N = {N}, K = {K}: at most {MOST_ROWS} rows, N 1 to {MOST_VOCAB}, K 1 to {MOST_INNER}")
     if not (x2.is_contiguous() and w.is_contiguous() and w_scale.is_contiguous()):
         x2, w, w_scale = x2.contiguous(), w.contiguous(), w_scale.contiguous()
-    dtype, dev = x.dtype, x.device
-    y = torch.empty((M, N), dtype=dtype, device=dev)
-    need = _int8_scratch(M, N, K)
-    scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _call(_lib.lib().ygg_int8_linear, dev, x2.data_ptr(), _TYPES[dtype], w.data_ptr(), w_scale.data_ptr(), M, N, K, y.data_ptr(),
-          _ptr(scratch), need)
+    y = _native().int8_linear(x2, w, w_scale)
     return y if x.dim() == 2 else y.reshape(x.shape[:-1] + (N,))
 
 
