@@ -2,7 +2,7 @@
 // nodes. In C++ for the host's time: a training step's backward pass runs on autograd's own thread, where a node in Python waits
 // for the interpreter lock (a step of 16 rows 96 us with Python nodes, 52 with these), and a call's allocations are most of its
 // cost (one row's log-probabilities 12.6 us from Python, 6.5 from here). Arguments
-// are checked by yggdrasil_amd/ops.py; the library's entries come as addresses, so that there is one copy of it.
+// are checked by yggdrasil_amd/ops.py, those of plain calls here; the library's entries come as addresses, so that there is one copy of it.
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
@@ -180,6 +180,38 @@ Tensor int8_linear(const Tensor &x, const Tensor &w, const Tensor &w_scale) {
     return y;
 }
 
+// The calls on tensors that need no reshaping, checked here; nothing where they do, or where a check fails and ops.py says why
+bool floats(const Tensor &t, int64_t dim) {
+    const auto d = t.scalar_type();
+    return t.is_cuda() && (d == at::kFloat || d == at::kBFloat16 || d == at::kHalf) && t.dim() == dim && t.is_contiguous();
+}
+bool like(const Tensor &t, const Tensor &other, at::ScalarType type, int64_t dim) {
+    return t.device() == other.device() && t.scalar_type() == type && t.dim() == dim && t.is_contiguous();
+}
+bool within(int64_t v, int64_t lo, int64_t hi) { return v >= lo && v <= hi; }
+
+std::optional<std::tuple<Maybe, Tensor, Maybe, Maybe>> plain_token_logprobs(const Tensor &x, const Maybe &targets, int64_t top) {
+    if (!floats(x, 2) || !within(x.size(1), 1, YGG_MOST_VOCAB) || !within(top, 0, YGG_MOST_TOP)) return std::nullopt;
+    if (targets && !((like(*targets, x, at::kInt, 1) || like(*targets, x, at::kLong, 1)) && targets->size(0) == x.size(0)))
+        return std::nullopt;
+    return token_logprobs(x, targets, top);
+}
+Maybe plain_grouped_matmul(const Tensor &x, const Tensor &w, const Tensor &offsets, const Maybe &order) {
+    if (!floats(x, 2) || !like(w, x, x.scalar_type(), 3) || w.size(2) != x.size(1) || x.size(0) > YGG_MOST_ROWS ||
+        !within(w.size(0), 1, YGG_MOST_EXPERTS) || !within(w.size(1), 1, YGG_MOST_INNER) || !within(w.size(2), 1, YGG_MOST_INNER) ||
+        !like(offsets, x, at::kInt, 1) || offsets.size(0) != w.size(0) + 1)
+        return std::nullopt;
+    if (order && !(like(*order, x, at::kInt, 1) && order->size(0) == x.size(0))) return std::nullopt;
+    return grouped_matmul(x, w, offsets, order);
+}
+Maybe plain_int8_linear(const Tensor &x, const Tensor &w, const Tensor &w_scale) {
+    if (!floats(x, 2) || (x.requires_grad() && at::GradMode::is_enabled()) || !like(w, x, at::kChar, 2) || w.size(1) != x.size(1) ||
+        x.size(0) > YGG_MOST_ROWS || !within(w.size(0), 1, YGG_MOST_VOCAB) || !within(w.size(1), 1, YGG_MOST_INNER) ||
+        !like(w_scale, x, at::kFloat, 1) || w_scale.size(0) != w.size(0))
+        return std::nullopt;
+    return int8_linear(x, w, w_scale);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_ygg_torch, m) {
@@ -187,4 +219,7 @@ PYBIND11_MODULE(_ygg_torch, m) {
     m.def("token_logprobs", &token_logprobs);
     m.def("grouped_matmul", &grouped_matmul);
     m.def("int8_linear", &int8_linear);
+    m.def("plain_token_logprobs", &plain_token_logprobs);
+    m.def("plain_grouped_matmul", &plain_grouped_matmul);
+    m.def("plain_int8_linear", &plain_int8_linear);
 }

@@ -41,6 +41,16 @@ def _on(t, device, name: str, dtypes, shape=None) -> None:
         raise ValueError(f"{name} of shape {tuple(t.shape)}, expected {tuple(shape)}")
 
 
+def _tensors(x, *others) -> bool:
+    """A device tensor, and tensors: what the native calls take as they are."""
+    if not (type(x) is torch.Tensor and x.is_cuda):
+        return False
+    for t in others:
+        if type(t) is not torch.Tensor:
+            return False
+    return True
+
+
 _ENTRIES = ("ygg_logprobs_scratch", "ygg_logprobs", "ygg_logprobs_grad", "ygg_grouped_matmul", "ygg_grouped_grad_x",
             "ygg_grouped_grad_w", "ygg_int8_scratch", "ygg_int8_linear", "ygg_last_error")
 _module = None
@@ -89,6 +99,10 @@ def token_logprobs(logits, targets=None, top: int = 0) -> LogProbs:
     log-probability -inf), and a row of them alone has log-probability -inf, entropy 0 and no gradient. A target of -1 is no
     token: its log-probability is 0, without a gradient. Other targets outside [0, V), and rows that hold a NaN or +inf,
     give NaN."""
+    if (_tensors(logits) if targets is None else _tensors(logits, targets)) and type(top) is int:
+        r = _native().plain_token_logprobs(logits, targets, top)
+        if r is not None:
+            return LogProbs(*r)
     _floats(logits, "logits")
     if logits.dim() < 1 or not 1 <= logits.shape[-1] <= MOST_VOCAB:
         raise ValueError(f"logits of shape {tuple(logits.shape)}: the last axis holds 1 to {MOST_VOCAB} classes")
@@ -125,6 +139,10 @@ def grouped_matmul(x, w, offsets, order=None) -> torch.Tensor:
     """Rows x (M, K) times the matrix of the expert each takes, w (E, N, K) -> y (M, N) in their type, y_i = w[expert] x_i.
     offsets (E + 1) int32, rising from 0: expert e takes the places offsets[e] to offsets[e + 1] - 1, of any number. Place p
     is row order[p] (order (M) int32, a permutation; None: row p). Rows past offsets[E] get 0. Differentiable in x and w."""
+    if _tensors(x, w, offsets) if order is None else _tensors(x, w, offsets, order):
+        y = _native().plain_grouped_matmul(x, w, offsets, order)
+        if y is not None:
+            return y
     _floats(x, "x")
     if x.dim() != 2:
         raise ValueError(f"x of shape {tuple(x.shape)}, expected (M, K)")
@@ -162,6 +180,10 @@ def int8_linear(x, w, w_scale) -> torch.Tensor:
     """x (..., K) times an int8 matrix w (N, K) whose row n has the scale w_scale[n] (f32) -> (..., N) in x's type. Each row
     of x is quantised to int8 with a scale of its own, max |row| / 127, and the products are summed in whole numbers. A row
     that holds a NaN or an infinity gives NaN. For serving: there is no gradient."""
+    if _tensors(x, w, w_scale):
+        y = _native().plain_int8_linear(x, w, w_scale)
+        if y is not None:
+            return y
     _floats(x, "x")
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError("int8_linear has no gradient: call it under torch.no_grad() or with x.detach()")
