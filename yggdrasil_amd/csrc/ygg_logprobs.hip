@@ -432,29 +432,34 @@ template <class T, int kU> __global__ __launch_bounds__(256) void wide_kernel(Lo
 // A row's parts, at most 64, joined by a workgroup. Each part's keys fall; with j = ceil(top / parts), the top-th largest of
 // the parts' first keys (j = 1) or the least of their j th bounds the row's: at least `top` of the parts' keys reach it.
 template <class T> __global__ __launch_bounds__(256) void wide_join_kernel(LogprobsArgs a, Wide w) {
+    constexpr int kFirst = 4;
     __shared__ TopShared sh;
     const int64_t row = blockIdx.x;
     const int tid = threadIdx.x, l = tid & 63;
     const T *x = (const T *)a.x + row * a.stride;
+    const uint64_t *keys = w.keys + row * w.parts * a.top;
+    const int j = (a.top + w.parts - 1) / w.parts, all = w.parts * a.top;
+    // every load that waits for none: together
     int64_t t = -1;
     if (a.target_bytes) t = target_at(a.targets, a.target_bytes, row);
-    const float vt = t >= 0 && t < a.V ? to_f32(x[t]) : 0.0f;
+    const float4 s = w.sums[row * w.parts + min(l, w.parts - 1)];
+    uint64_t mine = 0, first[kFirst] = {};
+    if (a.top) {
+        mine = keys[min(l, w.parts - 1) * a.top + j - 1];
+#pragma unroll
+        for (int i = 0; i < kFirst; i++) first[i] = keys[min(tid + 256 * i, all - 1)];
+    }
     if (tid == 0) sh.count = 0;
+    const float vt = t >= 0 && t < a.V ? to_f32(x[t]) : 0.0f;
     Sums z;
     z.clear();
-    if (l < w.parts) {
-        const float4 s = w.sums[row * w.parts + l];
-        z.m = s.x, z.n = s.y, z.r = s.z, z.s = s.w;
-    }
+    if (l < w.parts) z.m = s.x, z.n = s.y, z.r = s.z, z.s = s.w;
+    else mine = 0;
     z.join_lanes<64>();
     Row o;
     o.of(z);
     if (tid == 0) put_row(a, row, o, t, vt);
     if (!a.top) return;
-    const uint64_t *keys = w.keys + row * w.parts * a.top;
-    const int j = (a.top + w.parts - 1) / w.parts, all = w.parts * a.top;
-    uint64_t mine = 0;
-    if (l < w.parts) mine = keys[l * a.top + j - 1];
     uint64_t bound;
     if (j == 1) {
         int above = 0;
@@ -468,14 +473,17 @@ template <class T> __global__ __launch_bounds__(256) void wide_join_kernel(Logpr
         bound = ~max_key(l < w.parts ? ~mine : 0, 64);
     }
     __syncthreads();
-    if (!o.bad) {
-        for (int i = tid; i < all; i += 256) {
-            const uint64_t key = keys[i];
-            if (key && key >= bound) {
-                const int at = atomicAdd(&sh.count, 1);
-                if (at < kHold) sh.keys[at] = key;
-            }
+    auto keep = [&](uint64_t key) {
+        if (key && key >= bound) {
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < kHold) sh.keys[at] = key;
         }
+    };
+    if (!o.bad) {
+#pragma unroll
+        for (int i = 0; i < kFirst; i++)
+            if (tid + 256 * i < all) keep(first[i]);
+        for (int i = tid + 256 * kFirst; i < all; i += 256) keep(keys[i]);
     }
     __syncthreads();
     const int count = sh.count;
@@ -564,7 +572,6 @@ template <class T, int kU> __global__ __launch_bounds__(256) void grad_kernel(Lo
 }
 
 constexpr int kNarrow = 2048;    // most entries of a row held in registers
-constexpr int kWideU = 4;
 
 // Parts of a wide row: enough workgroups for 4 a CU, each of at least 4096 entries. Rows of up to 32768 are not worth the second
 // launch (16 rows of 10426: 15 us in parts, 10 whole).
@@ -599,8 +606,13 @@ template <class T> hipError_t go(const LogprobsArgs &a, void *scratch, hipStream
     w.sums = (float4 *)scratch;
     w.keys = (uint64_t *)((char *)scratch + (a.rows * w.parts * 16 + 255) / 256 * 256);
     if (a.rows * w.parts > INT32_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((wide_kernel<T, kWideU>), dim3((unsigned)(a.rows * w.parts)), dim3(256), 0, st, a, w);
-    if (w.parts > 1) hipLaunchKernelGGL(wide_join_kernel<T>, dim3((unsigned)a.rows), dim3(256), 0, st, a, w);
+    const dim3 grid((unsigned)(a.rows * w.parts)), block(256);
+    if (w.parts == 1) {
+        hipLaunchKernelGGL((wide_kernel<T, 4>), grid, block, 0, st, a, w);
+    } else {
+        hipLaunchKernelGGL((wide_kernel<T, 16 / kC>), grid, block, 0, st, a, w);     // 4096 entries at a time: a part
+        hipLaunchKernelGGL(wide_join_kernel<T>, dim3((unsigned)a.rows), block, 0, st, a, w);
+    }
     return hipGetLastError();
 }
 
