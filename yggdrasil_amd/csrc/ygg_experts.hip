@@ -48,16 +48,18 @@ template <int kI> __device__ __forceinline__ Piece piece_at(const Groups &g, int
 template <int kI> __device__ __forceinline__ Piece piece_from(const Groups &g, int place) {
     const int lane = threadIdx.x & 63;
     int lo = 0, n = g.E + 1;
-    while (n > 1) {
-        const int step = (n + 63) / 64, e = lane * step;
-        const bool before = e < n && (e == 0 || first_of(g, lo + e) <= place);
-        const int at = (63 - __builtin_clzll(__ballot(before))) * step;
-        lo += at;
-        n = min(step, n - at);
+    for (;;) {
+        // the last step has a lane for every expert left and for the one after: the owner's ends too
+        const int step = (n + 62) / 63, e = lane * step, at = lo + e;
+        const int v = at == 0 ? 0 : at <= g.E ? clamp_at(g.offsets[at], g.M) : g.M;
+        const int k = 63 - __builtin_clzll(__ballot(e < n && (e == 0 || v <= place)));
+        if (step == 1) {
+            const int first = __builtin_amdgcn_readlane(v, k), end = __builtin_amdgcn_readlane(v, k + 1);
+            return {__builtin_amdgcn_readfirstlane(lo + k), place, place >= first && (place - first) % kI == 0 ? min(end - place, kI) : 0};
+        }
+        lo += k * step;
+        n = min(step, n - k * step);
     }
-    lo = __builtin_amdgcn_readfirstlane(lo);
-    const int first = first_of(g, lo);
-    return {lo, place, place >= first && (place - first) % kI == 0 ? min(end_of(g, lo) - place, kI) : 0};
 }
 
 // out[row][o] = sum over r of in[row][r] * (TR ? w[e][r][o] : w[e][o][r]): dimensions O and R
@@ -161,10 +163,13 @@ __global__ __launch_bounds__(64 * kW) void few_rows_kernel(const T *in, const T 
     constexpr int kE = 16 / sizeof(T), kStep = 4 * kE, kU = 8;
     __shared__ f32x4 parts[kW][64];
     const int t = tile_of(blockIdx.x, gridDim.x), o0 = t % cols * 16;
+    const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, d = l & 15, q = l >> 4;
+    // by place the rows' numbers need not wait for the search
+    int row = by_place && t / cols + d < g.M ? row_of(g, t / cols + d) : -1;
     const Piece pc = by_place ? piece_from<16>(g, t / cols) : piece_at<16>(g, t / cols);
     if (pc.count <= 0) return;
-    const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, d = l & 15, q = l >> 4;
-    const int row = d < pc.count ? row_of(g, pc.first + d) : -1;
+    if (!by_place && d < pc.count) row = row_of(g, pc.first + d);
+    if (d >= pc.count) row = -1;
     f32x4 acc = {0, 0, 0, 0};
     if (pc.e < g.E) {
         const int steps = (R + kStep - 1) / kStep, per = (steps + kW - 1) / kW, end = min(per * (wave + 1), steps);
