@@ -401,3 +401,51 @@ def test_outputs_alone_and_kept_graphs():
     assert ((sum(one) - whole).abs() <= 2.0 ** -20 * size + 1e-30).all()
     with torch.no_grad():
         assert not ops.token_logprobs(x, t).logp.requires_grad
+
+
+def masked_rows(V, dtype, low):
+    """Rows whose masked entries hold a finite value far below the others: whole threads, waves and parts of a row see nothing
+    else before (or after) they meet an allowed one."""
+    x, t = rows_of(8, V, dtype, V, 2.0)
+    x[0, :V // 2] = low                             # the first half
+    x[1, V // 2:] = low                             # the last half
+    x[2, :min(4096, V - 5)] = low                   # a whole part
+    x[3, torch.rand(V, generator=torch.Generator().manual_seed(V)).cuda() < 0.9] = low
+    x[4, 3:] = low                                  # three left, fewer than the alternatives
+    x[5, :V - 1] = low                              # one left, the last
+    x[6, :-3] = low
+    x[6, :7] = -INF                                 # both masks in one row
+    x[7, V // 3:V // 3 + 700] = low
+    t[:] = torch.tensor([V - 1, 0, V - 2, V // 5, 1, V - 1, V - 3, 2])
+    return x, t
+
+
+@pytest.mark.parametrize("dtype, low", [(torch.float32, -1.0), (torch.float32, -1e38), (torch.float32, -1e9), (torch.bfloat16, -1.0),
+                                        (torch.bfloat16, -1e38), (torch.float16, -1.0)], ids=str)
+@pytest.mark.parametrize("V", [300, 2048, 2049, 9001, 40000, 131072])
+def test_masks_of_a_finite_value(V, dtype, low):
+    """low -1: the type's lowest value."""
+    x, t = masked_rows(V, dtype, torch.finfo(dtype).min if low == -1 else low)
+    r = check(x, t, 7)
+    check(x, t.int(), 0)
+    assert torch.isfinite(r.entropy).all() and torch.isfinite(r.logp).all()
+    assert r.entropy[5] == 0 and r.logp[5] == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("V", [300, 2049, 9001, 40000, 131072])
+@pytest.mark.parametrize("of_logp, of_entropy", [(True, False), (False, True), (True, True)])
+def test_gradient_under_masks_of_a_finite_value(V, dtype, of_logp, of_entropy):
+    from yggdrasil_amd import ops
+    x, t = masked_rows(V, dtype, torch.finfo(dtype).min)
+    x.requires_grad_()
+    gl, gh, _ = _weights(8, 0, V)
+    gl, gh = gl * of_logp, gh * of_entropy
+    r = ops.token_logprobs(x, t)
+    outs = [(r.logp, gl)] * of_logp + [(r.entropy, gh)] * of_entropy
+    dx, = torch.autograd.grad([o for o, _ in outs], x, [w.cuda() for _, w in outs])
+    ref, tol = _grad64(x, t, 0, gl, gh, None)
+    step = torch.finfo(dtype).eps / 2
+    small = {torch.float32: 2.0 ** -126, torch.bfloat16: 2.0 ** -126, torch.float16: 2.0 ** -25}[dtype]
+    err = (dx.double().cpu() - ref).abs()
+    assert (err <= tol + step * (ref.abs() + tol) + small).all(), (err - tol - step * ref.abs()).max()

@@ -20,6 +20,7 @@ namespace ygg {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLowest = -3.402823466e38f;
+constexpr float kGone = -1000.0f;    // exp of it is 0 in f32, and a count times it is finite
 
 __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
 
@@ -67,9 +68,10 @@ __device__ __forceinline__ int64_t target_at(const void *t, int bytes, int64_t r
 struct Sums {
     float m, n, r, s;
     __device__ __forceinline__ void clear() { m = kLowest, n = r = s = 0; }
-    // to the maximum `to`, at least m
+    // to the maximum `to`, at least m, and by far so where entries are masked by the type's lowest value: w d must not overflow,
+    // as f would make it 0 times infinity
     __device__ __forceinline__ void move(float to) {
-        const float d = __builtin_fmaxf(m - to, kLowest), f = exp_of(d), w = r + n;
+        const float d = __builtin_fmaxf(m - to, kGone), f = exp_of(d), w = r + n;
         const bool same = m == to;
         s = same ? s : f * __builtin_fmaf(w, d, s);
         r = same ? r : f * w;
