@@ -274,7 +274,7 @@ int ygg_logprobs(const void *d_logits, int type, int64_t rows, int V, int64_t st
 
 /* The logits' gradient (rows, V), contiguous, in the logits' type, from the gradients of ygg_logprobs' outputs (NULL: none
    comes from that output) and its d_entropy, d_top_ids and d_stats. Zero for a row of -inf alone; a target of -1 takes no
-   part, a bad one makes its row NaN. */
+   part, a bad one makes any other row NaN, masked entries included. */
 int ygg_logprobs_grad(const void *d_logits, int type, int64_t rows, int V, int64_t stride, const void *d_targets,
                       int target_bytes, int top, const float *d_entropy, const int32_t *d_top_ids, const float *d_stats,
                       const float *d_g_logp, const float *d_g_entropy, const float *d_g_top, void *d_out, void *stream);

@@ -449,3 +449,21 @@ def test_gradient_under_masks_of_a_finite_value(V, dtype, of_logp, of_entropy):
     small = {torch.float32: 2.0 ** -126, torch.bfloat16: 2.0 ** -126, torch.float16: 2.0 ** -25}[dtype]
     err = (dx.double().cpu() - ref).abs()
     assert (err <= tol + step * (ref.abs() + tol) + small).all(), (err - tol - step * ref.abs()).max()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("V", [9, 256, 3000])
+def test_bad_targets_make_their_whole_gradient_row_nan(V, dtype):
+    """Masked entries and those whose probability underflows among them; a row without a distribution has no gradient all the
+    same, and the other rows keep theirs."""
+    from yggdrasil_amd import ops
+    x, t = rows_of(6, V, dtype, V, 1.0)
+    x[:, 1::3] = -INF
+    x[:, 2] = -30000.0
+    x[4] = -INF
+    t[:] = torch.tensor([0, V, -2, 1 << 40, V + 7, -1])
+    x.requires_grad_()
+    ops.token_logprobs(x, t).logp.sum().backward()
+    g = x.grad
+    assert torch.isnan(g[1:4]).all()
+    assert (g[4] == 0).all() and (g[5] == 0).all() and torch.isfinite(g[0]).all()

@@ -528,7 +528,7 @@ template <class T, int kU> __global__ __launch_bounds__(256) void grad_kernel(Lo
     if (a.g_top)
         for (int k = 0; k < a.top; k++)
             if (a.top_ids[row * a.top + k] >= 0) all += a.g_top[row * a.top + k];
-    const bool none = st.x == -INFINITY;
+    const bool none = st.x == -INFINITY, bad = all != all;
     u32x4 p[kU];
     if (blocks > 1 && (int)(blockIdx.x % blocks + 1) * kU * 256 * kC <= a.V) {
 #pragma unroll
@@ -550,7 +550,7 @@ template <class T, int kU> __global__ __launch_bounds__(256) void grad_kernel(Lo
         for (int j = 0; j < kC; j++) {
             const float lp = v[j] - st.x - st.y, q = exp_of(lp);
             const float d = -q * __builtin_fmaf(gh, lp + H, all);
-            v[j] = q == 0 ? 0.0f : d;
+            v[j] = q == 0 && !bad ? 0.0f : d;
         }
         if (t >= c && t < c + kC) {
 #pragma unroll
