@@ -396,3 +396,19 @@ def test_second_derivatives_are_refused():
     for g in (gx, gw):
         with pytest.raises(RuntimeError, match="second derivative"):
             g.sum().backward(retain_graph=True)
+
+
+def test_forward_mode_derivatives_are_refused():
+    import torch.autograd.forward_ad as fwd
+    from yggdrasil_amd import ops
+    leaves, x, w, dy = make(12, 3, 8, 16, torch.float32)
+    offsets, _ = ops.group_rows(leaves.cuda(), 3)
+    x, w, dy = x.cuda(), w.cuda(), dy.cuda()
+    with fwd.dual_level():
+        for a, b in ((fwd.make_dual(x, x), w), (x, fwd.make_dual(w, w)), (fwd.make_dual(x, x)[:, ::2], w[:, :, ::2])):
+            with pytest.raises(RuntimeError, match="forward"):
+                ops.grouped_matmul(a, b, offsets)
+        xg = x.clone().requires_grad_()
+        y = ops.grouped_matmul(xg, w, offsets)
+        with pytest.raises(RuntimeError, match="forward"):
+            torch.autograd.grad(y, xg, fwd.make_dual(dy, dy))

@@ -182,3 +182,13 @@ def test_large_tiles(M, N, K):
                                      (32, 70, 1024), (33, 70, 1024), (77, 100, 2049), (1, 20, 33000), (600, 700, 64)])
 def test_borders_between_the_kernels(M, N, K, dtype):
     check(*make(M, N, K, dtype, M + N + K))
+
+
+def test_forward_mode_derivatives_are_refused():
+    import torch.autograd.forward_ad as fwd
+    from yggdrasil_amd import ops
+    x, w, ws = make(4, 6, 8, torch.float32)
+    with fwd.dual_level():
+        for a, s in ((fwd.make_dual(x, x), ws), (x, fwd.make_dual(ws, ws)), (fwd.make_dual(x, x).reshape(2, 2, 8), ws)):
+            with pytest.raises((RuntimeError, ValueError), match="forward"), torch.no_grad():
+                ops.int8_linear(a, w, s)

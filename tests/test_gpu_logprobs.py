@@ -467,3 +467,29 @@ def test_bad_targets_make_their_whole_gradient_row_nan(V, dtype):
     g = x.grad
     assert torch.isnan(g[1:4]).all()
     assert (g[4] == 0).all() and (g[5] == 0).all() and torch.isfinite(g[0]).all()
+
+
+def test_forward_mode_derivatives_are_refused():
+    import torch.autograd.forward_ad as fwd
+    from yggdrasil_amd import ops
+    x, t = rows_of(3, 20, torch.float32, 0)
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for bad in (dual, dual.reshape(3, 1, 20)[:, 0], dual[:, :17]):
+            with pytest.raises(RuntimeError, match="forward"):
+                ops.token_logprobs(bad, t)
+            with pytest.raises(RuntimeError, match="forward"), torch.no_grad():
+                ops.token_logprobs(bad, top=2)
+        # a tangent of the gradient that comes in
+        y = x.clone().requires_grad_()
+        r = ops.token_logprobs(y, t)
+        g = torch.ones(3, device="cuda")
+        with pytest.raises(RuntimeError, match="forward"):
+            torch.autograd.grad(r.logp, y, fwd.make_dual(g, g))
+        want = ops.token_logprobs(x, t)             # nothing in hand has a tangent
+        assert torch.equal(r.logp.detach(), want.logp)
+    assert torch.equal(ops.token_logprobs(x, t).logp, want.logp)
+    for f in (lambda: torch.func.jvp(lambda v: ops.token_logprobs(v, t).logp, (x,), (x,)),
+              lambda: torch.func.vmap(lambda v: ops.token_logprobs(v).entropy)(x)):
+        with pytest.raises(RuntimeError):           # transforms of torch.func hold no tensor that a kernel could read
+            f()

@@ -52,6 +52,13 @@ int type_of(const Tensor &t) { return t.scalar_type() == at::kFloat ? 0 : t.scal
 void *stream_of(const Tensor &t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 template <class T = void> T *ptr(const Tensor &t) { return t.defined() ? (T *)t.data_ptr() : nullptr; }
 Tensor empty(const Tensor &like, at::IntArrayRef size, at::ScalarType type) { return at::empty(size, like.options().dtype(type)); }
+// Forward-mode derivatives are refused: there are none here, and a tangent that is left out would count as zero. A tensor that
+// has one need not require a gradient.
+void no_tangents(const char *name, std::initializer_list<Tensor> tensors) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Tensor &t : tensors)
+        if (t.defined() && t._fw_grad(0).defined()) throw std::runtime_error(std::string(name) + " has no forward-mode derivative");
+}
 // gradients of gradients are refused where they are asked for, not when a graph is only kept
 variable_list once(variable_list grads, const char *name) {
     if (!at::GradMode::is_enabled()) return grads;
@@ -108,6 +115,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
             const at::AutoGradMode none(false);
             auto f32 = [](const Tensor &g) { return g.defined() ? g.to(at::kFloat).contiguous() : g; };
             const int at_logp = t.defined(), at_top = at_logp + 1;
+            for (const Tensor &g : grads) no_tangents("token_logprobs' gradient", {g});
             const Tensor ge = f32(grads[0]), gl = at_logp ? f32(grads[1]) : Tensor(), gt = top_ids.defined() ? f32(grads[at_top]) : Tensor();
             const int64_t rows = x.size(0), V = x.size(1);
             dx = empty(x, {rows, V}, x.scalar_type());
@@ -121,6 +129,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
 };
 // logp, entropy, top_logp, top_ids; None where there are none
 std::tuple<Maybe, Tensor, Maybe, Maybe> token_logprobs(const Tensor &x, const Maybe &targets, int64_t top) {
+    no_tangents("token_logprobs", {x});
     auto some = [](const Tensor &t) { return t.defined() ? Maybe(t) : Maybe(); };
     if (x.requires_grad() && at::GradMode::is_enabled()) {
         const variable_list r = TokenLogprobs::apply(x, targets, top);
@@ -155,6 +164,7 @@ struct GroupedMatmul : torch::autograd::Function<GroupedMatmul> {
         variable_list out;
         {
             const at::AutoGradMode none(false);
+            no_tangents("grouped_matmul's gradient", {grads[0]});
             const Tensor dy = grads[0].contiguous();
             if (to_x) out.push_back(grouped(api.grouped_grad_x, dy, w, offsets, order, x.size(0), w.sizes(), x.sizes()));
             if (to_w) out.push_back(grouped(api.grouped_grad_w, dy, x, offsets, order, x.size(0), w.sizes(), w.sizes()));
@@ -164,11 +174,13 @@ struct GroupedMatmul : torch::autograd::Function<GroupedMatmul> {
     }
 };
 Tensor grouped_matmul(const Tensor &x, const Tensor &w, const Tensor &offsets, const Maybe &order) {
+    no_tangents("grouped_matmul", {x, w});
     if ((x.requires_grad() || w.requires_grad()) && at::GradMode::is_enabled()) return GroupedMatmul::apply(x, w, offsets, order);
     return grouped(api.grouped_matmul, x, w, offsets, order.value_or(Tensor()), x.size(0), w.sizes(), {x.size(0), w.size(1)});
 }
 
 Tensor int8_linear(const Tensor &x, const Tensor &w, const Tensor &w_scale) {
+    no_tangents("int8_linear", {x, w_scale});
     const c10::DeviceGuard guard(x.device());
     const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
     Tensor y = empty(x, {M, N}, x.scalar_type());

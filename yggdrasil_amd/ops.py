@@ -9,7 +9,7 @@ The kernels are those of csrc/ygg_logprobs.hip, csrc/ygg_experts.hip and csrc/yg
 include/ygg_hip.h, on the current torch stream of the tensors' device (csrc/ygg_torch.cpp: allocation, the call, autograd).
 Nothing waits for the GPU, so a call can be captured into a graph; values that only the GPU holds (tokens, offsets, an order)
 are not checked here, and bad ones give wrong or NaN values, never an access out of bounds. Types: float32, bfloat16 and
-float16.
+float16. Derivatives are first ones in reverse mode: second ones and forward-mode tangents are refused.
 """
 from __future__ import annotations
 
