@@ -412,3 +412,20 @@ def test_forward_mode_derivatives_are_refused():
         y = ops.grouped_matmul(xg, w, offsets)
         with pytest.raises(RuntimeError, match="forward"):
             torch.autograd.grad(y, xg, fwd.make_dual(dy, dy))
+
+
+def test_group_rows_takes_no_leaf_modulo_32_bits():
+    """int64 leaves outside int32 belong to no expert, as others outside the range."""
+    from yggdrasil_amd import ops
+    leaves = torch.tensor([2 ** 32 + 1, 1, -2 ** 32, 0, 2 ** 31, -2 ** 63, 2 ** 63 - 1, 2, 2 ** 40 + 2, -2 ** 31 - 1], device="cuda")
+    offsets, order = ops.group_rows(leaves, 3)
+    assert offsets.tolist() == [0, 1, 2, 3] and order.tolist() == [3, 1, 7, 0, 2, 4, 5, 6, 8, 9]
+    x, w = torch.randn(10, 16, device="cuda"), torch.randn(3, 8, 16, device="cuda", requires_grad=True)
+    y = ops.grouped_matmul(x, w, offsets, order)
+    none = [0, 2, 4, 5, 6, 8, 9]
+    assert (y[none] == 0).all() and (y[[1, 3, 7]] != 0).all()
+    x2 = x.clone()
+    x2[none] = 0
+    want, = torch.autograd.grad(ops.grouped_matmul(x2, w, offsets, order).sum(), w)
+    got, = torch.autograd.grad(y.sum(), w)
+    assert torch.equal(got, want)

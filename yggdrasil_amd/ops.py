@@ -128,8 +128,8 @@ def group_rows(leaves, n_experts: int):
         raise ValueError("leaves must be an int32 or int64 tensor on a ROCm device")
     if not 1 <= n_experts <= MOST_EXPERTS:
         raise ValueError(f"n_experts {n_experts}: 1 to {MOST_EXPERTS}")
-    x = leaves.reshape(-1).to(torch.int32)
-    x = torch.where((x >= 0) & (x < n_experts), x, n_experts)
+    x = leaves.reshape(-1)
+    x = torch.where((x >= 0) & (x < n_experts), x, n_experts).to(torch.int32)      # in this order: int64 ones may not fit
     by, order = torch.sort(x, stable=True)
     ends = torch.arange(n_experts + 1, dtype=torch.int32, device=x.device)
     return torch.searchsorted(by, ends, out_int32=True), order.to(torch.int32)
