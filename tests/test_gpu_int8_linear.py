@@ -192,3 +192,15 @@ def test_forward_mode_derivatives_are_refused():
         for a, s in ((fwd.make_dual(x, x), ws), (x, fwd.make_dual(ws, ws)), (fwd.make_dual(x, x).reshape(2, 2, 8), ws)):
             with pytest.raises((RuntimeError, ValueError), match="forward"), torch.no_grad():
                 ops.int8_linear(a, w, s)
+
+
+def test_no_gradient_of_the_scales():
+    """As for x: refused where it would be asked for."""
+    from yggdrasil_amd import ops
+    x, w, ws = make(4, 6, 8, torch.float32)
+    want = ops.int8_linear(x, w, ws)
+    for s in (ws.clone().requires_grad_(), torch.nn.Parameter(ws.clone())):
+        with pytest.raises(ValueError, match="gradient"):
+            ops.int8_linear(x, w, s)
+        with torch.no_grad():
+            assert torch.equal(ops.int8_linear(x, w, s), want)

@@ -217,8 +217,9 @@ Maybe plain_grouped_matmul(const Tensor &x, const Tensor &w, const Tensor &offse
     return grouped_matmul(x, w, offsets, order);
 }
 Maybe plain_int8_linear(const Tensor &x, const Tensor &w, const Tensor &w_scale) {
-    if (!floats(x, 2) || (x.requires_grad() && at::GradMode::is_enabled()) || !like(w, x, at::kChar, 2) || w.size(1) != x.size(1) ||
-        x.size(0) > YGG_MOST_ROWS || !within(w.size(0), 1, YGG_MOST_VOCAB) || !within(w.size(1), 1, YGG_MOST_INNER) ||
+    if (!floats(x, 2) || ((x.requires_grad() || w_scale.requires_grad()) && at::GradMode::is_enabled()) ||
+        !like(w, x, at::kChar, 2) || w.size(1) != x.size(1) || x.size(0) > YGG_MOST_ROWS ||
+        !within(w.size(0), 1, YGG_MOST_VOCAB) || !within(w.size(1), 1, YGG_MOST_INNER) ||
         !like(w_scale, x, at::kFloat, 1) || w_scale.size(0) != w.size(0))
         return std::nullopt;
     return int8_linear(x, w, w_scale);

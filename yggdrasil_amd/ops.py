@@ -195,6 +195,8 @@ def int8_linear(x, w, w_scale) -> torch.Tensor:
         raise ValueError(f"w of shape {tuple(w.shape)}, expected (N, {K})")
     N = w.shape[0]
     _on(w_scale, x.device, "w_scale", (torch.float32,), (N,))
+    if w_scale.requires_grad and torch.is_grad_enabled():
+        raise ValueError("int8_linear has no gradient: call it under torch.no_grad() or with w_scale.detach()")
     x2 = x if x.dim() == 2 else x.reshape(-1, K)
     M = x2.shape[0]
     if M > MOST_ROWS or not 1 <= N <= MOST_VOCAB or not 1 <= K <= MOST_INNER:
