@@ -297,10 +297,10 @@ __device__ __forceinline__ Rsrc rsrc_of(const void *p, uint32_t bytes) {
 }
 constexpr uint32_t kFar = 0x80000000u;   // past every descriptor's size
 // 16 bytes a lane to LDS from `lds` on (a wave's number: the same for all its lanes), lane after lane. The load has no output
-// registers; the caller waits for it.
+// registers; the caller waits for it. It takes the LDS address in m0: as an operand, so that the compiler knows what m0 holds.
 __device__ __forceinline__ void load_lds(Rsrc r, uint32_t offset, uint32_t lds) {
     lds = __builtin_amdgcn_readfirstlane((int)lds);
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(r), "s"(lds) : "memory");
+    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(r), "{m0}"(lds) : "memory");
 }
 template <int kCount> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kCount) : "memory"); }
 __device__ __forceinline__ void turn_over() {
