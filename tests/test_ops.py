@@ -114,3 +114,29 @@ def test_native_errors_are_raised():
     with pytest.raises(RuntimeError, match="NULL|type|outside"):
         ops._native()
         _lib.check(_lib.lib().ygg_int8_linear(None, 7, None, None, 1, 1, 1, None, None, 0, None))
+
+
+@pytest.mark.gpu
+def test_the_torch_part_raises_the_librarys_errors():
+    """Sizes that ops.py would refuse, given to the torch part itself: the library refuses them and its message is raised. No
+    kernel runs."""
+    m = ops._native()
+    x, w = torch.zeros(2, ops.MOST_INNER + 1, device="cuda"), torch.zeros(3, ops.MOST_INNER + 1, dtype=torch.int8, device="cuda")
+    with pytest.raises(RuntimeError, match=r"K 131073 outside \[1, 131072\] \(error 5\)"):
+        m.int8_linear(x, w, torch.ones(3, device="cuda"))
+    with pytest.raises(RuntimeError, match=r"top 65 outside \[0, 64\] \(error 5\)"):
+        m.token_logprobs(torch.zeros(2, 100, device="cuda"), None, 65)
+    off = torch.zeros(2, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match=r"K 131073 outside \[1, 131072\] \(error 5\)"):
+        m.grouped_matmul(x, torch.zeros(1, 1, ops.MOST_INNER + 1, device="cuda"), off, None)
+
+
+def test_the_limits_are_the_headers():
+    import re
+    from pathlib import Path
+    text = (Path(__file__).resolve().parents[1] / "include" / "ygg_hip.h").read_text()
+    names = re.findall(r"YGG_(MOST_[A-Z]+) = ([0-9 <]+)", text)
+    assert len(names) == 5
+    for name, value in names:
+        a = [int(v) for v in value.split("<<")]
+        assert getattr(ops, name) == (a[0] if len(a) == 1 else a[0] << a[1]), name
