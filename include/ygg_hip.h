@@ -251,6 +251,7 @@ void ygg_float_free(ygg_fmodel *m);
 /* ---- Operators of an output head (no counterpart in the reference, whose step holds them inside): the products of
    routed experts, an int8 projection of float rows, and the log-probabilities of given tokens, with the gradients a
    training step takes. They run on the caller's current device and stream, wait for nothing and allocate nothing.
+   Any number of rows of logits; products whose sizes make more tiles than a launch takes (2^32 threads) are refused.
    type: 0 f32, 1 bf16, 2 f16. Sums, maxima and softmax statistics are held in 32 bits; an output is rounded once. ---- */
 enum {
     YGG_MOST_TOP = 64,             /* alternatives of a row */

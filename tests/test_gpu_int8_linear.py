@@ -204,3 +204,12 @@ def test_no_gradient_of_the_scales():
             ops.int8_linear(x, w, s)
         with torch.no_grad():
             assert torch.equal(ops.int8_linear(x, w, s), want)
+
+
+def test_as_many_rows_as_a_call_takes():
+    """2^24 rows: their scales and integers come from two launches."""
+    from yggdrasil_amd import ops
+    M, N, K = 1 << 24, 2, 16
+    x, w, ws = make(1 << 12, N, K, torch.float16)
+    y = ops.int8_linear(x.repeat(M >> 12, 1), w, ws)
+    assert torch.equal(y.view(-1, 1 << 12, N), check(x, w, ws).expand(M >> 12, 1 << 12, N))

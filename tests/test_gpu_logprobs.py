@@ -493,3 +493,23 @@ def test_forward_mode_derivatives_are_refused():
               lambda: torch.func.vmap(lambda v: ops.token_logprobs(v).entropy)(x)):
         with pytest.raises(RuntimeError):           # transforms of torch.func hold no tensor that a kernel could read
             f()
+
+
+def test_more_rows_than_a_launch_takes():
+    """2^26 rows of 64 lanes are 2^32 threads: the last ones come from a second launch."""
+    from yggdrasil_amd import ops
+    n, V, top = (1 << 26) + 1000, 17, 9
+    x = torch.randn(1 << 12, V, device="cuda", generator=torch.Generator("cuda").manual_seed(0)).bfloat16()
+    x = x.repeat((n >> 12) + 1, 1)[:n]
+    t = torch.arange(n, dtype=torch.int32, device="cuda") % V
+    x[-1], x[-2, 3], t[-3] = -INF, math.nan, -1
+    r = ops.token_logprobs(x, t, top=top)
+    for at in (slice(0, 3000), slice((1 << 26) - 3000, (1 << 26) + 3000), slice(n - 3000, n)):
+        check(x[at], t[at], top)
+        want = ops.token_logprobs(x[at], t[at], top=top)
+        assert all(torch.equal(a[at].nan_to_num(7.0), b.nan_to_num(7.0)) for a, b in zip(r, want))
+    # every row: the pattern comes again after 2^12 rows, the targets after V
+    whole = ops.token_logprobs(x[:1 << 12], top=top)
+    most = n >> 12 << 12
+    assert bool((r.entropy[:most].view(-1, 1 << 12) == whole.entropy).all())
+    assert bool((r.top_ids[:most].view(-1, 1 << 12, top) == whole.top_ids).all())

@@ -140,3 +140,15 @@ def test_the_limits_are_the_headers():
     for name, value in names:
         a = [int(v) for v in value.split("<<")]
         assert getattr(ops, name) == (a[0] if len(a) == 1 else a[0] << a[1]), name
+
+
+@pytest.mark.parametrize("entry, N, K", [("ygg_grouped_matmul", 2048, 8), ("ygg_grouped_matmul", 1 << 17, 1 << 17),
+                                         ("ygg_grouped_grad_x", 8, 8192), ("ygg_grouped_grad_w", 8, 2048),
+                                         ("ygg_grouped_grad_w", 1 << 17, 1 << 17)])
+@pytest.mark.parametrize("type", [0, 1, 2])
+def test_more_tiles_than_a_launch_takes(entry, N, K, type):
+    """A launch holds less than 2^32 threads: sizes within the limits that make more are refused as arguments, not by the
+    device."""
+    L = _lib.lib()
+    assert getattr(L, entry)(P, P, type, P, None, 1 << 21, 1 << 20, N, K, P, None) == 5
+    assert b"launch takes" in L.ygg_last_error()

@@ -1212,6 +1212,12 @@ int ygg_step(const ygg_model *m, const int32_t *d_tokens, const int8_t *d_state_
 
 static const char *const kTypeHelp = "type %d: 0 f32, 1 bf16, 2 f16";
 static const char *const kOpLimits = "%s %lld outside [%d, %d]";
+#define OP_TRY(expr)                                                                                              \
+    do {                                                                                                          \
+        hipError_t e_ = (expr);                                                                                   \
+        if (e_ == ygg::kTooLarge) return fail(YGG_ERR_ARG, "more workgroups than a launch takes (2^32 threads)"); \
+        if (e_ != hipSuccess) return fail(YGG_ERR_DEVICE, "%s: %s", #expr, hipGetErrorString(e_));                \
+    } while (0)
 
 int64_t ygg_logprobs_scratch(int type, int64_t rows, int V, int top) {
     if (type < 0 || type > 2 || rows < 1 || V < 1 || top < 0 || top > YGG_MOST_TOP) return 0;
@@ -1236,7 +1242,7 @@ int ygg_logprobs(const void *d_logits, int type, int64_t rows, int V, int64_t st
         return fail(YGG_ERR_ARG, "scratch of %lld bytes, %lld wanted", (long long)scratch_bytes, (long long)need);
     const ygg::LogprobsArgs a = {d_logits, rows, stride, V, top, target_bytes, d_targets, d_logp, d_entropy, d_top_logp,
                                  d_top_ids, (float2 *)d_stats};
-    HIP_TRY(ygg::launch_logprobs(type, a, d_scratch, (hipStream_t)stream));
+    OP_TRY(ygg::launch_logprobs(type, a, d_scratch, (hipStream_t)stream));
     return YGG_OK;
 }
 
@@ -1254,7 +1260,7 @@ int ygg_logprobs_grad(const void *d_logits, int type, int64_t rows, int V, int64
         return fail(YGG_ERR_ARG, "NULL buffer");
     const ygg::LogprobsGradArgs a = {d_logits, rows, stride, V, top, target_bytes, d_targets, d_entropy, d_top_ids,
                                      (const float2 *)d_stats, d_g_logp, d_g_entropy, top ? d_g_top : nullptr, d_out};
-    HIP_TRY(ygg::launch_logprobs_grad(type, a, (hipStream_t)stream));
+    OP_TRY(ygg::launch_logprobs_grad(type, a, (hipStream_t)stream));
     return YGG_OK;
 }
 
@@ -1274,7 +1280,7 @@ int ygg_grouped_matmul(const void *d_x, const void *d_w, int type, const int32_t
     if (int rc = check_grouped(type, d_offsets, M, E, N, K)) return rc;
     if (M == 0) return YGG_OK;
     if (!d_x || !d_w || !d_y) return fail(YGG_ERR_ARG, "NULL buffer");
-    HIP_TRY(ygg::launch_grouped_matmul(type, d_x, d_w, {d_offsets, d_order, M, E}, N, K, d_y, (hipStream_t)stream));
+    OP_TRY(ygg::launch_grouped_matmul(type, d_x, d_w, {d_offsets, d_order, M, E}, N, K, d_y, (hipStream_t)stream));
     return YGG_OK;
 }
 
@@ -1283,7 +1289,7 @@ int ygg_grouped_grad_x(const void *d_dy, const void *d_w, int type, const int32_
     if (int rc = check_grouped(type, d_offsets, M, E, N, K)) return rc;
     if (M == 0) return YGG_OK;
     if (!d_dy || !d_w || !d_dx) return fail(YGG_ERR_ARG, "NULL buffer");
-    HIP_TRY(ygg::launch_grouped_grad_x(type, d_dy, d_w, {d_offsets, d_order, M, E}, N, K, d_dx, (hipStream_t)stream));
+    OP_TRY(ygg::launch_grouped_grad_x(type, d_dy, d_w, {d_offsets, d_order, M, E}, N, K, d_dx, (hipStream_t)stream));
     return YGG_OK;
 }
 
@@ -1291,7 +1297,7 @@ int ygg_grouped_grad_w(const void *d_dy, const void *d_x, int type, const int32_
                        int E, int N, int K, void *d_dw, void *stream) {
     if (int rc = check_grouped(type, d_offsets, M, E, N, K)) return rc;
     if (!d_dw || (M > 0 && (!d_dy || !d_x))) return fail(YGG_ERR_ARG, "NULL buffer");
-    HIP_TRY(ygg::launch_grouped_grad_w(type, d_dy, d_x, {d_offsets, d_order, M, E}, N, K, d_dw, (hipStream_t)stream));
+    OP_TRY(ygg::launch_grouped_grad_w(type, d_dy, d_x, {d_offsets, d_order, M, E}, N, K, d_dw, (hipStream_t)stream));
     return YGG_OK;
 }
 
@@ -1311,7 +1317,7 @@ int ygg_int8_linear(const void *d_x, int type, const int8_t *d_w, const float *d
     const int64_t need = ygg::int8_scratch(M, N, K);
     if (need && (!d_scratch || scratch_bytes < need))
         return fail(YGG_ERR_ARG, "scratch of %lld bytes, %lld wanted", (long long)scratch_bytes, (long long)need);
-    HIP_TRY(ygg::launch_int8_linear(type, d_x, d_w, d_w_scale, M, N, K, d_y, d_scratch, (hipStream_t)stream));
+    OP_TRY(ygg::launch_int8_linear(type, d_x, d_w, d_w_scale, M, N, K, d_y, d_scratch, (hipStream_t)stream));
     return YGG_OK;
 }
 

@@ -453,7 +453,7 @@ hipError_t go_rows(const void *in, const void *w, const Groups &g, int O, int R,
         const int cols = (O + 255) / 256;
         const int64_t rows = (int64_t)g.M / 256 + g.E + 2;
         if (aligned16(in, in_row) && aligned16(w, w_row) && g.M * in_row < kMostBytes && O * in_row < kMostBytes &&
-            g.M >= 128 * (int64_t)g.E && (rows - g.E / 2) * cols >= 256 && rows * cols <= INT32_MAX) {
+            g.M >= 128 * (int64_t)g.E && (rows - g.E / 2) * cols >= 256 && rows * cols <= most_blocks(512)) {
             hipLaunchKernelGGL((rows_turn_kernel<T, 8, 4, 2, 4, TR>), dim3((unsigned)(rows * cols)), dim3(512), 0, st,
                                (const T *)in, (const T *)w, g, O, R, (T *)out, cols, 16);
             return hipGetLastError();
@@ -463,7 +463,7 @@ hipError_t go_rows(const void *in, const void *w, const Groups &g, int O, int R,
         constexpr int FI = decltype(fi)::value, WI = decltype(wi)::value, WO = decltype(wo)::value, kI = 16 * FI * WI, kO = 64 * WO;
         const int cols = (O + kO - 1) / kO;
         const int64_t slots = (int64_t)g.M / kI + g.E + 2, rows = std::min<int64_t>(slots, g.M);
-        if (rows * cols > INT32_MAX) return hipErrorInvalidValue;
+        if (rows * cols > most_blocks(64 * WI * WO)) return kTooLarge;
         hipLaunchKernelGGL((rows_kernel<T, FI, 4, WI, WO, TR>), dim3((unsigned)(rows * cols)), dim3(64 * WI * WO), 0, st,
                            (const T *)in, (const T *)w, g, O, R, (T *)out, cols, 16, slots > g.M);
         return hipGetLastError();
@@ -491,7 +491,7 @@ hipError_t go_rows(const void *in, const void *w, const Groups &g, int O, int R,
             if (!small && !(aligned16(in, in_row) && aligned16(w, w_row)) && (int64_t)g.M * ((O + 63) / 64) >= 256) return tiles(one, one, one);
             const int cols = (O + 15) / 16;
             const int64_t slots = (int64_t)g.M / 16 + g.E + 2, rows = std::min<int64_t>(slots, g.M);
-            if (rows * cols > INT32_MAX) return hipErrorInvalidValue;
+            if (rows * cols > most_blocks(in_row <= 1024 ? 64 : 256)) return kTooLarge;
             if (in_row <= 1024)
                 hipLaunchKernelGGL((few_rows_kernel<T, 1>), dim3((unsigned)(rows * cols)), dim3(64), 0, st, (const T *)in,
                                    (const T *)w, g, O, R, (T *)out, cols, slots > g.M);
@@ -519,7 +519,7 @@ hipError_t go_grad_w(const void *dy, const void *x, const Groups &g, int N, int 
         const int tn = (N + 255) / 256, tk = (K + 255) / 256;
         const int64_t tiles = (int64_t)g.E * tn * tk, dy_row = (int64_t)N * sizeof(T), x_row = (int64_t)K * sizeof(T);
         if (aligned16(dy, dy_row) && aligned16(x, x_row) && g.M * dy_row < kMostBytes && g.M * x_row < kMostBytes &&
-            tiles >= 256 && tiles <= INT32_MAX && N >= 192 && K >= 192) {
+            tiles >= 256 && tiles <= most_blocks(512) && N >= 192 && K >= 192) {
             hipLaunchKernelGGL((grad_w_turn_kernel<T, 8, 4, 2, 4>), dim3((unsigned)tiles), dim3(512), 0, st, (const T *)dy,
                                (const T *)x, g, N, K, (T *)dw, tn, tk);
             return hipGetLastError();
@@ -532,7 +532,7 @@ hipError_t go_grad_w(const void *dy, const void *x, const Groups &g, int N, int 
             const int tn = (N + 16 * FN - 1) / (16 * FN), tk = (K + 63) / 64;
             const int64_t early = g.M >= kLong ? ((int64_t)g.M / kLong + 1) * ((N + 15) / 16) * tk : 0;
             const int64_t tiles = (int64_t)g.E * tn * tk + early;
-            if (tiles > INT32_MAX) return hipErrorInvalidValue;
+            if (tiles > most_blocks(256)) return kTooLarge;
             hipLaunchKernelGGL((grad_w_small_kernel<T, FN>), dim3((unsigned)tiles), dim3(256), 0, st, (const T *)dy, (const T *)x, g, N,
                                K, (T *)dw, tk, (int)early);
             return hipGetLastError();
@@ -543,7 +543,7 @@ hipError_t go_grad_w(const void *dy, const void *x, const Groups &g, int N, int 
         constexpr int FI = decltype(fi)::value, WI = decltype(wi)::value, WO = decltype(wo)::value, kI = 16 * FI * WI, kO = 64 * WO;
         const int tn = (N + kI - 1) / kI, tk = (K + kO - 1) / kO;
         const int64_t tiles = (int64_t)g.E * tn * tk;
-        if (tiles > INT32_MAX) return hipErrorInvalidValue;
+        if (tiles > most_blocks(64 * WI * WO)) return kTooLarge;
         hipLaunchKernelGGL((grad_w_kernel<T, FI, 4, WI, WO>), dim3((unsigned)tiles), dim3(64 * WI * WO), 0, st, (const T *)dy,
                            (const T *)x, g, N, K, (T *)dw, tn, tk);
         return hipGetLastError();

@@ -2,6 +2,9 @@
 // q = x / s_i rounded to nearest with ties to even, and multiplied by an int8 matrix with a scale for each of its rows,
 // y_in = (sum_k q_ik w_nk) ws_n s_i (multiplied in this order: a row's scale may be near the ends of f32's range). The
 // integer sums are exact in 32 bits (K <= 131072). A row with a NaN or an infinity has a NaN scale, so it is NaN throughout.
+#include <algorithm>
+
+#include "../../include/ygg_hip.h"
 #include "ygg_gemm.h"
 #include "ygg_ops.h"
 
@@ -241,14 +244,17 @@ hipError_t go(const void *x, const int8_t *w, const float *ws, int M, int N, int
         constexpr int FI = decltype(fi)::value;
         const int cols = (N + 15) / 16;
         const int64_t tiles = (int64_t)((M + 16 * FI - 1) / (16 * FI)) * cols;
-        if (tiles > INT32_MAX) return hipErrorInvalidValue;
+        if (tiles > most_blocks(256)) return kTooLarge;
         hipLaunchKernelGGL((few_int8_kernel<T, FI, decltype(fused)::value>), dim3((unsigned)tiles), dim3(256), 0, st, (const T *)x,
                            q, scale, w, ws, M, N, K, padded(K), (T *)y, cols);
         return hipGetLastError();
     };
     using std::integral_constant;
     if (K >= 16 && fits_fused<T>(M, K)) return few(integral_constant<int, 1>(), std::true_type());
-    hipLaunchKernelGGL(quantize_kernel<T>, dim3(M), dim3(256), 0, st, (const T *)x, K, padded(K), q, scale);
+    const int half = YGG_MOST_ROWS / 2;     // 2^32 threads are too many for a launch
+    for (int i = 0; i < M; i += half)
+        hipLaunchKernelGGL(quantize_kernel<T>, dim3(std::min(M - i, half)), dim3(256), 0, st, (const T *)x + (int64_t)i * K, K,
+                           padded(K), q + (int64_t)i * padded(K), scale + i);
     // w is read once for 16 or 32 rows, by four waves a workgroup; more rows, or a short K, go by tiles (8192 x 4096: 16 rows
     // 10 us for 20, 32 rows 14 for 20, 64 rows 25 for 21), but where there are few of those (77 rows, 1000 x 4096: 8 for 17)
     const int64_t tiles64 = (int64_t)((M + 63) / 64) * ((N + 63) / 64);
@@ -257,7 +263,7 @@ hipError_t go(const void *x, const int8_t *w, const float *ws, int M, int N, int
     // tiles of 256 x 256 straight to LDS where there are enough of them: 8192 x 4096 x 8192 228 us against 424
     const int64_t big = (int64_t)((M + 255) / 256) * ((N + 255) / 256);
     if (K % 16 == 0 && (uintptr_t)w % 16 == 0 && (int64_t)M * padded(K) < 0x78000000 && (int64_t)N * K < 0x78000000 && big >= 256 &&
-        big <= INT32_MAX) {
+        big <= most_blocks(512)) {
         hipLaunchKernelGGL((int8_turn_kernel<T, 8, 4, 2, 4>), dim3((unsigned)big), dim3(512), 0, st, q, scale, w, ws, M, N, K,
                            padded(K), (T *)y, (N + 255) / 256, 16);
         return hipGetLastError();
@@ -266,7 +272,7 @@ hipError_t go(const void *x, const int8_t *w, const float *ws, int M, int N, int
         constexpr int FI = decltype(fi)::value, WO = decltype(wo)::value, kI = 32 * FI, kO = 64 * WO;
         const int cols = (N + kO - 1) / kO;
         const int64_t tiles = (int64_t)((M + kI - 1) / kI) * cols;
-        if (tiles > INT32_MAX) return hipErrorInvalidValue;
+        if (tiles > most_blocks(128 * WO)) return kTooLarge;
         hipLaunchKernelGGL((int8_kernel<T, FI, 4, 2, WO>), dim3((unsigned)tiles), dim3(128 * WO), 0, st, q, scale, w, ws, M, N, K,
                            padded(K), (T *)y, cols, 16);
         return hipGetLastError();

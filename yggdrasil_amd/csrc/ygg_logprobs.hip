@@ -583,14 +583,41 @@ int parts_of(int64_t rows, int V) {
     return (int)(want < most ? want < 64 ? want : 64 : most < 64 ? most : 64);
 }
 
+// the arguments from row n on
+template <class P> void move_on(P *&p, int64_t n) {
+    if (p) p += n;
+}
+void move_on(const void *&p, int64_t bytes) { p = p ? (const char *)p + bytes : p; }
+void skip_rows(LogprobsArgs &a, int64_t n, int size) {
+    move_on(a.x, n * a.stride * size), move_on(a.targets, n * a.target_bytes);
+    move_on(a.logp, n), move_on(a.entropy, n), move_on(a.stats, n);
+    move_on(a.top_logp, n * a.top), move_on(a.top_ids, n * a.top);
+}
+void skip_rows(LogprobsGradArgs &a, int64_t n, int size) {
+    move_on(a.x, n * a.stride * size), move_on(a.targets, n * a.target_bytes);
+    move_on(a.entropy, n), move_on(a.stats, n), move_on(a.top_ids, n * a.top);
+    move_on(a.g_logp, n), move_on(a.g_entropy, n), move_on(a.g_top, n * a.top);
+    a.dx = (char *)a.dx + n * a.V * size;
+}
+// launch(a) for up to `most` rows at a time: what one launch takes
+template <class T, class A, class F> hipError_t by_rows(A a, int64_t most, F launch) {
+    const int64_t rows = a.rows;
+    for (int64_t done = 0; done < rows; done += most) {
+        a.rows = rows - done < most ? rows - done : most;
+        launch(a);
+        if (hipError_t e = hipGetLastError()) return e;
+        skip_rows(a, most, sizeof(T));
+    }
+    return hipSuccess;
+}
+
 template <class T> hipError_t go(const LogprobsArgs &a, void *scratch, hipStream_t st) {
     constexpr int kC = 16 / sizeof(T);
     auto narrow = [&](auto g, auto u) {
-        constexpr int kG = decltype(g)::value, kU = decltype(u)::value;
-        const int64_t blocks = (a.rows + 256 / kG - 1) / (256 / kG);
-        if (blocks > INT32_MAX) return hipErrorInvalidValue;
-        hipLaunchKernelGGL((narrow_kernel<T, kG, kU>), dim3((unsigned)blocks), dim3(256), 0, st, a);
-        return hipGetLastError();
+        constexpr int kG = decltype(g)::value, kU = decltype(u)::value, kRows = 256 / kG;
+        return by_rows<T>(a, most_blocks(256) * kRows, [&](const LogprobsArgs &b) {
+            hipLaunchKernelGGL((narrow_kernel<T, kG, kU>), dim3((unsigned)((b.rows + kRows - 1) / kRows)), dim3(256), 0, st, b);
+        });
     };
     using std::integral_constant;
     // 16 lanes hold 8 alternatives with room for as many more that reach the bound, or all of 16 classes
@@ -607,14 +634,15 @@ template <class T> hipError_t go(const LogprobsArgs &a, void *scratch, hipStream
     w.width = ((a.V + w.parts - 1) / w.parts + kC - 1) / kC * kC;
     w.sums = (float4 *)scratch;
     w.keys = (uint64_t *)((char *)scratch + (a.rows * w.parts * 16 + 255) / 256 * 256);
-    if (a.rows * w.parts > INT32_MAX) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)(a.rows * w.parts)), block(256);
+    const dim3 block(256);
     if (w.parts == 1) {
-        hipLaunchKernelGGL((wide_kernel<T, 4>), grid, block, 0, st, a, w);
-    } else {
-        hipLaunchKernelGGL((wide_kernel<T, 16 / kC>), grid, block, 0, st, a, w);     // 4096 entries at a time: a part
-        hipLaunchKernelGGL(wide_join_kernel<T>, dim3((unsigned)a.rows), block, 0, st, a, w);
+        return by_rows<T>(a, most_blocks(256), [&](const LogprobsArgs &b) {
+            hipLaunchKernelGGL((wide_kernel<T, 4>), dim3((unsigned)b.rows), block, 0, st, b, w);
+        });
     }
+    // fewer than 1024 rows; 4096 entries at a time: a part
+    hipLaunchKernelGGL((wide_kernel<T, 16 / kC>), dim3((unsigned)(a.rows * w.parts)), block, 0, st, a, w);
+    hipLaunchKernelGGL(wide_join_kernel<T>, dim3((unsigned)a.rows), block, 0, st, a, w);
     return hipGetLastError();
 }
 
@@ -624,10 +652,10 @@ template <class T> hipError_t go_grad(const LogprobsGradArgs &a, hipStream_t st)
     int shift = 0;
     while (shift < 8 && (kU << shift) < pieces) shift++;
     const int blocks = shift < 8 ? 1 : (pieces + kU * 256 - 1) / (kU * 256);
-    const int64_t grid = ((a.rows + (1 << (8 - shift)) - 1) >> (8 - shift)) * blocks;
-    if (grid > INT32_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((grad_kernel<T, kU>), dim3((unsigned)grid), dim3(256), 0, st, a, shift, blocks);
-    return hipGetLastError();
+    return by_rows<T>(a, most_blocks(256) / blocks << (8 - shift), [&](const LogprobsGradArgs &b) {
+        const int64_t grid = ((b.rows + (1 << (8 - shift)) - 1) >> (8 - shift)) * blocks;
+        hipLaunchKernelGGL((grad_kernel<T, kU>), dim3((unsigned)grid), dim3(256), 0, st, b, shift, blocks);
+    });
 }
 
 }  // namespace

@@ -11,6 +11,11 @@ inline int op_bytes(int type) { return type == kOpF32 ? 4 : 2; }
 
 constexpr int kMostTop = 64;   // most alternatives of a row
 
+// Workgroups that a launch takes: it holds less than 2^32 threads along a dimension. Rows of logits past that go in several
+// launches, a product's sizes that make more are refused with kTooLarge (HIP's own answer to such a launch).
+constexpr int64_t most_blocks(int threads) { return UINT32_MAX / (uint32_t)threads; }
+constexpr hipError_t kTooLarge = hipErrorInvalidConfiguration;
+
 struct LogprobsArgs {
     const void *x;             // rows of V logits, `stride` values apart
     int64_t rows, stride;
