@@ -143,3 +143,31 @@ def test_host_api_errors(tmp_path):
         Yggdrasil.load("model.bin", backend="jax")
     with pytest.raises(FileNotFoundError):
         Yggdrasil.load(tmp_path / "none.bin")
+
+
+@pytest.mark.parametrize("lacks, word", [("torch", "no torch"), ("rocm", "without ROCm"), ("g++", "no g++"), ("", "")])
+def test_the_library_builds_without_what_the_torch_part_takes(monkeypatch, capsys, lacks, word):
+    """`python -m yggdrasil_amd.build` where torch or g++ is absent: the library, and a word on what is left out."""
+    import sys
+
+    import torch
+    from yggdrasil_amd import build
+    built = []
+    monkeypatch.setattr(sys, "argv", ["build"])
+    monkeypatch.setattr(build, "build_library", lambda verbose=False: built.append("library"))
+    if lacks:
+        run = build._run
+        monkeypatch.setattr(build, "_run", lambda cmd, cwd=None: run(["false"]) if lacks == "g++" else run(cmd, cwd))
+    else:
+        monkeypatch.setattr(build, "build_torch", lambda verbose=False: built.append("torch"))
+    if lacks == "torch":
+        monkeypatch.setitem(sys.modules, "torch", None)
+    elif lacks == "rocm":
+        monkeypatch.setattr(torch.version, "hip", None)
+        monkeypatch.setattr(build, "build_torch", lambda verbose=False: built.append("torch"))
+    elif lacks == "g++":
+        monkeypatch.setattr(build.shutil, "which", lambda name: None)
+    build.main()
+    out = capsys.readouterr().out
+    assert built == (["library"] if lacks else ["library", "torch"])
+    assert (word in out and "not built" in out) if lacks else "not built" not in out

@@ -1,7 +1,7 @@
 """Build the gfx950 library (libygg_hip.so, in this package directory), the operators on torch tensors and, for the tests, the
 CPU oracle.
 
-    python -m yggdrasil_amd.build            # the HIP library and the operators' torch part
+    python -m yggdrasil_amd.build            # the HIP library and, where torch and g++ are, the operators' torch part
     python -m yggdrasil_amd.build --oracle   # also oracle/libygg_oracle.so and, where /root/reference exists,
                                              # the reference kernel in oracle/_ref/
 
@@ -70,6 +70,17 @@ def build_library(verbose: bool = False) -> Path:
     return LIB
 
 
+def torch_part_missing() -> str:
+    """What build_torch needs and this machine lacks, or "": the library itself takes neither."""
+    try:
+        import torch
+    except ImportError:
+        return "no torch"
+    if torch.version.hip is None:
+        return "a torch without ROCm"
+    return "" if shutil.which("g++") else "no g++"
+
+
 def build_torch(verbose: bool = False) -> Path:
     """The operators on torch tensors (csrc/ygg_torch.cpp, host code): _ygg_torch in this package directory."""
     import sysconfig
@@ -101,7 +112,11 @@ def main():
     ap.add_argument("--oracle", action="store_true")
     a = ap.parse_args()
     build_library(verbose=True)
-    build_torch(verbose=True)
+    why = torch_part_missing()
+    if why:
+        print(f"not built: the operators' torch part ({why}); the library has their C-ABI all the same")
+    else:
+        build_torch(verbose=True)
     if a.oracle:
         build_oracle(verbose=True)
 
