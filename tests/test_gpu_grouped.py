@@ -429,3 +429,24 @@ def test_group_rows_takes_no_leaf_modulo_32_bits():
     want, = torch.autograd.grad(ops.grouped_matmul(x2, w, offsets, order).sum(), w)
     got, = torch.autograd.grad(y.sum(), w)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("M, E, dtype", [(7, 5, torch.int32), (4096, 16384, torch.int32), (16001, 64, torch.int64),
+                                         (65536, 1024, torch.int32)])
+def test_group_rows_in_graphs(M, E, dtype):
+    """Every replay, with eager work and synchronizations between them, equals the eager call."""
+    from yggdrasil_amd import ops
+    leaves = torch.randint(E, (M,), device="cuda", dtype=dtype)
+    ops.group_rows(leaves, E)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        offsets, order = ops.group_rows(leaves, E)
+    for k in range(5):
+        now = torch.randint(-2, E + 2, (M,), device="cuda", dtype=dtype)
+        leaves.copy_(now)
+        g.replay()
+        torch.cuda.synchronize()
+        want = ops.group_rows(now, E)
+        torch.cuda.synchronize()
+        assert torch.equal(offsets, want[0]) and torch.equal(order, want[1]), k
