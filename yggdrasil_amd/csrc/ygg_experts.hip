@@ -445,7 +445,8 @@ bool aligned16(const void *p, int64_t row_bytes) { return (uintptr_t)p % 16 == 0
 constexpr int64_t kMostBytes = 0x78000000;   // of an operand with 32-bit offsets: kFar and a few steps stay past it
 
 // Tiles of 256 x 256 straight to LDS pay where an expert's rows fill half of one and there are tiles for the 256 CUs: on
-// 16384 x 4096 x 4096 f16 over 8 experts 416 us against 655 of the 128 x 128 tiles through registers, which take the rest.
+// 16384 x 4096 x 4096 f16 over 8 experts 502 us a call against 692 with the 128 x 128 tiles through registers, which take the
+// rest (a quarter of the rows go to two of the experts, the others anywhere; even loads 532 against 704).
 template <class T, bool TR>
 hipError_t go_rows(const void *in, const void *w, const Groups &g, int O, int R, void *out, hipStream_t st) {
     const int64_t in_row = (int64_t)R * sizeof(T), w_row = TR ? (int64_t)O * sizeof(T) : in_row;

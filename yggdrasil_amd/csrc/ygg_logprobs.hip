@@ -12,7 +12,8 @@
 // The most likely tokens: every lane's largest value is known from the maximum's pass, and of the 16 or 64 of them the
 // top-th largest is a bound that at least `top` entries reach and few others; those are gathered in LDS and each counts the
 // keys (value, then lower index) above its own: its place. Where too many reach the bound (values in an order that hurts,
-// or equal), the places are found one by one.
+// or equal, also masked ones of a finite value where fewer than `top` are left), the places are found one by one, a pass each:
+// 20 of 8 x 131072 equal bf16 46 us for 13, 5 of 4095 x 50257 464 for 119.
 #include "ygg_ops.h"
 #include "ygg_optype.h"
 
@@ -177,8 +178,9 @@ __device__ __forceinline__ float max_of_rows(float v) {
     return __builtin_fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
 }
 
-// Rows of up to kG kC kU entries, kG lanes a row with the row in their registers. 64 rows of 256 bytes by 16 lanes each keep
-// 2 to 3 us of arithmetic a wave against the loads of the others: 262144 rows of 256 f32 are bound by both.
+// Rows of up to kG kC kU entries, kG lanes a row with the row in their registers: a wave's arithmetic runs while the others' rows
+// are on their way. 262144 rows of 256 f32 with 5 alternatives, 4 rows a wave: 67 us for 55 at a large copy's rate, VALU and
+// reading both busy.
 template <class T, int kG, int kU> __global__ __launch_bounds__(256) void narrow_kernel(LogprobsArgs a) {
     constexpr int kC = 16 / sizeof(T), kN = kU * kC, kRows = 256 / kG;
     __shared__ uint64_t keys[256];
