@@ -513,3 +513,16 @@ def test_more_rows_than_a_launch_takes():
     most = n >> 12 << 12
     assert bool((r.entropy[:most].view(-1, 1 << 12) == whole.entropy).all())
     assert bool((r.top_ids[:most].view(-1, 1 << 12, top) == whole.top_ids).all())
+
+
+def test_a_single_rows_stride_is_not_used():
+    """One row's distance to the next may be anything, through the C-ABI."""
+    import ctypes
+    from yggdrasil_amd import _lib, ops
+    x, _ = rows_of(1, 300, torch.float32, 8)
+    want = ops.token_logprobs(x)
+    for stride in (0, -5, 2 ** 62, -2 ** 63):
+        got = torch.full((1,), 7.0, device="cuda")
+        _lib.check(_lib.lib().ygg_logprobs(x.data_ptr(), 0, 1, 300, ctypes.c_int64(stride), None, 0, 0, None, got.data_ptr(), None,
+                                           None, None, None, 0, torch.cuda.current_stream().cuda_stream))
+        assert torch.equal(got, want.entropy)

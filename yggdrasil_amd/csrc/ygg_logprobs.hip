@@ -604,13 +604,13 @@ void skip_rows(LogprobsGradArgs &a, int64_t n, int size) {
 // launch(a) for up to `most` rows at a time: what one launch takes
 template <class T, class A, class F> hipError_t by_rows(A a, int64_t most, F launch) {
     const int64_t rows = a.rows;
-    for (int64_t done = 0; done < rows; done += most) {
+    for (int64_t done = 0;; skip_rows(a, most, sizeof(T))) {     // only to rows that there are: a single one may have any stride
         a.rows = rows - done < most ? rows - done : most;
         launch(a);
         if (hipError_t e = hipGetLastError()) return e;
-        skip_rows(a, most, sizeof(T));
+        done += a.rows;
+        if (done == rows) return hipSuccess;
     }
-    return hipSuccess;
 }
 
 template <class T> hipError_t go(const LogprobsArgs &a, void *scratch, hipStream_t st) {
