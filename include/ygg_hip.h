@@ -301,6 +301,58 @@ int64_t ygg_int8_scratch(int M, int N, int K);
 int ygg_int8_linear(const void *d_x, int type, const int8_t *d_w, const float *d_w_scale, int M, int N, int K, void *d_y,
                     void *d_scratch, int64_t scratch_bytes, void *stream);
 
+/* ---- Operators of a recurrent block that is trained and served beside the model (the reference trains with JAX: its scan
+   yggdrasil/scan.py:6-15, its norm yggdrasil/model.py:92-93, its clipping yggdrasil/train.py:64-68). As those above: on the
+   caller's current device and stream, without a wait or an allocation; types 0 f32, 1 bf16, 2 f16. Scratch is device
+   memory of the bytes that the _scratch entry gives, 256-byte aligned, that no other call uses until this one has run. ---- */
+#define YGG_MOST_STEPS (1 << 30)             /* steps of a recurrence */
+#define YGG_MOST_VALUES ((int64_t)1 << 40)   /* values of a tensor that is clipped */
+
+/* y = (x - mean) / sqrt(variance + eps) * weight + bias of rows of n values, `stride` values apart; y (rows, n) contiguous, in
+   x's type. weight and bias (n) in weight_type (0 or x's type), NULL: ones and zeros. d_stats (rows, 2) or NULL: what the
+   gradients want. */
+int ygg_layer_norm(const void *d_x, int type, int64_t rows, int n, int64_t stride, const void *d_weight, const void *d_bias,
+                   int weight_type, float eps, void *d_y, float *d_stats, void *stream);
+/* The gradients, from dy (rows, n) contiguous: of the rows (contiguous, in x's type), of weight and bias (in weight_type;
+   zero without rows). NULL: not wanted; scratch is wanted for those of weight and bias alone. */
+int64_t ygg_layer_norm_scratch(int type, int64_t rows, int n);
+int ygg_layer_norm_grad(const void *d_x, int type, int64_t rows, int n, int64_t stride, const void *d_weight, int weight_type,
+                        const float *d_stats, const void *d_dy, void *d_dx, void *d_dweight, void *d_dbias, void *d_scratch,
+                        int64_t scratch_bytes, void *stream);
+
+/* h_t = gate_t h_{t-1} + x_t over T steps of B sequences of n channels. gate (type gate_type: 0 or x's) and x lie with the
+   channels of a step next to each other, steps and sequences any distance apart (gate_t, gate_b, x_t, x_b values, at least
+   0). d_state (B, n) f32 is h_{-1} (NULL: zeros); d_h (B, T, n) contiguous in x's type, d_last (B, n) f32 the last state
+   (what d_state holds where there are no steps), memory of its own. States are held in f32; runs of steps are joined by the products
+   of their gates, so gates are meant to be at most 1 in magnitude: others have to keep the products of any run of steps
+   finite. */
+int64_t ygg_gated_scan_scratch(int type, int gate_type, int64_t B, int64_t T, int n);
+int ygg_gated_scan(const void *d_gate, int gate_type, int64_t gate_b, int64_t gate_t, const void *d_x, int type, int64_t x_b,
+                   int64_t x_t, int64_t B, int64_t T, int n, const float *d_state, void *d_h, float *d_last, void *d_scratch,
+                   int64_t scratch_bytes, void *stream);
+/* The gradients, from those of h (contiguous, NULL: zeros) and of the last state (NULL: zeros) and from h as ygg_gated_scan left
+   it: of x and the gates (B, T, n) contiguous in their types, of the state (B, n) f32. NULL: not wanted. */
+int ygg_gated_scan_grad(const void *d_gate, int gate_type, int64_t gate_b, int64_t gate_t, const void *d_h, int type, int64_t B,
+                        int64_t T, int n, const float *d_state, const void *d_dh, const float *d_dlast, void *d_dx, void *d_dgate,
+                        float *d_dstate, void *d_scratch, int64_t scratch_bytes, void *stream);
+
+/* The gated projections of a feed-forward block: x (M, K), w (2, N, K) contiguous, g = x w[0]^T, u = x w[1]^T, y (M, N) =
+   act(g) u in x's type; act: 0 silu (g sigmoid(g)), 1 gelu (g Phi(g)), 2 sigmoid. N up to YGG_MOST_INNER / 2. d_gu (M, 2, N)
+   in x's type or NULL: g and u, which the gradients want. */
+int ygg_gated_linear(const void *d_x, const void *d_w, int type, int act, int M, int N, int K, void *d_y, void *d_gu, void *stream);
+/* The gradients, from dy (M, N): of the rows and of w. NULL: not wanted. */
+int64_t ygg_gated_linear_scratch(int type, int M, int N, int K);
+int ygg_gated_linear_grad(const void *d_x, const void *d_w, const void *d_gu, const void *d_dy, int type, int act, int M, int N, int K,
+                          void *d_dx, void *d_dw, void *d_scratch, int64_t scratch_bytes, void *stream);
+
+/* d_norm (1): the root of the sum of the squares of all values of `count` tensors, summed in 64 bits. d_out (NULL: the norm
+   alone): each tensor times min(1, most / norm), each value rounded once; a norm that is no finite number changes nothing. The
+   arrays (of device addresses, sizes and types) are host memory that is read before the call returns; d_out may hold the
+   tensors themselves, but no two tensors may overlap otherwise. */
+int64_t ygg_clip_scratch(const int64_t *sizes, int count);
+int ygg_clip_grad_norm(const void *const *d_tensors, const int64_t *sizes, const int *types, int count, double most,
+                       void *const *d_out, float *d_norm, void *d_scratch, int64_t scratch_bytes, void *stream);
+
 /* Message of the last failed call on this thread ("" if none). */
 const char *ygg_last_error(void);
 

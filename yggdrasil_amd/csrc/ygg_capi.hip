@@ -933,7 +933,7 @@ int set_error(int code, const char *msg) { return fail(code, "%s", msg); }
 
 extern "C" {
 
-int ygg_version(void) { return 12; }
+int ygg_version(void) { return 13; }
 
 const char *ygg_last_error(void) { return g_err.c_str(); }
 
@@ -1318,6 +1318,156 @@ int ygg_int8_linear(const void *d_x, int type, const int8_t *d_w, const float *d
     if (need && (!d_scratch || scratch_bytes < need))
         return fail(YGG_ERR_ARG, "scratch of %lld bytes, %lld wanted", (long long)scratch_bytes, (long long)need);
     OP_TRY(ygg::launch_int8_linear(type, d_x, d_w, d_w_scale, M, N, K, d_y, d_scratch, (hipStream_t)stream));
+    return YGG_OK;
+}
+
+// ---- the operators of a recurrent block
+
+int ygg_layer_norm(const void *d_x, int type, int64_t rows, int n, int64_t stride, const void *d_weight, const void *d_bias,
+                   int weight_type, float eps, void *d_y, float *d_stats, void *stream) {
+    if (type < 0 || type > 2) return fail(YGG_ERR_ARG, kTypeHelp, type);
+    if (weight_type != 0 && weight_type != type) return fail(YGG_ERR_ARG, "weight_type %d: 0 or the rows' (%d)", weight_type, type);
+    if (rows < 0) return fail(YGG_ERR_ARG, "negative rows (%lld)", (long long)rows);
+    if (n < 1 || n > YGG_MOST_INNER) return fail(YGG_ERR_ARG, kOpLimits, "n", (long long)n, 1, YGG_MOST_INNER);
+    if (stride < n && rows > 1) return fail(YGG_ERR_ARG, "rows of %d values %lld apart", n, (long long)stride);
+    if (!(eps >= 0.0f) || eps == __builtin_huge_valf()) return fail(YGG_ERR_ARG, "eps %g: finite and >= 0", (double)eps);
+    if (rows == 0) return YGG_OK;
+    if (!d_x || !d_y) return fail(YGG_ERR_ARG, "NULL buffer");
+    const ygg::NormArgs a = {d_x, rows, stride, n, weight_type == 0, d_weight, d_bias, eps, d_y, d_stats};
+    OP_TRY(ygg::launch_norm(type, a, (hipStream_t)stream));
+    return YGG_OK;
+}
+
+int64_t ygg_layer_norm_scratch(int type, int64_t rows, int n) {
+    if (type < 0 || type > 2 || rows < 1 || n < 1 || n > YGG_MOST_INNER) return 0;
+    return ygg::norm_grad_scratch(type, rows, n);
+}
+
+int ygg_layer_norm_grad(const void *d_x, int type, int64_t rows, int n, int64_t stride, const void *d_weight, int weight_type,
+                        const float *d_stats, const void *d_dy, void *d_dx, void *d_dweight, void *d_dbias, void *d_scratch,
+                        int64_t scratch_bytes, void *stream) {
+    if (type < 0 || type > 2) return fail(YGG_ERR_ARG, kTypeHelp, type);
+    if (weight_type != 0 && weight_type != type) return fail(YGG_ERR_ARG, "weight_type %d: 0 or the rows' (%d)", weight_type, type);
+    if (rows < 0) return fail(YGG_ERR_ARG, "negative rows (%lld)", (long long)rows);
+    if (n < 1 || n > YGG_MOST_INNER) return fail(YGG_ERR_ARG, kOpLimits, "n", (long long)n, 1, YGG_MOST_INNER);
+    if (stride < n && rows > 1) return fail(YGG_ERR_ARG, "rows of %d values %lld apart", n, (long long)stride);
+    if (rows > 0 && (!d_x || !d_stats || !d_dy)) return fail(YGG_ERR_ARG, "NULL buffer");
+    const int64_t need = rows && (d_dweight || d_dbias) ? ygg::norm_grad_scratch(type, rows, n) : 0;
+    if (need && (!d_scratch || scratch_bytes < need))
+        return fail(YGG_ERR_ARG, "scratch of %lld bytes, %lld wanted", (long long)scratch_bytes, (long long)need);
+    const ygg::NormGradArgs a = {d_x, rows, stride, n, weight_type == 0, d_weight, d_stats, d_dy, d_dx, d_dweight, d_dbias};
+    OP_TRY(ygg::launch_norm_grad(type, a, d_scratch, (hipStream_t)stream));
+    return YGG_OK;
+}
+
+// sizes of a recurrence: an error code, or 0
+static int check_scan(int type, int gate_type, int64_t B, int64_t T, int n) {
+    if (type < 0 || type > 2) return fail(YGG_ERR_ARG, kTypeHelp, type);
+    if (gate_type != 0 && gate_type != type) return fail(YGG_ERR_ARG, "gate_type %d: 0 or x's (%d)", gate_type, type);
+    if (B < 0 || B > YGG_MOST_ROWS) return fail(YGG_ERR_ARG, kOpLimits, "B", (long long)B, 0, YGG_MOST_ROWS);
+    if (T < 0 || T > YGG_MOST_STEPS) return fail(YGG_ERR_ARG, kOpLimits, "T", (long long)T, 0, YGG_MOST_STEPS);
+    if (n < 1 || n > YGG_MOST_INNER) return fail(YGG_ERR_ARG, kOpLimits, "n", (long long)n, 1, YGG_MOST_INNER);
+    return YGG_OK;
+}
+
+int64_t ygg_gated_scan_scratch(int type, int gate_type, int64_t B, int64_t T, int n) {
+    if (type < 0 || type > 2 || B < 1 || B > YGG_MOST_ROWS || T < 1 || T > YGG_MOST_STEPS || n < 1 || n > YGG_MOST_INNER) return 0;
+    return ygg::scan_scratch(type, gate_type, B, T, n);
+}
+
+int ygg_gated_scan(const void *d_gate, int gate_type, int64_t gate_b, int64_t gate_t, const void *d_x, int type, int64_t x_b,
+                   int64_t x_t, int64_t B, int64_t T, int n, const float *d_state, void *d_h, float *d_last, void *d_scratch,
+                   int64_t scratch_bytes, void *stream) {
+    if (int rc = check_scan(type, gate_type, B, T, n)) return rc;
+    if (gate_b < 0 || gate_t < 0 || x_b < 0 || x_t < 0) return fail(YGG_ERR_ARG, "negative strides");
+    if (B == 0) return YGG_OK;
+    if (!d_last || (T > 0 && (!d_gate || !d_x || !d_h))) return fail(YGG_ERR_ARG, "NULL buffer");
+    const int64_t need = T ? ygg::scan_scratch(type, gate_type, B, T, n) : 0;
+    if (need && (!d_scratch || scratch_bytes < need))
+        return fail(YGG_ERR_ARG, "scratch of %lld bytes, %lld wanted", (long long)scratch_bytes, (long long)need);
+    const ygg::ScanArgs a = {d_gate, d_x, gate_b, gate_t, x_b, x_t, B, T, n, d_state, d_h, d_last};
+    OP_TRY(ygg::launch_scan(type, gate_type, a, d_scratch, (hipStream_t)stream));
+    return YGG_OK;
+}
+
+int ygg_gated_scan_grad(const void *d_gate, int gate_type, int64_t gate_b, int64_t gate_t, const void *d_h, int type, int64_t B,
+                        int64_t T, int n, const float *d_state, const void *d_dh, const float *d_dlast, void *d_dx, void *d_dgate,
+                        float *d_dstate, void *d_scratch, int64_t scratch_bytes, void *stream) {
+    if (int rc = check_scan(type, gate_type, B, T, n)) return rc;
+    if (gate_b < 0 || gate_t < 0) return fail(YGG_ERR_ARG, "negative strides");
+    if (B == 0 || (T == 0 && !d_dstate)) return YGG_OK;
+    if (T > 0 && (!d_gate || (d_dgate && !d_h))) return fail(YGG_ERR_ARG, "NULL buffer");
+    const int64_t need = T ? ygg::scan_scratch(type, gate_type, B, T, n) : 0;
+    if (need && (!d_scratch || scratch_bytes < need))
+        return fail(YGG_ERR_ARG, "scratch of %lld bytes, %lld wanted", (long long)scratch_bytes, (long long)need);
+    const ygg::ScanGradArgs a = {d_gate, d_h, d_dh, gate_b, gate_t, B, T, n, d_state, d_dlast, d_dx, d_dgate, d_dstate};
+    OP_TRY(ygg::launch_scan_grad(type, gate_type, a, d_scratch, (hipStream_t)stream));
+    return YGG_OK;
+}
+
+// sizes of the gated projections: an error code, or 0. N: half of what a product of both takes
+static int check_gated(int type, int act, int M, int N, int K) {
+    if (type < 0 || type > 2) return fail(YGG_ERR_ARG, kTypeHelp, type);
+    if (act < 0 || act > 2) return fail(YGG_ERR_ARG, "act %d: 0 silu, 1 gelu, 2 sigmoid", act);
+    if (M < 0 || M > YGG_MOST_ROWS) return fail(YGG_ERR_ARG, kOpLimits, "M", (long long)M, 0, YGG_MOST_ROWS);
+    if (N < 1 || N > YGG_MOST_INNER / 2) return fail(YGG_ERR_ARG, kOpLimits, "N", (long long)N, 1, YGG_MOST_INNER / 2);
+    if (K < 1 || K > YGG_MOST_INNER) return fail(YGG_ERR_ARG, kOpLimits, "K", (long long)K, 1, YGG_MOST_INNER);
+    return YGG_OK;
+}
+
+int ygg_gated_linear(const void *d_x, const void *d_w, int type, int act, int M, int N, int K, void *d_y, void *d_gu, void *stream) {
+    if (int rc = check_gated(type, act, M, N, K)) return rc;
+    if (M == 0) return YGG_OK;
+    if (!d_x || !d_w || !d_y) return fail(YGG_ERR_ARG, "NULL buffer");
+    OP_TRY(ygg::launch_gated(type, act, d_x, d_w, M, N, K, d_y, d_gu, (hipStream_t)stream));
+    return YGG_OK;
+}
+
+int64_t ygg_gated_linear_scratch(int type, int M, int N, int K) {
+    if (type < 0 || type > 2 || M < 0 || M > YGG_MOST_ROWS || N < 1 || N > YGG_MOST_INNER / 2 || K < 1 || K > YGG_MOST_INNER) return 0;
+    return ygg::gated_grad_scratch(type, M, N, K);
+}
+
+int ygg_gated_linear_grad(const void *d_x, const void *d_w, const void *d_gu, const void *d_dy, int type, int act, int M, int N, int K,
+                          void *d_dx, void *d_dw, void *d_scratch, int64_t scratch_bytes, void *stream) {
+    if (int rc = check_gated(type, act, M, N, K)) return rc;
+    if ((M == 0 || !d_dx) && !d_dw) return YGG_OK;
+    if ((M > 0 && (!d_x || !d_w || !d_gu || !d_dy))) return fail(YGG_ERR_ARG, "NULL buffer");
+    const int64_t need = ygg::gated_grad_scratch(type, M, N, K);
+    if (!d_scratch || scratch_bytes < need)
+        return fail(YGG_ERR_ARG, "scratch of %lld bytes, %lld wanted", (long long)scratch_bytes, (long long)need);
+    OP_TRY(ygg::launch_gated_grad(type, act, d_x, d_w, d_gu, d_dy, M, N, K, M ? d_dx : nullptr, d_dw, d_scratch, (hipStream_t)stream));
+    return YGG_OK;
+}
+
+static int check_tensors(const int64_t *sizes, const int *types, int count) {
+    if (count < 0) return fail(YGG_ERR_ARG, "negative count (%d)", count);
+    if (count && !sizes) return fail(YGG_ERR_ARG, "NULL sizes");
+    for (int i = 0; i < count; i++) {
+        if (sizes[i] < 0 || sizes[i] > YGG_MOST_VALUES) return fail(YGG_ERR_ARG, "tensor %d: %lld values", i, (long long)sizes[i]);
+        if (types && (types[i] < 0 || types[i] > 2)) return fail(YGG_ERR_ARG, kTypeHelp, types[i]);
+    }
+    return YGG_OK;
+}
+
+int64_t ygg_clip_scratch(const int64_t *sizes, int count) {
+    if (count < 0 || (count && !sizes)) return 0;
+    for (int i = 0; i < count; i++)
+        if (sizes[i] < 0 || sizes[i] > YGG_MOST_VALUES) return 0;
+    return ygg::clip_scratch(sizes, count);
+}
+
+int ygg_clip_grad_norm(const void *const *d_tensors, const int64_t *sizes, const int *types, int count, double most,
+                       void *const *d_out, float *d_norm, void *d_scratch, int64_t scratch_bytes, void *stream) {
+    if (int rc = check_tensors(sizes, types, count)) return rc;
+    if (!(most >= 0.0)) return fail(YGG_ERR_ARG, "most %g: at least 0", most);
+    if (!d_norm || (count && (!d_tensors || !types))) return fail(YGG_ERR_ARG, "NULL argument");
+    for (int i = 0; i < count; i++)
+        if (sizes[i] && (!d_tensors[i] || (d_out && !d_out[i]))) return fail(YGG_ERR_ARG, "NULL buffer of tensor %d", i);
+    const int64_t need = ygg::clip_scratch(sizes, count);
+    if (!d_scratch || scratch_bytes < need)
+        return fail(YGG_ERR_ARG, "scratch of %lld bytes, %lld wanted", (long long)scratch_bytes, (long long)need);
+    OP_TRY(ygg::launch_clip(d_tensors, sizes, types, count, most, d_out, d_norm, d_scratch, (hipStream_t)stream));
     return YGG_OK;
 }
 

@@ -14,6 +14,7 @@
 // keys (value, then lower index) above its own: its place. Where too many reach the bound (values in an order that hurts,
 // or equal, also masked ones of a finite value where fewer than `top` are left), the places are found one by one, a pass each:
 // 20 of 8 x 131072 equal bf16 46 us for 13, 5 of 4095 x 50257 464 for 119.
+#include "ygg_lanes.h"
 #include "ygg_ops.h"
 #include "ygg_optype.h"
 
@@ -36,28 +37,6 @@ __device__ __forceinline__ float unordered(uint32_t u) {
 __device__ __forceinline__ uint64_t key_of(float v, int c) { return (uint64_t)ordered(v + 0.0f) << 32 | (uint32_t)~c; }
 __device__ __forceinline__ int index_of(uint64_t key) { return (int)~(uint32_t)key; }
 
-// A value joined over groups of kG lanes (16 or 64), the same in each of them
-template <int kControl> __device__ __forceinline__ uint32_t rotated(uint32_t v) {
-    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kControl, 0xf, 0xf, true);
-}
-template <int kG, class V, class F> __device__ __forceinline__ V join(V v, F f) {
-    static_assert(sizeof(V) == 4, "");
-    auto turn = [&](uint32_t o) { v = f(v, __builtin_bit_cast(V, o)); };
-    turn(rotated<0x128>(__builtin_bit_cast(uint32_t, v)));    // row_ror of 8, 4, 2, 1
-    turn(rotated<0x124>(__builtin_bit_cast(uint32_t, v)));
-    turn(rotated<0x122>(__builtin_bit_cast(uint32_t, v)));
-    turn(rotated<0x121>(__builtin_bit_cast(uint32_t, v)));
-    if constexpr (kG == 64) {
-        uint32_t u = __builtin_bit_cast(uint32_t, v);
-        u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(u, u, false, false));
-        v = f(__builtin_bit_cast(V, (uint32_t)r[0]), __builtin_bit_cast(V, (uint32_t)r[1]));
-        u = __builtin_bit_cast(uint32_t, v);
-        r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(u, u, false, false));
-        v = f(__builtin_bit_cast(V, (uint32_t)r[0]), __builtin_bit_cast(V, (uint32_t)r[1]));
-    }
-    return v;
-}
-template <int kG> __device__ __forceinline__ float sum_of(float v) { return join<kG>(v, [](float a, float b) { return a + b; }); }
 template <int kG> __device__ __forceinline__ float max_of(float v) {
     return join<kG>(v, [](float a, float b) { return __builtin_fmaxf(a, b); });
 }

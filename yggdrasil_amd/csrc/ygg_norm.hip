@@ -1,0 +1,514 @@
+// Layer norm of rows and its gradients. With m and v a row's mean and variance and z = (x - m) / sqrt(v + eps):
+//   y = z w + b;   q = w dy, dx = (q - mean(q) - z mean(q z)) / sqrt(v + eps);   dw = sum over rows of dy z, db = of dy.
+//
+// A row is held in the registers of 4, 16 or 64 lanes or of a workgroup, 16 bytes a load, so that it is read once: the mean and
+// then the squares about it are joined in f32. A workgroup's waves first take each its own mean and squares M2 and are joined by
+//   m = sum n_i m_i / n,  M2 = sum M2_i + n_i (m_i - m)^2,
+// which takes one barrier instead of two and cancels nothing. The backward pass reads x and dy once, writes dx, and keeps its
+// columns' sums of dy z and dy in registers over all of a workgroup's rows; the workgroups' sums are added in their order by a
+// second kernel, so that they come out the same every time. Rows wider than the registers hold are read again.
+#include <algorithm>
+
+#include "ygg_lanes.h"
+#include "ygg_ops.h"
+#include "ygg_optype.h"
+
+namespace ygg {
+namespace {
+
+template <class T> constexpr int kEach = 16 / (int)sizeof(T);    // values of a piece
+
+// piece i of lane `lane` of kL: its first column
+template <class T, int kL> __device__ __forceinline__ int column(int i, int lane) { return (i * kL + lane) * kEach<T>; }
+
+// A row's pieces; columns that there are not come as zero
+template <class T, int kL, int kP>
+__device__ __forceinline__ void load_row(u32x4 (&v)[kP], const T *p, int n, int lane) {
+    constexpr int kE = kEach<T>;
+    if (n % kE == 0) {
+#pragma unroll
+        for (int i = 0; i < kP; i++) v[i] = load16(p + min(column<T, kL>(i, lane), n - kE));
+#pragma unroll
+        for (int i = 0; i < kP; i++)
+            if (column<T, kL>(i, lane) >= n) v[i] = u32x4{0, 0, 0, 0};
+    } else if (n > kE) {
+#pragma unroll
+        for (int i = 0; i < kP; i++) v[i] = load16_end(p + column<T, kL>(i, lane), n - column<T, kL>(i, lane));
+    } else {
+#pragma unroll
+        for (int i = 0; i < kP; i++) v[i] = load16(p + column<T, kL>(i, lane), n - column<T, kL>(i, lane));
+    }
+}
+
+// kN values of a weight from column c on, in f32; `other` where there are none
+template <class T, int kN> __device__ __forceinline__ void load_weight(float *f, const T *p, int c, int n, float other) {
+    if (!p) {
+#pragma unroll
+        for (int j = 0; j < kN; j++) f[j] = other;
+        return;
+    }
+    constexpr int kE = kEach<T>;
+#pragma unroll
+    for (int k = 0; k < kN; k += kE) {
+        u32x4 v;
+        if (c + k + kE <= n) v = load16(p + c + k);
+        else v = load16(p + min(c + k, n - 1), n - c - k);
+        float t[kE];
+        unpack(v, t, T());
+#pragma unroll
+        for (int j = 0; j < kE && j < kN; j++) f[k + j] = t[j];
+    }
+}
+template <class T, int kN>
+__device__ __forceinline__ void load_weight(float *f, const void *p, bool wide, int c, int n, float other) {
+    if (wide) load_weight<float, kN>(f, (const float *)p, c, n, other);
+    else load_weight<T, kN>(f, (const T *)p, c, n, other);
+}
+
+// The mean and 1 / sqrt(variance + eps) of a row held by kL lanes. waves: LDS of a workgroup of more than a wave, another one
+// than the row before's.
+template <class T, int kL, int kP>
+__device__ __forceinline__ float2 moments(const u32x4 (&x)[kP], int n, float eps, int lane, float2 *waves) {
+    constexpr int kE = kEach<T>;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kP; i++) {
+        float f[kE];
+        unpack(x[i], f, T());
+#pragma unroll
+        for (int j = 0; j < kE; j++) sum += f[j];
+    }
+    constexpr int kIn = kL < 64 ? kL : 64;
+    // the wave's values: whole pieces of 64 lanes, the last one cut
+    const int wave = lane / 64;
+    auto held = [&](int w) {
+        int h = 0;
+#pragma unroll
+        for (int i = 0; i < kP; i++) h += min(max(n - (i * kL + w * 64) * kE, 0), 64 * kE);
+        return h;
+    };
+    const float mine = kL <= 64 ? (float)n : (float)held(wave);
+    float mean = sum_of<kIn>(sum) / fmaxf(mine, 1.0f);
+    float squares = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kP; i++) {
+        float f[kE];
+        unpack(x[i], f, T());
+        const int left = n - column<T, kL>(i, lane);
+#pragma unroll
+        for (int j = 0; j < kE; j++) {
+            const float d = j < left ? f[j] - mean : 0.0f;
+            squares = __builtin_fmaf(d, d, squares);
+        }
+    }
+    squares = sum_of<kIn>(squares);
+    if constexpr (kL > 64) {
+        if (lane % 64 == 0) waves[wave] = make_float2(mean, squares);
+        __syncthreads();
+        float total = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kL / 64; w++) total = __builtin_fmaf((float)held(w), waves[w].x, total);
+        mean = total / (float)n;
+        squares = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kL / 64; w++) {
+            const float d = waves[w].x - mean;
+            squares += __builtin_fmaf((float)held(w) * d, d, waves[w].y);
+        }
+    }
+    return make_float2(mean, 1.0f / sqrtf(squares / (float)n + eps));
+}
+
+// kL lanes a row, kP pieces a lane. Up to kHold values a lane the weights stay in registers over a workgroup's rows.
+constexpr int kHold = 32;
+template <class T, int kL, int kP>
+__global__ __launch_bounds__(kL > 256 ? kL : 256) void norm_kernel(const NormArgs a) {
+    constexpr int kThreads = kL > 256 ? kL : 256, kRows = kThreads / kL, kE = kEach<T>;
+    constexpr bool kHeld = kL <= 256 && kP * kE <= kHold;
+    __shared__ float2 waves[2][kThreads / 64];
+    const int lane = threadIdx.x % kL, n = a.n;
+    float w[kP][kE], b[kP][kE];
+    if constexpr (kHeld) {
+#pragma unroll
+        for (int i = 0; i < kP; i++) {
+            load_weight<T, kE>(w[i], a.weight, a.wide, column<T, kL>(i, lane), n, 1.0f);
+            load_weight<T, kE>(b[i], a.bias, a.wide, column<T, kL>(i, lane), n, 0.0f);
+        }
+    }
+    const int64_t hop = (int64_t)gridDim.x * kRows;
+    int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kL;
+    if (row >= a.rows) return;     // whole groups of lanes; of a workgroup a row, none
+    u32x4 x[kP], next[kP];
+    load_row<T, kL>(next, (const T *)a.x + row * a.stride, n, lane);
+    for (int turn = 0; row < a.rows; row += hop, turn ^= 1) {
+#pragma unroll
+        for (int i = 0; i < kP; i++) x[i] = next[i];
+        if (row + hop < a.rows) load_row<T, kL>(next, (const T *)a.x + (row + hop) * a.stride, n, lane);
+        const float2 s = moments<T, kL>(x, n, a.eps, lane, waves[turn]);
+        if (a.stats && lane == 0) ((float2 *)a.stats)[row] = s;
+        T *y = (T *)a.y + row * n;
+#pragma unroll
+        for (int i = 0; i < kP; i++) {
+            const int c = column<T, kL>(i, lane);
+            if (c >= n) break;
+            if constexpr (!kHeld) {
+                load_weight<T, kE>(w[i], a.weight, a.wide, c, n, 1.0f);
+                load_weight<T, kE>(b[i], a.bias, a.wide, c, n, 0.0f);
+            }
+            float f[kE];
+            unpack(x[i], f, T());
+#pragma unroll
+            for (int j = 0; j < kE; j++) f[j] = __builtin_fmaf((f[j] - s.x) * s.y, w[i][j], b[i][j]);
+            store_run<T, kE>(y + c, f, n - c);
+        }
+    }
+}
+
+// values joined over a workgroup of kThreads, the same in each thread
+template <int kThreads> __device__ __forceinline__ float sum_all(float v, float *lds) {
+    v = sum_of<64>(v);
+    __syncthreads();
+    if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = v;
+    __syncthreads();
+    v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; w++) v += lds[w];
+    return v;
+}
+// f(column, values of x (and dy, where there is one), how many of them exist) over a row's pieces
+template <class T, int kThreads, class F> __device__ __forceinline__ void each_piece(const T *x, const T *dy, int n, F f) {
+    constexpr int kE = kEach<T>;
+    for (int c = threadIdx.x * kE; c < n; c += kThreads * kE) {
+        float v[kE], d[kE];
+        unpack(load16(x + c, n - c), v, T());
+        if (dy) unpack(load16(dy + c, n - c), d, T());
+        f(c, v, d, n - c);
+    }
+}
+// Rows wider than the registers of a workgroup: three readings, the later ones from the caches where they hold the row
+template <class T> __global__ __launch_bounds__(1024) void norm_wide_kernel(const NormArgs a) {
+    constexpr int kE = kEach<T>;
+    __shared__ float lds[16];
+    const int n = a.n;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T *x = (const T *)a.x + row * a.stride;
+        float sum = 0.0f, squares = 0.0f;
+        each_piece<T, 1024>(x, (const T *)nullptr, n, [&](int, const float *v, const float *, int) {
+#pragma unroll
+            for (int j = 0; j < kE; j++) sum += v[j];
+        });
+        const float mean = sum_all<1024>(sum, lds) / (float)n;
+        each_piece<T, 1024>(x, (const T *)nullptr, n, [&](int, const float *v, const float *, int left) {
+#pragma unroll
+            for (int j = 0; j < kE; j++) {
+                const float d = j < left ? v[j] - mean : 0.0f;
+                squares = __builtin_fmaf(d, d, squares);
+            }
+        });
+        const float inv = 1.0f / sqrtf(sum_all<1024>(squares, lds) / (float)n + a.eps);
+        if (a.stats && threadIdx.x == 0) ((float2 *)a.stats)[row] = make_float2(mean, inv);
+        T *y = (T *)a.y + row * n;
+        each_piece<T, 1024>(x, (const T *)nullptr, n, [&](int c, const float *v, const float *, int left) {
+            float w[kE], b[kE], f[kE];
+            load_weight<T, kE>(w, a.weight, a.wide, c, n, 1.0f);
+            load_weight<T, kE>(b, a.bias, a.wide, c, n, 0.0f);
+#pragma unroll
+            for (int j = 0; j < kE; j++) f[j] = __builtin_fmaf((v[j] - mean) * inv, w[j], b[j]);
+            store_run<T, kE>(y + c, f, left);
+        });
+    }
+}
+
+// ---- backward: dx, and a workgroup's sums of dy z and dy over its rows into part[blockIdx][2][n]
+template <class T, int kL, int kP>
+__global__ __launch_bounds__(kL > 256 ? kL : 256) void norm_grad_kernel(const NormGradArgs a, float *part) {
+    constexpr int kThreads = kL > 256 ? kL : 256, kRows = kThreads / kL, kE = kEach<T>, kIn = kL < 64 ? kL : 64;
+    __shared__ float2 waves[2][kThreads / 64];
+    __shared__ float sums[kL <= 64 ? 2 : 1][kL <= 64 ? kL * kP * kE : 1];
+    const int lane = threadIdx.x % kL, n = a.n;
+    float w[kP][kE], aw[kP][kE], ab[kP][kE];
+#pragma unroll
+    for (int i = 0; i < kP; i++) {
+        load_weight<T, kE>(w[i], a.weight, a.wide, column<T, kL>(i, lane), n, 1.0f);
+#pragma unroll
+        for (int j = 0; j < kE; j++) aw[i][j] = ab[i][j] = 0.0f;
+    }
+    const int64_t hop = (int64_t)gridDim.x * kRows;
+    int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kL;
+    u32x4 x[kP], dy[kP], next_x[kP], next_dy[kP];
+    float2 s = {0, 0}, next_s = {0, 0};
+    auto load = [&](int64_t r) {
+        if (r >= a.rows) return;
+        load_row<T, kL>(next_x, (const T *)a.x + r * a.stride, n, lane);
+        load_row<T, kL>(next_dy, (const T *)a.dy + r * n, n, lane);
+        next_s = ((const float2 *)a.stats)[r];
+    };
+    load(row);
+    for (int turn = 0; row < a.rows; row += hop, turn ^= 1) {
+#pragma unroll
+        for (int i = 0; i < kP; i++) {
+            x[i] = next_x[i];
+            dy[i] = next_dy[i];
+        }
+        s = next_s;
+        load(row + hop);
+        float q1 = 0.0f, q2 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kP; i++) {
+            float f[kE], d[kE];
+            unpack(x[i], f, T());
+            unpack(dy[i], d, T());
+#pragma unroll
+            for (int j = 0; j < kE; j++) {
+                const float z = (f[j] - s.x) * s.y, q = w[i][j] * d[j];
+                aw[i][j] = __builtin_fmaf(d[j], z, aw[i][j]);
+                ab[i][j] += d[j];
+                q1 += q;
+                q2 = __builtin_fmaf(q, z, q2);
+            }
+        }
+        if (!a.dx) continue;
+        q1 = sum_of<kIn>(q1);
+        q2 = sum_of<kIn>(q2);
+        if constexpr (kL > 64) {
+            if (lane % 64 == 0) waves[turn][lane / 64] = make_float2(q1, q2);
+            __syncthreads();
+            q1 = q2 = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kL / 64; k++) {
+                q1 += waves[turn][k].x;
+                q2 += waves[turn][k].y;
+            }
+        }
+        q1 /= (float)n;
+        q2 /= (float)n;
+        T *dx = (T *)a.dx + row * n;
+#pragma unroll
+        for (int i = 0; i < kP; i++) {
+            const int c = column<T, kL>(i, lane);
+            if (c >= n) break;
+            float f[kE], d[kE];
+            unpack(x[i], f, T());
+            unpack(dy[i], d, T());
+#pragma unroll
+            for (int j = 0; j < kE; j++) {
+                const float z = (f[j] - s.x) * s.y, q = w[i][j] * d[j];
+                f[j] = (q - q1 - z * q2) * s.y;
+            }
+            store_run<T, kE>(dx + c, f, n - c);
+        }
+    }
+    if (!part) return;
+    float *out = part + (int64_t)blockIdx.x * 2 * n;
+    if constexpr (kL > 64) {
+#pragma unroll
+        for (int i = 0; i < kP; i++) {
+            const int c = column<T, kL>(i, lane);
+            store_run<float, kE>(out + c, aw[i], n - c);
+            store_run<float, kE>(out + n + c, ab[i], n - c);
+        }
+    } else {
+        // the wave's groups of lanes, then the waves one after the other
+#pragma unroll
+        for (int i = 0; i < kP; i++)
+#pragma unroll
+            for (int j = 0; j < kE; j++)
+#pragma unroll
+                for (int o = kL; o < 64; o *= 2) {
+                    aw[i][j] += __shfl_xor(aw[i][j], o);
+                    ab[i][j] += __shfl_xor(ab[i][j], o);
+                }
+        for (int k = 0; k < kThreads / 64; k++) {
+            if ((int)threadIdx.x / 64 == k && (int)threadIdx.x % 64 < kL) {
+#pragma unroll
+                for (int i = 0; i < kP; i++)
+#pragma unroll
+                    for (int j = 0; j < kE; j++) {
+                        const int c = column<T, kL>(i, lane) + j;
+                        sums[0][c] = k ? sums[0][c] + aw[i][j] : aw[i][j];
+                        sums[kL <= 64][c] = k ? sums[kL <= 64][c] + ab[i][j] : ab[i][j];
+                    }
+            }
+            __syncthreads();
+        }
+        for (int c = threadIdx.x; c < n; c += kThreads) {
+            out[c] = sums[0][c];
+            out[n + c] = sums[kL <= 64][c];
+        }
+    }
+}
+
+// Wider rows: dx by a workgroup a row, in two readings, and the columns' sums by a kernel of their own
+template <class T> __global__ __launch_bounds__(1024) void norm_grad_wide_kernel(const NormGradArgs a) {
+    constexpr int kE = kEach<T>;
+    __shared__ float lds[16];
+    const int n = a.n;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T *x = (const T *)a.x + row * a.stride, *dy = (const T *)a.dy + row * n;
+        const float2 s = ((const float2 *)a.stats)[row];
+        float q1 = 0.0f, q2 = 0.0f;
+        each_piece<T, 1024>(x, dy, n, [&](int c, const float *v, const float *d, int) {
+            float w[kE];
+            load_weight<T, kE>(w, a.weight, a.wide, c, n, 1.0f);
+#pragma unroll
+            for (int j = 0; j < kE; j++) {
+                const float q = w[j] * d[j];
+                q1 += q;
+                q2 = __builtin_fmaf(q, (v[j] - s.x) * s.y, q2);
+            }
+        });
+        q1 = sum_all<1024>(q1, lds) / (float)n;
+        q2 = sum_all<1024>(q2, lds) / (float)n;
+        T *dx = (T *)a.dx + row * n;
+        each_piece<T, 1024>(x, dy, n, [&](int c, const float *v, const float *d, int left) {
+            float w[kE], f[kE];
+            load_weight<T, kE>(w, a.weight, a.wide, c, n, 1.0f);
+#pragma unroll
+            for (int j = 0; j < kE; j++) f[j] = (w[j] * d[j] - q1 - (v[j] - s.x) * s.y * q2) * s.y;
+            store_run<T, kE>(dx + c, f, left);
+        });
+    }
+}
+template <class T> __global__ __launch_bounds__(256) void norm_columns_kernel(const NormGradArgs a, float *part, int groups) {
+    constexpr int kE = kEach<T>;
+    const int n = a.n, g = blockIdx.x % groups, c = (blockIdx.x / groups * 256 + threadIdx.x) * kE;
+    if (c >= n) return;
+    float aw[kE], ab[kE];
+#pragma unroll
+    for (int j = 0; j < kE; j++) aw[j] = ab[j] = 0.0f;
+    for (int64_t row = g; row < a.rows; row += groups) {
+        const float2 s = ((const float2 *)a.stats)[row];
+        float v[kE], d[kE];
+        unpack(load16((const T *)a.x + row * a.stride + c, n - c), v, T());
+        unpack(load16((const T *)a.dy + row * n + c, n - c), d, T());
+#pragma unroll
+        for (int j = 0; j < kE; j++) {
+            aw[j] = __builtin_fmaf(d[j], (v[j] - s.x) * s.y, aw[j]);
+            ab[j] += d[j];
+        }
+    }
+    float *out = part + (int64_t)g * 2 * n + c;
+    store_run<float, kE>(out, aw, n - c);
+    store_run<float, kE>(out + n, ab, n - c);
+}
+
+// The groups' sums of a column, 16 runs of them side by side
+template <class W> __global__ __launch_bounds__(1024) void norm_join_kernel(const float *part, int groups, int n, W *dw, W *db) {
+    __shared__ float sums[16][64];
+    const int col = threadIdx.x % 64, run = threadIdx.x / 64;
+    const int64_t c = (int64_t)blockIdx.x * 64 + col;
+    float sum = 0.0f;
+    if (c < 2 * (int64_t)n) {
+        const int per = (groups + 15) / 16, end = min((run + 1) * per, groups);
+        int g = run * per;
+        for (; g + 4 <= end; g += 4) {
+            float v[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k] = part[(int64_t)(g + k) * 2 * n + c];
+#pragma unroll
+            for (int k = 0; k < 4; k++) sum += v[k];
+        }
+        for (; g < end; g++) sum += part[(int64_t)g * 2 * n + c];
+    }
+    sums[run][col] = sum;
+    __syncthreads();
+    if (run || c >= 2 * (int64_t)n) return;
+#pragma unroll
+    for (int k = 1; k < 16; k++) sum += sums[k][col];
+    if (c < n && dw) dw[c] = from_f32<W>(sum);
+    if (c >= n && db) db[c - n] = from_f32<W>(sum);
+}
+
+// The form that holds rows of n values: f(lanes, pieces), or false past all of them
+template <class T, class F> bool with_form(int n, F f) {
+    auto is = [&](auto l, auto p) {
+        constexpr int kL = decltype(l)::value, kP = decltype(p)::value;
+        if (n > kL * kP * kEach<T>) return false;
+        f(l, p);
+        return true;
+    };
+    constexpr std::integral_constant<int, 1> one{};
+    constexpr std::integral_constant<int, 2> two{};
+    constexpr std::integral_constant<int, 4> four{};
+    constexpr std::integral_constant<int, 16> l16{};
+    constexpr std::integral_constant<int, 64> l64{};
+    constexpr std::integral_constant<int, 256> l256{};
+    return is(four, one) || is(l16, one) || is(l16, two) || is(l16, four) || is(l64, two) || is(l64, four) || is(l256, two) ||
+           is(l256, four);
+}
+constexpr int kFewGroups = 512;     // workgroups of a backward pass: two on each CU
+int64_t groups_of(int64_t rows, int lanes) {
+    const int each = lanes >= 256 ? 1 : 256 / lanes;
+    return std::min<int64_t>((rows + each - 1) / each, kFewGroups);
+}
+template <class T> int64_t grad_groups(int64_t rows, int n) {
+    int64_t g = 0;
+    if (!with_form<T>(n, [&](auto l, auto) { g = groups_of(rows, decltype(l)::value); }) && n <= 512 * 2 * kEach<T>)
+        g = groups_of(rows, 512);
+    // the columns' kernel: a thousand workgroups or so
+    if (!g) g = std::min<int64_t>(rows, std::max(1, 1024 / ((n + 256 * kEach<T> - 1) / (256 * kEach<T>))));
+    return g;
+}
+
+template <class T> hipError_t go(const NormArgs &a, hipStream_t st) {
+    auto launch = [&](auto kernel, int threads, int64_t blocks, int most) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)std::min<int64_t>(blocks, most)), dim3(threads), 0, st, a);
+    };
+    if (!with_form<T>(a.n, [&](auto l, auto p) {
+            constexpr int kL = decltype(l)::value, kEachWg = 256 / kL;
+            launch(norm_kernel<T, kL, decltype(p)::value>, 256, (a.rows + kEachWg - 1) / kEachWg, 2048);
+        })) {
+        constexpr int kE = kEach<T>;
+        if (a.n <= 1024 * 2 * kE) launch(norm_kernel<T, 1024, 2>, 1024, a.rows, 1024);
+        else launch(norm_wide_kernel<T>, 1024, a.rows, 1024);
+    }
+    return hipGetLastError();
+}
+template <class T> hipError_t go_grad(const NormGradArgs &a, void *scratch, hipStream_t st) {
+    const bool sums = a.dw || a.db;
+    float *part = sums ? (float *)scratch : nullptr;
+    const int64_t groups = grad_groups<T>(a.rows, a.n);
+    if (a.rows && !with_form<T>(a.n, [&](auto l, auto p) {
+            hipLaunchKernelGGL((norm_grad_kernel<T, decltype(l)::value, decltype(p)::value>), dim3((unsigned)groups), dim3(256), 0, st,
+                               a, part);
+        })) {
+        constexpr int kE = kEach<T>;
+        if (a.n <= 512 * 2 * kE) {
+            hipLaunchKernelGGL((norm_grad_kernel<T, 512, 2>), dim3((unsigned)groups), dim3(512), 0, st, a, part);
+        } else {
+            if (a.dx)
+                hipLaunchKernelGGL(norm_grad_wide_kernel<T>, dim3((unsigned)std::min<int64_t>(a.rows, 1024)), dim3(1024), 0, st, a);
+            if (part) {
+                const int slabs = (a.n + 256 * kE - 1) / (256 * kE);
+                hipLaunchKernelGGL(norm_columns_kernel<T>, dim3((unsigned)(groups * slabs)), dim3(256), 0, st, a, part, (int)groups);
+            }
+        }
+    }
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !sums) return e;
+    const unsigned blocks = (unsigned)((2 * (int64_t)a.n + 63) / 64);
+    if (a.wide)
+        hipLaunchKernelGGL(norm_join_kernel<float>, dim3(blocks), dim3(1024), 0, st, part, (int)groups, a.n, (float *)a.dw, (float *)a.db);
+    else
+        hipLaunchKernelGGL(norm_join_kernel<T>, dim3(blocks), dim3(1024), 0, st, part, (int)groups, a.n, (T *)a.dw, (T *)a.db);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+int64_t norm_grad_scratch(int type, int64_t rows, int n) {
+    const int64_t groups = type == kOpF32 ? grad_groups<float>(rows, n) : grad_groups<bf16_t>(rows, n);
+    return groups * 2 * n * 4;
+}
+hipError_t launch_norm(int type, const NormArgs &a, hipStream_t st) {
+    if (type == kOpF32) return go<float>(a, st);
+    if (type == kOpBf16) return go<bf16_t>(a, st);
+    return go<f16_t>(a, st);
+}
+hipError_t launch_norm_grad(int type, const NormGradArgs &a, void *scratch, hipStream_t st) {
+    if (type == kOpF32) return go_grad<float>(a, scratch, st);
+    if (type == kOpBf16) return go_grad<bf16_t>(a, scratch, st);
+    return go_grad<f16_t>(a, scratch, st);
+}
+
+}  // namespace ygg

@@ -1,5 +1,7 @@
 // The output head's operators: log-probabilities of given tokens (ygg_logprobs.hip), products of routed experts
-// (ygg_experts.hip) and the int8 projection of float rows (ygg_int8.hip). Every launcher is called with checked sizes.
+// (ygg_experts.hip) and the int8 projection of float rows (ygg_int8.hip); and a recurrent block's: layer norm (ygg_norm.hip), the
+// gated recurrence (ygg_gated_scan.hip), the gated projections (ygg_gated.hip) and clipping by the global norm (ygg_clip.hip).
+// Every launcher is called with checked sizes.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -56,5 +58,64 @@ hipError_t launch_grouped_grad_w(int type, const void *dy, const void *x, const 
 int64_t int8_scratch(int M, int N, int K);
 hipError_t launch_int8_linear(int type, const void *x, const int8_t *w, const float *w_scale, int M, int N, int K, void *y,
                               void *scratch, hipStream_t stream);
+
+struct NormArgs {
+    const void *x;                // rows of n values, `stride` values apart
+    int64_t rows, stride;
+    int n;
+    bool wide;                    // weight and bias in f32, else in x's type; NULL: ones, zeros
+    const void *weight, *bias;
+    float eps;
+    void *y;                      // rows of n, contiguous
+    float *stats;                 // a row's mean and 1 / sqrt(variance + eps); NULL: not kept
+};
+struct NormGradArgs {
+    const void *x;
+    int64_t rows, stride;
+    int n;
+    bool wide;
+    const void *weight;
+    const float *stats;
+    const void *dy;               // rows of n, contiguous, as dx is
+    void *dx, *dw, *db;           // NULL: not wanted
+};
+int64_t norm_grad_scratch(int type, int64_t rows, int n);
+hipError_t launch_norm(int type, const NormArgs &a, hipStream_t stream);
+hipError_t launch_norm_grad(int type, const NormGradArgs &a, void *scratch, hipStream_t stream);
+
+// h_t = gate_t h_{t-1} + x_t over T steps of B sequences of n channels; h, dh, dx and dgate (B, T, n) are contiguous
+struct ScanArgs {
+    const void *gate, *x;
+    int64_t gate_b, gate_t, x_b, x_t;     // values from a sequence, a step, to the next
+    int64_t B, T;
+    int n;
+    const float *state;                   // (B, n); NULL: zeros
+    void *h;
+    float *last;                          // (B, n)
+};
+struct ScanGradArgs {
+    const void *gate, *h, *dh;            // dh NULL: zeros
+    int64_t gate_b, gate_t;
+    int64_t B, T;
+    int n;
+    const float *state, *dlast;           // NULL: zeros
+    void *dx, *dgate;                     // NULL: not wanted
+    float *dstate;
+};
+int64_t scan_scratch(int type, int gate_type, int64_t B, int64_t T, int n);
+hipError_t launch_scan(int type, int gate_type, const ScanArgs &a, void *scratch, hipStream_t stream);
+hipError_t launch_scan_grad(int type, int gate_type, const ScanGradArgs &a, void *scratch, hipStream_t stream);
+
+// With x (M, K) and w (2, N, K): g = x w[0]^T, u = x w[1]^T, y (M, N) = act(g) u
+enum Activation { kSilu = 0, kGelu = 1, kSigmoid = 2 };
+hipError_t launch_gated(int type, int act, const void *x, const void *w, int M, int N, int K, void *y, void *gu, hipStream_t stream);
+int64_t gated_grad_scratch(int type, int M, int N, int K);
+hipError_t launch_gated_grad(int type, int act, const void *x, const void *w, const void *gu, const void *dy, int M, int N, int K,
+                             void *dx, void *dw, void *scratch, hipStream_t stream);
+
+// The norm of `count` tensors' values together; out (NULL: the norm alone) gets them times min(1, most / norm)
+int64_t clip_scratch(const int64_t *sizes, int count);
+hipError_t launch_clip(const void *const *tensors, const int64_t *sizes, const int *types, int count, double most, void *const *out,
+                       float *norm, void *scratch, hipStream_t stream);
 
 }  // namespace ygg

@@ -1,4 +1,4 @@
-// The output head's operators on torch tensors: allocation, the C-ABI call on the tensors' current stream, and the autograd
+// The operators of an output head and of a recurrent block on torch tensors: allocation, the C-ABI call on the tensors' current stream, and the autograd
 // nodes. In C++ for the host's time: a training step's backward pass runs on autograd's own thread, where a node in Python waits
 // for the interpreter lock (a step of 16 rows 96 us with Python nodes, 52 with these), and a call's allocations are most of its
 // cost (one row's log-probabilities 12.6 us from Python, 6.5 from here). Arguments
@@ -7,6 +7,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <map>
 #include <optional>
 #include <string>
@@ -29,6 +30,17 @@ struct {
     decltype(&ygg_grouped_grad_w) grouped_grad_w;
     decltype(&ygg_int8_scratch) int8_scratch;
     decltype(&ygg_int8_linear) int8_linear;
+    decltype(&ygg_layer_norm) layer_norm;
+    decltype(&ygg_layer_norm_scratch) layer_norm_scratch;
+    decltype(&ygg_layer_norm_grad) layer_norm_grad;
+    decltype(&ygg_gated_scan) gated_scan;
+    decltype(&ygg_gated_scan_scratch) gated_scan_scratch;
+    decltype(&ygg_gated_scan_grad) gated_scan_grad;
+    decltype(&ygg_gated_linear) gated_linear;
+    decltype(&ygg_gated_linear_scratch) gated_linear_scratch;
+    decltype(&ygg_gated_linear_grad) gated_linear_grad;
+    decltype(&ygg_clip_scratch) clip_scratch;
+    decltype(&ygg_clip_grad_norm) clip_grad_norm;
     decltype(&ygg_last_error) last_error;
 } api;
 
@@ -42,6 +54,17 @@ void bind(const std::map<std::string, uintptr_t> &at) {
     set(api.grouped_grad_w, "ygg_grouped_grad_w");
     set(api.int8_scratch, "ygg_int8_scratch");
     set(api.int8_linear, "ygg_int8_linear");
+    set(api.layer_norm, "ygg_layer_norm");
+    set(api.layer_norm_scratch, "ygg_layer_norm_scratch");
+    set(api.layer_norm_grad, "ygg_layer_norm_grad");
+    set(api.gated_scan, "ygg_gated_scan");
+    set(api.gated_scan_scratch, "ygg_gated_scan_scratch");
+    set(api.gated_scan_grad, "ygg_gated_scan_grad");
+    set(api.gated_linear, "ygg_gated_linear");
+    set(api.gated_linear_scratch, "ygg_gated_linear_scratch");
+    set(api.gated_linear_grad, "ygg_gated_linear_grad");
+    set(api.clip_scratch, "ygg_clip_scratch");
+    set(api.clip_grad_norm, "ygg_clip_grad_norm");
     set(api.last_error, "ygg_last_error");
 }
 
@@ -192,6 +215,244 @@ Tensor int8_linear(const Tensor &x, const Tensor &w, const Tensor &w_scale) {
     return y;
 }
 
+// ---------------------------------------------------------------------------------------------- a recurrent block's operators
+Tensor scratch_of(const Tensor &like, int64_t bytes) { return bytes ? empty(like, {bytes}, at::kByte) : Tensor(); }
+Tensor or_none(const Maybe &t) { return t.value_or(Tensor()); }
+bool wants_grad(std::initializer_list<Tensor> tensors) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor &t : tensors)
+        if (t.defined() && t.requires_grad()) return true;
+    return false;
+}
+// which of the tensors that a node got (undefined ones are none of its inputs) a backward pass wants gradients of
+std::vector<bool> wanted(AutogradContext *ctx, std::initializer_list<bool> given) {
+    std::vector<bool> want;
+    size_t edge = 0;
+    for (bool g : given) want.push_back(g && ctx->needs_input_grad(edge++));
+    return want;
+}
+
+// rows (M, n) any distance apart -> y, and a row's mean and inverse deviation if they are kept
+std::pair<Tensor, Tensor> layer_norm_of(const Tensor &x, const Tensor &w, const Tensor &b, double eps, bool keep) {
+    const c10::DeviceGuard guard(x.device());
+    const int64_t rows = x.size(0), n = x.size(1);
+    Tensor y = empty(x, {rows, n}, x.scalar_type()), stats;
+    if (keep) stats = empty(x, {rows, 2}, at::kFloat);
+    const Tensor &any = w.defined() ? w : b;
+    check(api.layer_norm(x.data_ptr(), type_of(x), rows, n, rows > 1 ? x.stride(0) : n, ptr(w), ptr(b), any.defined() ? type_of(any) : 0,
+                         eps, y.data_ptr(), ptr<float>(stats), stream_of(x)));
+    return {y, stats};
+}
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Maybe &w, const Maybe &b, double eps) {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        auto [y, stats] = layer_norm_of(x, or_none(w), or_none(b), eps, true);
+        ctx->save_for_backward({x, or_none(w), stats});
+        ctx->saved_data["type"] = w ? (int64_t)type_of(*w) : b ? (int64_t)type_of(*b) : 0;
+        ctx->saved_data["w"] = w.has_value();
+        ctx->saved_data["b"] = b.has_value();
+        return y;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        const variable_list s = ctx->get_saved_variables();
+        const Tensor &x = s[0], &w = s[1], &stats = s[2];
+        const std::vector<bool> want = wanted(ctx, {true, ctx->saved_data["w"].toBool(), ctx->saved_data["b"].toBool()});
+        const c10::DeviceGuard guard(x.device());
+        variable_list out(3), made;
+        {
+            const at::AutoGradMode none(false);
+            no_tangents("layer_norm's gradient", {grads[0]});
+            const Tensor dy = grads[0].contiguous();
+            const int64_t rows = x.size(0), n = x.size(1), type = ctx->saved_data["type"].toInt();
+            const at::ScalarType kind = type == 0 ? at::kFloat : x.scalar_type();
+            if (want[0]) out[0] = empty(x, {rows, n}, x.scalar_type());
+            for (int k : {1, 2})
+                if (want[k]) out[k] = empty(x, {n}, kind);
+            const int64_t need = want[1] || want[2] ? api.layer_norm_scratch(type_of(x), rows, n) : 0;
+            const Tensor scratch = scratch_of(x, need);
+            check(api.layer_norm_grad(x.data_ptr(), type_of(x), rows, n, rows > 1 ? x.stride(0) : n, ptr(w), type, ptr<float>(stats),
+                                      dy.data_ptr(), ptr(out[0]), ptr(out[1]), ptr(out[2]), ptr(scratch), need, stream_of(x)));
+            for (const Tensor &t : out)
+                if (t.defined()) made.push_back(t);
+        }
+        made = once(std::move(made), "layer_norm");
+        size_t k = 0;
+        for (Tensor &t : out)
+            if (t.defined()) t = made[k++];
+        out.push_back(Tensor());
+        return out;
+    }
+};
+Tensor layer_norm(const Tensor &x, const Maybe &w, const Maybe &b, double eps) {
+    no_tangents("layer_norm", {x, or_none(w), or_none(b)});
+    if (wants_grad({x, or_none(w), or_none(b)})) return LayerNorm::apply(x, w, b, eps);
+    return layer_norm_of(x, or_none(w), or_none(b), eps, false).first;
+}
+
+// gate, x (B, T, n), a step's channels next to each other; state (B, n) or undefined -> h, the last state
+std::pair<Tensor, Tensor> gated_scan_of(const Tensor &gate, const Tensor &x, const Tensor &state) {
+    const c10::DeviceGuard guard(x.device());
+    const int64_t B = x.size(0), T = x.size(1), n = x.size(2);
+    Tensor h = empty(x, {B, T, n}, x.scalar_type()), last = empty(x, {B, n}, at::kFloat);
+    const int64_t need = api.gated_scan_scratch(type_of(x), type_of(gate), B, T, n);
+    const Tensor scratch = scratch_of(x, need);
+    check(api.gated_scan(gate.data_ptr(), type_of(gate), gate.stride(0), gate.stride(1), x.data_ptr(), type_of(x), x.stride(0), x.stride(1),
+                         B, T, n, ptr<float>(state), h.data_ptr(), ptr<float>(last), ptr(scratch), need, stream_of(x)));
+    return {h, last};
+}
+struct GatedScan : torch::autograd::Function<GatedScan> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &gate, const Tensor &x, const Maybe &state) {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        auto [h, last] = gated_scan_of(gate, x, or_none(state));
+        ctx->save_for_backward({gate, h, or_none(state)});
+        ctx->set_materialize_grads(false);
+        return {h, last};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        const variable_list s = ctx->get_saved_variables();
+        const Tensor &gate = s[0], &h = s[1], &state = s[2];
+        const std::vector<bool> want = wanted(ctx, {true, true, state.defined()});
+        const c10::DeviceGuard guard(h.device());
+        variable_list out(3), made;
+        {
+            const at::AutoGradMode none(false);
+            for (const Tensor &g : grads) no_tangents("gated_scan's gradient", {g});
+            const Tensor dh = grads[0].defined() ? grads[0].contiguous() : Tensor(), dlast = grads[1].defined() ? grads[1].contiguous() : Tensor();
+            const int64_t B = h.size(0), T = h.size(1), n = h.size(2);
+            if (want[0]) out[0] = empty(h, {B, T, n}, gate.scalar_type());
+            if (want[1]) out[1] = empty(h, {B, T, n}, h.scalar_type());
+            if (want[2]) out[2] = empty(h, {B, n}, at::kFloat);
+            const int64_t need = api.gated_scan_scratch(type_of(h), type_of(gate), B, T, n);
+            const Tensor scratch = scratch_of(h, need);
+            check(api.gated_scan_grad(gate.data_ptr(), type_of(gate), gate.stride(0), gate.stride(1), h.data_ptr(), type_of(h), B, T, n,
+                                      ptr<float>(state), ptr(dh), ptr<float>(dlast), ptr(out[1]), ptr(out[0]), ptr<float>(out[2]),
+                                      ptr(scratch), need, stream_of(h)));
+            for (const Tensor &t : out)
+                if (t.defined()) made.push_back(t);
+        }
+        made = once(std::move(made), "gated_scan");
+        size_t k = 0;
+        for (Tensor &t : out)
+            if (t.defined()) t = made[k++];
+        return out;
+    }
+};
+std::pair<Tensor, Tensor> gated_scan(const Tensor &gate, const Tensor &x, const Maybe &state) {
+    no_tangents("gated_scan", {gate, x, or_none(state)});
+    if (wants_grad({gate, x, or_none(state)})) {
+        const variable_list r = GatedScan::apply(gate, x, state);
+        return {r[0], r[1]};
+    }
+    return gated_scan_of(gate, x, or_none(state));
+}
+
+// x (M, K), w (2, N, K) -> y, and g and u (M, 2, N) if they are kept
+std::pair<Tensor, Tensor> gated_linear_of(const Tensor &x, const Tensor &w, int64_t act, bool keep) {
+    const c10::DeviceGuard guard(x.device());
+    const int64_t M = x.size(0), N = w.size(1), K = x.size(1);
+    Tensor y = empty(x, {M, N}, x.scalar_type()), gu;
+    if (keep) gu = empty(x, {M, 2, N}, x.scalar_type());
+    check(api.gated_linear(x.data_ptr(), w.data_ptr(), type_of(x), act, M, N, K, y.data_ptr(), ptr(gu), stream_of(x)));
+    return {y, gu};
+}
+struct GatedLinear : torch::autograd::Function<GatedLinear> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, int64_t act) {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        auto [y, gu] = gated_linear_of(x, w, act, true);
+        ctx->save_for_backward({x, w, gu});
+        ctx->saved_data["act"] = act;
+        return y;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        const variable_list s = ctx->get_saved_variables();
+        const Tensor &x = s[0], &w = s[1], &gu = s[2];
+        const bool to_x = ctx->needs_input_grad(0), to_w = ctx->needs_input_grad(1);
+        const c10::DeviceGuard guard(x.device());
+        variable_list out;
+        {
+            const at::AutoGradMode none(false);
+            no_tangents("gated_linear's gradient", {grads[0]});
+            const Tensor dy = grads[0].contiguous();
+            const int64_t M = x.size(0), N = w.size(1), K = x.size(1), need = api.gated_linear_scratch(type_of(x), M, N, K);
+            const Tensor scratch = scratch_of(x, need);
+            if (to_x) out.push_back(empty(x, {M, K}, x.scalar_type()));
+            if (to_w) out.push_back(empty(x, {2, N, K}, x.scalar_type()));
+            check(api.gated_linear_grad(x.data_ptr(), w.data_ptr(), gu.data_ptr(), dy.data_ptr(), type_of(x), ctx->saved_data["act"].toInt(),
+                                        M, N, K, to_x ? out[0].data_ptr() : nullptr, to_w ? out[to_x].data_ptr() : nullptr, ptr(scratch),
+                                        need, stream_of(x)));
+        }
+        out = once(std::move(out), "gated_linear");
+        return {to_x ? out[0] : Tensor(), to_w ? out[to_x] : Tensor(), Tensor()};
+    }
+};
+Tensor gated_linear(const Tensor &x, const Tensor &w, int64_t act) {
+    no_tangents("gated_linear", {x, w});
+    if (wants_grad({x, w})) return GatedLinear::apply(x, w, act);
+    return gated_linear_of(x, w, act, false).first;
+}
+
+// The norm of the tensors' values together and, with clip, the tensors times min(1, most / norm): into out, tensors of their
+// sizes and types (themselves among them), or new ones. Memory that is written may be no other tensor's.
+struct Range {
+    uintptr_t from, end;
+    size_t i;
+};
+std::vector<Range> ranges_of(const std::vector<Tensor> &tensors) {
+    std::vector<Range> r;
+    for (size_t i = 0; i < tensors.size(); i++) {
+        const uintptr_t p = (uintptr_t)tensors[i].data_ptr();
+        if (tensors[i].numel()) r.push_back({p, p + tensors[i].nbytes(), i});
+    }
+    return r;
+}
+std::pair<std::vector<Tensor>, Tensor> clip_grad_norm(std::vector<Tensor> in, double most, bool clip, const std::optional<std::vector<Tensor>> &to) {
+    const Tensor first = in.at(0);
+    for (const Tensor &t : in) no_tangents("clip_grad_norm", {t});
+    const c10::DeviceGuard guard(first.device());
+    const at::AutoGradMode none(false);
+    std::vector<Tensor> out;
+    if (clip && to) {
+        out = *to;
+        for (const Tensor &t : out)
+            if (t.layout() != at::kStrided || !t.is_non_overlapping_and_dense()) throw py::value_error("out must hold dense tensors");
+        std::vector<Range> written = ranges_of(out);
+        std::sort(written.begin(), written.end(), [](const Range &a, const Range &b) { return a.from < b.from; });
+        for (size_t k = 1; k < written.size(); k++)
+            if (written[k].from < written[k - 1].end) throw py::value_error("two tensors that clip_grad_norm writes share memory");
+        for (const Range &r : ranges_of(in)) {
+            // the written ones that end past r's begin: those from here on
+            auto w = std::upper_bound(written.begin(), written.end(), r.from, [](uintptr_t p, const Range &b) { return p < b.end; });
+            for (; w != written.end() && w->from < r.end; ++w)
+                if (w->i != r.i || w->from != r.from) throw py::value_error("clip_grad_norm would write into memory of another of its tensors");
+        }
+    }
+    std::vector<const void *> from(in.size());
+    std::vector<void *> into(in.size());
+    std::vector<int64_t> sizes(in.size());
+    std::vector<int> types(in.size());
+    for (size_t i = 0; i < in.size(); i++) {
+        // values go in the order they lie in memory, the same in both
+        if (!in[i].is_non_overlapping_and_dense()) in[i] = in[i].contiguous();
+        if (clip) {
+            if (!to) out.push_back(at::empty_like(in[i]));
+            if (out[i].strides() != in[i].strides()) in[i] = at::empty_like(out[i]).copy_(in[i]);
+            into[i] = out[i].data_ptr();
+        }
+        from[i] = in[i].data_ptr();
+        sizes[i] = in[i].numel();
+        types[i] = type_of(in[i]);
+    }
+    Tensor norm = empty(first, {}, at::kFloat);
+    const int64_t need = api.clip_scratch(sizes.data(), (int)sizes.size());
+    const Tensor scratch = scratch_of(first, need);
+    check(api.clip_grad_norm(from.data(), sizes.data(), types.data(), (int)sizes.size(), most, clip ? into.data() : nullptr,
+                             norm.data_ptr<float>(), ptr(scratch), need, stream_of(first)));
+    if (clip && to)
+        for (const Tensor &t : out)
+            if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    return {out, norm};
+}
+
 // The calls on tensors that need no reshaping, checked here; nothing where they do, or where a check fails and ops.py says why
 bool floats(const Tensor &t, int64_t dim) {
     const auto d = t.scalar_type();
@@ -225,6 +486,29 @@ Maybe plain_int8_linear(const Tensor &x, const Tensor &w, const Tensor &w_scale)
     return int8_linear(x, w, w_scale);
 }
 
+bool vector_like(const Maybe &t, const Tensor &x, int64_t n) {
+    return !t || ((like(*t, x, at::kFloat, 1) || like(*t, x, x.scalar_type(), 1)) && t->size(0) == n);
+}
+Maybe plain_layer_norm(const Tensor &x, const Maybe &w, const Maybe &b, double eps) {
+    if (!floats(x, 2) || !within(x.size(1), 1, YGG_MOST_INNER) || !vector_like(w, x, x.size(1)) || !vector_like(b, x, x.size(1)) ||
+        (w && b && w->scalar_type() != b->scalar_type()) || !(eps >= 0) || !(eps <= 1e30))
+        return std::nullopt;
+    return layer_norm(x, w, b, eps);
+}
+std::optional<std::pair<Tensor, Tensor>> plain_gated_scan(const Tensor &gate, const Tensor &x, const Maybe &state) {
+    if (!floats(x, 3) || !(like(gate, x, at::kFloat, 3) || like(gate, x, x.scalar_type(), 3)) || gate.sizes() != x.sizes() ||
+        !within(x.size(0), 0, YGG_MOST_ROWS) || !within(x.size(1), 0, YGG_MOST_STEPS) || !within(x.size(2), 1, YGG_MOST_INNER))
+        return std::nullopt;
+    if (state && !(like(*state, x, at::kFloat, 2) && state->size(0) == x.size(0) && state->size(1) == x.size(2))) return std::nullopt;
+    return gated_scan(gate, x, state);
+}
+Maybe plain_gated_linear(const Tensor &x, const Tensor &w, int64_t act) {
+    if (!floats(x, 2) || !like(w, x, x.scalar_type(), 3) || w.size(0) != 2 || w.size(2) != x.size(1) || x.size(0) > YGG_MOST_ROWS ||
+        !within(w.size(1), 1, YGG_MOST_INNER / 2) || !within(x.size(1), 1, YGG_MOST_INNER))
+        return std::nullopt;
+    return gated_linear(x, w, act);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_ygg_torch, m) {
@@ -232,7 +516,14 @@ PYBIND11_MODULE(_ygg_torch, m) {
     m.def("token_logprobs", &token_logprobs);
     m.def("grouped_matmul", &grouped_matmul);
     m.def("int8_linear", &int8_linear);
+    m.def("layer_norm", &layer_norm);
+    m.def("gated_scan", &gated_scan);
+    m.def("gated_linear", &gated_linear);
+    m.def("clip_grad_norm", &clip_grad_norm);
     m.def("plain_token_logprobs", &plain_token_logprobs);
     m.def("plain_grouped_matmul", &plain_grouped_matmul);
     m.def("plain_int8_linear", &plain_int8_linear);
+    m.def("plain_layer_norm", &plain_layer_norm);
+    m.def("plain_gated_scan", &plain_gated_scan);
+    m.def("plain_gated_linear", &plain_gated_linear);
 }

@@ -1,12 +1,18 @@
-"""Operators of an output head on the GPU, for programs that train, score or serve one next to the model's own step:
+"""Operators of an output head and of a recurrent block on the GPU, for programs that train, score or serve them next to the
+model's own step:
 
     r = token_logprobs(logits, tokens, top=5)       # .logp, .entropy, .top_logp, .top_ids; differentiable
     offsets, order = group_rows(leaves, experts)    # rows by the expert they take
     y = grouped_matmul(x, w, offsets, order)        # y_i = W[expert of i] x_i; differentiable
     y = int8_linear(x, w_int8, w_scale)             # rows quantised to int8, an int8 matrix with scales
 
-The kernels are those of csrc/ygg_logprobs.hip, csrc/ygg_experts.hip and csrc/ygg_int8.hip, through the C-ABI of
-include/ygg_hip.h, on the current torch stream of the tensors' device (csrc/ygg_torch.cpp: allocation, the call, autograd).
+    y = layer_norm(x, weight, bias)                 # differentiable
+    h, last = gated_scan(gate, x, state)            # h_t = gate_t h_{t-1} + x_t; differentiable
+    y = gated_linear(x, w, "silu")                  # silu(x w[0]^T) (x w[1]^T); differentiable
+    grads, norm = clip_grad_norm(grads, 1.0)        # by the norm of all of them
+
+The kernels are those of csrc/ygg_logprobs.hip, ygg_experts.hip and ygg_int8.hip, and of ygg_norm.hip, ygg_gated_scan.hip,
+ygg_gated.hip and ygg_clip.hip, through the C-ABI of include/ygg_hip.h, on the current torch stream of the tensors' device (csrc/ygg_torch.cpp: allocation, the call, autograd).
 Nothing waits for the GPU, so a call can be captured into a graph; values that only the GPU holds (tokens, offsets, an order)
 are not checked here, and bad ones give wrong or NaN values, never an access out of bounds. Types: float32, bfloat16 and
 float16. Derivatives are first ones in reverse mode: second ones and forward-mode tangents are refused.
@@ -26,6 +32,9 @@ MOST_VOCAB = 1 << 24
 MOST_ROWS = 1 << 24
 MOST_EXPERTS = 1 << 20
 MOST_INNER = 1 << 17
+MOST_STEPS = 1 << 30
+MOST_VALUES = 1 << 40
+ACTIVATIONS = {"silu": 0, "gelu": 1, "sigmoid": 2}
 
 
 def _floats(t, name: str) -> torch.Tensor:
@@ -52,7 +61,9 @@ def _tensors(x, *others) -> bool:
 
 
 _ENTRIES = ("ygg_logprobs_scratch", "ygg_logprobs", "ygg_logprobs_grad", "ygg_grouped_matmul", "ygg_grouped_grad_x",
-            "ygg_grouped_grad_w", "ygg_int8_scratch", "ygg_int8_linear", "ygg_last_error")
+            "ygg_grouped_grad_w", "ygg_int8_scratch", "ygg_int8_linear", "ygg_layer_norm", "ygg_layer_norm_scratch",
+            "ygg_layer_norm_grad", "ygg_gated_scan", "ygg_gated_scan_scratch", "ygg_gated_scan_grad", "ygg_gated_linear",
+            "ygg_gated_linear_scratch", "ygg_gated_linear_grad", "ygg_clip_scratch", "ygg_clip_grad_norm", "ygg_last_error")
 _module = None
 
 
@@ -207,4 +218,138 @@ def int8_linear(x, w, w_scale) -> torch.Tensor:
     return y if x.dim() == 2 else y.reshape(x.shape[:-1] + (N,))
 
 
-__all__ = ["LogProbs", "token_logprobs", "group_rows", "grouped_matmul", "quantize_weight", "int8_linear"]
+# ---------------------------------------------------------------------------------------------- a recurrent block
+def layer_norm(x, weight=None, bias=None, eps: float = 1e-5) -> torch.Tensor:
+    """x (..., n) -> (x - mean) / sqrt(variance + eps) * weight + bias over the last axis, in x's type. weight and bias (n) are
+    f32 or in x's type, both the same; None: ones, zeros. Mean and variance (the mean of the squares about the mean) are in
+    f32. Differentiable in all three; the gradients of weight and bias are summed in f32, in the same order every time. A row
+    that holds a NaN or an infinity is NaN."""
+    if type(eps) is float and _tensors(x, *[t for t in (weight, bias) if t is not None]):
+        y = _native().plain_layer_norm(x, weight, bias, eps)
+        if y is not None:
+            return y
+    _floats(x, "x")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MOST_INNER:
+        raise ValueError(f"x of shape {tuple(x.shape)}: the last axis holds 1 to {MOST_INNER} values")
+    n = x.shape[-1]
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is not None:
+            _on(t, x.device, name, (torch.float32, x.dtype), (n,))
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError(f"weight in {weight.dtype}, bias in {bias.dtype}: both in one type")
+    if not (isinstance(eps, (int, float)) and 0 <= eps <= 1e30):
+        raise ValueError(f"eps {eps!r}: a finite number of at least 0")
+    weight = weight if weight is None else weight.contiguous()
+    bias = bias if bias is None else bias.contiguous()
+    return _native().layer_norm(_rows(x), weight, bias, float(eps)).reshape(x.shape)
+
+
+def _steps(t: torch.Tensor) -> torch.Tensor:
+    """t (B, T, n), a step's channels next to each other; a copy where they are not."""
+    return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
+
+
+def gated_scan(gate, x, state=None):
+    """The gated recurrence h_t = gate_t h_{t-1} + x_t of every channel: gate and x (B, T, n), the gate in f32 or in x's type, and
+    the state before the first step (B, n) f32 (None: zeros) -> h (B, T, n) in x's type and the last state (B, n) f32. For
+    serving, one step at a time with the state carried on; for training, differentiable in all three, over long sequences.
+
+    States are held in f32. Runs of steps are joined by the products of their gates: gates are meant to be at most 1 in
+    magnitude, and others have to keep the product of every run of steps finite. A gate of 0 begins anew (a document's first
+    step); a step with gate 1 and x 0 keeps the state (padding behind a sequence's end leaves the last state right). The gate's
+    gradient takes h as it was returned, in x's type."""
+    if _tensors(x, gate) if state is None else _tensors(x, gate, state):
+        r = _native().plain_gated_scan(gate, x, state)
+        if r is not None:
+            return r
+    _floats(x, "x")
+    if x.dim() != 3:
+        raise ValueError(f"x of shape {tuple(x.shape)}, expected (B, T, n)")
+    _on(gate, x.device, "gate", (torch.float32, x.dtype), x.shape)
+    B, T, n = x.shape
+    if B > MOST_ROWS or T > MOST_STEPS or not 1 <= n <= MOST_INNER:
+        raise ValueError(f"B = {B}, T = {T}, n = {n}: at most {MOST_ROWS} sequences of {MOST_STEPS} steps, n 1 to {MOST_INNER}")
+    if state is not None:
+        _on(state, x.device, "state", (torch.float32,), (B, n))
+        state = state.contiguous()
+    return _native().gated_scan(_steps(gate), _steps(x), state)
+
+
+def gated_linear(x, w, activation: str = "silu") -> torch.Tensor:
+    """The gated projections of a feed-forward block in one kernel: x (..., K), w (2, N, K) in x's type ->
+    act(x w[0]^T) (x w[1]^T) (..., N) in x's type, act "silu" (g sigmoid(g)), "gelu" (g Phi(g)) or "sigmoid". Sums and
+    the product are in f32, rounded once. Differentiable in x and w: for that, both projections are kept in x's type, and the
+    gradients' products take their factors in it."""
+    act = ACTIVATIONS.get(activation) if isinstance(activation, str) else None
+    if act is None:
+        raise ValueError(f"activation {activation!r}: one of {', '.join(ACTIVATIONS)}")
+    if _tensors(x, w):
+        y = _native().plain_gated_linear(x, w, act)
+        if y is not None:
+            return y
+    _floats(x, "x")
+    if x.dim() < 1:
+        raise ValueError("x needs an axis of K values")
+    K = x.shape[-1]
+    _on(w, x.device, "w", (x.dtype,))
+    if w.dim() != 3 or w.shape[0] != 2 or w.shape[2] != K:
+        raise ValueError(f"w of shape {tuple(w.shape)}, expected (2, N, {K})")
+    N = w.shape[1]
+    if not 1 <= N <= MOST_INNER // 2 or not 1 <= K <= MOST_INNER:
+        raise ValueError(f"N = {N}, K = {K}: N 1 to {MOST_INNER // 2}, K 1 to {MOST_INNER}")
+    x2 = x.reshape(-1, K).contiguous()
+    if len(x2) > MOST_ROWS:
+        raise ValueError(f"{len(x2)} rows: at most {MOST_ROWS}")
+    return _native().gated_linear(x2, w.contiguous(), act).reshape(x.shape[:-1] + (N,))
+
+
+def _clip(grads, most: float, clip: bool, out=None):
+    grads = list(grads)
+    some = [i for i, g in enumerate(grads) if g is not None]
+    if not some:
+        raise ValueError("no gradients")
+    tensors = [grads[i] for i in some]
+    for g in tensors:
+        _floats(g, "a gradient")
+        if g.device != tensors[0].device or g.layout != torch.strided or g.numel() > MOST_VALUES:
+            raise ValueError(f"gradients must be dense tensors on one device, of at most {MOST_VALUES} values each")
+        if clip and g.requires_grad and torch.is_grad_enabled():
+            raise ValueError("clip_grad_norm has no gradient: call it under torch.no_grad() or with detached tensors")
+    if out is not None:
+        out = list(out)
+        if len(out) != len(grads) or any((o is None) != (g is None) for o, g in zip(out, grads)):
+            raise ValueError("out must hold a tensor for every gradient, and None where there is none")
+        to = [out[i] for i in some]
+        for o, g in zip(to, tensors):
+            _on(o, g.device, "out", (g.dtype,), g.shape)
+            if o.requires_grad and torch.is_grad_enabled():
+                raise ValueError("out must hold tensors that require no gradient")
+        return out, _native().clip_grad_norm(tensors, most, clip, to)[1]
+    r, norm = _native().clip_grad_norm(tensors, most, clip, None)
+    if clip and len(some) < len(grads):
+        whole = [None] * len(grads)
+        for i, t in zip(some, r):
+            whole[i] = t
+        r = whole
+    return r, norm
+
+
+def grad_norm(grads) -> torch.Tensor:
+    """The norm of all values of the tensors together (None: left out), the root of the sum of their squares: () f32, squares
+    summed in 64 bits, in the same order every time."""
+    with torch.no_grad():
+        return _clip(grads, 0.0, False)[1]
+
+
+def clip_grad_norm(grads, max_norm: float, out=None):
+    """Gradients (None: there is none) brought to a norm of at most max_norm together: each times min(1, max_norm / norm), rounded
+    once -> the list of them, and the norm that they had, () f32. New tensors, or out: tensors of their shapes and types, also
+    the gradients themselves (out=grads: in place); no others may share memory with what is written. A norm that is NaN or
+    infinite leaves the values as they are; the caller sees it in the norm. Nothing waits for the GPU."""
+    if not (isinstance(max_norm, (int, float)) and max_norm >= 0):
+        raise ValueError(f"max_norm {max_norm!r}: a number of at least 0")
+    return _clip(grads, float(max_norm), True, out)
+
+
+__all__ = ["LogProbs", "token_logprobs", "group_rows", "grouped_matmul", "quantize_weight", "int8_linear", "layer_norm",
+           "gated_scan", "gated_linear", "grad_norm", "clip_grad_norm"]
