@@ -337,8 +337,9 @@ int ygg_gated_scan_grad(const void *d_gate, int gate_type, int64_t gate_b, int64
                         float *d_dstate, void *d_scratch, int64_t scratch_bytes, void *stream);
 
 /* The gated projections of a feed-forward block: x (M, K), w (2, N, K) contiguous, g = x w[0]^T, u = x w[1]^T, y (M, N) =
-   act(g) u in x's type; act: 0 silu (g sigmoid(g)), 1 gelu (g Phi(g)), 2 sigmoid. N up to YGG_MOST_INNER / 2. d_gu (M, 2, N)
-   in x's type or NULL: g and u, which the gradients want. */
+   act(g) u in x's type; act: 0 silu (g sigmoid(g)), 1 gelu (g Phi(g)), 2 sigmoid. N up to YGG_MOST_INNER / 2. d_gu: NULL or
+   memory of ygg_gated_linear_kept bytes for g and u, which the gradients want (f32, or its upper 24 bits for 16-bit types). */
+int64_t ygg_gated_linear_kept(int type, int M, int N);
 int ygg_gated_linear(const void *d_x, const void *d_w, int type, int act, int M, int N, int K, void *d_y, void *d_gu, void *stream);
 /* The gradients, from dy (M, N): of the rows and of w. NULL: not wanted. */
 int64_t ygg_gated_linear_scratch(int type, int M, int N, int K);

@@ -125,7 +125,9 @@ def test_nothing_to_do_is_done():
     assert L.ygg_gated_linear_grad(*{**GATED_GRAD, "dx": None, "dw": None}.values()) == 0
     assert L.ygg_layer_norm_scratch(0, 0, 8) == 0 and L.ygg_layer_norm_scratch(5, 1, 8) == 0
     assert L.ygg_gated_scan_scratch(0, 0, 0, 8, 8) == 0 and L.ygg_gated_scan_scratch(0, 0, 512, 100, 1024) == 0
-    assert L.ygg_gated_linear_scratch(7, 1, 1, 1) == 0 and L.ygg_clip_scratch(None, 3) == 0
+    assert L.ygg_gated_linear_scratch(7, 1, 1, 1) == 0 and L.ygg_gated_linear_scratch(1, 0, 8, 8) == 0
+    assert L.ygg_gated_linear_kept(1, 0, 8) == 0 and L.ygg_gated_linear_kept(1, 5, 8) == 240 and L.ygg_gated_linear_kept(0, 5, 8) == 320
+    assert L.ygg_clip_scratch(None, 3) == 0
 
 
 def test_the_limits_are_the_headers():

@@ -1423,6 +1423,11 @@ int ygg_gated_linear(const void *d_x, const void *d_w, int type, int act, int M,
     return YGG_OK;
 }
 
+int64_t ygg_gated_linear_kept(int type, int M, int N) {
+    if (type < 0 || type > 2 || M < 0 || M > YGG_MOST_ROWS || N < 1 || N > YGG_MOST_INNER / 2) return 0;
+    return ygg::gated_kept(type, M, N);
+}
+
 int64_t ygg_gated_linear_scratch(int type, int M, int N, int K) {
     if (type < 0 || type > 2 || M < 0 || M > YGG_MOST_ROWS || N < 1 || N > YGG_MOST_INNER / 2 || K < 1 || K > YGG_MOST_INNER) return 0;
     return ygg::gated_grad_scratch(type, M, N, K);
@@ -1434,7 +1439,7 @@ int ygg_gated_linear_grad(const void *d_x, const void *d_w, const void *d_gu, co
     if ((M == 0 || !d_dx) && !d_dw) return YGG_OK;
     if ((M > 0 && (!d_x || !d_w || !d_gu || !d_dy))) return fail(YGG_ERR_ARG, "NULL buffer");
     const int64_t need = ygg::gated_grad_scratch(type, M, N, K);
-    if (!d_scratch || scratch_bytes < need)
+    if (need && (!d_scratch || scratch_bytes < need))
         return fail(YGG_ERR_ARG, "scratch of %lld bytes, %lld wanted", (long long)scratch_bytes, (long long)need);
     OP_TRY(ygg::launch_gated_grad(type, act, d_x, d_w, d_gu, d_dy, M, N, K, M ? d_dx : nullptr, d_dw, d_scratch, (hipStream_t)stream));
     return YGG_OK;

@@ -3,9 +3,12 @@
 //
 // A tile computes g and u of the same columns: a wave's 64 columns of the columns' operand are 32 rows of Wg and the 32 rows of
 // Wu below them, so a lane ends up with 8 neighbouring values of g and the same 8 of u, in f32, and takes their product there. For a
-// backward pass g and u are kept in the inputs' type (a rounding more in dy's factors, the size of the one that dg and du take
-// to enter the matrix cores), one row of 2 N values each: dg and du are laid out alike, so that with w as (2 N, K) both
-// gradients are single products, those of ygg_experts.hip with one expert that takes every row.
+// backward pass g and u are kept: of 16-bit types the upper 24 bits of f32, so that the only roundings that the gradients have and
+// g and u's own do not are those of dg and du on their way into the matrix cores and the results'. dg and du lie in rows of
+// 2 N values: with w as (2 N, K) each gradient is a single product,
+//   dx = [dg du] w,  dw = [dg du]^T x,
+// of operands in tiles of their own; where the tiles are few for the 256 CUs the reduction is cut too, and the parts, in f32, are
+// added in their order.
 #include <algorithm>
 
 #include "ygg_gemm.h"
@@ -38,24 +41,89 @@ template <class F> __host__ __device__ __forceinline__ auto with_act(int act, F 
     return f(std::integral_constant<int, kSigmoid>());
 }
 
+constexpr int kBand = 16;     // rows of tiles of a band
+
 // the row of w of a tile's column o, the tile's outputs beginning at n0
 __device__ __forceinline__ int row_of_w(int o, int n0, int N) { return (o & 32 ? N : 0) + min(n0 + (o >> 6) * 32 + (o & 31), N - 1); }
 
+// g and u of M rows of 2 N values, kept for the backward pass: f32, or its upper 24 bits, first all values' 16 and then their 8
+// (in 16 bits alone the gradients were 1.8 times as far off as a rounding, in 24 1.4; the 16384 x 4096 of a bf16 case take the memory
+// 134 MB longer on the way out and in)
+template <class T> struct Kept {
+    static constexpr int kBytes = sizeof(T) == 4 ? 4 : 3;
+    char *p;
+    int64_t count;
+    // kN values from place `at` on, of which the first `left` exist
+    template <int kN> __device__ __forceinline__ void put(int64_t at, const float *v, int left) const {
+        if constexpr (sizeof(T) == 4) {
+            store_run<float, kN>((float *)p + at, v, left);
+        } else {
+            uint32_t b[kN];
+#pragma unroll
+            for (int j = 0; j < kN; j++)      // to nearest; a NaN must not carry into the sign
+                b[j] = v[j] == v[j] ? __builtin_bit_cast(uint32_t, v[j]) + 0x80u : 0x7fc00000u;
+            typedef uint32_t hi_t __attribute__((ext_vector_type(kN / 2), aligned(1)));
+            typedef uint32_t lo_t __attribute__((ext_vector_type(kN / 4), aligned(1)));
+            uint16_t *hi = (uint16_t *)p + at;
+            uint8_t *lo = (uint8_t *)p + 2 * count + at;
+            if (left >= kN) {
+                hi_t h;
+                lo_t l;
+#pragma unroll
+                for (int j = 0; j < kN / 2; j++) h[j] = b[2 * j] >> 16 | (b[2 * j + 1] & 0xffff0000u);
+#pragma unroll
+                for (int j = 0; j < kN / 4; j++)
+                    l[j] = (b[4 * j] >> 8 & 0xffu) | (b[4 * j + 1] & 0xff00u) | (b[4 * j + 2] & 0xff00u) << 8 | (b[4 * j + 3] & 0xff00u) << 16;
+                *(hi_t *)hi = h;
+                *(lo_t *)lo = l;
+            } else {
+#pragma unroll
+                for (int j = 0; j < kN; j++)
+                    if (j < left) {
+                        hi[j] = (uint16_t)(b[j] >> 16);
+                        lo[j] = (uint8_t)(b[j] >> 8);
+                    }
+            }
+        }
+    }
+    template <int kN> __device__ __forceinline__ void get(int64_t at, float *v, int left) const {
+        if constexpr (sizeof(T) == 4) {
+            static_assert(kN == 4, "");
+            unpack(load16((const float *)p + at, left), v, 0.0f);
+        } else {
+            static_assert(kN == 8, "");
+            const u32x4 h = load16((const uint16_t *)p + at, left);
+            const uint8_t *lo = (const uint8_t *)p + 2 * count + at;
+            u32x2 l = {0, 0};
+            if (left >= kN) {
+                __builtin_memcpy(&l, lo, 8);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kN; j++)
+                    if (j < left) l[j / 4] |= (uint32_t)lo[j] << 8 * (j % 4);
+            }
+#pragma unroll
+            for (int j = 0; j < kN; j++)
+                v[j] = __builtin_bit_cast(float, (h[j / 2] >> 16 * (j % 2)) << 16 | (l[j / 4] >> 8 * (j % 4) & 0xffu) << 8);
+        }
+    }
+};
+
 // kN neighbouring outputs of a row
 template <class T, int kAct, int kN>
-__device__ __forceinline__ void put_outputs(const float *g, const float *u, int row, int n, int N, T *y, T *gu) {
+__device__ __forceinline__ void put_outputs(const float *g, const float *u, int row, int n, int N, T *y, const Kept<T> &gu) {
     float v[kN];
 #pragma unroll
     for (int j = 0; j < kN; j++) v[j] = act_of<kAct>(g[j]) * u[j];
     store_run<T, kN>(y + (int64_t)row * N + n, v, N - n);
-    if (gu) {
-        T *p = gu + (int64_t)row * 2 * N + n;
-        store_run<T, kN>(p, g, N - n);
-        store_run<T, kN>(p + N, u, N - n);
+    if (gu.p) {
+        const int64_t at = (int64_t)row * 2 * N + n;
+        gu.template put<kN>(at, g, N - n);
+        gu.template put<kN>(at + N, u, N - n);
     }
 }
 template <class T, int kAct, int FI, class Acc>
-__device__ __forceinline__ void put_tile(Acc (&acc)[FI][4], int row0, int part, int M, int n0, int N, T *y, T *gu, int i0) {
+__device__ __forceinline__ void put_tile(Acc (&acc)[FI][4], int row0, int part, int M, int n0, int N, T *y, const Kept<T> &gu, int i0) {
     const int l = threadIdx.x & 63, n = n0 + part * 32 + 8 * (l >> 4);
     if (n >= N) return;
 #pragma unroll
@@ -66,7 +134,7 @@ __device__ __forceinline__ void put_tile(Acc (&acc)[FI][4], int row0, int part, 
 }
 
 template <class T, int FI, int WI, int WO, int kAct>
-__global__ __launch_bounds__(64 * WI * WO) void gated_kernel(const T *x, const T *w, int M, int N, int K, T *y, T *gu, int cols, int band) {
+__global__ __launch_bounds__(64 * WI * WO) void gated_kernel(const T *x, const T *w, int M, int N, int K, T *y, Kept<T> gu, int cols, int band) {
     constexpr int kThreads = 64 * WI * WO, kI = 16 * FI * WI, kO = 64 * WO;
     typedef Along<T, kI, kThreads, FI, true> A;
     typedef Along<T, kO, kThreads, 4, false> B;
@@ -88,7 +156,7 @@ __global__ __launch_bounds__(64 * WI * WO) void gated_kernel(const T *x, const T
 
 // Aligned rows, straight to LDS
 template <class T, int kAct>
-__global__ __launch_bounds__(512) void gated_turn_kernel(const T *x, const T *w, int M, int N, int K, T *y, T *gu, int cols, int band) {
+__global__ __launch_bounds__(512) void gated_turn_kernel(const T *x, const T *w, int M, int N, int K, T *y, Kept<T> gu, int cols, int band) {
     typedef AlongLds<T, 8, 2, true> A;
     typedef AlongLds<T, 4, 4, false> B;
     typedef TurnTile<T, 8, 4, 2, 4, A, B> Tl;
@@ -108,7 +176,7 @@ __global__ __launch_bounds__(512) void gated_turn_kernel(const T *x, const T *w,
 
 // Few rows: 16 of them by 16 outputs a workgroup, whose kW waves take a part of K each, fragments straight from memory
 template <class T, int kW, int kAct>
-__global__ __launch_bounds__(64 * kW) void gated_few_kernel(const T *x, const T *w, int M, int N, int K, T *y, T *gu, int cols) {
+__global__ __launch_bounds__(64 * kW) void gated_few_kernel(const T *x, const T *w, int M, int N, int K, T *y, Kept<T> gu, int cols) {
     constexpr int kE = 16 / sizeof(T), kStep = 4 * kE, kU = 4;
     __shared__ f32x4 parts[kW][2][64];
     const int t = tile_of(blockIdx.x, gridDim.x), n0 = t % cols * 16, l = threadIdx.x & 63, wave = threadIdx.x >> 6, d = l & 15, q = l >> 4;
@@ -161,23 +229,18 @@ __global__ __launch_bounds__(64 * kW) void gated_few_kernel(const T *x, const T 
     if (row < M && n < N) put_outputs<T, kAct, 4>((const float *)&acc[0], (const float *)&acc[1], row, n, N, y, gu);
 }
 
-// dg and du of pieces of 16 bytes of dy; and the one expert's offsets
+// dg and du of pieces of 16 bytes of dy
 template <class T, int kAct>
-__global__ __launch_bounds__(256) void gated_slope_kernel(const T *gu, const T *dy, int M, int N, T *dgu, int32_t *offsets) {
+__global__ __launch_bounds__(256) void gated_slope_kernel(Kept<T> gu, const T *dy, int M, int N, T *dgu) {
     constexpr int kE = 16 / sizeof(T);
     const int per = (N + kE - 1) / kE;
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / per;
-    if (id == 0) {
-        offsets[0] = 0;
-        offsets[1] = M;
-    }
     if (row >= M) return;
     const int n = (int)(id % per) * kE, left = N - n;
-    const T *p = gu + row * 2 * N + n, *q = dy + row * N + n;
     float g[kE], u[kE], d[kE];
-    unpack(load16(p, left), g, T());
-    unpack(load16(p + N, left), u, T());
-    unpack(load16(q, left), d, T());
+    gu.template get<kE>(row * 2 * N + n, g, left);
+    gu.template get<kE>(row * 2 * N + n + N, u, left);
+    unpack(load16(dy + row * N + n, left), d, T());
 #pragma unroll
     for (int j = 0; j < kE; j++) {
         float slope;
@@ -190,11 +253,100 @@ __global__ __launch_bounds__(256) void gated_slope_kernel(const T *gu, const T *
     store_run<T, kE>(out + N, u, left);
 }
 
+// ---- the gradients' products: out (I, O) = sum over r of A(i, r) b(r, o). kRows: A is a (I, R), else a^T, a (R, I). A workgroup takes the
+// steps of its part of the reduction; of more than one part, the sums go to `sums` in f32, part after part.
+struct Dense {
+    const void *a, *b;
+    int I, O, R;
+    void *out;
+    float *sums;
+    int tiles, cols, per;       // tiles of a part, tiles along O, steps of a part
+};
+template <class T> struct DenseOut {
+    const Dense &g;
+    int part, i0, o0;
+    template <class N> __device__ __forceinline__ void operator()(int i, int o, const float *v, N) const {
+        if (i0 + i >= g.I || o0 + o >= g.O) return;
+        const int64_t at = (int64_t)(i0 + i) * g.O + o0 + o;
+        if (g.sums) store_run<float, N::value>(g.sums + (int64_t)part * g.I * g.O + at, v, g.O - o0 - o);
+        else store_run<T, N::value>((T *)g.out + at, v, g.O - o0 - o);
+    }
+};
+template <class T, int FI, int WI, int WO, bool kRows>
+__global__ __launch_bounds__(64 * WI * WO) void dense_kernel(const Dense g) {
+    constexpr int kThreads = 64 * WI * WO, kI = 16 * FI * WI, kO = 64 * WO;
+    typedef std::conditional_t<kRows, Along<T, kI, kThreads, FI, true>, Across<T, kI, kThreads>> A;
+    typedef Across<T, kO, kThreads> B;
+    typedef Tile<T, FI, 4, WI, WO, A, B> Tl;
+    __shared__ __align__(128) char lds[Tl::kLds];
+    const int part = blockIdx.x / g.tiles;
+    const Place t = place_of(tile_of(blockIdx.x % g.tiles, g.tiles), g.tiles / g.cols, g.cols, kBand);
+    const int i0 = t.row * kI, o0 = t.col * kO, steps = (g.R + A::kStep - 1) / A::kStep, first = part * g.per;
+    Tl tile;
+    A a;
+    B b;
+    if constexpr (kRows) a.begin([&](int i) { return (const T *)g.a + (int64_t)min(i0 + i, g.I - 1) * g.R; });
+    else a.begin((const T *)g.a, i0, g.I);
+    b.begin((const T *)g.b, o0, g.O);
+    tile.run(a, b, lds, min(g.per, steps - first), [&](int s) {
+        const int r0 = (first + s) * A::kStep;
+        if constexpr (kRows) a.load(r0, g.R);
+        else a.load([&](int i) { return r0 + A::r_of(i) < g.R ? (int64_t)(r0 + A::r_of(i)) * g.I : -1; });
+        b.load([&](int i) { return r0 + B::r_of(i) < g.R ? (int64_t)(r0 + B::r_of(i)) * g.O : -1; });
+    });
+    const DenseOut<T> put = {g, part, i0, o0};
+    tile.template each<false>([&](int i, int o, const typename Tl::Acc *v, auto n) { put(i, o, (const float *)v, n); });
+}
+template <class T, bool kRows> __global__ __launch_bounds__(512) void dense_turn_kernel(const Dense g) {
+    constexpr int kSize = sizeof(T);
+    typedef std::conditional_t<kRows, AlongLds<T, 8, 2, true>, AcrossLds<T, 8, 2>> A;
+    typedef AcrossLds<T, 4, 4> B;
+    typedef TurnTile<T, 8, 4, 2, 4, A, B> Tl;
+    __shared__ __align__(1024) char lds[Tl::kLds];
+    const int part = blockIdx.x / g.tiles;
+    const Place t = place_of(tile_of(blockIdx.x % g.tiles, g.tiles), g.tiles / g.cols, g.cols, kBand);
+    const int i0 = t.row * 256, o0 = t.col * 256, steps = (g.R + B::kStep - 1) / B::kStep, first = part * g.per;
+    const uint32_t a_row = (kRows ? g.R : g.I) * kSize, b_row = g.O * kSize;
+    Tl tile;
+    A a;
+    B b;
+    if constexpr (kRows) a.begin(g.a, g.I * a_row, a_row, [&](int i) { return i0 + i < g.I ? (uint32_t)(i0 + i) * a_row : kFar; });
+    else a.begin(g.a, g.R * a_row, i0 * kSize, (g.I - i0) * kSize);
+    b.begin(g.b, g.R * b_row, o0 * kSize, (g.O - o0) * kSize);
+    tile.clear();
+    auto row = [&](int s, int in_step, uint32_t bytes) {
+        const int r = (first + s) * B::kStep + in_step;
+        return r < g.R ? (uint32_t)r * bytes : kFar;
+    };
+    tile.run(lds, min(g.per, steps - first),
+             [&](auto h, int s, uint32_t to) {
+                 if constexpr (kRows) a.template load<decltype(h)::value>(first + s, to);
+                 else a.template load<decltype(h)::value>(to, [&](int i) { return row(s, A::r_of(i), a_row); });
+             },
+             [&](auto h, int s, uint32_t to) { b.template load<decltype(h)::value>(to, [&](int i) { return row(s, B::r_of(i), b_row); }); },
+             [](int) {}, kRows ? min(g.I - i0, 256) : 256);
+    const DenseOut<T> put = {g, part, i0, o0};
+    tile.template each<false>([&](int i, int o, const typename Tl::Acc *v, auto n) { put(i, o, (const float *)v, n); });
+}
+// the parts' sums, added in their order
+template <class T> __global__ __launch_bounds__(256) void parts_kernel(const float *sums, int parts, int64_t count, T *out) {
+    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (at >= count) return;
+    const int left = (int)min(count - at, (int64_t)4);
+    float v[4], p[4];
+    unpack(load16(sums + at, left), v, 0.0f);
+    for (int k = 1; k < parts; k++) {
+        unpack(load16(sums + k * count + at, left), p, 0.0f);
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] += p[j];
+    }
+    store_run<T, 4>(out + at, v, left);
+}
+
 bool aligned16(const void *p, int64_t row_bytes) { return (uintptr_t)p % 16 == 0 && row_bytes % 16 == 0; }
 constexpr int64_t kMostBytes = 0x78000000;   // of an operand with 32-bit offsets: kFar and a few steps stay past it
-constexpr int kBand = 16;
-
-template <class T, int kAct> hipError_t go(const void *x, const void *w, int M, int N, int K, void *y, void *gu, hipStream_t st) {
+template <class T, int kAct> hipError_t go(const void *x, const void *w, int M, int N, int K, void *y, void *kept, hipStream_t st) {
+    const Kept<T> gu = {(char *)kept, (int64_t)M * 2 * N};
     const int64_t row = (int64_t)K * sizeof(T);
     if constexpr (sizeof(T) == 2) {
         const int cols = (N + 127) / 128;
@@ -202,14 +354,14 @@ template <class T, int kAct> hipError_t go(const void *x, const void *w, int M, 
         if (aligned16(x, row) && aligned16(w, row) && M * row < kMostBytes && 2 * N * row < kMostBytes && tiles >= 256 &&
             tiles <= most_blocks(512)) {
             hipLaunchKernelGGL((gated_turn_kernel<T, kAct>), dim3((unsigned)tiles), dim3(512), 0, st, (const T *)x, (const T *)w, M, N, K,
-                               (T *)y, (T *)gu, cols, kBand);
+                               (T *)y, gu, cols, kBand);
             return hipGetLastError();
         }
     }
     if (M <= 16) {
         const int cols = (N + 15) / 16;
         hipLaunchKernelGGL((gated_few_kernel<T, 4, kAct>), dim3((unsigned)cols), dim3(256), 0, st, (const T *)x, (const T *)w, M, N, K,
-                           (T *)y, (T *)gu, cols);
+                           (T *)y, gu, cols);
         return hipGetLastError();
     }
     auto tiles = [&](auto fi, auto wi, auto wo) {
@@ -218,7 +370,7 @@ template <class T, int kAct> hipError_t go(const void *x, const void *w, int M, 
         const int64_t all = ((int64_t)M + kI - 1) / kI * cols;
         if (all > most_blocks(64 * WI * WO)) return kTooLarge;
         hipLaunchKernelGGL((gated_kernel<T, FI, WI, WO, kAct>), dim3((unsigned)all), dim3(64 * WI * WO), 0, st, (const T *)x,
-                           (const T *)w, M, N, K, (T *)y, (T *)gu, cols, kBand);
+                           (const T *)w, M, N, K, (T *)y, gu, cols, kBand);
         return hipGetLastError();
     };
     constexpr std::integral_constant<int, 2> two{};
@@ -226,12 +378,58 @@ template <class T, int kAct> hipError_t go(const void *x, const void *w, int M, 
     const int64_t tiles128 = ((int64_t)M + 127) / 128 * ((N + 63) / 64);
     return tiles128 >= 512 ? tiles(four, two, two) : tiles(two, two, two);
 }
-template <class T, int kAct> hipError_t go_slope(const void *gu, const void *dy, int M, int N, void *dgu, int32_t *offsets, hipStream_t st) {
+template <class T, int kAct> hipError_t go_slope(const void *gu, const void *dy, int M, int N, void *dgu, hipStream_t st) {
     constexpr int kE = 16 / sizeof(T);
-    const int64_t blocks = std::max<int64_t>(((int64_t)M * ((N + kE - 1) / kE) + 255) / 256, 1);   // without rows for the offsets
+    const int64_t blocks = ((int64_t)M * ((N + kE - 1) / kE) + 255) / 256;
+    if (blocks == 0) return hipSuccess;
     if (blocks > most_blocks(256)) return kTooLarge;
-    hipLaunchKernelGGL((gated_slope_kernel<T, kAct>), dim3((unsigned)blocks), dim3(256), 0, st, (const T *)gu, (const T *)dy, M, N, (T *)dgu,
-                       offsets);
+    hipLaunchKernelGGL((gated_slope_kernel<T, kAct>), dim3((unsigned)blocks), dim3(256), 0, st, Kept<T>{(char *)gu, (int64_t)M * 2 * N},
+                       (const T *)dy, M, N, (T *)dgu);
+    return hipGetLastError();
+}
+
+// How a product is cut: 256 x 256 tiles straight to LDS where rows are aligned (`turn`), else kI rows of a tile; the reduction in parts
+struct Plan {
+    bool turn, large;
+    int cols, parts, per;
+    int64_t tiles;
+};
+Plan plan_of(int size, bool rows, int I, int O, int R, bool aligned) {
+    const int64_t a_bytes = (int64_t)I * R * size, b_bytes = (int64_t)R * O * size;
+    const int step = 128 / size, steps = (R + step - 1) / step;
+    Plan p = {};
+    auto cut = [&](int ti, int to, int64_t want, int least) {
+        p.cols = (O + to - 1) / to;
+        p.tiles = ((int64_t)I + ti - 1) / ti * p.cols;
+        const int64_t parts = std::max<int64_t>(std::min<int64_t>(want / std::max<int64_t>(p.tiles, 1), steps / least), 1);
+        p.per = (int)std::max<int64_t>((steps + parts - 1) / parts, 1);
+        p.parts = std::max((steps + p.per - 1) / p.per, 1);      // without rows there is still the weights' gradient, zero
+    };
+    if (size == 2 && aligned && (rows ? R : I) % 8 == 0 && O % 8 == 0 && a_bytes < kMostBytes && b_bytes < kMostBytes && I >= 192 && O >= 192) {
+        cut(256, 256, 256, 8);
+        p.turn = p.tiles * p.parts >= 128;
+        if (p.turn) return p;
+    }
+    p.large = ((int64_t)I + 127) / 128 * ((O + 127) / 128) >= 512;
+    cut(p.large ? 128 : 64, 128, 768, 6);
+    return p;
+}
+int64_t part_bytes(const Plan &p, int I, int O) { return p.parts > 1 ? (int64_t)p.parts * I * O * 4 : 0; }
+template <class T, bool kRows>
+hipError_t go_dense(const void *a, const void *b, int I, int O, int R, void *out, const Plan &p, void *sums, hipStream_t st) {
+    const int64_t blocks = p.tiles * p.parts, count = (int64_t)I * O;
+    if (blocks > most_blocks(512)) return kTooLarge;
+    const Dense g = {a, b, I, O, R, out, p.parts > 1 ? (float *)sums : nullptr, (int)p.tiles, p.cols, p.per};
+    if (p.turn) {
+        if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((dense_turn_kernel<T, kRows>), dim3((unsigned)blocks), dim3(512), 0, st, g);
+    } else if (p.large) {
+        hipLaunchKernelGGL((dense_kernel<T, 4, 2, 2, kRows>), dim3((unsigned)blocks), dim3(256), 0, st, g);
+    } else {
+        hipLaunchKernelGGL((dense_kernel<T, 2, 2, 2, kRows>), dim3((unsigned)blocks), dim3(256), 0, st, g);
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.parts == 1) return e;
+    hipLaunchKernelGGL(parts_kernel<T>, dim3((unsigned)((count + 1023) / 1024)), dim3(256), 0, st, (const float *)sums, p.parts, count, (T *)out);
     return hipGetLastError();
 }
 template <class F> hipError_t with_type(int type, F f) {
@@ -247,18 +445,32 @@ hipError_t launch_gated(int type, int act, const void *x, const void *w, int M, 
         return with_act(act, [&](auto k) { return go<decltype(one), decltype(k)::value>(x, w, M, N, K, y, gu, st); });
     });
 }
-int64_t gated_grad_scratch(int type, int M, int N, int) { return 256 + (int64_t)M * 2 * N * op_bytes(type); }
+int64_t gated_kept(int type, int M, int N) { return (int64_t)M * 2 * N * (type == kOpF32 ? 4 : 3); }
+// dg and du, then the parts' sums of one product at a time; whether the rows turn out to be aligned or not
+int64_t dgu_bytes(int type, int M, int N) { return ((int64_t)M * 2 * N * op_bytes(type) + 255) / 256 * 256; }
+int64_t gated_grad_scratch(int type, int M, int N, int K) {
+    const int size = op_bytes(type);
+    int64_t sums = 0;
+    for (bool aligned : {false, true})
+        sums = std::max({sums, part_bytes(plan_of(size, true, M, K, 2 * N, aligned), M, K), part_bytes(plan_of(size, false, 2 * N, K, M, aligned), 2 * N, K)});
+    return dgu_bytes(type, M, N) + sums;
+}
 hipError_t launch_gated_grad(int type, int act, const void *x, const void *w, const void *gu, const void *dy, int M, int N, int K,
                              void *dx, void *dw, void *scratch, hipStream_t st) {
-    int32_t *offsets = (int32_t *)scratch;
-    void *dgu = (char *)scratch + 256;
+    void *dgu = scratch, *sums = (char *)scratch + dgu_bytes(type, M, N);
+    const int size = op_bytes(type);
     hipError_t e = with_type(type, [&](auto one) {
-        return with_act(act, [&](auto k) { return go_slope<decltype(one), decltype(k)::value>(gu, dy, M, N, dgu, offsets, st); });
+        return with_act(act, [&](auto k) { return go_slope<decltype(one), decltype(k)::value>(gu, dy, M, N, dgu, st); });
     });
-    const Groups g = {offsets, nullptr, M, 1};
-    if (e == hipSuccess && dx) e = launch_grouped_grad_x(type, dgu, w, g, 2 * N, K, dx, st);
-    if (e == hipSuccess && dw) e = launch_grouped_grad_w(type, dgu, x, g, 2 * N, K, dw, st);
-    return e;
+    if (e != hipSuccess) return e;
+    return with_type(type, [&](auto one) {
+        typedef decltype(one) T;
+        hipError_t e = hipSuccess;
+        if (dx) e = go_dense<T, true>(dgu, w, M, K, 2 * N, dx, plan_of(size, true, M, K, 2 * N, (uintptr_t)w % 16 == 0), sums, st);
+        if (e == hipSuccess && dw)
+            e = go_dense<T, false>(dgu, x, 2 * N, K, M, dw, plan_of(size, false, 2 * N, K, M, (uintptr_t)x % 16 == 0), sums, st);
+        return e;
+    });
 }
 
 }  // namespace ygg

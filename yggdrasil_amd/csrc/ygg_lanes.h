@@ -7,13 +7,14 @@
 
 namespace ygg {
 
-// A value joined over groups of kG lanes (4, 16 or 64), the same in each of them
+// A value joined over groups of kG lanes (1, 4, 16 or 64), the same in each of them
 template <int kControl> __device__ __forceinline__ uint32_t rotated(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kControl, 0xf, 0xf, true);
 }
 template <int kG, class V, class F> __device__ __forceinline__ V join(V v, F f) {
     static_assert(sizeof(V) == 4, "");
     auto turn = [&](uint32_t o) { v = f(v, __builtin_bit_cast(V, o)); };
+    if constexpr (kG == 1) return v;
     if constexpr (kG == 4) {
         turn(rotated<0xb1>(__builtin_bit_cast(uint32_t, v)));     // quad_perm 1 0 3 2, 2 3 0 1
         turn(rotated<0x4e>(__builtin_bit_cast(uint32_t, v)));

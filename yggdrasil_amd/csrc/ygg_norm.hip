@@ -18,26 +18,30 @@ namespace {
 
 template <class T> constexpr int kEach = 16 / (int)sizeof(T);    // values of a piece
 
-// piece i of lane `lane` of kL: its first column
-template <class T, int kL> __device__ __forceinline__ int column(int i, int lane) { return (i * kL + lane) * kEach<T>; }
-
-// A row's pieces; columns that there are not come as zero
-template <class T, int kL, int kP>
-__device__ __forceinline__ void load_row(u32x4 (&v)[kP], const T *p, int n, int lane) {
-    constexpr int kE = kEach<T>;
-    if (n % kE == 0) {
-#pragma unroll
-        for (int i = 0; i < kP; i++) v[i] = load16(p + min(column<T, kL>(i, lane), n - kE));
-#pragma unroll
-        for (int i = 0; i < kP; i++)
-            if (column<T, kL>(i, lane) >= n) v[i] = u32x4{0, 0, 0, 0};
-    } else if (n > kE) {
-#pragma unroll
-        for (int i = 0; i < kP; i++) v[i] = load16_end(p + column<T, kL>(i, lane), n - column<T, kL>(i, lane));
-    } else {
-#pragma unroll
-        for (int i = 0; i < kP; i++) v[i] = load16(p + column<T, kL>(i, lane), n - column<T, kL>(i, lane));
+// A row of n values in pieces: piece i of lane `lane` of kL. The last piece of a row that it does not fill begins earlier, so that
+// nothing in the rows' loop is cut: its first `skip` values are the piece's before it, computed and written twice alike and left
+// out of the sums. kTiny: rows of less than a piece, one lane's.
+template <class T, int kL, bool kTiny> struct Pieces {
+    static constexpr int kE = kEach<T>;
+    int n, lane;
+    __device__ __forceinline__ int at(int i) const { return (i * kL + lane) * kE; }
+    __device__ __forceinline__ int column(int i) const { return kTiny ? 0 : min(at(i), n - kE); }
+    __device__ __forceinline__ bool some(int i) const { return at(i) < n; }
+    __device__ __forceinline__ int skip(int i) const { return at(i) - column(i); }
+    // all lanes' pieces are whole and their own
+    __device__ __forceinline__ bool whole(int i) const { return !kTiny && (i + 1) * kL * kE <= n; }
+    // value j of piece i is summed here
+    __device__ __forceinline__ bool own(int i, int j) const { return kTiny ? lane == 0 && j < n : j >= skip(i); }
+    __device__ __forceinline__ u32x4 load(const T *p, int i) const { return kTiny ? load16(p, n) : load16(p + column(i)); }
+    template <class O> __device__ __forceinline__ void store(O *p, const float *f, int i) const {
+        if (some(i)) store_run<O, kE>(p + column(i), f, kTiny ? n : kE);
     }
+};
+
+// What was unpacked from these before is not held until it is wanted again, but unpacked again
+template <int kP> __device__ __forceinline__ void let_go(u32x4 (&v)[kP]) {
+#pragma unroll
+    for (int i = 0; i < kP; i++) asm volatile("" : "+v"(v[i])::"memory");
 }
 
 // kN values of a weight from column c on, in f32; `other` where there are none
@@ -67,99 +71,123 @@ __device__ __forceinline__ void load_weight(float *f, const void *p, bool wide, 
 
 // The mean and 1 / sqrt(variance + eps) of a row held by kL lanes. waves: LDS of a workgroup of more than a wave, another one
 // than the row before's.
-template <class T, int kL, int kP>
-__device__ __forceinline__ float2 moments(const u32x4 (&x)[kP], int n, float eps, int lane, float2 *waves) {
-    constexpr int kE = kEach<T>;
-    float sum = 0.0f;
+template <class T, int kL, bool kTiny, int kP>
+__device__ __forceinline__ float2 moments(u32x4 (&x)[kP], const Pieces<T, kL, kTiny> &at, float eps, float2 *waves) {
+    constexpr int kE = kEach<T>, kIn = kL < 64 ? kL : 64;
+    const int n = at.n;
+    // f(a value of the row that is this lane's)
+    auto each = [&](auto f) {
 #pragma unroll
-    for (int i = 0; i < kP; i++) {
-        float f[kE];
-        unpack(x[i], f, T());
+        for (int i = 0; i < kP; i++) {
+            float v[kE];
+            unpack(x[i], v, T());
+            if (at.whole(i)) {
 #pragma unroll
-        for (int j = 0; j < kE; j++) sum += f[j];
-    }
-    constexpr int kIn = kL < 64 ? kL : 64;
-    // the wave's values: whole pieces of 64 lanes, the last one cut
-    const int wave = lane / 64;
+                for (int j = 0; j < kE; j++) f(v[j], true);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kE; j++) f(v[j], at.own(i, j));
+            }
+        }
+    };
+    float sum = 0.0f, squares = 0.0f;
+    each([&](float v, bool own) { sum += own ? v : 0.0f; });
+    // the values that a wave holds
     auto held = [&](int w) {
         int h = 0;
 #pragma unroll
         for (int i = 0; i < kP; i++) h += min(max(n - (i * kL + w * 64) * kE, 0), 64 * kE);
-        return h;
+        return (float)h;
     };
-    const float mine = kL <= 64 ? (float)n : (float)held(wave);
-    float mean = sum_of<kIn>(sum) / fmaxf(mine, 1.0f);
-    float squares = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kP; i++) {
-        float f[kE];
-        unpack(x[i], f, T());
-        const int left = n - column<T, kL>(i, lane);
-#pragma unroll
-        for (int j = 0; j < kE; j++) {
-            const float d = j < left ? f[j] - mean : 0.0f;
-            squares = __builtin_fmaf(d, d, squares);
-        }
-    }
+    const int wave = at.lane / 64;
+    float mean = sum_of<kIn>(sum) / fmaxf(kL <= 64 ? (float)n : held(wave), 1.0f);
+    let_go(x);
+    each([&](float v, bool own) {
+        const float d = own ? v - mean : 0.0f;
+        squares = __builtin_fmaf(d, d, squares);
+    });
     squares = sum_of<kIn>(squares);
     if constexpr (kL > 64) {
-        if (lane % 64 == 0) waves[wave] = make_float2(mean, squares);
+        if (at.lane % 64 == 0) waves[wave] = make_float2(mean, squares);
         __syncthreads();
         float total = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kL / 64; w++) total = __builtin_fmaf((float)held(w), waves[w].x, total);
+        for (int w = 0; w < kL / 64; w++) total = __builtin_fmaf(held(w), waves[w].x, total);
         mean = total / (float)n;
         squares = 0.0f;
 #pragma unroll
         for (int w = 0; w < kL / 64; w++) {
             const float d = waves[w].x - mean;
-            squares += __builtin_fmaf((float)held(w) * d, d, waves[w].y);
+            squares += __builtin_fmaf(held(w) * d, d, waves[w].y);
         }
     }
     return make_float2(mean, 1.0f / sqrtf(squares / (float)n + eps));
 }
 
-// kL lanes a row, kP pieces a lane. Up to kHold values a lane the weights stay in registers over a workgroup's rows.
-constexpr int kHold = 32;
-template <class T, int kL, int kP>
-__global__ __launch_bounds__(kL > 256 ? kL : 256) void norm_kernel(const NormArgs a) {
-    constexpr int kThreads = kL > 256 ? kL : 256, kRows = kThreads / kL, kE = kEach<T>;
-    constexpr bool kHeld = kL <= 256 && kP * kE <= kHold;
-    __shared__ float2 waves[2][kThreads / 64];
-    const int lane = threadIdx.x % kL, n = a.n;
-    float w[kP][kE], b[kP][kE];
-    if constexpr (kHeld) {
+// A weight in f32 in LDS, in the order its lanes read it, 16 bytes each: in registers it would hold the rows off the CU
+template <class T, int kL, int kP> struct Held {
+    static constexpr int kE = kEach<T>;
+    float v[kP][kE / 4][kL][4];
+    template <int kThreads, bool kTiny> __device__ __forceinline__ void fill(const void *p, bool wide, int n, float other) {
+        for (int k = threadIdx.x; k < kP * kL; k += kThreads) {
+            const Pieces<T, kL, kTiny> at = {n, k % kL};
+            float f[kE];
+            load_weight<T, kE>(f, p, wide, at.column(k / kL), n, other);
 #pragma unroll
-        for (int i = 0; i < kP; i++) {
-            load_weight<T, kE>(w[i], a.weight, a.wide, column<T, kL>(i, lane), n, 1.0f);
-            load_weight<T, kE>(b[i], a.bias, a.wide, column<T, kL>(i, lane), n, 0.0f);
+            for (int j = 0; j < kE; j++) v[k / kL][j / 4][k % kL][j % 4] = f[j];
         }
     }
+    __device__ __forceinline__ void get(float *f, int i, int lane) const {
+#pragma unroll
+        for (int j = 0; j < kE; j++) f[j] = v[i][j / 4][lane][j % 4];
+    }
+};
+
+// kL lanes a row, kP pieces a lane; the next row's loads are on their way while a row is normed
+template <class T, int kL, int kP, bool kTiny>
+__global__ __launch_bounds__(kL > 256 ? kL : 256) void norm_kernel(const NormArgs a) {
+    constexpr int kThreads = kL > 256 ? kL : 256, kRows = kThreads / kL, kE = kEach<T>;
+    __shared__ float2 waves[2][kThreads / 64];
+    constexpr bool kHeld = kL <= 256 || kP <= 2;      // wider rows' weights do not fit LDS: from the caches for each row
+    __shared__ Held<T, kHeld ? kL : 1, kHeld ? kP : 1> w, b;
+    const Pieces<T, kL, kTiny> at = {a.n, (int)threadIdx.x % kL};
     const int64_t hop = (int64_t)gridDim.x * kRows;
     int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kL;
-    if (row >= a.rows) return;     // whole groups of lanes; of a workgroup a row, none
     u32x4 x[kP], next[kP];
-    load_row<T, kL>(next, (const T *)a.x + row * a.stride, n, lane);
+    auto load = [&](int64_t r) {
+        if (r >= a.rows) return;
+#pragma unroll
+        for (int i = 0; i < kP; i++) next[i] = at.load((const T *)a.x + r * a.stride, i);
+    };
+    load(row);
+    if constexpr (kHeld) {
+        w.template fill<kThreads, kTiny>(a.weight, a.wide, a.n, 1.0f);
+        b.template fill<kThreads, kTiny>(a.bias, a.wide, a.n, 0.0f);
+        __syncthreads();
+    }
     for (int turn = 0; row < a.rows; row += hop, turn ^= 1) {
 #pragma unroll
         for (int i = 0; i < kP; i++) x[i] = next[i];
-        if (row + hop < a.rows) load_row<T, kL>(next, (const T *)a.x + (row + hop) * a.stride, n, lane);
-        const float2 s = moments<T, kL>(x, n, a.eps, lane, waves[turn]);
-        if (a.stats && lane == 0) ((float2 *)a.stats)[row] = s;
-        T *y = (T *)a.y + row * n;
+        load(row + hop);
+        const float2 s = moments(x, at, a.eps, waves[turn]);
+        if (a.stats && at.lane == 0) ((float2 *)a.stats)[row] = s;
+        let_go(x);
+        const float c = -s.x * s.y;        // z = x / deviation + c: its rounding is one more of the mean's
+        T *y = (T *)a.y + row * a.n;
 #pragma unroll
         for (int i = 0; i < kP; i++) {
-            const int c = column<T, kL>(i, lane);
-            if (c >= n) break;
-            if constexpr (!kHeld) {
-                load_weight<T, kE>(w[i], a.weight, a.wide, c, n, 1.0f);
-                load_weight<T, kE>(b[i], a.bias, a.wide, c, n, 0.0f);
-            }
-            float f[kE];
+            float f[kE], wf[kE], bf[kE];
             unpack(x[i], f, T());
+            if constexpr (kHeld) {
+                w.get(wf, i, at.lane);
+                b.get(bf, i, at.lane);
+            } else {
+                load_weight<T, kE>(wf, a.weight, a.wide, at.column(i), a.n, 1.0f);
+                load_weight<T, kE>(bf, a.bias, a.wide, at.column(i), a.n, 0.0f);
+            }
 #pragma unroll
-            for (int j = 0; j < kE; j++) f[j] = __builtin_fmaf((f[j] - s.x) * s.y, w[i][j], b[i][j]);
-            store_run<T, kE>(y + c, f, n - c);
+            for (int j = 0; j < kE; j++) f[j] = __builtin_fmaf(__builtin_fmaf(f[j], s.y, c), wf[j], bf[j]);
+            at.store(y, f, i);
         }
     }
 }
@@ -220,30 +248,34 @@ template <class T> __global__ __launch_bounds__(1024) void norm_wide_kernel(cons
 }
 
 // ---- backward: dx, and a workgroup's sums of dy z and dy over its rows into part[blockIdx][2][n]
-template <class T, int kL, int kP>
+template <class T, int kL, int kP, bool kTiny>
 __global__ __launch_bounds__(kL > 256 ? kL : 256) void norm_grad_kernel(const NormGradArgs a, float *part) {
     constexpr int kThreads = kL > 256 ? kL : 256, kRows = kThreads / kL, kE = kEach<T>, kIn = kL < 64 ? kL : 64;
     __shared__ float2 waves[2][kThreads / 64];
     __shared__ float sums[kL <= 64 ? 2 : 1][kL <= 64 ? kL * kP * kE : 1];
-    const int lane = threadIdx.x % kL, n = a.n;
-    float w[kP][kE], aw[kP][kE], ab[kP][kE];
+    __shared__ Held<T, kL, kP> w;
+    const int n = a.n;
+    const Pieces<T, kL, kTiny> at = {n, (int)threadIdx.x % kL};
+    float aw[kP][kE], ab[kP][kE];
 #pragma unroll
-    for (int i = 0; i < kP; i++) {
-        load_weight<T, kE>(w[i], a.weight, a.wide, column<T, kL>(i, lane), n, 1.0f);
+    for (int i = 0; i < kP; i++)
 #pragma unroll
         for (int j = 0; j < kE; j++) aw[i][j] = ab[i][j] = 0.0f;
-    }
     const int64_t hop = (int64_t)gridDim.x * kRows;
     int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kL;
     u32x4 x[kP], dy[kP], next_x[kP], next_dy[kP];
     float2 s = {0, 0}, next_s = {0, 0};
     auto load = [&](int64_t r) {
         if (r >= a.rows) return;
-        load_row<T, kL>(next_x, (const T *)a.x + r * a.stride, n, lane);
-        load_row<T, kL>(next_dy, (const T *)a.dy + r * n, n, lane);
+#pragma unroll
+        for (int i = 0; i < kP; i++) next_x[i] = at.load((const T *)a.x + r * a.stride, i);
+#pragma unroll
+        for (int i = 0; i < kP; i++) next_dy[i] = at.load((const T *)a.dy + r * n, i);
         next_s = ((const float2 *)a.stats)[r];
     };
     load(row);
+    w.template fill<kThreads, kTiny>(a.weight, a.wide, n, 1.0f);
+    __syncthreads();
     for (int turn = 0; row < a.rows; row += hop, turn ^= 1) {
 #pragma unroll
         for (int i = 0; i < kP; i++) {
@@ -252,26 +284,32 @@ __global__ __launch_bounds__(kL > 256 ? kL : 256) void norm_grad_kernel(const No
         }
         s = next_s;
         load(row + hop);
+        const float c = -s.x * s.y;
         float q1 = 0.0f, q2 = 0.0f;
 #pragma unroll
         for (int i = 0; i < kP; i++) {
-            float f[kE], d[kE];
+            float f[kE], d[kE], wf[kE];
             unpack(x[i], f, T());
             unpack(dy[i], d, T());
+            w.get(wf, i, at.lane);
+            if (!at.whole(i)) {
+#pragma unroll
+                for (int j = 0; j < kE; j++) d[j] = at.own(i, j) ? d[j] : 0.0f;
+            }
 #pragma unroll
             for (int j = 0; j < kE; j++) {
-                const float z = (f[j] - s.x) * s.y, q = w[i][j] * d[j];
+                const float z = __builtin_fmaf(f[j], s.y, c), q = wf[j] * d[j];
                 aw[i][j] = __builtin_fmaf(d[j], z, aw[i][j]);
                 ab[i][j] += d[j];
                 q1 += q;
                 q2 = __builtin_fmaf(q, z, q2);
             }
+            __builtin_amdgcn_sched_barrier(0);     // a piece at a time, for the registers
         }
-        if (!a.dx) continue;
         q1 = sum_of<kIn>(q1);
         q2 = sum_of<kIn>(q2);
         if constexpr (kL > 64) {
-            if (lane % 64 == 0) waves[turn][lane / 64] = make_float2(q1, q2);
+            if (at.lane % 64 == 0) waves[turn][at.lane / 64] = make_float2(q1, q2);
             __syncthreads();
             q1 = q2 = 0.0f;
 #pragma unroll
@@ -280,33 +318,38 @@ __global__ __launch_bounds__(kL > 256 ? kL : 256) void norm_grad_kernel(const No
                 q2 += waves[turn][k].y;
             }
         }
-        q1 /= (float)n;
-        q2 /= (float)n;
+        if (!a.dx) continue;       // not before the joins: the compiler would hold all the values that they add until then
+        q1 *= -s.y / (float)n;
+        q2 *= -s.y / (float)n;
+        let_go(x);
+        let_go(dy);
         T *dx = (T *)a.dx + row * n;
 #pragma unroll
         for (int i = 0; i < kP; i++) {
-            const int c = column<T, kL>(i, lane);
-            if (c >= n) break;
-            float f[kE], d[kE];
+            float f[kE], d[kE], wf[kE];
             unpack(x[i], f, T());
             unpack(dy[i], d, T());
+            w.get(wf, i, at.lane);
 #pragma unroll
             for (int j = 0; j < kE; j++) {
-                const float z = (f[j] - s.x) * s.y, q = w[i][j] * d[j];
-                f[j] = (q - q1 - z * q2) * s.y;
+                const float z = __builtin_fmaf(f[j], s.y, c);
+                f[j] = __builtin_fmaf(z, q2, __builtin_fmaf(wf[j] * s.y, d[j], q1));
             }
-            store_run<T, kE>(dx + c, f, n - c);
+            at.store(dx, f, i);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
     if (!part) return;
     float *out = part + (int64_t)blockIdx.x * 2 * n;
     if constexpr (kL > 64) {
 #pragma unroll
-        for (int i = 0; i < kP; i++) {
-            const int c = column<T, kL>(i, lane);
-            store_run<float, kE>(out + c, aw[i], n - c);
-            store_run<float, kE>(out + n + c, ab[i], n - c);
-        }
+        for (int i = 0; i < kP; i++)
+#pragma unroll
+            for (int j = 0; j < kE; j++) {
+                if (!at.some(i) || !at.own(i, j)) continue;
+                out[at.column(i) + j] = aw[i][j];
+                out[n + at.column(i) + j] = ab[i][j];
+            }
     } else {
         // the wave's groups of lanes, then the waves one after the other
 #pragma unroll
@@ -324,7 +367,8 @@ __global__ __launch_bounds__(kL > 256 ? kL : 256) void norm_grad_kernel(const No
                 for (int i = 0; i < kP; i++)
 #pragma unroll
                     for (int j = 0; j < kE; j++) {
-                        const int c = column<T, kL>(i, lane) + j;
+                        if (!at.some(i) || !at.own(i, j)) continue;
+                        const int c = at.column(i) + j;
                         sums[0][c] = k ? sums[0][c] + aw[i][j] : aw[i][j];
                         sums[kL <= 64][c] = k ? sums[kL <= 64][c] + ab[i][j] : ab[i][j];
                     }
@@ -419,22 +463,24 @@ template <class W> __global__ __launch_bounds__(1024) void norm_join_kernel(cons
     if (c >= n && db) db[c - n] = from_f32<W>(sum);
 }
 
-// The form that holds rows of n values: f(lanes, pieces), or false past all of them
+// The form that holds rows of n values: f(lanes, pieces, whether rows are less than a piece), or false past all of them
 template <class T, class F> bool with_form(int n, F f) {
-    auto is = [&](auto l, auto p) {
+    auto is = [&](auto l, auto p, auto tiny) {
         constexpr int kL = decltype(l)::value, kP = decltype(p)::value;
-        if (n > kL * kP * kEach<T>) return false;
-        f(l, p);
+        if (n > (decltype(tiny)::value ? kEach<T> - 1 : kL * kP * kEach<T>)) return false;
+        f(l, p, tiny);
         return true;
     };
     constexpr std::integral_constant<int, 1> one{};
     constexpr std::integral_constant<int, 2> two{};
+    constexpr std::integral_constant<int, 3> three{};
     constexpr std::integral_constant<int, 4> four{};
     constexpr std::integral_constant<int, 16> l16{};
     constexpr std::integral_constant<int, 64> l64{};
     constexpr std::integral_constant<int, 256> l256{};
-    return is(four, one) || is(l16, one) || is(l16, two) || is(l16, four) || is(l64, two) || is(l64, four) || is(l256, two) ||
-           is(l256, four);
+    constexpr std::false_type no{};
+    return is(one, one, std::true_type()) || is(one, one, no) || is(four, one, no) || is(four, two, no) || is(l16, one, no) || is(l16, two, no) || is(l16, four, no) ||
+           is(l64, two, no) || is(l64, three, no) || is(l64, four, no) || is(l256, two, no) || is(l256, three, no) || is(l256, four, no);
 }
 constexpr int kFewGroups = 512;     // workgroups of a backward pass: two on each CU
 int64_t groups_of(int64_t rows, int lanes) {
@@ -443,7 +489,7 @@ int64_t groups_of(int64_t rows, int lanes) {
 }
 template <class T> int64_t grad_groups(int64_t rows, int n) {
     int64_t g = 0;
-    if (!with_form<T>(n, [&](auto l, auto) { g = groups_of(rows, decltype(l)::value); }) && n <= 512 * 2 * kEach<T>)
+    if (!with_form<T>(n, [&](auto l, auto, auto) { g = groups_of(rows, decltype(l)::value); }) && n <= 512 * 4 * kEach<T>)
         g = groups_of(rows, 512);
     // the columns' kernel: a thousand workgroups or so
     if (!g) g = std::min<int64_t>(rows, std::max(1, 1024 / ((n + 256 * kEach<T> - 1) / (256 * kEach<T>))));
@@ -454,12 +500,15 @@ template <class T> hipError_t go(const NormArgs &a, hipStream_t st) {
     auto launch = [&](auto kernel, int threads, int64_t blocks, int most) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)std::min<int64_t>(blocks, most)), dim3(threads), 0, st, a);
     };
-    if (!with_form<T>(a.n, [&](auto l, auto p) {
-            constexpr int kL = decltype(l)::value, kEachWg = 256 / kL;
-            launch(norm_kernel<T, kL, decltype(p)::value>, 256, (a.rows + kEachWg - 1) / kEachWg, 2048);
+    if (!with_form<T>(a.n, [&](auto l, auto p, auto tiny) {
+            // as many workgroups as the weights in LDS let the CUs hold together, so that all begin and end at once
+            constexpr int kL = decltype(l)::value, kRows = 256 / kL, kLds = 2 * kL * decltype(p)::value * kEach<T> * 4 + 64;
+            launch(norm_kernel<T, kL, decltype(p)::value, decltype(tiny)::value>, 256, (a.rows + kRows - 1) / kRows,
+                   256 * std::min(8, 160 * 1024 / kLds));
         })) {
         constexpr int kE = kEach<T>;
-        if (a.n <= 1024 * 2 * kE) launch(norm_kernel<T, 1024, 2>, 1024, a.rows, 1024);
+        if (a.n <= 1024 * 2 * kE) launch(norm_kernel<T, 1024, 2, false>, 1024, a.rows, 256);
+        else if (a.n <= 1024 * 4 * kE) launch(norm_kernel<T, 1024, 4, false>, 1024, a.rows, 256);
         else launch(norm_wide_kernel<T>, 1024, a.rows, 1024);
     }
     return hipGetLastError();
@@ -468,13 +517,13 @@ template <class T> hipError_t go_grad(const NormGradArgs &a, void *scratch, hipS
     const bool sums = a.dw || a.db;
     float *part = sums ? (float *)scratch : nullptr;
     const int64_t groups = grad_groups<T>(a.rows, a.n);
-    if (a.rows && !with_form<T>(a.n, [&](auto l, auto p) {
-            hipLaunchKernelGGL((norm_grad_kernel<T, decltype(l)::value, decltype(p)::value>), dim3((unsigned)groups), dim3(256), 0, st,
+    if (a.rows && !with_form<T>(a.n, [&](auto l, auto p, auto tiny) {
+            hipLaunchKernelGGL((norm_grad_kernel<T, decltype(l)::value, decltype(p)::value, decltype(tiny)::value>), dim3((unsigned)groups), dim3(256), 0, st,
                                a, part);
         })) {
         constexpr int kE = kEach<T>;
-        if (a.n <= 512 * 2 * kE) {
-            hipLaunchKernelGGL((norm_grad_kernel<T, 512, 2>), dim3((unsigned)groups), dim3(512), 0, st, a, part);
+        if (a.n <= 512 * 4 * kE) {
+            hipLaunchKernelGGL((norm_grad_kernel<T, 512, 4, false>), dim3((unsigned)groups), dim3(512), 0, st, a, part);
         } else {
             if (a.dx)
                 hipLaunchKernelGGL(norm_grad_wide_kernel<T>, dim3((unsigned)std::min<int64_t>(a.rows, 1024)), dim3(1024), 0, st, a);

@@ -109,6 +109,7 @@ hipError_t launch_scan_grad(int type, int gate_type, const ScanGradArgs &a, void
 // With x (M, K) and w (2, N, K): g = x w[0]^T, u = x w[1]^T, y (M, N) = act(g) u
 enum Activation { kSilu = 0, kGelu = 1, kSigmoid = 2 };
 hipError_t launch_gated(int type, int act, const void *x, const void *w, int M, int N, int K, void *y, void *gu, hipStream_t stream);
+int64_t gated_kept(int type, int M, int N);    // bytes of gu
 int64_t gated_grad_scratch(int type, int M, int N, int K);
 hipError_t launch_gated_grad(int type, int act, const void *x, const void *w, const void *gu, const void *dy, int M, int N, int K,
                              void *dx, void *dw, void *scratch, hipStream_t stream);

@@ -37,6 +37,7 @@ struct {
     decltype(&ygg_gated_scan_scratch) gated_scan_scratch;
     decltype(&ygg_gated_scan_grad) gated_scan_grad;
     decltype(&ygg_gated_linear) gated_linear;
+    decltype(&ygg_gated_linear_kept) gated_linear_kept;
     decltype(&ygg_gated_linear_scratch) gated_linear_scratch;
     decltype(&ygg_gated_linear_grad) gated_linear_grad;
     decltype(&ygg_clip_scratch) clip_scratch;
@@ -61,6 +62,7 @@ void bind(const std::map<std::string, uintptr_t> &at) {
     set(api.gated_scan_scratch, "ygg_gated_scan_scratch");
     set(api.gated_scan_grad, "ygg_gated_scan_grad");
     set(api.gated_linear, "ygg_gated_linear");
+    set(api.gated_linear_kept, "ygg_gated_linear_kept");
     set(api.gated_linear_scratch, "ygg_gated_linear_scratch");
     set(api.gated_linear_grad, "ygg_gated_linear_grad");
     set(api.clip_scratch, "ygg_clip_scratch");
@@ -346,12 +348,12 @@ std::pair<Tensor, Tensor> gated_scan(const Tensor &gate, const Tensor &x, const 
     return gated_scan_of(gate, x, or_none(state));
 }
 
-// x (M, K), w (2, N, K) -> y, and g and u (M, 2, N) if they are kept
+// x (M, K), w (2, N, K) -> y, and g and u if they are kept
 std::pair<Tensor, Tensor> gated_linear_of(const Tensor &x, const Tensor &w, int64_t act, bool keep) {
     const c10::DeviceGuard guard(x.device());
     const int64_t M = x.size(0), N = w.size(1), K = x.size(1);
     Tensor y = empty(x, {M, N}, x.scalar_type()), gu;
-    if (keep) gu = empty(x, {M, 2, N}, x.scalar_type());
+    if (keep) gu = empty(x, {api.gated_linear_kept(type_of(x), M, N)}, at::kByte);
     check(api.gated_linear(x.data_ptr(), w.data_ptr(), type_of(x), act, M, N, K, y.data_ptr(), ptr(gu), stream_of(x)));
     return {y, gu};
 }
@@ -410,6 +412,7 @@ std::pair<std::vector<Tensor>, Tensor> clip_grad_norm(std::vector<Tensor> in, do
     for (const Tensor &t : in) no_tangents("clip_grad_norm", {t});
     const c10::DeviceGuard guard(first.device());
     const at::AutoGradMode none(false);
+    at::AutoDispatchBelowADInplaceOrView below;      // for the time of many allocations
     std::vector<Tensor> out;
     if (clip && to) {
         out = *to;
@@ -434,7 +437,7 @@ std::pair<std::vector<Tensor>, Tensor> clip_grad_norm(std::vector<Tensor> in, do
         // values go in the order they lie in memory, the same in both
         if (!in[i].is_non_overlapping_and_dense()) in[i] = in[i].contiguous();
         if (clip) {
-            if (!to) out.push_back(at::empty_like(in[i]));
+            if (!to) out.push_back(at::empty_strided(in[i].sizes(), in[i].strides(), in[i].options()));
             if (out[i].strides() != in[i].strides()) in[i] = at::empty_like(out[i]).copy_(in[i]);
             into[i] = out[i].data_ptr();
         }
@@ -502,6 +505,21 @@ std::optional<std::pair<Tensor, Tensor>> plain_gated_scan(const Tensor &gate, co
     if (state && !(like(*state, x, at::kFloat, 2) && state->size(0) == x.size(0) && state->size(1) == x.size(2))) return std::nullopt;
     return gated_scan(gate, x, state);
 }
+std::optional<std::pair<std::vector<Tensor>, Tensor>> plain_clip_grad_norm(const std::vector<Tensor> &in, double most, bool clip,
+                                                                          const std::optional<std::vector<Tensor>> &to) {
+    if (in.empty() || !(most >= 0) || (to && to->size() != in.size())) return std::nullopt;
+    const bool grad = at::GradMode::is_enabled();
+    auto plain = [&](const Tensor &t) {
+        const auto d = t.scalar_type();
+        return t.is_cuda() && t.layout() == at::kStrided && (d == at::kFloat || d == at::kBFloat16 || d == at::kHalf) &&
+               t.device() == in[0].device() && t.numel() <= YGG_MOST_VALUES && !(clip && grad && t.requires_grad());
+    };
+    for (size_t i = 0; i < in.size(); i++) {
+        if (!plain(in[i])) return std::nullopt;
+        if (to && ((*to)[i].scalar_type() != in[i].scalar_type() || (*to)[i].sizes() != in[i].sizes() || !plain((*to)[i]))) return std::nullopt;
+    }
+    return clip_grad_norm(in, most, clip, to);
+}
 Maybe plain_gated_linear(const Tensor &x, const Tensor &w, int64_t act) {
     if (!floats(x, 2) || !like(w, x, x.scalar_type(), 3) || w.size(0) != 2 || w.size(2) != x.size(1) || x.size(0) > YGG_MOST_ROWS ||
         !within(w.size(1), 1, YGG_MOST_INNER / 2) || !within(x.size(1), 1, YGG_MOST_INNER))
@@ -526,4 +544,5 @@ PYBIND11_MODULE(_ygg_torch, m) {
     m.def("plain_layer_norm", &plain_layer_norm);
     m.def("plain_gated_scan", &plain_gated_scan);
     m.def("plain_gated_linear", &plain_gated_linear);
+    m.def("plain_clip_grad_norm", &plain_clip_grad_norm);
 }

@@ -63,7 +63,7 @@ def _tensors(x, *others) -> bool:
 _ENTRIES = ("ygg_logprobs_scratch", "ygg_logprobs", "ygg_logprobs_grad", "ygg_grouped_matmul", "ygg_grouped_grad_x",
             "ygg_grouped_grad_w", "ygg_int8_scratch", "ygg_int8_linear", "ygg_layer_norm", "ygg_layer_norm_scratch",
             "ygg_layer_norm_grad", "ygg_gated_scan", "ygg_gated_scan_scratch", "ygg_gated_scan_grad", "ygg_gated_linear",
-            "ygg_gated_linear_scratch", "ygg_gated_linear_grad", "ygg_clip_scratch", "ygg_clip_grad_norm", "ygg_last_error")
+            "ygg_gated_linear_kept", "ygg_gated_linear_scratch", "ygg_gated_linear_grad", "ygg_clip_scratch", "ygg_clip_grad_norm", "ygg_last_error")
 _module = None
 
 
@@ -278,8 +278,8 @@ def gated_scan(gate, x, state=None):
 def gated_linear(x, w, activation: str = "silu") -> torch.Tensor:
     """The gated projections of a feed-forward block in one kernel: x (..., K), w (2, N, K) in x's type ->
     act(x w[0]^T) (x w[1]^T) (..., N) in x's type, act "silu" (g sigmoid(g)), "gelu" (g Phi(g)) or "sigmoid". Sums and
-    the product are in f32, rounded once. Differentiable in x and w: for that, both projections are kept in x's type, and the
-    gradients' products take their factors in it."""
+    the product are in f32, rounded once. Differentiable in x and w: for that, both projections are kept (in f32, or its upper 24
+    bits for 16-bit types), and the gradients' products take their factors in x's type."""
     act = ACTIVATIONS.get(activation) if isinstance(activation, str) else None
     if act is None:
         raise ValueError(f"activation {activation!r}: one of {', '.join(ACTIVATIONS)}")
@@ -305,6 +305,11 @@ def gated_linear(x, w, activation: str = "silu") -> torch.Tensor:
 
 def _clip(grads, most: float, clip: bool, out=None):
     grads = list(grads)
+    out = out if out is None else list(out)
+    if grads and _tensors(*grads) and (out is None or (out and _tensors(*out))):
+        r = _native().plain_clip_grad_norm(grads, most, clip, out)
+        if r is not None:
+            return (r[0] if out is None else out), r[1]
     some = [i for i, g in enumerate(grads) if g is not None]
     if not some:
         raise ValueError("no gradients")
@@ -316,7 +321,6 @@ def _clip(grads, most: float, clip: bool, out=None):
         if clip and g.requires_grad and torch.is_grad_enabled():
             raise ValueError("clip_grad_norm has no gradient: call it under torch.no_grad() or with detached tensors")
     if out is not None:
-        out = list(out)
         if len(out) != len(grads) or any((o is None) != (g is None) for o, g in zip(out, grads)):
             raise ValueError("out must hold a tensor for every gradient, and None where there is none")
         to = [out[i] for i in some]
