@@ -323,18 +323,22 @@ int ygg_layer_norm_grad(const void *d_x, int type, int64_t rows, int n, int64_t 
 /* h_t = gate_t h_{t-1} + x_t over T steps of B sequences of n channels. gate (type gate_type: 0 or x's) and x lie with the
    channels of a step next to each other, steps and sequences any distance apart (gate_t, gate_b, x_t, x_b values, at least
    0). d_state (B, n) f32 is h_{-1} (NULL: zeros); d_h (B, T, n) contiguous in x's type, d_last (B, n) f32 the last state
-   (what d_state holds where there are no steps), memory of its own. States are held in f32; runs of steps are joined by the products
+   (what d_state holds where there are no steps), memory of its own. d_kept: NULL, or f32 memory of ygg_gated_scan_kept
+   bytes (0: none) for every 64th state, which the gates' gradient wants. States are held in f32; runs of steps are joined by the products
    of their gates, so gates are meant to be at most 1 in magnitude: others have to keep the products of any run of steps
    finite. */
 int64_t ygg_gated_scan_scratch(int type, int gate_type, int64_t B, int64_t T, int n);
+int64_t ygg_gated_scan_kept(int64_t B, int64_t T, int n);
 int ygg_gated_scan(const void *d_gate, int gate_type, int64_t gate_b, int64_t gate_t, const void *d_x, int type, int64_t x_b,
-                   int64_t x_t, int64_t B, int64_t T, int n, const float *d_state, void *d_h, float *d_last, void *d_scratch,
-                   int64_t scratch_bytes, void *stream);
-/* The gradients, from those of h (contiguous, NULL: zeros) and of the last state (NULL: zeros) and from h as ygg_gated_scan left
-   it: of x and the gates (B, T, n) contiguous in their types, of the state (B, n) f32. NULL: not wanted. */
-int ygg_gated_scan_grad(const void *d_gate, int gate_type, int64_t gate_b, int64_t gate_t, const void *d_h, int type, int64_t B,
-                        int64_t T, int n, const float *d_state, const void *d_dh, const float *d_dlast, void *d_dx, void *d_dgate,
-                        float *d_dstate, void *d_scratch, int64_t scratch_bytes, void *stream);
+                   int64_t x_t, int64_t B, int64_t T, int n, const float *d_state, void *d_h, float *d_last, float *d_kept,
+                   void *d_scratch, int64_t scratch_bytes, void *stream);
+/* The gradients, from those of h (contiguous, NULL: zeros) and of the last state (NULL: zeros): of x and the gates (B, T, n)
+   contiguous in their types, of the state (B, n) f32. NULL: not wanted. d_x, d_state and d_kept, as ygg_gated_scan took and
+   left them, are read for the gates' gradient alone. */
+int ygg_gated_scan_grad(const void *d_gate, int gate_type, int64_t gate_b, int64_t gate_t, const void *d_x, int type, int64_t x_b,
+                        int64_t x_t, int64_t B, int64_t T, int n, const float *d_state, const float *d_kept, const void *d_dh,
+                        const float *d_dlast, void *d_dx, void *d_dgate, float *d_dstate, void *d_scratch, int64_t scratch_bytes,
+                        void *stream);
 
 /* The gated projections of a feed-forward block: x (M, K), w (2, N, K) contiguous, g = x w[0]^T, u = x w[1]^T, y (M, N) =
    act(g) u in x's type; act: 0 silu (g sigmoid(g)), 1 gelu (g Phi(g)), 2 sigmoid. N up to YGG_MOST_INNER / 2. d_gu: NULL or

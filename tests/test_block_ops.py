@@ -56,8 +56,8 @@ def test_layer_norm_grad_refuses(kw, word):
     refused("ygg_layer_norm_grad", NORM_GRAD, kw, word)
 
 
-SCAN = dict(gate=P, gate_type=0, gate_b=8, gate_t=8, x=P, type=1, x_b=8, x_t=8, B=1, T=4, n=8, state=None, h=P, last=P, scratch=P, bytes=1 << 40,
-            stream=None)
+SCAN = dict(gate=P, gate_type=0, gate_b=8, gate_t=8, x=P, type=1, x_b=8, x_t=8, B=1, T=4, n=8, state=None, h=P, last=P, kept=None, scratch=P,
+            bytes=1 << 40, stream=None)
 
 
 @pytest.mark.parametrize("kw, word", [
@@ -69,13 +69,14 @@ def test_gated_scan_refuses(kw, word):
     refused("ygg_gated_scan", SCAN, kw, word)
 
 
-SCAN_GRAD = dict(gate=P, gate_type=0, gate_b=8, gate_t=8, h=P, type=1, B=1, T=4, n=8, state=None, dh=P, dlast=None, dx=P, dg=P, ds=None, scratch=P,
-                 bytes=1 << 40, stream=None)
+SCAN_GRAD = dict(gate=P, gate_type=0, gate_b=8, gate_t=8, x=P, type=1, x_b=8, x_t=8, B=1, T=4, n=8, state=None, kept=P, dh=P, dlast=None, dx=P,
+                 dg=P, ds=None, scratch=P, bytes=1 << 40, stream=None)
 
 
 @pytest.mark.parametrize("kw, word", [
     (dict(type=3), b"type"), (dict(gate_type=2), b"gate_type"), (dict(B=-1), b"B "), (dict(T=-1), b"T "), (dict(n=0), b"n "),
-    (dict(gate_b=-8), b"strides"), (dict(gate=None), b"NULL"), (dict(h=None), b"NULL"), (dict(T=1 << 20, scratch=None), b"scratch")])
+    (dict(gate_b=-8), b"strides"), (dict(x_t=-8), b"strides"), (dict(gate=None), b"NULL"), (dict(x=None), b"NULL"),
+    (dict(T=65, kept=None), b"NULL"), (dict(T=1 << 20, scratch=None), b"scratch")])
 def test_gated_scan_grad_refuses(kw, word):
     refused("ygg_gated_scan_grad", SCAN_GRAD, kw, word)
 
@@ -125,6 +126,7 @@ def test_nothing_to_do_is_done():
     assert L.ygg_gated_linear_grad(*{**GATED_GRAD, "dx": None, "dw": None}.values()) == 0
     assert L.ygg_layer_norm_scratch(0, 0, 8) == 0 and L.ygg_layer_norm_scratch(5, 1, 8) == 0
     assert L.ygg_gated_scan_scratch(0, 0, 0, 8, 8) == 0 and L.ygg_gated_scan_scratch(0, 0, 512, 100, 1024) == 0
+    assert [L.ygg_gated_scan_kept(2, t, 5) for t in (0, 1, 64, 65, 128, 129, 4096)] == [0, 0, 0, 40, 40, 80, 63 * 40]
     assert L.ygg_gated_linear_scratch(7, 1, 1, 1) == 0 and L.ygg_gated_linear_scratch(1, 0, 8, 8) == 0
     assert L.ygg_gated_linear_kept(1, 0, 8) == 0 and L.ygg_gated_linear_kept(1, 5, 8) == 240 and L.ygg_gated_linear_kept(0, 5, 8) == 320
     assert L.ygg_clip_scratch(None, 3) == 0

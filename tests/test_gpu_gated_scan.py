@@ -4,7 +4,7 @@ channels from one on, gates of 0 and 1, strides.
 Tolerance: a term x_s times the t - s gates after it goes through at most 2 (t - s) + 8 roundings in f32 (each step of its way is
 added once and its gates are multiplied once), so with S the recurrence of the magnitudes and W the one that counts steps,
 W_t = |a_t| (W_{t-1} + S_{t-1}), h is off by at most u (2 W + 8 S), u = 2^-24; backwards alike. The gates' gradient takes h
-rounded to its type. Then half a step of the output's type."""
+in f32. Then half a step of the output's type."""
 import math
 
 import pytest
@@ -75,7 +75,6 @@ def check(gate, x, state, dh, dlast, on_device=None):
     near(dx, rx, tx, "dx")
     near(ds, rs, ts, "dstate")
     prior = torch.cat([torch.zeros_like(th[:, :1]), th[:, :-1]], 1)
-    prior = prior + (torch.finfo(x.dtype).eps / 2) * (before.abs() + prior) + LEAST[x.dtype]
     near(dg, rx * before, rx.abs() * prior + tx * (before.abs() + prior) + 2 * U * (rx * before).abs(), "dgate")
 
 

@@ -21,7 +21,8 @@ SYMBOLS = ("ygg_load", "ygg_load_blob", "ygg_model_info", "ygg_free", "ygg_step"
            "ygg_float_run_scratch", "ygg_float_nll", "ygg_float_take_errors",
            "ygg_float_free", "ygg_logprobs_scratch", "ygg_logprobs", "ygg_logprobs_grad", "ygg_grouped_matmul",
            "ygg_grouped_grad_x", "ygg_grouped_grad_w", "ygg_int8_scratch", "ygg_int8_linear", "ygg_layer_norm",
-           "ygg_layer_norm_scratch", "ygg_layer_norm_grad", "ygg_gated_scan_scratch", "ygg_gated_scan", "ygg_gated_scan_grad",
+           "ygg_layer_norm_scratch", "ygg_layer_norm_grad", "ygg_gated_scan_scratch", "ygg_gated_scan_kept", "ygg_gated_scan",
+           "ygg_gated_scan_grad",
            "ygg_gated_linear", "ygg_gated_linear_kept", "ygg_gated_linear_scratch", "ygg_gated_linear_grad", "ygg_clip_scratch", "ygg_clip_grad_norm",
            "ygg_kernel_name",
            "ygg_spec_stats", "ygg_last_error", "ygg_version")
@@ -116,15 +117,16 @@ def lib() -> ctypes.CDLL:
     L.ygg_layer_norm_scratch.argtypes = [i32, i64, i32]
     L.ygg_layer_norm_grad.argtypes = [vp, i32, i64, i32, i64, vp, i32, vp, vp, vp, vp, vp, vp, i64, vp]
     L.ygg_gated_scan_scratch.argtypes = [i32, i32, i64, i64, i32]
-    L.ygg_gated_scan.argtypes = [vp, i32, i64, i64, vp, i32, i64, i64, i64, i64, i32, vp, vp, vp, vp, i64, vp]
-    L.ygg_gated_scan_grad.argtypes = [vp, i32, i64, i64, vp, i32, i64, i64, i32, vp, vp, vp, vp, vp, vp, vp, i64, vp]
+    L.ygg_gated_scan_kept.argtypes = [i64, i64, i32]
+    L.ygg_gated_scan.argtypes = [vp, i32, i64, i64, vp, i32, i64, i64, i64, i64, i32, vp, vp, vp, vp, vp, i64, vp]
+    L.ygg_gated_scan_grad.argtypes = [vp, i32, i64, i64, vp, i32, i64, i64, i64, i64, i32, vp, vp, vp, vp, vp, vp, vp, vp, i64, vp]
     L.ygg_gated_linear.argtypes = [vp, vp, i32, i32, i32, i32, i32, vp, vp, vp]
     L.ygg_gated_linear_kept.argtypes = [i32, i32, i32]
     L.ygg_gated_linear_scratch.argtypes = [i32, i32, i32, i32]
     L.ygg_gated_linear_grad.argtypes = [vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, vp, vp, i64, vp]
     L.ygg_clip_scratch.argtypes = [vp, i32]
     L.ygg_clip_grad_norm.argtypes = [vp, vp, vp, i32, ctypes.c_double, vp, vp, vp, i64, vp]
-    for f in (L.ygg_layer_norm_scratch, L.ygg_gated_scan_scratch, L.ygg_gated_linear_kept, L.ygg_gated_linear_scratch,
+    for f in (L.ygg_layer_norm_scratch, L.ygg_gated_scan_scratch, L.ygg_gated_scan_kept, L.ygg_gated_linear_kept, L.ygg_gated_linear_scratch,
               L.ygg_clip_scratch):
         f.restype = i64
     L.ygg_last_error.argtypes = []

@@ -1375,9 +1375,14 @@ int64_t ygg_gated_scan_scratch(int type, int gate_type, int64_t B, int64_t T, in
     return ygg::scan_scratch(type, gate_type, B, T, n);
 }
 
+int64_t ygg_gated_scan_kept(int64_t B, int64_t T, int n) {
+    if (B < 1 || B > YGG_MOST_ROWS || T < 1 || T > YGG_MOST_STEPS || n < 1 || n > YGG_MOST_INNER) return 0;
+    return ygg::scan_kept(B, T, n);
+}
+
 int ygg_gated_scan(const void *d_gate, int gate_type, int64_t gate_b, int64_t gate_t, const void *d_x, int type, int64_t x_b,
-                   int64_t x_t, int64_t B, int64_t T, int n, const float *d_state, void *d_h, float *d_last, void *d_scratch,
-                   int64_t scratch_bytes, void *stream) {
+                   int64_t x_t, int64_t B, int64_t T, int n, const float *d_state, void *d_h, float *d_last, float *d_kept,
+                   void *d_scratch, int64_t scratch_bytes, void *stream) {
     if (int rc = check_scan(type, gate_type, B, T, n)) return rc;
     if (gate_b < 0 || gate_t < 0 || x_b < 0 || x_t < 0) return fail(YGG_ERR_ARG, "negative strides");
     if (B == 0) return YGG_OK;
@@ -1385,22 +1390,23 @@ int ygg_gated_scan(const void *d_gate, int gate_type, int64_t gate_b, int64_t ga
     const int64_t need = T ? ygg::scan_scratch(type, gate_type, B, T, n) : 0;
     if (need && (!d_scratch || scratch_bytes < need))
         return fail(YGG_ERR_ARG, "scratch of %lld bytes, %lld wanted", (long long)scratch_bytes, (long long)need);
-    const ygg::ScanArgs a = {d_gate, d_x, gate_b, gate_t, x_b, x_t, B, T, n, d_state, d_h, d_last};
+    const ygg::ScanArgs a = {d_gate, d_x, gate_b, gate_t, x_b, x_t, B, T, n, d_state, d_h, d_last, d_kept};
     OP_TRY(ygg::launch_scan(type, gate_type, a, d_scratch, (hipStream_t)stream));
     return YGG_OK;
 }
 
-int ygg_gated_scan_grad(const void *d_gate, int gate_type, int64_t gate_b, int64_t gate_t, const void *d_h, int type, int64_t B,
-                        int64_t T, int n, const float *d_state, const void *d_dh, const float *d_dlast, void *d_dx, void *d_dgate,
-                        float *d_dstate, void *d_scratch, int64_t scratch_bytes, void *stream) {
+int ygg_gated_scan_grad(const void *d_gate, int gate_type, int64_t gate_b, int64_t gate_t, const void *d_x, int type, int64_t x_b,
+                        int64_t x_t, int64_t B, int64_t T, int n, const float *d_state, const float *d_kept, const void *d_dh,
+                        const float *d_dlast, void *d_dx, void *d_dgate, float *d_dstate, void *d_scratch, int64_t scratch_bytes,
+                        void *stream) {
     if (int rc = check_scan(type, gate_type, B, T, n)) return rc;
-    if (gate_b < 0 || gate_t < 0) return fail(YGG_ERR_ARG, "negative strides");
+    if (gate_b < 0 || gate_t < 0 || x_b < 0 || x_t < 0) return fail(YGG_ERR_ARG, "negative strides");
     if (B == 0 || (T == 0 && !d_dstate)) return YGG_OK;
-    if (T > 0 && (!d_gate || (d_dgate && !d_h))) return fail(YGG_ERR_ARG, "NULL buffer");
+    if (T > 0 && (!d_gate || (d_dgate && (!d_x || (!d_kept && ygg::scan_kept(B, T, n)))))) return fail(YGG_ERR_ARG, "NULL buffer");
     const int64_t need = T ? ygg::scan_scratch(type, gate_type, B, T, n) : 0;
     if (need && (!d_scratch || scratch_bytes < need))
         return fail(YGG_ERR_ARG, "scratch of %lld bytes, %lld wanted", (long long)scratch_bytes, (long long)need);
-    const ygg::ScanGradArgs a = {d_gate, d_h, d_dh, gate_b, gate_t, B, T, n, d_state, d_dlast, d_dx, d_dgate, d_dstate};
+    const ygg::ScanGradArgs a = {d_gate, d_x, d_dh, gate_b, gate_t, x_b, x_t, B, T, n, d_state, d_dlast, d_kept, d_dx, d_dgate, d_dstate};
     OP_TRY(ygg::launch_scan_grad(type, gate_type, a, d_scratch, (hipStream_t)stream));
     return YGG_OK;
 }

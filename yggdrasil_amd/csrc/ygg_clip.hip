@@ -24,6 +24,7 @@ struct Table {
     uint32_t first[kTensors + 1];   // a tensor's first workgroup
     uint8_t type[kTensors];
     int count, chunk;
+    bool past;                      // the results, past the caches
 };
 static_assert(sizeof(Table) < 4000, "more than a launch's arguments");
 struct Share {
@@ -132,7 +133,7 @@ __global__ __launch_bounds__(kThreads) void scale_kernel(const Table tab, const 
             unpack(v, t, T());
 #pragma unroll
             for (int j = 0; j < kE; j++) t[j] = (float)((double)t[j] * f);
-            store_run<T, kE>(out + c, t, s.count - c);
+            store_run<T, kE>(out + c, t, s.count - c, tab.past);
         };
         int c = threadIdx.x * kE;
         for (; c + (kU - 1) * kThreads * kE + kE <= s.count; c += kU * kThreads * kE) {
@@ -169,6 +170,8 @@ hipError_t launch_clip(const void *const *tensors, const int64_t *sizes, const i
                        float *norm, void *scratch, hipStream_t st) {
     double *by = (double *)scratch, *part = by + 1;
     const int chunk = chunk_of(sizes, count);
+    int64_t bytes = 0;
+    for (int i = 0; i < count; i++) bytes += sizes[i] * op_bytes(types[i]);
     // f(a table of up to kTensors tensors, its workgroups, those before them)
     auto tables = [&](auto f) {
         int64_t before = 0;
@@ -192,6 +195,7 @@ hipError_t launch_clip(const void *const *tensors, const int64_t *sizes, const i
             tab.first[n] = (uint32_t)blocks;
             tab.count = n;
             tab.chunk = chunk;
+            tab.past = bytes >= kPastBytes;
             f(tab, (unsigned)blocks, before);
             const hipError_t e = hipGetLastError();
             if (e != hipSuccess) return e;

@@ -23,6 +23,7 @@
 
 #include <type_traits>
 
+#include "ygg_lanes.h"
 #include "ygg_optype.h"
 
 namespace ygg {
@@ -481,13 +482,6 @@ template <class T, int FI, int FO, int WI, int WO, class A, class B> struct Turn
     }
     template <bool kDealt, class F> __device__ __forceinline__ void each(F put) { each_run<T, kDealt>(acc, row0(), col0(), put); }
 };
-
-// Workgroups go round the 8 XCDs in turn, each with an L2 of its own: a run of neighbouring tiles to each
-__device__ __forceinline__ int tile_of(int id, int tiles) {
-    const int most = (tiles + 7) / 8, full = tiles - (most - 1) * 8;   // the first `full` XCDs have `most`
-    const int x = id & 7;
-    return (x < full ? x * most : full * most + (x - full) * (most - 1)) + (id >> 3);
-}
 
 // Tile t of rows x cols of them, by bands of `band` rows, down each column of a band: neighbours share both operands
 struct Place {

@@ -1,4 +1,4 @@
-// Values joined over the lanes of a wave, in the lanes' registers.
+// Values joined over the lanes of a wave, in the lanes' registers, and the order of workgroups.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -35,5 +35,12 @@ template <int kG, class V, class F> __device__ __forceinline__ V join(V v, F f) 
     return v;
 }
 template <int kG> __device__ __forceinline__ float sum_of(float v) { return join<kG>(v, [](float a, float b) { return a + b; }); }
+
+// Workgroups go round the 8 XCDs in turn, each with an L2 of its own: a run of neighbouring tiles to each
+__device__ __forceinline__ int tile_of(int id, int tiles) {
+    const int most = (tiles + 7) / 8, full = tiles - (most - 1) * 8;   // the first `full` XCDs have `most`
+    const int x = id & 7;
+    return (x < full ? x * most : full * most + (x - full) * (most - 1)) + (id >> 3);
+}
 
 }  // namespace ygg

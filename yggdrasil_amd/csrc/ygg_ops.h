@@ -68,6 +68,7 @@ struct NormArgs {
     float eps;
     void *y;                      // rows of n, contiguous
     float *stats;                 // a row's mean and 1 / sqrt(variance + eps); NULL: not kept
+    bool past = false;            // the launcher's: results past the caches
 };
 struct NormGradArgs {
     const void *x;
@@ -78,6 +79,7 @@ struct NormGradArgs {
     const float *stats;
     const void *dy;               // rows of n, contiguous, as dx is
     void *dx, *dw, *db;           // NULL: not wanted
+    bool past = false;
 };
 int64_t norm_grad_scratch(int type, int64_t rows, int n);
 hipError_t launch_norm(int type, const NormArgs &a, hipStream_t stream);
@@ -92,16 +94,20 @@ struct ScanArgs {
     const float *state;                   // (B, n); NULL: zeros
     void *h;
     float *last;                          // (B, n)
+    float *kept;                          // what the gates' gradient wants, scan_kept bytes; NULL: nothing
+    bool past = false;                    // the launcher's: results past the caches
 };
 struct ScanGradArgs {
-    const void *gate, *h, *dh;            // dh NULL: zeros
-    int64_t gate_b, gate_t;
+    const void *gate, *x, *dh;            // dh NULL: zeros
+    int64_t gate_b, gate_t, x_b, x_t;
     int64_t B, T;
     int n;
-    const float *state, *dlast;           // NULL: zeros
+    const float *state, *dlast, *kept;    // NULL: zeros; x, state and kept are read for dgate alone
     void *dx, *dgate;                     // NULL: not wanted
     float *dstate;
+    bool past = false;
 };
+int64_t scan_kept(int64_t B, int64_t T, int n);
 int64_t scan_scratch(int type, int gate_type, int64_t B, int64_t T, int n);
 hipError_t launch_scan(int type, int gate_type, const ScanArgs &a, void *scratch, hipStream_t stream);
 hipError_t launch_scan_grad(int type, int gate_type, const ScanGradArgs &a, void *scratch, hipStream_t stream);

@@ -35,6 +35,7 @@ struct {
     decltype(&ygg_layer_norm_grad) layer_norm_grad;
     decltype(&ygg_gated_scan) gated_scan;
     decltype(&ygg_gated_scan_scratch) gated_scan_scratch;
+    decltype(&ygg_gated_scan_kept) gated_scan_kept;
     decltype(&ygg_gated_scan_grad) gated_scan_grad;
     decltype(&ygg_gated_linear) gated_linear;
     decltype(&ygg_gated_linear_kept) gated_linear_kept;
@@ -60,6 +61,7 @@ void bind(const std::map<std::string, uintptr_t> &at) {
     set(api.layer_norm_grad, "ygg_layer_norm_grad");
     set(api.gated_scan, "ygg_gated_scan");
     set(api.gated_scan_scratch, "ygg_gated_scan_scratch");
+    set(api.gated_scan_kept, "ygg_gated_scan_kept");
     set(api.gated_scan_grad, "ygg_gated_scan_grad");
     set(api.gated_linear, "ygg_gated_linear");
     set(api.gated_linear_kept, "ygg_gated_linear_kept");
@@ -73,7 +75,8 @@ void bind(const std::map<std::string, uintptr_t> &at) {
 void check(int rc) {
     if (rc) throw std::runtime_error(std::string(api.last_error()) + " (error " + std::to_string(rc) + ")");
 }
-int type_of(const Tensor &t) { return t.scalar_type() == at::kFloat ? 0 : t.scalar_type() == at::kBFloat16 ? 1 : 2; }
+int type_of(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : 2; }
+int type_of(const Tensor &t) { return type_of(t.scalar_type()); }
 void *stream_of(const Tensor &t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 template <class T = void> T *ptr(const Tensor &t) { return t.defined() ? (T *)t.data_ptr() : nullptr; }
 Tensor empty(const Tensor &like, at::IntArrayRef size, at::ScalarType type) { return at::empty(size, like.options().dtype(type)); }
@@ -291,44 +294,51 @@ Tensor layer_norm(const Tensor &x, const Maybe &w, const Maybe &b, double eps) {
     return layer_norm_of(x, or_none(w), or_none(b), eps, false).first;
 }
 
-// gate, x (B, T, n), a step's channels next to each other; state (B, n) or undefined -> h, the last state
-std::pair<Tensor, Tensor> gated_scan_of(const Tensor &gate, const Tensor &x, const Tensor &state) {
+// gate, x (B, T, n), a step's channels next to each other; state (B, n) or undefined -> h, the last state, and
+// what the gate's gradient wants if it is kept
+std::tuple<Tensor, Tensor, Tensor> gated_scan_of(const Tensor &gate, const Tensor &x, const Tensor &state, bool keep) {
     const c10::DeviceGuard guard(x.device());
     const int64_t B = x.size(0), T = x.size(1), n = x.size(2);
-    Tensor h = empty(x, {B, T, n}, x.scalar_type()), last = empty(x, {B, n}, at::kFloat);
+    Tensor h = empty(x, {B, T, n}, x.scalar_type()), last = empty(x, {B, n}, at::kFloat), kept;
+    if (keep) kept = scratch_of(x, api.gated_scan_kept(B, T, n));
     const int64_t need = api.gated_scan_scratch(type_of(x), type_of(gate), B, T, n);
     const Tensor scratch = scratch_of(x, need);
     check(api.gated_scan(gate.data_ptr(), type_of(gate), gate.stride(0), gate.stride(1), x.data_ptr(), type_of(x), x.stride(0), x.stride(1),
-                         B, T, n, ptr<float>(state), h.data_ptr(), ptr<float>(last), ptr(scratch), need, stream_of(x)));
-    return {h, last};
+                         B, T, n, ptr<float>(state), h.data_ptr(), ptr<float>(last), ptr<float>(kept), ptr(scratch), need, stream_of(x)));
+    return {h, last, kept};
 }
 struct GatedScan : torch::autograd::Function<GatedScan> {
     static variable_list forward(AutogradContext *ctx, const Tensor &gate, const Tensor &x, const Maybe &state) {
         at::AutoDispatchBelowADInplaceOrView guard;
-        auto [h, last] = gated_scan_of(gate, x, or_none(state));
-        ctx->save_for_backward({gate, h, or_none(state)});
+        const bool keep = gate.requires_grad();
+        auto [h, last, kept] = gated_scan_of(gate, x, or_none(state), keep);
+        ctx->save_for_backward({gate, keep ? x : Tensor(), keep ? or_none(state) : Tensor(), kept});
+        ctx->saved_data["type"] = (int64_t)x.scalar_type();
+        ctx->saved_data["state"] = state.has_value();
         ctx->set_materialize_grads(false);
         return {h, last};
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         const variable_list s = ctx->get_saved_variables();
-        const Tensor &gate = s[0], &h = s[1], &state = s[2];
-        const std::vector<bool> want = wanted(ctx, {true, true, state.defined()});
-        const c10::DeviceGuard guard(h.device());
+        const Tensor &gate = s[0], &x = s[1], &state = s[2], &kept = s[3];
+        const at::ScalarType type = (at::ScalarType)ctx->saved_data["type"].toInt();
+        const std::vector<bool> want = wanted(ctx, {true, true, ctx->saved_data["state"].toBool()});
+        const c10::DeviceGuard guard(gate.device());
         variable_list out(3), made;
         {
             const at::AutoGradMode none(false);
             for (const Tensor &g : grads) no_tangents("gated_scan's gradient", {g});
             const Tensor dh = grads[0].defined() ? grads[0].contiguous() : Tensor(), dlast = grads[1].defined() ? grads[1].contiguous() : Tensor();
-            const int64_t B = h.size(0), T = h.size(1), n = h.size(2);
-            if (want[0]) out[0] = empty(h, {B, T, n}, gate.scalar_type());
-            if (want[1]) out[1] = empty(h, {B, T, n}, h.scalar_type());
-            if (want[2]) out[2] = empty(h, {B, n}, at::kFloat);
-            const int64_t need = api.gated_scan_scratch(type_of(h), type_of(gate), B, T, n);
-            const Tensor scratch = scratch_of(h, need);
-            check(api.gated_scan_grad(gate.data_ptr(), type_of(gate), gate.stride(0), gate.stride(1), h.data_ptr(), type_of(h), B, T, n,
-                                      ptr<float>(state), ptr(dh), ptr<float>(dlast), ptr(out[1]), ptr(out[0]), ptr<float>(out[2]),
-                                      ptr(scratch), need, stream_of(h)));
+            const int64_t B = gate.size(0), T = gate.size(1), n = gate.size(2);
+            if (want[0]) out[0] = empty(gate, {B, T, n}, gate.scalar_type());
+            if (want[1]) out[1] = empty(gate, {B, T, n}, type);
+            if (want[2]) out[2] = empty(gate, {B, n}, at::kFloat);
+            const int64_t need = api.gated_scan_scratch(type_of(type), type_of(gate), B, T, n);
+            const Tensor scratch = scratch_of(gate, need);
+            check(api.gated_scan_grad(gate.data_ptr(), type_of(gate), gate.stride(0), gate.stride(1), ptr(x), type_of(type),
+                                      x.defined() ? x.stride(0) : 0, x.defined() ? x.stride(1) : 0, B, T, n, ptr<float>(state),
+                                      ptr<float>(kept), ptr(dh), ptr<float>(dlast), ptr(out[1]), ptr(out[0]), ptr<float>(out[2]),
+                                      ptr(scratch), need, stream_of(gate)));
             for (const Tensor &t : out)
                 if (t.defined()) made.push_back(t);
         }
@@ -345,7 +355,8 @@ std::pair<Tensor, Tensor> gated_scan(const Tensor &gate, const Tensor &x, const 
         const variable_list r = GatedScan::apply(gate, x, state);
         return {r[0], r[1]};
     }
-    return gated_scan_of(gate, x, or_none(state));
+    auto [h, last, kept] = gated_scan_of(gate, x, or_none(state), false);
+    return {h, last};
 }
 
 // x (M, K), w (2, N, K) -> y, and g and u if they are kept

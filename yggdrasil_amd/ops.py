@@ -62,7 +62,7 @@ def _tensors(x, *others) -> bool:
 
 _ENTRIES = ("ygg_logprobs_scratch", "ygg_logprobs", "ygg_logprobs_grad", "ygg_grouped_matmul", "ygg_grouped_grad_x",
             "ygg_grouped_grad_w", "ygg_int8_scratch", "ygg_int8_linear", "ygg_layer_norm", "ygg_layer_norm_scratch",
-            "ygg_layer_norm_grad", "ygg_gated_scan", "ygg_gated_scan_scratch", "ygg_gated_scan_grad", "ygg_gated_linear",
+            "ygg_layer_norm_grad", "ygg_gated_scan", "ygg_gated_scan_scratch", "ygg_gated_scan_kept", "ygg_gated_scan_grad", "ygg_gated_linear",
             "ygg_gated_linear_kept", "ygg_gated_linear_scratch", "ygg_gated_linear_grad", "ygg_clip_scratch", "ygg_clip_grad_norm", "ygg_last_error")
 _module = None
 
@@ -256,8 +256,8 @@ def gated_scan(gate, x, state=None):
 
     States are held in f32. Runs of steps are joined by the products of their gates: gates are meant to be at most 1 in
     magnitude, and others have to keep the product of every run of steps finite. A gate of 0 begins anew (a document's first
-    step); a step with gate 1 and x 0 keeps the state (padding behind a sequence's end leaves the last state right). The gate's
-    gradient takes h as it was returned, in x's type."""
+    step); a step with gate 1 and x 0 keeps the state (padding behind a sequence's end leaves the last state right). For the gate's
+    gradient every 64th state is kept, in f32, and the others are computed again from x."""
     if _tensors(x, gate) if state is None else _tensors(x, gate, state):
         r = _native().plain_gated_scan(gate, x, state)
         if r is not None:
