@@ -88,7 +88,8 @@ def test_shapes(M, N, K, dtype, act):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
-@pytest.mark.parametrize("M, N, K", [(4100, 2056, 136), (2050, 4104, 72), (1030, 1100, 2040), (2000, 1001, 203), (16, 5000, 1024), (12, 4097, 511)])
+@pytest.mark.parametrize("M, N, K", [(4100, 2056, 136), (2050, 4104, 72), (1030, 1100, 2040), (2000, 1001, 203), (16, 5000, 1024), (12, 4097, 511),
+                                     (6150, 1100, 515), (1500, 1003, 1000)])
 def test_large(M, N, K, dtype):
     """Whole and cut tiles of each kernel."""
     check(*make(M, N, K, dtype, seed=M), "silu")

@@ -229,11 +229,13 @@ __global__ __launch_bounds__(64 * kW) void gated_few_kernel(const T *x, const T 
     if (row < M && n < N) put_outputs<T, kAct, 4>((const float *)&acc[0], (const float *)&acc[1], row, n, N, y, gu);
 }
 
+// dg and du lie `half` values apart in rows of 2 half, N up to whole 16 bytes, so that the products' loads are aligned; zeros between.
+__host__ __device__ constexpr int half_of(int size, int N) { return (N + 16 / size - 1) / (16 / size) * (16 / size); }
 // dg and du of pieces of 16 bytes of dy
 template <class T, int kAct>
 __global__ __launch_bounds__(256) void gated_slope_kernel(Kept<T> gu, const T *dy, int M, int N, T *dgu) {
     constexpr int kE = 16 / sizeof(T);
-    const int per = (N + kE - 1) / kE;
+    const int half = half_of(sizeof(T), N), per = half / kE;
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / per;
     if (row >= M) return;
     const int n = (int)(id % per) * kE, left = N - n;
@@ -248,26 +250,31 @@ __global__ __launch_bounds__(256) void gated_slope_kernel(Kept<T> gu, const T *d
         g[j] = d[j] * u[j] * slope;
         u[j] = d[j] * a;
     }
-    T *out = dgu + row * 2 * N + n;
-    store_run<T, kE>(out, g, left);
-    store_run<T, kE>(out + N, u, left);
+    T *out = dgu + row * 2 * half + n;
+    store_run<T, kE>(out, g, kE);
+    store_run<T, kE>(out + half, u, kE);
 }
 
-// ---- the gradients' products: out (I, O) = sum over r of A(i, r) b(r, o). kRows: A is a (I, R), else a^T, a (R, I). A workgroup takes the
-// steps of its part of the reduction; of more than one part, the sums go to `sums` in f32, part after part.
+// ---- the gradients' products: out (I, O) = sum over r of A(i, r) b(r, o), b's rows `pitch` values apart. kRows: A is a (I, 2 half), the r's
+// those of dg and du; else a^T, a (R, 2 half), the i's those of dg and du. A workgroup takes the steps of its part of the reduction; of more
+// than one part, the sums go to `sums` in f32, part after part.
 struct Dense {
     const void *a, *b;
-    int I, O, R;
+    int I, O, R, pitch;
+    int N, half;
     void *out;
     float *sums;
     int tiles, cols, per;       // tiles of a part, tiles along O, steps of a part
+    // the row of w that a column of dg and du belongs to, or -1
+    __device__ __forceinline__ int place(int k) const { return k < N ? k : k >= half && k < half + N ? k - half + N : -1; }
 };
-template <class T> struct DenseOut {
+template <class T, bool kRows> struct DenseOut {
     const Dense &g;
     int part, i0, o0;
     template <class N> __device__ __forceinline__ void operator()(int i, int o, const float *v, N) const {
-        if (i0 + i >= g.I || o0 + o >= g.O) return;
-        const int64_t at = (int64_t)(i0 + i) * g.O + o0 + o;
+        const int row = kRows ? (i0 + i < g.I ? i0 + i : -1) : g.place(i0 + i);
+        if (row < 0 || o0 + o >= g.O) return;
+        const int64_t at = (int64_t)row * g.O + o0 + o;
         if (g.sums) store_run<float, N::value>(g.sums + (int64_t)part * g.I * g.O + at, v, g.O - o0 - o);
         else store_run<T, N::value>((T *)g.out + at, v, g.O - o0 - o);
     }
@@ -279,22 +286,29 @@ __global__ __launch_bounds__(64 * WI * WO) void dense_kernel(const Dense g) {
     typedef Across<T, kO, kThreads> B;
     typedef Tile<T, FI, 4, WI, WO, A, B> Tl;
     __shared__ __align__(128) char lds[Tl::kLds];
-    const int part = blockIdx.x / g.tiles;
+    const int part = blockIdx.x / g.tiles, wide = 2 * g.half, R = kRows ? wide : g.R;
     const Place t = place_of(tile_of(blockIdx.x % g.tiles, g.tiles), g.tiles / g.cols, g.cols, kBand);
-    const int i0 = t.row * kI, o0 = t.col * kO, steps = (g.R + A::kStep - 1) / A::kStep, first = part * g.per;
+    const int i0 = t.row * kI, o0 = t.col * kO, steps = (R + A::kStep - 1) / A::kStep, first = part * g.per;
     Tl tile;
     A a;
     B b;
-    if constexpr (kRows) a.begin([&](int i) { return (const T *)g.a + (int64_t)min(i0 + i, g.I - 1) * g.R; });
-    else a.begin((const T *)g.a, i0, g.I);
+    if constexpr (kRows) a.begin([&](int i) { return (const T *)g.a + (int64_t)min(i0 + i, g.I - 1) * wide; });
+    else a.begin((const T *)g.a, i0, wide);
     b.begin((const T *)g.b, o0, g.O);
     tile.run(a, b, lds, min(g.per, steps - first), [&](int s) {
         const int r0 = (first + s) * A::kStep;
-        if constexpr (kRows) a.load(r0, g.R);
-        else a.load([&](int i) { return r0 + A::r_of(i) < g.R ? (int64_t)(r0 + A::r_of(i)) * g.I : -1; });
-        b.load([&](int i) { return r0 + B::r_of(i) < g.R ? (int64_t)(r0 + B::r_of(i)) * g.O : -1; });
+        if constexpr (kRows) {
+            a.load(r0, R);
+            b.load([&](int i) {
+                const int r = g.place(r0 + B::r_of(i));
+                return r >= 0 ? (int64_t)r * g.pitch : -1;
+            });
+        } else {
+            a.load([&](int i) { return r0 + A::r_of(i) < R ? (int64_t)(r0 + A::r_of(i)) * wide : -1; });
+            b.load([&](int i) { return r0 + B::r_of(i) < R ? (int64_t)(r0 + B::r_of(i)) * g.pitch : -1; });
+        }
     });
-    const DenseOut<T> put = {g, part, i0, o0};
+    const DenseOut<T, kRows> put = {g, part, i0, o0};
     tile.template each<false>([&](int i, int o, const typename Tl::Acc *v, auto n) { put(i, o, (const float *)v, n); });
 }
 template <class T, bool kRows> __global__ __launch_bounds__(512) void dense_turn_kernel(const Dense g) {
@@ -303,30 +317,41 @@ template <class T, bool kRows> __global__ __launch_bounds__(512) void dense_turn
     typedef AcrossLds<T, 4, 4> B;
     typedef TurnTile<T, 8, 4, 2, 4, A, B> Tl;
     __shared__ __align__(1024) char lds[Tl::kLds];
-    const int part = blockIdx.x / g.tiles;
+    const int part = blockIdx.x / g.tiles, wide = 2 * g.half, R = kRows ? wide : g.R;
     const Place t = place_of(tile_of(blockIdx.x % g.tiles, g.tiles), g.tiles / g.cols, g.cols, kBand);
-    const int i0 = t.row * 256, o0 = t.col * 256, steps = (g.R + B::kStep - 1) / B::kStep, first = part * g.per;
-    const uint32_t a_row = (kRows ? g.R : g.I) * kSize, b_row = g.O * kSize;
+    const int i0 = t.row * 256, o0 = t.col * 256, steps = (R + B::kStep - 1) / B::kStep, first = part * g.per;
+    const uint32_t a_row = wide * kSize, b_row = g.pitch * kSize;
     Tl tile;
     A a;
     B b;
     if constexpr (kRows) a.begin(g.a, g.I * a_row, a_row, [&](int i) { return i0 + i < g.I ? (uint32_t)(i0 + i) * a_row : kFar; });
-    else a.begin(g.a, g.R * a_row, i0 * kSize, (g.I - i0) * kSize);
-    b.begin(g.b, g.R * b_row, o0 * kSize, (g.O - o0) * kSize);
+    else a.begin(g.a, g.R * a_row, i0 * kSize, (wide - i0) * kSize);
+    b.begin(g.b, (kRows ? 2 * g.N : g.R) * b_row, o0 * kSize, (g.O - o0) * kSize);
     tile.clear();
-    auto row = [&](int s, int in_step, uint32_t bytes) {
-        const int r = (first + s) * B::kStep + in_step;
-        return r < g.R ? (uint32_t)r * bytes : kFar;
-    };
+    auto row = [&](int r, uint32_t bytes) { return r >= 0 && r < R ? (uint32_t)r * bytes : kFar; };
     tile.run(lds, min(g.per, steps - first),
              [&](auto h, int s, uint32_t to) {
                  if constexpr (kRows) a.template load<decltype(h)::value>(first + s, to);
-                 else a.template load<decltype(h)::value>(to, [&](int i) { return row(s, A::r_of(i), a_row); });
+                 else a.template load<decltype(h)::value>(to, [&](int i) { return row((first + s) * B::kStep + A::r_of(i), a_row); });
              },
-             [&](auto h, int s, uint32_t to) { b.template load<decltype(h)::value>(to, [&](int i) { return row(s, B::r_of(i), b_row); }); },
+             [&](auto h, int s, uint32_t to) {
+                 b.template load<decltype(h)::value>(to, [&](int i) {
+                     const int r = (first + s) * B::kStep + B::r_of(i);
+                     return row(kRows ? g.place(r) : r, b_row);
+                 });
+             },
              [](int) {}, kRows ? min(g.I - i0, 256) : 256);
-    const DenseOut<T> put = {g, part, i0, o0};
+    const DenseOut<T, kRows> put = {g, part, i0, o0};
     tile.template each<false>([&](int i, int o, const typename Tl::Acc *v, auto n) { put(i, o, (const float *)v, n); });
+}
+// rows of n values, `pitch` of whole 16 bytes apart
+template <class T> __global__ __launch_bounds__(256) void spaced_kernel(const T *in, int64_t rows, int n, int pitch, T *out) {
+    constexpr int kE = 16 / sizeof(T);
+    const int per = pitch / kE;
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / per;
+    if (row >= rows) return;
+    const int c = (int)(id % per) * kE;
+    *(u32x4 *)(out + row * pitch + c) = load16(in + row * n + c, n - c);
 }
 // the parts' sums, added in their order
 template <class T> __global__ __launch_bounds__(256) void parts_kernel(const float *sums, int parts, int64_t count, T *out) {
@@ -380,7 +405,7 @@ template <class T, int kAct> hipError_t go(const void *x, const void *w, int M, 
 }
 template <class T, int kAct> hipError_t go_slope(const void *gu, const void *dy, int M, int N, void *dgu, hipStream_t st) {
     constexpr int kE = 16 / sizeof(T);
-    const int64_t blocks = ((int64_t)M * ((N + kE - 1) / kE) + 255) / 256;
+    const int64_t blocks = ((int64_t)M * (half_of(sizeof(T), N) / kE) + 255) / 256;
     if (blocks == 0) return hipSuccess;
     if (blocks > most_blocks(256)) return kTooLarge;
     hipLaunchKernelGGL((gated_slope_kernel<T, kAct>), dim3((unsigned)blocks), dim3(256), 0, st, Kept<T>{(char *)gu, (int64_t)M * 2 * N},
@@ -388,38 +413,58 @@ template <class T, int kAct> hipError_t go_slope(const void *gu, const void *dy,
     return hipGetLastError();
 }
 
-// How a product is cut: 256 x 256 tiles straight to LDS where rows are aligned (`turn`), else kI rows of a tile; the reduction in parts
+// How a product is cut: 256 x 256 tiles straight to LDS (`turn`), which wants b's rows aligned: of a width that is no multiple of 16
+// bytes they are laid out anew (`spaced`); else kI rows of a tile
 struct Plan {
-    bool turn, large;
-    int cols, parts, per;
+    bool turn, large, spaced;
+    int cols, parts, per, pitch;
     int64_t tiles;
 };
-Plan plan_of(int size, bool rows, int I, int O, int R, bool aligned) {
-    const int64_t a_bytes = (int64_t)I * R * size, b_bytes = (int64_t)R * O * size;
-    const int step = 128 / size, steps = (R + step - 1) / step;
+// rows: out (M, K) over 2 half r's; else out (2 N, K) over M
+Plan plan_of(int size, bool rows, int M, int N, int K, bool aligned) {
+    const int half = half_of(size, N), step = 128 / size, I = rows ? M : 2 * half, R = rows ? 2 * half : M, steps = (R + step - 1) / step;
     Plan p = {};
     auto cut = [&](int ti, int to, int64_t want, int least) {
-        p.cols = (O + to - 1) / to;
+        p.cols = (K + to - 1) / to;
         p.tiles = ((int64_t)I + ti - 1) / ti * p.cols;
         const int64_t parts = std::max<int64_t>(std::min<int64_t>(want / std::max<int64_t>(p.tiles, 1), steps / least), 1);
         p.per = (int)std::max<int64_t>((steps + parts - 1) / parts, 1);
         p.parts = std::max((steps + p.per - 1) / p.per, 1);      // without rows there is still the weights' gradient, zero
     };
-    if (size == 2 && aligned && (rows ? R : I) % 8 == 0 && O % 8 == 0 && a_bytes < kMostBytes && b_bytes < kMostBytes && I >= 192 && O >= 192) {
+    p.pitch = half_of(size, K);
+    const int64_t a_bytes = (int64_t)M * 2 * half * size, b_bytes = (int64_t)(rows ? 2 * N : M) * p.pitch * size;
+    p.spaced = p.pitch != K;
+    if (size == 2 && (aligned || p.spaced) && a_bytes < kMostBytes && b_bytes < kMostBytes && I >= 192 && K >= 192) {
         cut(256, 256, 256, 8);
-        p.turn = p.tiles * p.parts >= 128;
+        p.turn = p.tiles * p.parts >= 96;
         if (p.turn) return p;
     }
-    p.large = ((int64_t)I + 127) / 128 * ((O + 127) / 128) >= 512;
+    p.spaced = false;
+    p.pitch = K;
+    p.large = ((int64_t)I + 127) / 128 * ((K + 127) / 128) >= 512;
     cut(p.large ? 128 : 64, 128, 768, 6);
     return p;
 }
-int64_t part_bytes(const Plan &p, int I, int O) { return p.parts > 1 ? (int64_t)p.parts * I * O * 4 : 0; }
-template <class T, bool kRows>
-hipError_t go_dense(const void *a, const void *b, int I, int O, int R, void *out, const Plan &p, void *sums, hipStream_t st) {
-    const int64_t blocks = p.tiles * p.parts, count = (int64_t)I * O;
+// device memory of a product, behind each other: b laid out anew, the parts' sums
+int64_t spaced_bytes(const Plan &p, int size, bool rows, int M, int N) {
+    return p.spaced ? ((int64_t)(rows ? 2 * N : M) * p.pitch * size + 255) / 256 * 256 : 0;
+}
+int64_t part_bytes(const Plan &p, bool rows, int M, int N, int K) { return p.parts > 1 ? (int64_t)p.parts * (rows ? M : 2 * N) * K * 4 : 0; }
+template <class T, bool kRows> hipError_t go_dense(const void *a, const void *b, int M, int N, int K, void *out, void *scratch, hipStream_t st) {
+    const Plan p = plan_of(sizeof(T), kRows, M, N, K, (uintptr_t)b % 16 == 0);
+    float *sums = (float *)((char *)scratch + spaced_bytes(p, sizeof(T), kRows, M, N));
+    const int64_t blocks = p.tiles * p.parts, I = kRows ? M : 2 * N, count = I * K;
     if (blocks > most_blocks(512)) return kTooLarge;
-    const Dense g = {a, b, I, O, R, out, p.parts > 1 ? (float *)sums : nullptr, (int)p.tiles, p.cols, p.per};
+    if (p.spaced) {
+        constexpr int kE = 16 / sizeof(T);
+        const int64_t rows = kRows ? 2 * N : M, pieces = (rows * (p.pitch / kE) + 255) / 256;
+        if (pieces > most_blocks(256)) return kTooLarge;
+        hipLaunchKernelGGL(spaced_kernel<T>, dim3((unsigned)pieces), dim3(256), 0, st, (const T *)b, rows, K, p.pitch, (T *)scratch);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        b = scratch;
+    }
+    const Dense g = {a, b, (int)I, K, M, p.pitch, N, half_of(sizeof(T), N), out, p.parts > 1 ? sums : nullptr, (int)p.tiles, p.cols, p.per};
     if (p.turn) {
         if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((dense_turn_kernel<T, kRows>), dim3((unsigned)blocks), dim3(512), 0, st, g);
     } else if (p.large) {
@@ -446,19 +491,21 @@ hipError_t launch_gated(int type, int act, const void *x, const void *w, int M, 
     });
 }
 int64_t gated_kept(int type, int M, int N) { return (int64_t)M * 2 * N * (type == kOpF32 ? 4 : 3); }
-// dg and du, then the parts' sums of one product at a time; whether the rows turn out to be aligned or not
-int64_t dgu_bytes(int type, int M, int N) { return ((int64_t)M * 2 * N * op_bytes(type) + 255) / 256 * 256; }
+// dg and du, then what one product at a time takes; whether its operand turns out to be aligned or not
+int64_t dgu_bytes(int type, int M, int N) { return ((int64_t)M * 2 * half_of(op_bytes(type), N) * op_bytes(type) + 255) / 256 * 256; }
 int64_t gated_grad_scratch(int type, int M, int N, int K) {
     const int size = op_bytes(type);
-    int64_t sums = 0;
+    int64_t most = 0;
     for (bool aligned : {false, true})
-        sums = std::max({sums, part_bytes(plan_of(size, true, M, K, 2 * N, aligned), M, K), part_bytes(plan_of(size, false, 2 * N, K, M, aligned), 2 * N, K)});
-    return dgu_bytes(type, M, N) + sums;
+        for (bool rows : {false, true}) {
+            const Plan p = plan_of(size, rows, M, N, K, aligned);
+            most = std::max(most, spaced_bytes(p, size, rows, M, N) + part_bytes(p, rows, M, N, K));
+        }
+    return dgu_bytes(type, M, N) + most;
 }
 hipError_t launch_gated_grad(int type, int act, const void *x, const void *w, const void *gu, const void *dy, int M, int N, int K,
                              void *dx, void *dw, void *scratch, hipStream_t st) {
-    void *dgu = scratch, *sums = (char *)scratch + dgu_bytes(type, M, N);
-    const int size = op_bytes(type);
+    void *dgu = scratch, *rest = (char *)scratch + dgu_bytes(type, M, N);
     hipError_t e = with_type(type, [&](auto one) {
         return with_act(act, [&](auto k) { return go_slope<decltype(one), decltype(k)::value>(gu, dy, M, N, dgu, st); });
     });
@@ -466,9 +513,8 @@ hipError_t launch_gated_grad(int type, int act, const void *x, const void *w, co
     return with_type(type, [&](auto one) {
         typedef decltype(one) T;
         hipError_t e = hipSuccess;
-        if (dx) e = go_dense<T, true>(dgu, w, M, K, 2 * N, dx, plan_of(size, true, M, K, 2 * N, (uintptr_t)w % 16 == 0), sums, st);
-        if (e == hipSuccess && dw)
-            e = go_dense<T, false>(dgu, x, 2 * N, K, M, dw, plan_of(size, false, 2 * N, K, M, (uintptr_t)x % 16 == 0), sums, st);
+        if (dx) e = go_dense<T, true>(dgu, w, M, N, K, dx, rest, st);
+        if (e == hipSuccess && dw) e = go_dense<T, false>(dgu, x, M, N, K, dw, rest, st);
         return e;
     });
 }
