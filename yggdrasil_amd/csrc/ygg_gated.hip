@@ -86,26 +86,41 @@ template <class T> struct Kept {
             }
         }
     }
-    template <int kN> __device__ __forceinline__ void get(int64_t at, float *v, int left) const {
-        if constexpr (sizeof(T) == 4) {
-            static_assert(kN == 4, "");
-            unpack(load16((const float *)p + at, left), v, 0.0f);
-        } else {
-            static_assert(kN == 8, "");
-            const u32x4 h = load16((const uint16_t *)p + at, left);
-            const uint8_t *lo = (const uint8_t *)p + 2 * count + at;
-            u32x2 l = {0, 0};
-            if (left >= kN) {
-                __builtin_memcpy(&l, lo, 8);
-            } else {
-#pragma unroll
-                for (int j = 0; j < kN; j++)
-                    if (j < left) l[j / 4] |= (uint32_t)lo[j] << 8 * (j % 4);
-            }
-#pragma unroll
-            for (int j = 0; j < kN; j++)
-                v[j] = __builtin_bit_cast(float, (h[j / 2] >> 16 * (j % 2)) << 16 | (l[j / 4] >> 8 * (j % 4) & 0xffu) << 8);
+    // what is kept of 16 bytes of values, as it lies there; past: past the caches, which would not hold it until it is read again
+    struct Piece {
+        u32x4 hi;
+        u32x2 lo;
+    };
+    template <bool kPast> __device__ __forceinline__ Piece load(int64_t at) const {
+        typedef uint32_t hi_t __attribute__((ext_vector_type(4), aligned(1)));
+        typedef uint32_t lo_t __attribute__((ext_vector_type(2), aligned(1)));
+        Piece v = {};
+        const hi_t *hi = (const hi_t *)(p + at * (sizeof(T) == 4 ? 4 : 2));
+        v.hi = kPast ? __builtin_nontemporal_load(hi) : *hi;
+        if constexpr (sizeof(T) == 2) {
+            const lo_t *lo = (const lo_t *)(p + 2 * count + at);
+            v.lo = kPast ? __builtin_nontemporal_load(lo) : *lo;
         }
+        return v;
+    }
+    // the first `left` of a piece
+    __device__ __forceinline__ Piece load(int64_t at, int left) const {
+        Piece v = {};
+        if constexpr (sizeof(T) == 4) {
+            v.hi = load16((const float *)p + at, left);
+        } else {
+            v.hi = load16((const uint16_t *)p + at, left);
+            const uint8_t *lo = (const uint8_t *)p + 2 * count + at;
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (j < left) v.lo[j / 4] |= (uint32_t)lo[j] << 8 * (j % 4);
+        }
+        return v;
+    }
+    static __device__ __forceinline__ void values(const Piece &v, float *f) {
+#pragma unroll
+        for (int j = 0; j < 16 / (int)sizeof(T); j++)
+            f[j] = __builtin_bit_cast(float, sizeof(T) == 4 ? v.hi[j] : (v.hi[j / 2] >> 16 * (j % 2)) << 16 | (v.lo[j / 4] >> 8 * (j % 4) & 0xffu) << 8);
     }
 };
 
@@ -232,17 +247,29 @@ __global__ __launch_bounds__(64 * kW) void gated_few_kernel(const T *x, const T 
 // dg and du lie `half` values apart in rows of 2 half, N up to whole 16 bytes, so that the products' loads are aligned; zeros between.
 __host__ __device__ constexpr int half_of(int size, int N) { return (N + 16 / size - 1) / (16 / size) * (16 / size); }
 // dg and du of pieces of 16 bytes of dy
-template <class T, int kAct>
+template <class T, int kAct, bool kPast>
 __global__ __launch_bounds__(256) void gated_slope_kernel(Kept<T> gu, const T *dy, int M, int N, T *dgu) {
     constexpr int kE = 16 / sizeof(T);
     const int half = half_of(sizeof(T), N), per = half / kE;
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / per;
     if (row >= M) return;
     const int n = (int)(id % per) * kE, left = N - n;
+    const int64_t at = row * 2 * N + n;
+    typename Kept<T>::Piece gp, up;
+    u32x4 dp;
+    if (left >= kE) {
+        gp = gu.template load<kPast>(at);
+        up = gu.template load<kPast>(at + N);
+        dp = load16(dy + row * N + n);
+    } else {
+        gp = gu.load(at, left);
+        up = gu.load(at + N, left);
+        dp = load16(dy + row * N + n, left);
+    }
     float g[kE], u[kE], d[kE];
-    gu.template get<kE>(row * 2 * N + n, g, left);
-    gu.template get<kE>(row * 2 * N + n + N, u, left);
-    unpack(load16(dy + row * N + n, left), d, T());
+    Kept<T>::values(gp, g);
+    Kept<T>::values(up, u);
+    unpack(dp, d, T());
 #pragma unroll
     for (int j = 0; j < kE; j++) {
         float slope;
@@ -251,8 +278,8 @@ __global__ __launch_bounds__(256) void gated_slope_kernel(Kept<T> gu, const T *d
         u[j] = d[j] * a;
     }
     T *out = dgu + row * 2 * half + n;
-    store_run<T, kE>(out, g, kE);
-    store_run<T, kE>(out + half, u, kE);
+    store_run<T, kE>(out, g, kE, kPast);
+    store_run<T, kE>(out + half, u, kE, kPast);
 }
 
 // ---- the gradients' products: out (I, O) = sum over r of A(i, r) b(r, o), b's rows `pitch` values apart. kRows: A is a (I, 2 half), the r's
@@ -408,8 +435,12 @@ template <class T, int kAct> hipError_t go_slope(const void *gu, const void *dy,
     const int64_t blocks = ((int64_t)M * (half_of(sizeof(T), N) / kE) + 255) / 256;
     if (blocks == 0) return hipSuccess;
     if (blocks > most_blocks(256)) return kTooLarge;
-    hipLaunchKernelGGL((gated_slope_kernel<T, kAct>), dim3((unsigned)blocks), dim3(256), 0, st, Kept<T>{(char *)gu, (int64_t)M * 2 * N},
-                       (const T *)dy, M, N, (T *)dgu);
+    const Kept<T> kept = {(char *)gu, (int64_t)M * 2 * N};
+    // 16384 x 4096 bf16: 184 us with the caches, 145 past them
+    if (kept.count * Kept<T>::kBytes >= kPastBytes)
+        hipLaunchKernelGGL((gated_slope_kernel<T, kAct, true>), dim3((unsigned)blocks), dim3(256), 0, st, kept, (const T *)dy, M, N, (T *)dgu);
+    else
+        hipLaunchKernelGGL((gated_slope_kernel<T, kAct, false>), dim3((unsigned)blocks), dim3(256), 0, st, kept, (const T *)dy, M, N, (T *)dgu);
     return hipGetLastError();
 }
 

@@ -19,7 +19,7 @@
 // through the segments from the last one, whose values the memory's cache still holds, and neighbouring segments are one XCD's.
 // States, maps and their joins are in f32; h, dx and da are rounded to their types once, on the way out.
 //
-// The memory bounds it. 16 x 4096 x 2048 bf16: forward 160 us (2 readings and a writing of 268 MB, 5.0 TB/s), backward 276 us (3 and
+// The memory bounds it. 16 x 4096 x 2048 bf16: forward 155 us (2 readings and a writing of 268 MB, 5.2 TB/s), backward 273 us (3 and
 // 2, 4.9 TB/s); 131072 x 256 bf16 with gates in f32: 33 us for the segments' maps, 49 for the states. Workgroups of 512 threads
 // (295 us backward) and of half as many channels (300) were slower.
 #include <algorithm>
@@ -69,7 +69,7 @@ template <class T, int kV> struct Few {
         } else {
             any a;
             __builtin_memcpy(&a, w, sizeof(w));
-            if (past) __builtin_nontemporal_store(a, (any *)p);
+            if (past) store_past(a, p);
             else *(any *)p = a;
         }
     }

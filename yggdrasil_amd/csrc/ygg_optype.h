@@ -100,9 +100,16 @@ template <class T, int kN, class V> __device__ __forceinline__ void store_run(T 
 }
 
 // The same past the caches where `past`. A result that is larger than the memory's cache (256 MB) has pushed its own beginning out
-// by the time that it is whole, and the inputs with it: written past it, it leaves them for the next reader. Layer norm of 268 MB bf16
-// 106 us with the caches, 90 past them, the recurrence's 268 MB 165 and 153, clipping of 320 MB 189 and 162.
+// by the time that it is whole, and the inputs with it: written past it, it leaves them for the next reader. Of 268 MB bf16 layer norm's
+// gradient took 166 us with the caches and 157 past them, the recurrence 165 and 155, clipping of 320 MB 189 and 162.
 constexpr int64_t kPastBytes = 256 << 20;
+// Of a branch's two stores that differ in this alone the compiler makes one, without it: the asm keeps them apart.
+template <class V> __device__ __forceinline__ void store_past(V v, void *p) {
+    typedef V any __attribute__((aligned(1)));
+    asm volatile("" ::: "memory");
+    __builtin_nontemporal_store(v, (any *)p);
+    asm volatile("" ::: "memory");
+}
 template <class T, int kN, class V> __device__ __forceinline__ void store_run(T *p, const V *v, int left, bool past) {
     typedef uint32_t any __attribute__((ext_vector_type(kN * sizeof(T) / 4), aligned(1)));
     if (!past || left < kN) return store_run<T, kN>(p, v, left);
@@ -111,7 +118,7 @@ template <class T, int kN, class V> __device__ __forceinline__ void store_run(T 
     for (int j = 0; j < kN; j++) t[j] = from_f32<T>(v[j]);
     any a;
     __builtin_memcpy(&a, t, sizeof(a));
-    __builtin_nontemporal_store(a, (any *)p);
+    store_past(a, p);
 }
 
 }  // namespace ygg
