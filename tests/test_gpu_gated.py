@@ -103,6 +103,14 @@ def test_few_rows(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("M, N, K", [(32, 4100, 136), (33, 2048, 520), (70, 1500, 72), (100, 1300, 1031), (256, 1024, 264), (250, 1000, 96),
+                                     (512, 1020, 200), (17, 8200, 40), (64, 8190, 64)])
+def test_few_tiles(M, N, K, dtype):
+    """Batches between a tile's rows and many: each form of the kernel without a tile in LDS, and where they end."""
+    check(*make(M, N, K, dtype, seed=N), "silu", train=M == 100)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
 def test_off_an_alignment_and_strides(dtype):
     x, w, dy = make(70, 96, 160, dtype, seed=1)
     for at in (1, 3):

@@ -189,59 +189,84 @@ __global__ __launch_bounds__(512) void gated_turn_kernel(const T *x, const T *w,
     put_tile<T, kAct>(tile.acc, Tl::row0(), Tl::col0() / 64, M, n0, N, y, gu, i0);
 }
 
-// Few rows: 16 of them by 16 outputs a workgroup, whose kW waves take a part of K each, fragments straight from memory
-template <class T, int kW, int kAct>
-__global__ __launch_bounds__(64 * kW) void gated_few_kernel(const T *x, const T *w, int M, int N, int K, T *y, Kept<T> gu, int cols) {
-    constexpr int kE = 16 / sizeof(T), kStep = 4 * kE, kU = 4;
-    __shared__ f32x4 parts[kW][2][64];
-    const int t = tile_of(blockIdx.x, gridDim.x), n0 = t % cols * 16, l = threadIdx.x & 63, wave = threadIdx.x >> 6, d = l & 15, q = l >> 4;
-    const int row = t / cols * 16 + d;
-    f32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-    const int steps = (K + kStep - 1) / kStep, per = (steps + kW - 1) / kW, end = min(per * (wave + 1), steps);
-    const T *gp = w + (int64_t)min(n0 + d, N - 1) * K + q * kE, *up = gp + (int64_t)N * K, *xp = x + (int64_t)min(row, M - 1) * K + q * kE;
-    const int last = K - q * kE;
+// Few tiles: 16 FR rows by 16 FC outputs a workgroup, whose four waves take a part of K each, fragments straight from memory
+template <class T, int FR, int FC, int kAct>
+__global__ __launch_bounds__(256) void gated_few_kernel(const T *x, const T *w, int M, int N, int K, T *y, Kept<T> gu, int cols) {
+    constexpr int kE = 16 / sizeof(T), kStep = 4 * kE, kU = FR == 1 ? 4 : 2;
+    __shared__ f32x4 parts[4][FR * FC][2][64];
+    // the rows' tiles of a column of outputs follow each other: they share its weights
+    const int t = tile_of(blockIdx.x, gridDim.x), tall = gridDim.x / cols, n0 = t / tall * 16 * FC, m0 = t % tall * 16 * FR;
+    const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, d = l & 15, q = l >> 4;
+    f32x4 acc[FR][FC][2];
+#pragma unroll
+    for (int i = 0; i < FR; i++)
+#pragma unroll
+        for (int o = 0; o < FC; o++) acc[i][o][0] = acc[i][o][1] = f32x4{0, 0, 0, 0};
+    const int steps = (K + kStep - 1) / kStep, per = (steps + 3) / 4, end = min(per * (wave + 1), steps);
+    const T *wp[FC], *xp[FR];
+    const int64_t to_u = (int64_t)N * K;
+#pragma unroll
+    for (int o = 0; o < FC; o++) wp[o] = w + (int64_t)min(n0 + 16 * o + d, N - 1) * K + q * kE;
+#pragma unroll
+    for (int i = 0; i < FR; i++) xp[i] = x + (int64_t)min(m0 + 16 * i + d, M - 1) * K + q * kE;
     int s = per * wave;
     for (; s + kU <= end && (s + kU) * kStep <= K; s += kU) {
-        u32x4 a[kU], b[kU], c[kU];
+        u32x4 a[kU][FC][2], c[kU][FR];
 #pragma unroll
-        for (int k = 0; k < kU; k++) {
-            a[k] = load16(gp + (s + k) * kStep);
-            b[k] = load16(up + (s + k) * kStep);
-        }
+        for (int k = 0; k < kU; k++)
 #pragma unroll
-        for (int k = 0; k < kU; k++) c[k] = load16(xp + (s + k) * kStep);
+            for (int o = 0; o < FC; o++) {
+                a[k][o][0] = load16(wp[o] + (s + k) * kStep);
+                a[k][o][1] = load16(wp[o] + to_u + (s + k) * kStep);
+            }
 #pragma unroll
-        for (int k = 0; k < kU; k++) {
-            acc[0] = Mma<T>::run(a[k], c[k], acc[0]);
-            acc[1] = Mma<T>::run(b[k], c[k], acc[1]);
-        }
+        for (int k = 0; k < kU; k++)
+#pragma unroll
+            for (int i = 0; i < FR; i++) c[k][i] = load16(xp[i] + (s + k) * kStep);
+#pragma unroll
+        for (int k = 0; k < kU; k++)
+#pragma unroll
+            for (int i = 0; i < FR; i++)
+#pragma unroll
+                for (int o = 0; o < FC; o++) {
+                    acc[i][o][0] = Mma<T>::run(a[k][o][0], c[k][i], acc[i][o][0]);
+                    acc[i][o][1] = Mma<T>::run(a[k][o][1], c[k][i], acc[i][o][1]);
+                }
     }
+    const int last = K - q * kE;
+    auto load_end = [&](const T *p) { return K >= kE ? load16_end(p + s * kStep, last - s * kStep) : load16(p + s * kStep, last - s * kStep); };
     for (; s < end; s++) {
-        const int n = last - s * kStep;
-        u32x4 a, b, c;
-        if (K >= kE) {
-            a = load16_end(gp + s * kStep, n);
-            b = load16_end(up + s * kStep, n);
-            c = load16_end(xp + s * kStep, n);
-        } else {
-            a = load16(gp + s * kStep, n);
-            b = load16(up + s * kStep, n);
-            c = load16(xp + s * kStep, n);
-        }
-        acc[0] = Mma<T>::run(a, c, acc[0]);
-        acc[1] = Mma<T>::run(b, c, acc[1]);
-    }
-    parts[wave][0][l] = acc[0];
-    parts[wave][1][l] = acc[1];
-    __syncthreads();
-    if (wave) return;
+        u32x4 c[FR];
 #pragma unroll
-    for (int i = 1; i < kW; i++) {
-        acc[0] += parts[i][0][l];
-        acc[1] += parts[i][1][l];
+        for (int i = 0; i < FR; i++) c[i] = load_end(xp[i]);
+#pragma unroll
+        for (int o = 0; o < FC; o++) {
+            const u32x4 a = load_end(wp[o]), b = load_end(wp[o] + to_u);
+#pragma unroll
+            for (int i = 0; i < FR; i++) {
+                acc[i][o][0] = Mma<T>::run(a, c[i], acc[i][o][0]);
+                acc[i][o][1] = Mma<T>::run(b, c[i], acc[i][o][1]);
+            }
+        }
     }
-    const int n = n0 + 4 * q;
-    if (row < M && n < N) put_outputs<T, kAct, 4>((const float *)&acc[0], (const float *)&acc[1], row, n, N, y, gu);
+#pragma unroll
+    for (int i = 0; i < FR; i++)
+#pragma unroll
+        for (int o = 0; o < FC; o++) {
+            parts[wave][i * FC + o][0][l] = acc[i][o][0];
+            parts[wave][i * FC + o][1][l] = acc[i][o][1];
+        }
+    __syncthreads();
+    for (int f = wave; f < FR * FC; f += 4) {
+        f32x4 g = parts[0][f][0][l], u = parts[0][f][1][l];
+#pragma unroll
+        for (int k = 1; k < 4; k++) {
+            g += parts[k][f][0][l];
+            u += parts[k][f][1][l];
+        }
+        const int row = m0 + 16 * (f / FC) + d, n = n0 + 16 * (f % FC) + 4 * q;
+        if (row < M && n < N) put_outputs<T, kAct, 4>((const float *)&g, (const float *)&u, row, n, N, y, gu);
+    }
 }
 
 // dg and du lie `half` values apart in rows of 2 half, N up to whole 16 bytes, so that the products' loads are aligned; zeros between.
@@ -410,12 +435,25 @@ template <class T, int kAct> hipError_t go(const void *x, const void *w, int M, 
             return hipGetLastError();
         }
     }
-    if (M <= 16) {
-        const int cols = (N + 15) / 16;
-        hipLaunchKernelGGL((gated_few_kernel<T, 4, kAct>), dim3((unsigned)cols), dim3(256), 0, st, (const T *)x, (const T *)w, M, N, K,
-                           (T *)y, gu, cols);
+    auto few = [&](auto fr, auto fc) {
+        constexpr int FR = decltype(fr)::value, FC = decltype(fc)::value;
+        const int cols = (N + 16 * FC - 1) / (16 * FC);
+        hipLaunchKernelGGL((gated_few_kernel<T, FR, FC, kAct>), dim3((unsigned)(cols * ((M + 16 * FR - 1) / (16 * FR)))), dim3(256), 0, st,
+                           (const T *)x, (const T *)w, M, N, K, (T *)y, gu, cols);
         return hipGetLastError();
-    }
+    };
+    constexpr std::integral_constant<int, 1> one{};
+    constexpr std::integral_constant<int, 2> two{};
+    constexpr std::integral_constant<int, 4> four{};
+    // Few tiles, as long as they are no more than the CUs: the smallest that are. bf16, in the tiles below and in these: 32 x 4096 x 1024
+    // (rows, K, N) 34 and 16.5 us, 128 x 4096 x 1024 34 and 17, 256 x 4096 x 1024 35 and 25, 32 x 4096 x 8192 46 and 26, 64 x 4096 x 8192
+    // 46 and 35; of twice as many as the CUs 128 x 4096 x 8192 46 and 60. The largest is no gain for 16-bit rows
+    // off an alignment of 16 bytes (512 x 777 x 1001 13 and 17; f32 36 and 22).
+    auto fits = [&](int fr, int fc) { return ((int64_t)M + 16 * fr - 1) / (16 * fr) * ((N + 16 * fc - 1) / (16 * fc)) <= 256; };
+    if (M <= 16) return few(one, one);
+    if (fits(2, 1)) return few(two, one);
+    if (fits(2, 2)) return few(two, two);
+    if (fits(4, 2) && (sizeof(T) == 4 || row % 16 == 0)) return few(four, two);
     auto tiles = [&](auto fi, auto wi, auto wo) {
         constexpr int FI = decltype(fi)::value, WI = decltype(wi)::value, WO = decltype(wo)::value, kI = 16 * FI * WI;
         const int cols = (N + 32 * WO - 1) / (32 * WO);
@@ -425,8 +463,6 @@ template <class T, int kAct> hipError_t go(const void *x, const void *w, int M, 
                            (const T *)w, M, N, K, (T *)y, gu, cols, kBand);
         return hipGetLastError();
     };
-    constexpr std::integral_constant<int, 2> two{};
-    constexpr std::integral_constant<int, 4> four{};
     const int64_t tiles128 = ((int64_t)M + 127) / 128 * ((N + 63) / 64);
     return tiles128 >= 512 ? tiles(four, two, two) : tiles(two, two, two);
 }
