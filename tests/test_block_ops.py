@@ -51,7 +51,8 @@ NORM_GRAD = dict(x=P, type=1, rows=2, n=8, stride=8, w=P, w_type=0, stats=P, dy=
 
 @pytest.mark.parametrize("kw, word", [
     (dict(type=-1), b"type"), (dict(w_type=2), b"weight_type"), (dict(rows=-1), b"rows"), (dict(n=0), b"n "), (dict(stride=7), b"apart"),
-    (dict(stats=None), b"NULL"), (dict(dy=None), b"NULL"), (dict(x=None), b"NULL"), (dict(scratch=None), b"scratch"), (dict(bytes=8), b"scratch")])
+    (dict(stats=None), b"NULL"), (dict(dy=None), b"NULL"), (dict(x=None), b"NULL"), (dict(scratch=None), b"scratch"), (dict(bytes=8), b"scratch"),
+    (dict(n=20000, stride=20000, dw=None, db=None, scratch=None), b"scratch")])
 def test_layer_norm_grad_refuses(kw, word):
     refused("ygg_layer_norm_grad", NORM_GRAD, kw, word)
 

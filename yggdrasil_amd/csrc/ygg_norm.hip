@@ -249,7 +249,7 @@ template <class T> __global__ __launch_bounds__(1024) void norm_wide_kernel(cons
 
 // ---- backward: dx, and a workgroup's sums of dy z and dy over its rows into part[blockIdx][2][n]
 template <class T, int kL, int kP, bool kTiny>
-__global__ __launch_bounds__(kL > 256 ? kL : 256) void norm_grad_kernel(const NormGradArgs a, float *part) {
+__global__ __launch_bounds__(kL > 256 ? kL : 256, 2) void norm_grad_kernel(const NormGradArgs a, float *part) {
     constexpr int kThreads = kL > 256 ? kL : 256, kRows = kThreads / kL, kE = kEach<T>, kIn = kL < 64 ? kL : 64;
     __shared__ float2 waves[2][kThreads / 64];
     __shared__ float sums[kL <= 64 ? 2 : 1][kL <= 64 ? kL * kP * kE : 1];
@@ -382,8 +382,10 @@ __global__ __launch_bounds__(kL > 256 ? kL : 256) void norm_grad_kernel(const No
     }
 }
 
-// Wider rows: dx by a workgroup a row, in two readings, and the columns' sums by a kernel of their own
-template <class T> __global__ __launch_bounds__(1024) void norm_grad_wide_kernel(const NormGradArgs a) {
+// Wider rows, in two readings. The columns' sums by workgroups of a slab of columns and every groups-th row, which also leave each
+// wave's part of a row's sums of q and q z, as (rows, waves, 2); then dx by a workgroup a row, which adds those.
+template <class T> __host__ __device__ constexpr int waves_of(int n) { return (n + 64 * kEach<T> - 1) / (64 * kEach<T>); }
+template <class T> __global__ __launch_bounds__(1024) void norm_grad_wide_kernel(const NormGradArgs a, const float2 *given) {
     constexpr int kE = kEach<T>;
     __shared__ float lds[16];
     const int n = a.n;
@@ -391,16 +393,11 @@ template <class T> __global__ __launch_bounds__(1024) void norm_grad_wide_kernel
         const T *x = (const T *)a.x + row * a.stride, *dy = (const T *)a.dy + row * n;
         const float2 s = ((const float2 *)a.stats)[row];
         float q1 = 0.0f, q2 = 0.0f;
-        each_piece<T, 1024>(x, dy, n, [&](int c, const float *v, const float *d, int) {
-            float w[kE];
-            load_weight<T, kE>(w, a.weight, a.wide, c, n, 1.0f);
-#pragma unroll
-            for (int j = 0; j < kE; j++) {
-                const float q = w[j] * d[j];
-                q1 += q;
-                q2 = __builtin_fmaf(q, (v[j] - s.x) * s.y, q2);
-            }
-        });
+        for (int i = threadIdx.x; i < waves_of<T>(n); i += 1024) {
+            const float2 q = given[row * waves_of<T>(n) + i];
+            q1 += q.x;
+            q2 += q.y;
+        }
         q1 = sum_all<1024>(q1, lds) / (float)n;
         q2 = sum_all<1024>(q2, lds) / (float)n;
         T *dx = (T *)a.dx + row * n;
@@ -409,31 +406,60 @@ template <class T> __global__ __launch_bounds__(1024) void norm_grad_wide_kernel
             load_weight<T, kE>(w, a.weight, a.wide, c, n, 1.0f);
 #pragma unroll
             for (int j = 0; j < kE; j++) f[j] = (w[j] * d[j] - q1 - (v[j] - s.x) * s.y * q2) * s.y;
-            store_run<T, kE>(dx + c, f, left);
+            store_run<T, kE>(dx + c, f, left, a.past);
         });
     }
 }
-template <class T> __global__ __launch_bounds__(256) void norm_columns_kernel(const NormGradArgs a, float *part, int groups) {
-    constexpr int kE = kEach<T>;
-    const int n = a.n, g = blockIdx.x % groups, c = (blockIdx.x / groups * 256 + threadIdx.x) * kE;
-    if (c >= n) return;
-    float aw[kE], ab[kE];
+template <class T> __global__ __launch_bounds__(256) void norm_columns_kernel(const NormGradArgs a, float *part, int groups, float2 *given) {
+    constexpr int kE = kEach<T>, kU = 4;
+    const int n = a.n, g = blockIdx.x % groups, c = (blockIdx.x / groups * 256 + threadIdx.x) * kE, left = n - c;
+    const int wave = blockIdx.x / groups * 4 + threadIdx.x / 64, waves = waves_of<T>(n);
+    if (wave >= waves) return;      // lanes past the end go on with zeros
+    float aw[kE], ab[kE], w[kE];
 #pragma unroll
     for (int j = 0; j < kE; j++) aw[j] = ab[j] = 0.0f;
-    for (int64_t row = g; row < a.rows; row += groups) {
-        const float2 s = ((const float2 *)a.stats)[row];
-        float v[kE], d[kE];
-        unpack(load16((const T *)a.x + row * a.stride + c, n - c), v, T());
-        unpack(load16((const T *)a.dy + row * n + c, n - c), d, T());
+    load_weight<T, kE>(w, a.weight, a.wide, min(c, n - 1), n, 1.0f);
+    for (int64_t first = g; first < a.rows; first += kU * (int64_t)groups) {
+        u32x4 x[kU], dy[kU];
+        float2 s[kU];
 #pragma unroll
-        for (int j = 0; j < kE; j++) {
-            aw[j] = __builtin_fmaf(d[j], (v[j] - s.x) * s.y, aw[j]);
-            ab[j] += d[j];
+        for (int k = 0; k < kU; k++) {
+            const int64_t row = min(first + k * (int64_t)groups, a.rows - 1);
+            const T *xp = (const T *)a.x + row * a.stride, *dp = (const T *)a.dy + row * n;
+            if (left >= kE) {
+                x[k] = load16(xp + c);
+                dy[k] = load16(dp + c);
+            } else {
+                x[k] = load16(xp + min(c, n), left);
+                dy[k] = load16(dp + min(c, n), left);
+            }
+            s[k] = ((const float2 *)a.stats)[row];
+        }
+#pragma unroll
+        for (int k = 0; k < kU; k++) {
+            const int64_t row = first + k * (int64_t)groups;
+            if (row >= a.rows) break;
+            float v[kE], d[kE], q1 = 0.0f, q2 = 0.0f;
+            unpack(x[k], v, T());
+            unpack(dy[k], d, T());
+#pragma unroll
+            for (int j = 0; j < kE; j++) {
+                const float z = (v[j] - s[k].x) * s[k].y, q = w[j] * d[j];
+                aw[j] = __builtin_fmaf(d[j], z, aw[j]);
+                ab[j] += d[j];
+                q1 += j < left ? q : 0.0f;
+                q2 += j < left ? q * z : 0.0f;
+            }
+            if (!given) continue;
+            q1 = sum_of<64>(q1);
+            q2 = sum_of<64>(q2);
+            if (threadIdx.x % 64 == 0) given[row * waves + wave] = make_float2(q1, q2);
         }
     }
+    if (left <= 0 || !part) return;
     float *out = part + (int64_t)g * 2 * n + c;
-    store_run<float, kE>(out, aw, n - c);
-    store_run<float, kE>(out + n, ab, n - c);
+    store_run<float, kE>(out, aw, left);
+    store_run<float, kE>(out + n, ab, left);
 }
 
 // The groups' sums of a column, 16 runs of them side by side
@@ -534,12 +560,12 @@ template <class T> hipError_t go_grad(NormGradArgs a, void *scratch, hipStream_t
         if (a.n <= 512 * 4 * kE) {
             hipLaunchKernelGGL((norm_grad_kernel<T, 512, 4, false>), dim3((unsigned)groups), dim3(512), 0, st, a, part);
         } else {
+            const int slabs = (a.n + 256 * kE - 1) / (256 * kE);
+            float2 *given = a.dx ? (float2 *)((char *)scratch + groups * 2 * a.n * 4) : nullptr;
+            hipLaunchKernelGGL(norm_columns_kernel<T>, dim3((unsigned)(groups * slabs)), dim3(256), 0, st, a, part, (int)groups, given);
             if (a.dx)
-                hipLaunchKernelGGL(norm_grad_wide_kernel<T>, dim3((unsigned)std::min<int64_t>(a.rows, 1024)), dim3(1024), 0, st, a);
-            if (part) {
-                const int slabs = (a.n + 256 * kE - 1) / (256 * kE);
-                hipLaunchKernelGGL(norm_columns_kernel<T>, dim3((unsigned)(groups * slabs)), dim3(256), 0, st, a, part, (int)groups);
-            }
+                hipLaunchKernelGGL(norm_grad_wide_kernel<T>, dim3((unsigned)std::min<int64_t>(a.rows, 1024)), dim3(1024), 0, st, a,
+                                   (const float2 *)given);
         }
     }
     hipError_t e = hipGetLastError();
@@ -554,10 +580,12 @@ template <class T> hipError_t go_grad(NormGradArgs a, void *scratch, hipStream_t
 
 }  // namespace
 
-int64_t norm_grad_scratch(int type, int64_t rows, int n) {
-    const int64_t groups = type == kOpF32 ? grad_groups<float>(rows, n) : grad_groups<bf16_t>(rows, n);
-    return groups * 2 * n * 4;
+template <class T> bool wide_rows(int n) { return n > 512 * 4 * kEach<T>; }
+template <class T> int64_t scratch_of(int64_t rows, int n) {
+    return grad_groups<T>(rows, n) * 2 * n * 4 + (wide_rows<T>(n) ? rows * waves_of<T>(n) * 8 : 0);
 }
+int64_t norm_grad_scratch(int type, int64_t rows, int n) { return type == kOpF32 ? scratch_of<float>(rows, n) : scratch_of<bf16_t>(rows, n); }
+bool norm_grad_wide(int type, int n) { return type == kOpF32 ? wide_rows<float>(n) : wide_rows<bf16_t>(n); }
 hipError_t launch_norm(int type, const NormArgs &a, hipStream_t st) {
     if (type == kOpF32) return go<float>(a, st);
     if (type == kOpBf16) return go<bf16_t>(a, st);
