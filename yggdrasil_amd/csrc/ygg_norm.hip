@@ -28,6 +28,8 @@ template <class T, int kL, bool kTiny> struct Pieces {
     __device__ __forceinline__ int column(int i) const { return kTiny ? 0 : min(at(i), n - kE); }
     __device__ __forceinline__ bool some(int i) const { return at(i) < n; }
     __device__ __forceinline__ int skip(int i) const { return at(i) - column(i); }
+    // columns and masks are worked out again from here on: those of many pieces held more registers than the values
+    __device__ __forceinline__ void anew() { asm volatile("" : "+v"(lane)); }
     // all lanes' pieces are whole and their own
     __device__ __forceinline__ bool whole(int i) const { return !kTiny && (i + 1) * kL * kE <= n; }
     // value j of piece i is summed here
@@ -69,6 +71,20 @@ __device__ __forceinline__ void load_weight(float *f, const void *p, bool wide, 
     else load_weight<T, kN>(f, (const T *)p, c, n, other);
 }
 
+// a piece that is all there
+template <class T> __device__ __forceinline__ void whole_weight(float *f, const void *p, bool wide, int c, float other) {
+    constexpr int kE = kEach<T>;
+    if (!p) {
+#pragma unroll
+        for (int j = 0; j < kE; j++) f[j] = other;
+    } else if (wide) {
+#pragma unroll
+        for (int k = 0; k < kE; k += 4) unpack(load16((const float *)p + c + k), f + k, 0.0f);
+    } else {
+        unpack(load16((const T *)p + c), f, T());
+    }
+}
+
 // The mean and 1 / sqrt(variance + eps) of a row held by kL lanes. waves: LDS of a workgroup of more than a wave, another one
 // than the row before's.
 template <class T, int kL, bool kTiny, int kP>
@@ -88,6 +104,7 @@ __device__ __forceinline__ float2 moments(u32x4 (&x)[kP], const Pieces<T, kL, kT
 #pragma unroll
                 for (int j = 0; j < kE; j++) f(v[j], at.own(i, j));
             }
+            if constexpr (kP > 4) __builtin_amdgcn_sched_barrier(0);     // a piece at a time, for the registers
         }
     };
     float sum = 0.0f, squares = 0.0f;
@@ -150,28 +167,35 @@ __global__ __launch_bounds__(kL > 256 ? kL : 256) void norm_kernel(const NormArg
     __shared__ float2 waves[2][kThreads / 64];
     constexpr bool kHeld = kL <= 256 || kP <= 2;      // wider rows' weights do not fit LDS: from the caches for each row
     __shared__ Held<T, kHeld ? kL : 1, kHeld ? kP : 1> w, b;
-    const Pieces<T, kL, kTiny> at = {a.n, (int)threadIdx.x % kL};
+    Pieces<T, kL, kTiny> at = {a.n, (int)threadIdx.x % kL};
     const int64_t hop = (int64_t)gridDim.x * kRows;
     int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kL;
-    u32x4 x[kP], next[kP];
-    auto load = [&](int64_t r) {
+    constexpr bool kAhead = kL <= 256 || kP <= 4;     // more pieces leave no registers for the next row's
+    u32x4 x[kP], next[kAhead ? kP : 1];
+    auto load = [&](u32x4 *v, int64_t r) {
         if (r >= a.rows) return;
 #pragma unroll
-        for (int i = 0; i < kP; i++) next[i] = at.load((const T *)a.x + r * a.stride, i);
+        for (int i = 0; i < kP; i++) v[i] = at.load((const T *)a.x + r * a.stride, i);
     };
-    load(row);
+    if constexpr (kAhead) load(next, row);
     if constexpr (kHeld) {
         w.template fill<kThreads, kTiny>(a.weight, a.wide, a.n, 1.0f);
         b.template fill<kThreads, kTiny>(a.bias, a.wide, a.n, 0.0f);
         __syncthreads();
     }
     for (int turn = 0; row < a.rows; row += hop, turn ^= 1) {
+        if constexpr (kAhead) {
 #pragma unroll
-        for (int i = 0; i < kP; i++) x[i] = next[i];
-        load(row + hop);
+            for (int i = 0; i < kP; i++) x[i] = next[i];
+            load(next, row + hop);
+        } else {
+            load(x, row);
+            at.anew();
+        }
         const float2 s = moments(x, at, a.eps, waves[turn]);
         if (a.stats && at.lane == 0) ((float2 *)a.stats)[row] = s;
         let_go(x);
+        if constexpr (!kAhead) at.anew();
         const float c = -s.x * s.y;        // z = x / deviation + c: its rounding is one more of the mean's
         T *y = (T *)a.y + row * a.n;
 #pragma unroll
@@ -182,12 +206,13 @@ __global__ __launch_bounds__(kL > 256 ? kL : 256) void norm_kernel(const NormArg
                 w.get(wf, i, at.lane);
                 b.get(bf, i, at.lane);
             } else {
-                load_weight<T, kE>(wf, a.weight, a.wide, at.column(i), a.n, 1.0f);
-                load_weight<T, kE>(bf, a.bias, a.wide, at.column(i), a.n, 0.0f);
+                whole_weight<T>(wf, a.weight, a.wide, at.column(i), 1.0f);
+                whole_weight<T>(bf, a.bias, a.wide, at.column(i), 0.0f);
             }
 #pragma unroll
             for (int j = 0; j < kE; j++) f[j] = __builtin_fmaf(__builtin_fmaf(f[j], s.y, c), wf[j], bf[j]);
             at.store(y, f, i, a.past);
+            if constexpr (kP > 4) __builtin_amdgcn_sched_barrier(0);
         }
     }
 }
@@ -543,6 +568,8 @@ template <class T> hipError_t go(NormArgs a, hipStream_t st) {
         constexpr int kE = kEach<T>;
         if (a.n <= 1024 * 2 * kE) launch(norm_kernel<T, 1024, 2, false>, 1024, a.rows, 256);
         else if (a.n <= 1024 * 4 * kE) launch(norm_kernel<T, 1024, 4, false>, 1024, a.rows, 256);
+        else if (a.n <= 1024 * 8 * kE) launch(norm_kernel<T, 1024, 8, false>, 1024, a.rows, 256);
+        else if (a.n <= 1024 * 16 * kE) launch(norm_kernel<T, 1024, 16, false>, 1024, a.rows, 256);
         else launch(norm_wide_kernel<T>, 1024, a.rows, 1024);
     }
     return hipGetLastError();
