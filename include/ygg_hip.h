@@ -314,7 +314,7 @@ int ygg_int8_linear(const void *d_x, int type, const int8_t *d_w, const float *d
 int ygg_layer_norm(const void *d_x, int type, int64_t rows, int n, int64_t stride, const void *d_weight, const void *d_bias,
                    int weight_type, float eps, void *d_y, float *d_stats, void *stream);
 /* The gradients, from dy (rows, n) contiguous: of the rows (contiguous, in x's type), of weight and bias (in weight_type;
-   zero without rows). NULL: not wanted; scratch is wanted for those of weight and bias, and for rows of more than 8192 values. */
+   zero without rows). NULL: not wanted; scratch is wanted for those of weight and bias, and for rows of more than 16384 values. */
 int64_t ygg_layer_norm_scratch(int type, int64_t rows, int n);
 int ygg_layer_norm_grad(const void *d_x, int type, int64_t rows, int n, int64_t stride, const void *d_weight, int weight_type,
                         const float *d_stats, const void *d_dy, void *d_dx, void *d_dweight, void *d_dbias, void *d_scratch,

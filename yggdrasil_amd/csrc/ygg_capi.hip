@@ -1352,7 +1352,7 @@ int ygg_layer_norm_grad(const void *d_x, int type, int64_t rows, int n, int64_t 
     if (n < 1 || n > YGG_MOST_INNER) return fail(YGG_ERR_ARG, kOpLimits, "n", (long long)n, 1, YGG_MOST_INNER);
     if (stride < n && rows > 1) return fail(YGG_ERR_ARG, "rows of %d values %lld apart", n, (long long)stride);
     if (rows > 0 && (!d_x || !d_stats || !d_dy)) return fail(YGG_ERR_ARG, "NULL buffer");
-    const int64_t need = rows && (d_dweight || d_dbias || (d_dx && ygg::norm_grad_wide(type, n))) ? ygg::norm_grad_scratch(type, rows, n) : 0;
+    const int64_t need = rows && (d_dweight || d_dbias || (d_dx && ygg::norm_grad_wide(n))) ? ygg::norm_grad_scratch(type, rows, n) : 0;
     if (need && (!d_scratch || scratch_bytes < need))
         return fail(YGG_ERR_ARG, "scratch of %lld bytes, %lld wanted", (long long)scratch_bytes, (long long)need);
     const ygg::NormGradArgs a = {d_x, rows, stride, n, weight_type == 0, d_weight, d_stats, d_dy, d_dx, d_dweight, d_dbias};

@@ -165,7 +165,7 @@ template <class T, int kL, int kP, bool kTiny>
 __global__ __launch_bounds__(kL > 256 ? kL : 256) void norm_kernel(const NormArgs a) {
     constexpr int kThreads = kL > 256 ? kL : 256, kRows = kThreads / kL, kE = kEach<T>;
     __shared__ float2 waves[2][kThreads / 64];
-    constexpr bool kHeld = kL <= 256 || kP <= 2;      // wider rows' weights do not fit LDS: from the caches for each row
+    constexpr bool kHeld = kL <= 256;      // wider rows' weights come from the caches for each row, so that LDS holds off no workgroup
     __shared__ Held<T, kHeld ? kL : 1, kHeld ? kP : 1> w, b;
     Pieces<T, kL, kTiny> at = {a.n, (int)threadIdx.x % kL};
     const int64_t hop = (int64_t)gridDim.x * kRows;
@@ -195,7 +195,7 @@ __global__ __launch_bounds__(kL > 256 ? kL : 256) void norm_kernel(const NormArg
         const float2 s = moments(x, at, a.eps, waves[turn]);
         if (a.stats && at.lane == 0) ((float2 *)a.stats)[row] = s;
         let_go(x);
-        if constexpr (!kAhead) at.anew();
+        if constexpr (!kAhead || (kL == 1024 && sizeof(T) == 2)) at.anew();
         const float c = -s.x * s.y;        // z = x / deviation + c: its rounding is one more of the mean's
         T *y = (T *)a.y + row * a.n;
 #pragma unroll
@@ -278,14 +278,21 @@ __global__ __launch_bounds__(kL > 256 ? kL : 256, 2) void norm_grad_kernel(const
     constexpr int kThreads = kL > 256 ? kL : 256, kRows = kThreads / kL, kE = kEach<T>, kIn = kL < 64 ? kL : 64;
     __shared__ float2 waves[2][kThreads / 64];
     __shared__ float sums[kL <= 64 ? 2 : 1][kL <= 64 ? kL * kP * kE : 1];
-    __shared__ Held<T, kL, kP> w;
+    // the widest rows: the weight comes from the caches for each row, and the sums of dy lie in LDS, each thread's its own
+    constexpr bool kWide = kL > 512;
+    __shared__ Held<T, kWide ? 1 : kL, kWide ? 1 : kP> w;
+    __shared__ Held<T, kWide ? kL : 1, kWide ? kP : 1> b;
     const int n = a.n;
-    const Pieces<T, kL, kTiny> at = {n, (int)threadIdx.x % kL};
-    float aw[kP][kE], ab[kP][kE];
+    Pieces<T, kL, kTiny> at = {n, (int)threadIdx.x % kL};
+    float aw[kP][kE], ab[kWide ? 1 : kP][kE];
 #pragma unroll
     for (int i = 0; i < kP; i++)
 #pragma unroll
-        for (int j = 0; j < kE; j++) aw[i][j] = ab[i][j] = 0.0f;
+        for (int j = 0; j < kE; j++) {
+            aw[i][j] = 0.0f;
+            if constexpr (kWide) b.v[i][j / 4][threadIdx.x][j % 4] = 0.0f;
+            else ab[i][j] = 0.0f;
+        }
     const int64_t hop = (int64_t)gridDim.x * kRows;
     int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kL;
     u32x4 x[kP], dy[kP], next_x[kP], next_dy[kP];
@@ -299,16 +306,18 @@ __global__ __launch_bounds__(kL > 256 ? kL : 256, 2) void norm_grad_kernel(const
         next_s = ((const float2 *)a.stats)[r];
     };
     load(row);
-    w.template fill<kThreads, kTiny>(a.weight, a.wide, n, 1.0f);
+    if constexpr (!kWide) w.template fill<kThreads, kTiny>(a.weight, a.wide, n, 1.0f);
     __syncthreads();
     for (int turn = 0; row < a.rows; row += hop, turn ^= 1) {
+        if constexpr (kWide) load(row);
 #pragma unroll
         for (int i = 0; i < kP; i++) {
             x[i] = next_x[i];
             dy[i] = next_dy[i];
         }
         s = next_s;
-        load(row + hop);
+        if constexpr (kWide) at.anew();
+        else load(row + hop);
         const float c = -s.x * s.y;
         float q1 = 0.0f, q2 = 0.0f;
 #pragma unroll
@@ -316,7 +325,8 @@ __global__ __launch_bounds__(kL > 256 ? kL : 256, 2) void norm_grad_kernel(const
             float f[kE], d[kE], wf[kE];
             unpack(x[i], f, T());
             unpack(dy[i], d, T());
-            w.get(wf, i, at.lane);
+            if constexpr (kWide) whole_weight<T>(wf, a.weight, a.wide, at.column(i), 1.0f);
+            else w.get(wf, i, at.lane);
             if (!at.whole(i)) {
 #pragma unroll
                 for (int j = 0; j < kE; j++) d[j] = at.own(i, j) ? d[j] : 0.0f;
@@ -325,7 +335,8 @@ __global__ __launch_bounds__(kL > 256 ? kL : 256, 2) void norm_grad_kernel(const
             for (int j = 0; j < kE; j++) {
                 const float z = __builtin_fmaf(f[j], s.y, c), q = wf[j] * d[j];
                 aw[i][j] = __builtin_fmaf(d[j], z, aw[i][j]);
-                ab[i][j] += d[j];
+                if constexpr (kWide) b.v[i][j / 4][threadIdx.x][j % 4] += d[j];
+                else ab[i][j] += d[j];
                 q1 += q;
                 q2 = __builtin_fmaf(q, z, q2);
             }
@@ -348,13 +359,15 @@ __global__ __launch_bounds__(kL > 256 ? kL : 256, 2) void norm_grad_kernel(const
         q2 *= -s.y / (float)n;
         let_go(x);
         let_go(dy);
+        if constexpr (kWide) at.anew();
         T *dx = (T *)a.dx + row * n;
 #pragma unroll
         for (int i = 0; i < kP; i++) {
             float f[kE], d[kE], wf[kE];
             unpack(x[i], f, T());
             unpack(dy[i], d, T());
-            w.get(wf, i, at.lane);
+            if constexpr (kWide) whole_weight<T>(wf, a.weight, a.wide, at.column(i), 1.0f);
+            else w.get(wf, i, at.lane);
 #pragma unroll
             for (int j = 0; j < kE; j++) {
                 const float z = __builtin_fmaf(f[j], s.y, c);
@@ -373,7 +386,8 @@ __global__ __launch_bounds__(kL > 256 ? kL : 256, 2) void norm_grad_kernel(const
             for (int j = 0; j < kE; j++) {
                 if (!at.some(i) || !at.own(i, j)) continue;
                 out[at.column(i) + j] = aw[i][j];
-                out[n + at.column(i) + j] = ab[i][j];
+                if constexpr (kWide) out[n + at.column(i) + j] = b.v[i][j / 4][threadIdx.x][j % 4];
+                else out[n + at.column(i) + j] = ab[i][j];
             }
     } else {
         // the wave's groups of lanes, then the waves one after the other
@@ -533,6 +547,10 @@ template <class T, class F> bool with_form(int n, F f) {
     return is(one, one, std::true_type()) || is(one, one, no) || is(four, one, no) || is(four, two, no) || is(l16, one, no) || is(l16, two, no) || is(l16, four, no) ||
            is(l64, two, no) || is(l64, three, no) || is(l64, four, no) || is(l256, two, no) || is(l256, three, no) || is(l256, four, no);
 }
+// values of the widest rows that a backward pass's workgroup holds with their columns' sums: f32 in 1024 lanes, 16-bit types in 512
+// (1024 by 3 pieces of those spilled: 20000 bf16 303 us, in two readings 280)
+constexpr int kWidest = 16384;
+bool wide_rows(int n) { return n > kWidest; }
 constexpr int kFewGroups = 512;     // workgroups of a backward pass: two on each CU
 int64_t groups_of(int64_t rows, int lanes) {
     const int each = lanes >= 256 ? 1 : 256 / lanes;
@@ -540,8 +558,8 @@ int64_t groups_of(int64_t rows, int lanes) {
 }
 template <class T> int64_t grad_groups(int64_t rows, int n) {
     int64_t g = 0;
-    if (!with_form<T>(n, [&](auto l, auto, auto) { g = groups_of(rows, decltype(l)::value); }) && n <= 512 * 4 * kEach<T>)
-        g = groups_of(rows, 512);
+    if (!with_form<T>(n, [&](auto l, auto, auto) { g = groups_of(rows, decltype(l)::value); }) && !wide_rows(n))
+        g = std::min<int64_t>(rows, n <= 512 * 4 * kEach<T> ? kFewGroups : kFewGroups / 2);
     // the columns' kernel: a thousand workgroups or so
     if (!g) g = std::min<int64_t>(rows, std::max(1, 1024 / ((n + 256 * kEach<T> - 1) / (256 * kEach<T>))));
     return g;
@@ -566,7 +584,8 @@ template <class T> hipError_t go(NormArgs a, hipStream_t st) {
                    256 * std::min(8, 160 * 1024 / kLds));
         })) {
         constexpr int kE = kEach<T>;
-        if (a.n <= 1024 * 2 * kE) launch(norm_kernel<T, 1024, 2, false>, 1024, a.rows, 256);
+        if (a.n <= 512 * 3 * kE) launch(norm_kernel<T, 512, 3, false>, 512, a.rows, 512);
+        else if (a.n <= 512 * 4 * kE) launch(norm_kernel<T, 512, 4, false>, 512, a.rows, 512);
         else if (a.n <= 1024 * 4 * kE) launch(norm_kernel<T, 1024, 4, false>, 1024, a.rows, 256);
         else if (a.n <= 1024 * 8 * kE) launch(norm_kernel<T, 1024, 8, false>, 1024, a.rows, 256);
         else if (a.n <= 1024 * 16 * kE) launch(norm_kernel<T, 1024, 16, false>, 1024, a.rows, 256);
@@ -586,6 +605,9 @@ template <class T> hipError_t go_grad(NormGradArgs a, void *scratch, hipStream_t
         constexpr int kE = kEach<T>;
         if (a.n <= 512 * 4 * kE) {
             hipLaunchKernelGGL((norm_grad_kernel<T, 512, 4, false>), dim3((unsigned)groups), dim3(512), 0, st, a, part);
+        } else if (sizeof(T) == 4 && !wide_rows(a.n)) {
+            if constexpr (sizeof(T) == 4)
+                hipLaunchKernelGGL((norm_grad_kernel<T, 1024, 4, false>), dim3((unsigned)groups), dim3(1024), 0, st, a, part);
         } else {
             const int slabs = (a.n + 256 * kE - 1) / (256 * kE);
             float2 *given = a.dx ? (float2 *)((char *)scratch + groups * 2 * a.n * 4) : nullptr;
@@ -607,12 +629,11 @@ template <class T> hipError_t go_grad(NormGradArgs a, void *scratch, hipStream_t
 
 }  // namespace
 
-template <class T> bool wide_rows(int n) { return n > 512 * 4 * kEach<T>; }
 template <class T> int64_t scratch_of(int64_t rows, int n) {
-    return grad_groups<T>(rows, n) * 2 * n * 4 + (wide_rows<T>(n) ? rows * waves_of<T>(n) * 8 : 0);
+    return grad_groups<T>(rows, n) * 2 * n * 4 + (wide_rows(n) ? rows * waves_of<T>(n) * 8 : 0);
 }
 int64_t norm_grad_scratch(int type, int64_t rows, int n) { return type == kOpF32 ? scratch_of<float>(rows, n) : scratch_of<bf16_t>(rows, n); }
-bool norm_grad_wide(int type, int n) { return type == kOpF32 ? wide_rows<float>(n) : wide_rows<bf16_t>(n); }
+bool norm_grad_wide(int n) { return wide_rows(n); }
 hipError_t launch_norm(int type, const NormArgs &a, hipStream_t st) {
     if (type == kOpF32) return go<float>(a, st);
     if (type == kOpBf16) return go<bf16_t>(a, st);

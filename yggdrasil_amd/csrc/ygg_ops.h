@@ -82,7 +82,7 @@ struct NormGradArgs {
     bool past = false;
 };
 int64_t norm_grad_scratch(int type, int64_t rows, int n);
-bool norm_grad_wide(int type, int n);      // rows whose own gradient wants scratch too
+bool norm_grad_wide(int n);      // rows whose own gradient wants scratch too
 hipError_t launch_norm(int type, const NormArgs &a, hipStream_t stream);
 hipError_t launch_norm_grad(int type, const NormGradArgs &a, void *scratch, hipStream_t stream);
 

@@ -273,7 +273,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
             if (want[0]) out[0] = empty(x, {rows, n}, x.scalar_type());
             for (int k : {1, 2})
                 if (want[k]) out[k] = empty(x, {n}, kind);
-            const int64_t need = want[1] || want[2] || n > 8192 ? api.layer_norm_scratch(type_of(x), rows, n) : 0;
+            const int64_t need = want[1] || want[2] || n > 16384 ? api.layer_norm_scratch(type_of(x), rows, n) : 0;
             const Tensor scratch = scratch_of(x, need);
             check(api.layer_norm_grad(x.data_ptr(), type_of(x), rows, n, rows > 1 ? x.stride(0) : n, ptr(w), type, ptr<float>(stats),
                                       dy.data_ptr(), ptr(out[0]), ptr(out[1]), ptr(out[2]), ptr(scratch), need, stream_of(x)));
