@@ -326,7 +326,7 @@ int ygg_layer_norm_grad(const void *d_x, int type, int64_t rows, int n, int64_t 
    (what d_state holds where there are no steps), memory of its own. d_kept: NULL, or f32 memory of ygg_gated_scan_kept
    bytes (0: none) for every 64th state, which the gates' gradient wants. States are held in f32; runs of steps are joined by the products
    of their gates, so gates are meant to be at most 1 in magnitude: others have to keep the products of any run of steps
-   finite. */
+   finite, and a state that becomes infinite may come out as NaN later on. */
 int64_t ygg_gated_scan_scratch(int type, int gate_type, int64_t B, int64_t T, int n);
 int64_t ygg_gated_scan_kept(int64_t B, int64_t T, int n);
 int ygg_gated_scan(const void *d_gate, int gate_type, int64_t gate_b, int64_t gate_t, const void *d_x, int type, int64_t x_b,

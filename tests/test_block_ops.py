@@ -65,7 +65,8 @@ SCAN = dict(gate=P, gate_type=0, gate_b=8, gate_t=8, x=P, type=1, x_b=8, x_t=8, 
     (dict(type=3), b"type"), (dict(gate_type=2), b"gate_type"), (dict(B=-1), b"B "), (dict(B=(1 << 24) + 1), b"B "), (dict(T=-1), b"T "),
     (dict(T=(1 << 30) + 1), b"T "), (dict(n=0), b"n "), (dict(gate_t=-8), b"strides"), (dict(x_b=-1), b"strides"), (dict(gate=None), b"NULL"),
     (dict(x=None), b"NULL"), (dict(h=None), b"NULL"), (dict(last=None), b"NULL"), (dict(T=1 << 20, scratch=None), b"scratch"),
-    (dict(T=1 << 20, bytes=8), b"scratch"), (dict(B=1 << 24, T=64, n=1 << 17), b"launch takes")])
+    (dict(T=1 << 20, bytes=8), b"scratch"), (dict(B=1 << 24, T=64, n=1 << 17), b"launch takes"),
+    (dict(B=1 << 24, T=1 << 30, n=1 << 17), b"2^50")])
 def test_gated_scan_refuses(kw, word):
     refused("ygg_gated_scan", SCAN, kw, word)
 

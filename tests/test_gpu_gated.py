@@ -133,6 +133,9 @@ def test_leading_axes_and_no_rows():
     assert y.shape == (0, 5, 40)
     dx, dw = torch.autograd.grad(y.sum(), (e, w))
     assert dx.shape == e.shape and not dw.any()
+    # sizes whose operands would be laid out anew, had they rows
+    e, w = (torch.zeros(s, dtype=torch.bfloat16, device="cuda", requires_grad=True) for s in ((0, 777), (2, 4096, 777)))
+    assert not torch.autograd.grad(ops.gated_linear(e, w).sum(), w)[0].any()
 
 
 @pytest.mark.parametrize("act", ACTS)

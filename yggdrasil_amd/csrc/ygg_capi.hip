@@ -1361,12 +1361,14 @@ int ygg_layer_norm_grad(const void *d_x, int type, int64_t rows, int n, int64_t 
 }
 
 // sizes of a recurrence: an error code, or 0
+constexpr double kMostCells = 1125899906842624.0;    // whose bytes, and those of what is kept of them, 64 bits count
 static int check_scan(int type, int gate_type, int64_t B, int64_t T, int n) {
     if (type < 0 || type > 2) return fail(YGG_ERR_ARG, kTypeHelp, type);
     if (gate_type != 0 && gate_type != type) return fail(YGG_ERR_ARG, "gate_type %d: 0 or x's (%d)", gate_type, type);
     if (B < 0 || B > YGG_MOST_ROWS) return fail(YGG_ERR_ARG, kOpLimits, "B", (long long)B, 0, YGG_MOST_ROWS);
     if (T < 0 || T > YGG_MOST_STEPS) return fail(YGG_ERR_ARG, kOpLimits, "T", (long long)T, 0, YGG_MOST_STEPS);
     if (n < 1 || n > YGG_MOST_INNER) return fail(YGG_ERR_ARG, kOpLimits, "n", (long long)n, 1, YGG_MOST_INNER);
+    if ((double)B * (double)T * n > kMostCells) return fail(YGG_ERR_ARG, "%lld sequences of %lld steps of %d: past 2^50 values", (long long)B, (long long)T, n);
     return YGG_OK;
 }
 
@@ -1376,7 +1378,7 @@ int64_t ygg_gated_scan_scratch(int type, int gate_type, int64_t B, int64_t T, in
 }
 
 int64_t ygg_gated_scan_kept(int64_t B, int64_t T, int n) {
-    if (B < 1 || B > YGG_MOST_ROWS || T < 1 || T > YGG_MOST_STEPS || n < 1 || n > YGG_MOST_INNER) return 0;
+    if (B < 1 || B > YGG_MOST_ROWS || T < 1 || T > YGG_MOST_STEPS || n < 1 || n > YGG_MOST_INNER || (double)B * (double)T * n > kMostCells) return 0;
     return ygg::scan_kept(B, T, n);
 }
 

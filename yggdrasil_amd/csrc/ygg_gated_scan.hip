@@ -551,10 +551,9 @@ template <class TG, class F> auto with_width(int n, F f) {
     constexpr std::integral_constant<int, 1> one{};
     return n >= decltype(wide)::value ? f(wide) : f(one);
 }
-// steps of a thread
-template <class TX, class TG> constexpr int steps_of(bool back) { return back ? 4 : 8; }
-template <class TX, class TG> Cut cut_for(int64_t B, int64_t T, int n, bool back) {
-    return with_width<TG>(n, [&](auto v) { return cut_of(B, T, n, kCols * decltype(v)::value, kParts * steps_of<TX, TG>(back)); });
+constexpr int steps_of(bool back) { return back ? 4 : 8; }     // of a thread
+template <class TG> Cut cut_for(int64_t B, int64_t T, int n, bool back) {
+    return with_width<TG>(n, [&](auto v) { return cut_of(B, T, n, kCols * decltype(v)::value, kParts * steps_of(back)); });
 }
 
 bool writes_past(int64_t B, int64_t T, int n, int size) { return B * T * n * size >= kPastBytes; }
@@ -562,14 +561,14 @@ bool writes_past(int64_t B, int64_t T, int n, int size) { return B * T * n * siz
 template <class TX, class TG> hipError_t go(ScanArgs a, void *scratch, hipStream_t st) {
     a.past = writes_past(a.B, a.T, a.n, sizeof(TX));
     return with_width<TG>(a.n, [&](auto v) {
-        constexpr int kV = decltype(v)::value, kSteps = steps_of<TX, TG>(false);
+        constexpr int kV = decltype(v)::value, kSteps = steps_of(false);
         if (a.T <= 8) {
             const int64_t threads = a.B * ((a.n + kV - 1) / kV);
             if ((threads + 255) / 256 > most_blocks(256)) return kTooLarge;
             hipLaunchKernelGGL((step_kernel<TX, TG, kV>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a);
             return hipGetLastError();
         }
-        const Cut cut = cut_for<TX, TG>(a.B, a.T, a.n, false);
+        const Cut cut = cut_for<TG>(a.B, a.T, a.n, false);
         const int64_t blocks = a.B * cut.slabs * cut.segments;
         if (blocks > most_blocks(256)) return kTooLarge;
         if (cut.segments > 1) {
@@ -585,8 +584,8 @@ template <class TX, class TG> hipError_t go(ScanArgs a, void *scratch, hipStream
 template <class TX, class TG> hipError_t go_grad(ScanGradArgs a, void *scratch, hipStream_t st) {
     a.past = writes_past(a.B, a.T, a.n, sizeof(TX));
     return with_width<TG>(a.n, [&](auto v) {
-        constexpr int kV = decltype(v)::value, kSteps = steps_of<TX, TG>(true);
-        const Cut cut = cut_for<TX, TG>(a.B, a.T, a.n, true);
+        constexpr int kV = decltype(v)::value, kSteps = steps_of(true);
+        const Cut cut = cut_for<TG>(a.B, a.T, a.n, true);
         const int64_t blocks = a.B * cut.slabs * cut.segments;
         if (blocks > most_blocks(256)) return kTooLarge;
         if (cut.segments > 1) {
@@ -614,10 +613,8 @@ template <class F> auto with_types(int type, int gate_type, F f) {
 
 int64_t scan_kept(int64_t B, int64_t T, int n) { return B * kept_of(T) * n * 4; }
 int64_t scan_scratch(int type, int gate_type, int64_t B, int64_t T, int n) {
-    const int64_t most = with_types(type, gate_type, [&](auto x, auto g) {
-        typedef decltype(x) TX;
-        typedef decltype(g) TG;
-        return std::max(cut_for<TX, TG>(B, T, n, false).segments, cut_for<TX, TG>(B, T, n, true).segments);
+    const int64_t most = with_types(type, gate_type, [&](auto, auto g) {
+        return std::max(cut_for<decltype(g)>(B, T, n, false).segments, cut_for<decltype(g)>(B, T, n, true).segments);
     });
     return most > 1 ? B * most * 2 * n * 4 : 0;
 }

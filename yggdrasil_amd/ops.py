@@ -255,7 +255,8 @@ def gated_scan(gate, x, state=None):
     serving, one step at a time with the state carried on; for training, differentiable in all three, over long sequences.
 
     States are held in f32. Runs of steps are joined by the products of their gates: gates are meant to be at most 1 in
-    magnitude, and others have to keep the product of every run of steps finite. A gate of 0 begins anew (a document's first
+    magnitude, and others have to keep the product of every run of steps finite; a state that becomes infinite may come out as NaN
+    later on. A gate of 0 begins anew (a document's first
     step); a step with gate 1 and x 0 keeps the state (padding behind a sequence's end leaves the last state right). For the gate's
     gradient every 64th state is kept, in f32, and the others are computed again from x."""
     if _tensors(x, gate) if state is None else _tensors(x, gate, state):
