@@ -50,74 +50,51 @@ constexpr int kBand = 16;     // rows of tiles of a band
 // the row of w of a tile's column o, the tile's outputs beginning at n0
 __device__ __forceinline__ int row_of_w(int o, int n0, int N) { return (o & 32 ? N : 0) + min(n0 + (o >> 6) * 32 + (o & 31), N - 1); }
 
-// g and u of M rows of 2 N values, kept for the backward pass: f32, or its upper 24 bits, first all values' 16 and then their 8
+// What is kept of rows of N values lies `half` values apart, N up to a multiple of 8, so that it is read and written aligned and in whole
+// runs of a lane's 8 results
+__host__ __device__ constexpr int half_of(int N) { return (N + 7) / 8 * 8; }
+
+// g and u of M rows, kept for the backward pass, in rows of 2 half values: f32, or its upper 24 bits, first all values' 16 and then their 8
 // (in 16 bits alone the gradients were 1.8 times as far off as a rounding, in 24 1.4; the 16384 x 4096 of a bf16 case take the memory
 // 134 MB longer on the way out and in)
 template <class T> struct Kept {
     static constexpr int kBytes = sizeof(T) == 4 ? 4 : 3;
     char *p;
     int64_t count;
-    // kN values from place `at` on, of which the first `left` exist
-    template <int kN> __device__ __forceinline__ void put(int64_t at, const float *v, int left) const {
+    // kN values from place `at` on, which may go on behind the row's N
+    template <int kN> __device__ __forceinline__ void put(int64_t at, const float *v) const {
         if constexpr (sizeof(T) == 4) {
-            store_run<float, kN>((float *)p + at, v, left);
+            store_run<float, kN>((float *)p + at, v, kN);
         } else {
             uint32_t b[kN];
 #pragma unroll
             for (int j = 0; j < kN; j++)      // to nearest; a NaN must not carry into the sign
                 b[j] = v[j] == v[j] ? __builtin_bit_cast(uint32_t, v[j]) + 0x80u : 0x7fc00000u;
-            typedef uint32_t hi_t __attribute__((ext_vector_type(kN / 2), aligned(1)));
-            typedef uint32_t lo_t __attribute__((ext_vector_type(kN / 4), aligned(1)));
-            uint16_t *hi = (uint16_t *)p + at;
-            uint8_t *lo = (uint8_t *)p + 2 * count + at;
-            if (left >= kN) {
-                hi_t h;
-                lo_t l;
+            typedef uint32_t hi_t __attribute__((ext_vector_type(kN / 2)));
+            typedef uint32_t lo_t __attribute__((ext_vector_type(kN / 4)));
+            hi_t h;
+            lo_t l;
 #pragma unroll
-                for (int j = 0; j < kN / 2; j++) h[j] = b[2 * j] >> 16 | (b[2 * j + 1] & 0xffff0000u);
+            for (int j = 0; j < kN / 2; j++) h[j] = b[2 * j] >> 16 | (b[2 * j + 1] & 0xffff0000u);
 #pragma unroll
-                for (int j = 0; j < kN / 4; j++)
-                    l[j] = (b[4 * j] >> 8 & 0xffu) | (b[4 * j + 1] & 0xff00u) | (b[4 * j + 2] & 0xff00u) << 8 | (b[4 * j + 3] & 0xff00u) << 16;
-                *(hi_t *)hi = h;
-                *(lo_t *)lo = l;
-            } else {
-#pragma unroll
-                for (int j = 0; j < kN; j++)
-                    if (j < left) {
-                        hi[j] = (uint16_t)(b[j] >> 16);
-                        lo[j] = (uint8_t)(b[j] >> 8);
-                    }
-            }
+            for (int j = 0; j < kN / 4; j++)
+                l[j] = (b[4 * j] >> 8 & 0xffu) | (b[4 * j + 1] & 0xff00u) | (b[4 * j + 2] & 0xff00u) << 8 | (b[4 * j + 3] & 0xff00u) << 16;
+            *(hi_t *)(p + 2 * at) = h;
+            *(lo_t *)(p + 2 * count + at) = l;
         }
     }
-    // what is kept of 16 bytes of values, as it lies there; past: past the caches, which would not hold it until it is read again
+    // what is kept of 16 bytes of values, as it lies there; kPast: past the caches, which would not hold it until it is read again
     struct Piece {
         u32x4 hi;
         u32x2 lo;
     };
     template <bool kPast> __device__ __forceinline__ Piece load(int64_t at) const {
-        typedef uint32_t hi_t __attribute__((ext_vector_type(4), aligned(1)));
-        typedef uint32_t lo_t __attribute__((ext_vector_type(2), aligned(1)));
         Piece v = {};
-        const hi_t *hi = (const hi_t *)(p + at * (sizeof(T) == 4 ? 4 : 2));
+        const u32x4 *hi = (const u32x4 *)(p + at * (sizeof(T) == 4 ? 4 : 2));
         v.hi = kPast ? __builtin_nontemporal_load(hi) : *hi;
         if constexpr (sizeof(T) == 2) {
-            const lo_t *lo = (const lo_t *)(p + 2 * count + at);
+            const u32x2 *lo = (const u32x2 *)(p + 2 * count + at);
             v.lo = kPast ? __builtin_nontemporal_load(lo) : *lo;
-        }
-        return v;
-    }
-    // the first `left` of a piece
-    __device__ __forceinline__ Piece load(int64_t at, int left) const {
-        Piece v = {};
-        if constexpr (sizeof(T) == 4) {
-            v.hi = load16((const float *)p + at, left);
-        } else {
-            v.hi = load16((const uint16_t *)p + at, left);
-            const uint8_t *lo = (const uint8_t *)p + 2 * count + at;
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (j < left) v.lo[j / 4] |= (uint32_t)lo[j] << 8 * (j % 4);
         }
         return v;
     }
@@ -136,9 +113,10 @@ __device__ __forceinline__ void put_outputs(const float *g, const float *u, int 
     for (int j = 0; j < kN; j++) v[j] = act_of<kAct>(g[j]) * u[j];
     store_run<T, kN>(y + (int64_t)row * N + n, v, N - n);
     if (gu.p) {
-        const int64_t at = (int64_t)row * 2 * N + n;
-        gu.template put<kN>(at, g, N - n);
-        gu.template put<kN>(at + N, u, N - n);
+        const int half = half_of(N);
+        const int64_t at = (int64_t)row * 2 * half + n;
+        gu.template put<kN>(at, g);
+        gu.template put<kN>(at + half, u);
     }
 }
 template <class T, int kAct, int FI, class Acc>
@@ -273,28 +251,17 @@ __global__ __launch_bounds__(256) void gated_few_kernel(const T *x, const T *w, 
     }
 }
 
-// dg and du lie `half` values apart in rows of 2 half, N up to whole 16 bytes, so that the products' loads are aligned; zeros between.
-__host__ __device__ constexpr int half_of(int size, int N) { return (N + 16 / size - 1) / (16 / size) * (16 / size); }
-// dg and du of pieces of 16 bytes of dy
+// dg and du lie as g and u do, so that the products' loads are aligned, zeros behind N. A thread: 16 bytes of each
 template <class T, int kAct, bool kPast>
 __global__ __launch_bounds__(256) void gated_slope_kernel(Kept<T> gu, const T *dy, int M, int N, T *dgu) {
     constexpr int kE = 16 / sizeof(T);
-    const int half = half_of(sizeof(T), N), per = half / kE;
+    const int half = half_of(N), per = half / kE;
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / per;
     if (row >= M) return;
     const int n = (int)(id % per) * kE, left = N - n;
-    const int64_t at = row * 2 * N + n;
-    typename Kept<T>::Piece gp, up;
-    u32x4 dp;
-    if (left >= kE) {
-        gp = gu.template load<kPast>(at);
-        up = gu.template load<kPast>(at + N);
-        dp = load16(dy + row * N + n);
-    } else {
-        gp = gu.load(at, left);
-        up = gu.load(at + N, left);
-        dp = load16(dy + row * N + n, left);
-    }
+    const int64_t at = row * 2 * half + n;
+    const typename Kept<T>::Piece gp = gu.template load<kPast>(at), up = gu.template load<kPast>(at + half);
+    const u32x4 dp = left >= kE ? load16(dy + row * N + n) : load16(dy + row * N + n, left);
     float g[kE], u[kE], d[kE];
     Kept<T>::values(gp, g);
     Kept<T>::values(up, u);
@@ -303,8 +270,8 @@ __global__ __launch_bounds__(256) void gated_slope_kernel(Kept<T> gu, const T *d
     for (int j = 0; j < kE; j++) {
         float slope;
         const float a = act_of<kAct>(g[j], &slope);
-        g[j] = d[j] * u[j] * slope;
-        u[j] = d[j] * a;
+        g[j] = j < left ? d[j] * u[j] * slope : 0.0f;      // what lies behind N may be anything
+        u[j] = j < left ? d[j] * a : 0.0f;
     }
     T *out = dgu + row * 2 * half + n;
     store_run<T, kE>(out, g, kE, kPast);
@@ -427,7 +394,7 @@ template <class T> __global__ __launch_bounds__(256) void parts_kernel(const flo
 bool aligned16(const void *p, int64_t row_bytes) { return (uintptr_t)p % 16 == 0 && row_bytes % 16 == 0; }
 constexpr int64_t kMostBytes = 0x78000000;   // of an operand with 32-bit offsets: kFar and a few steps stay past it
 template <class T, int kAct> hipError_t go(const void *x, const void *w, int M, int N, int K, void *y, void *kept, hipStream_t st) {
-    const Kept<T> gu = {(char *)kept, (int64_t)M * 2 * N};
+    const Kept<T> gu = {(char *)kept, (int64_t)M * 2 * half_of(N)};
     const int64_t row = (int64_t)K * sizeof(T);
     if constexpr (sizeof(T) == 2) {
         const int cols = (N + 127) / 128;
@@ -468,14 +435,16 @@ template <class T, int kAct> hipError_t go(const void *x, const void *w, int M, 
         return hipGetLastError();
     };
     const int64_t tiles128 = ((int64_t)M + 127) / 128 * ((N + 63) / 64);
-    return tiles128 >= 512 ? tiles(four, two, two) : tiles(two, two, two);
+    // 128 rows a tile where there are more than one for each CU: 3000 x 2222 x 1111 (rows, K, N) bf16, 432 of them, 48 us, 65 with 64 rows;
+    // 1001 x 1000 x 2003, 256 of them, 19.8 and 19.1
+    return tiles128 >= 384 ? tiles(four, two, two) : tiles(two, two, two);
 }
 template <class T, int kAct> hipError_t go_slope(const void *gu, const void *dy, int M, int N, void *dgu, hipStream_t st) {
     constexpr int kE = 16 / sizeof(T);
-    const int64_t blocks = ((int64_t)M * (half_of(sizeof(T), N) / kE) + 255) / 256;
+    const int64_t blocks = ((int64_t)M * (half_of(N) / kE) + 255) / 256;
     if (blocks == 0) return hipSuccess;
     if (blocks > most_blocks(256)) return kTooLarge;
-    const Kept<T> kept = {(char *)gu, (int64_t)M * 2 * N};
+    const Kept<T> kept = {(char *)gu, (int64_t)M * 2 * half_of(N)};
     // 16384 x 4096 bf16: 184 us with the caches, 145 past them
     if (kept.count * Kept<T>::kBytes >= kPastBytes)
         hipLaunchKernelGGL((gated_slope_kernel<T, kAct, true>), dim3((unsigned)blocks), dim3(256), 0, st, kept, (const T *)dy, M, N, (T *)dgu);
@@ -493,7 +462,7 @@ struct Plan {
 };
 // rows: out (M, K) over 2 half r's; else out (2 N, K) over M
 Plan plan_of(int size, bool rows, int M, int N, int K, bool aligned) {
-    const int half = half_of(size, N), step = 128 / size, I = rows ? M : 2 * half, R = rows ? 2 * half : M, steps = (R + step - 1) / step;
+    const int half = half_of(N), step = 128 / size, I = rows ? M : 2 * half, R = rows ? 2 * half : M, steps = (R + step - 1) / step;
     Plan p = {};
     auto cut = [&](int ti, int to, int64_t want, int least) {
         p.cols = (K + to - 1) / to;
@@ -502,7 +471,7 @@ Plan plan_of(int size, bool rows, int M, int N, int K, bool aligned) {
         p.per = (int)std::max<int64_t>((steps + parts - 1) / parts, 1);
         p.parts = std::max((steps + p.per - 1) / p.per, 1);      // without rows there is still the weights' gradient, zero
     };
-    p.pitch = half_of(size, K);
+    p.pitch = half_of(K);
     const int64_t a_bytes = (int64_t)M * 2 * half * size, b_bytes = (int64_t)(rows ? 2 * N : M) * p.pitch * size;
     p.spaced = p.pitch != K;
     if (size == 2 && (aligned || p.spaced) && a_bytes < kMostBytes && b_bytes < kMostBytes && I >= 192 && K >= 192) {
@@ -538,7 +507,7 @@ template <class T, bool kRows> hipError_t go_dense(const void *a, const void *b,
         if (e != hipSuccess) return e;
         b = scratch;
     }
-    const Dense g = {a, b, (int)I, K, M, p.pitch, N, half_of(sizeof(T), N), out, p.parts > 1 ? sums : nullptr, (int)p.tiles, p.cols, p.per};
+    const Dense g = {a, b, (int)I, K, M, p.pitch, N, half_of(N), out, p.parts > 1 ? sums : nullptr, (int)p.tiles, p.cols, p.per};
     if (p.turn) {
         if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((dense_turn_kernel<T, kRows>), dim3((unsigned)blocks), dim3(512), 0, st, g);
     } else if (p.large) {
@@ -564,9 +533,9 @@ hipError_t launch_gated(int type, int act, const void *x, const void *w, int M, 
         return with_act(act, [&](auto k) { return go<decltype(one), decltype(k)::value>(x, w, M, N, K, y, gu, st); });
     });
 }
-int64_t gated_kept(int type, int M, int N) { return (int64_t)M * 2 * N * (type == kOpF32 ? 4 : 3); }
+int64_t gated_kept(int type, int M, int N) { return (int64_t)M * 2 * half_of(N) * (type == kOpF32 ? 4 : 3); }
 // dg and du, then what one product at a time takes; whether its operand turns out to be aligned or not
-int64_t dgu_bytes(int type, int M, int N) { return ((int64_t)M * 2 * half_of(op_bytes(type), N) * op_bytes(type) + 255) / 256 * 256; }
+int64_t dgu_bytes(int type, int M, int N) { return ((int64_t)M * 2 * half_of(N) * op_bytes(type) + 255) / 256 * 256; }
 int64_t gated_grad_scratch(int type, int M, int N, int K) {
     const int size = op_bytes(type);
     int64_t most = 0;
