@@ -20,7 +20,7 @@
 // States, maps and their joins are in f32; h, dx and da are rounded to their types once, on the way out.
 //
 // The memory bounds it. 16 x 4096 x 2048 bf16: forward 155 us (2 readings and a writing of 268 MB, 5.2 TB/s), backward 273 us (3 and
-// 2, 4.9 TB/s); 131072 x 256 bf16 with gates in f32: 33 us for the segments' maps, 49 for the states. Workgroups of 512 threads
+// 2, 4.9 TB/s); 131072 x 256 bf16 with gates in f32: 30 us for the segments' maps, 44 for the states. Workgroups of 512 threads
 // (295 us backward) and of half as many channels (300) were slower.
 #include <algorithm>
 
@@ -179,19 +179,33 @@ template <bool kBack, int kV> __device__ __forceinline__ void join_waves(const M
         }
     }
 }
-// the state at the begin of a segment: what `begin` is after the segments before it, whose maps lie `hop` values apart
-template <int kV> __device__ __forceinline__ void join_segments(const float *maps, int64_t hop, int n, int count, float *carry) {
-#pragma unroll 8
-    for (int s = 0; s < count; s++) {
-        float A[kV], H[kV];
+// carry: what the first segment begins with, then what the one after the `count` of these maps does. The maps lie `hop` values apart; each
+// part takes its share of them, side by side, and the parts are joined as those of a chunk (one after the other those of 131072 x 256 took 5 us longer)
+template <int kV> __device__ __forceinline__ void join_segments(const float *maps, int64_t hop, int n, int count, Maps<kV> &lds_a, Maps<kV> &lds_h, float *carry) {
+    if (count == 0) return;
+    const int per = (count + kParts - 1) / kParts, first = threadIdx.x / kCols * per, end = min(first + per, count);
+    float A[kV], H[kV], in[kV];
+#pragma unroll
+    for (int j = 0; j < kV; j++) A[j] = 1.0f, H[j] = 0.0f;
+#pragma unroll 4
+    for (int s = first; s < end; s++) {
+        Few<float, kV> a, h;
+        a.load(maps + s * hop);
+        h.load(maps + s * hop + n);
 #pragma unroll
         for (int j = 0; j < kV; j++) {
-            A[j] = maps[s * hop + j];
-            H[j] = maps[s * hop + n + j];
+            H[j] = __builtin_fmaf(a[j], H[j], h[j]);
+            A[j] *= a[j];
         }
-#pragma unroll
-        for (int j = 0; j < kV; j++) carry[j] = __builtin_fmaf(A[j], carry[j], H[j]);
     }
+#pragma unroll
+    for (int j = 0; j < kV; j++) {
+        const Scan<false> w(A[j], H[j], 0.0f);
+        lds_a.put(j, w.all_A);
+        lds_h.put(j, w.all_H);
+    }
+    __syncthreads();
+    join_waves<false>(lds_a, lds_h, carry, in);
 }
 
 // How a call is cut: `slabs` of a sequence, `segments` of `per` steps each
@@ -301,7 +315,7 @@ __global__ __launch_bounds__(kCols *kParts, 2) void scan_kernel(const ScanArgs a
     float carry[kV];
 #pragma unroll
     for (int j = 0; j < kV; j++) carry[j] = a.state ? a.state[at.b * n + at.c + j] : 0.0f;
-    join_segments<kV>(maps + at.b * cut.segments * 2 * n + at.c, 2 * n, n, s, carry);
+    join_segments<kV>(maps + at.b * cut.segments * 2 * n + at.c, 2 * n, n, s, lds_a[1], lds_h[1], carry);     // the chunks begin with [0]
     int buf = 0;
     for (int64_t chunk = from; chunk < end; chunk += kChunk, buf ^= 1) {
         const int64_t t0 = chunk + at.part * kSteps;
@@ -432,7 +446,7 @@ __global__ __launch_bounds__(kCols *kParts, 2) void scan_grad_kernel(const ScanG
         }
     };
     if (from < end) load(from);     // there may be no step at all
-    join_segments<kV>(maps + at.b * cut.segments * 2 * n + at.c, 2 * n, n, s, carry);
+    join_segments<kV>(maps + at.b * cut.segments * 2 * n + at.c, 2 * n, n, s, lds_a[1], lds_f[1], carry);
     int buf = 0;
     for (int64_t chunk = from; chunk < end; chunk += kChunk, buf ^= 1) {
         const int64_t t0 = cut.steps - 1 - (chunk + at.part * kSteps);     // the step of k is t0 - k
@@ -530,14 +544,14 @@ __global__ __launch_bounds__(kCols *kParts, 2) void scan_grad_kernel(const ScanG
     }
 }
 
-constexpr int kWant = 512;           // workgroups that fill the chip: two on each CU
-constexpr int kMostSegments = 128;   // maps that a workgroup of the second kernel joins
-Cut cut_of(int64_t B, int64_t T, int n, int wide, int chunk) {
+constexpr int kMostSegments = 256;   // maps that a workgroup of the second kernel joins
+// want: workgroups that fill the chip
+Cut cut_of(int64_t B, int64_t T, int n, int wide, int chunk, int want) {
     Cut c;
     c.slabs = (n + wide - 1) / wide;
     const int64_t columns = B * c.slabs, chunks = std::max<int64_t>((T + chunk - 1) / chunk, 1);
     // a segment is of two chunks or more
-    int64_t segments = columns >= kWant / 2 ? 1 : std::min<int64_t>(std::min<int64_t>((kWant + columns - 1) / columns, kMostSegments), chunks / 2);
+    int64_t segments = columns >= 256 ? 1 : std::min<int64_t>(std::min<int64_t>((want + columns - 1) / columns, kMostSegments), chunks / 2);
     segments = std::max<int64_t>(segments, 1);
     const int64_t per = (chunks + segments - 1) / segments;
     c.per = per * chunk;
@@ -552,8 +566,11 @@ template <class TG, class F> auto with_width(int n, F f) {
     return n >= decltype(wide)::value ? f(wide) : f(one);
 }
 constexpr int steps_of(bool back) { return back ? 4 : 8; }     // of a thread
-template <class TG> Cut cut_for(int64_t B, int64_t T, int n, bool back) {
-    return with_width<TG>(n, [&](auto v) { return cut_of(B, T, n, kCols * decltype(v)::value, kParts * steps_of(back)); });
+// Two workgroups on each CU, by the registers, three of the forward kernel of 16-bit values with gates in f32 (131072 x 256 bf16: 74 us of
+// kernels, 80 with two; the backward kernel of 5 x 1001 x 1003 f32 18 us with two and 20 with three)
+template <class TX, class TG> Cut cut_for(int64_t B, int64_t T, int n, bool back) {
+    const int want = !back && sizeof(TX) == 2 && sizeof(TG) == 4 ? 768 : 512;
+    return with_width<TG>(n, [&](auto v) { return cut_of(B, T, n, kCols * decltype(v)::value, kParts * steps_of(back), want); });
 }
 
 bool writes_past(int64_t B, int64_t T, int n, int size) { return B * T * n * size >= kPastBytes; }
@@ -568,7 +585,7 @@ template <class TX, class TG> hipError_t go(ScanArgs a, void *scratch, hipStream
             hipLaunchKernelGGL((step_kernel<TX, TG, kV>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a);
             return hipGetLastError();
         }
-        const Cut cut = cut_for<TG>(a.B, a.T, a.n, false);
+        const Cut cut = cut_for<TX, TG>(a.B, a.T, a.n, false);
         const int64_t blocks = a.B * cut.slabs * cut.segments;
         if (blocks > most_blocks(256)) return kTooLarge;
         if (cut.segments > 1) {
@@ -585,7 +602,7 @@ template <class TX, class TG> hipError_t go_grad(ScanGradArgs a, void *scratch, 
     a.past = writes_past(a.B, a.T, a.n, sizeof(TX));
     return with_width<TG>(a.n, [&](auto v) {
         constexpr int kV = decltype(v)::value, kSteps = steps_of(true);
-        const Cut cut = cut_for<TG>(a.B, a.T, a.n, true);
+        const Cut cut = cut_for<TX, TG>(a.B, a.T, a.n, true);
         const int64_t blocks = a.B * cut.slabs * cut.segments;
         if (blocks > most_blocks(256)) return kTooLarge;
         if (cut.segments > 1) {
@@ -613,8 +630,9 @@ template <class F> auto with_types(int type, int gate_type, F f) {
 
 int64_t scan_kept(int64_t B, int64_t T, int n) { return B * kept_of(T) * n * 4; }
 int64_t scan_scratch(int type, int gate_type, int64_t B, int64_t T, int n) {
-    const int64_t most = with_types(type, gate_type, [&](auto, auto g) {
-        return std::max(cut_for<decltype(g)>(B, T, n, false).segments, cut_for<decltype(g)>(B, T, n, true).segments);
+    const int64_t most = with_types(type, gate_type, [&](auto x, auto g) {
+        auto segments = [&](bool back) { return cut_for<decltype(x), decltype(g)>(B, T, n, back).segments; };
+        return std::max(segments(false), segments(true));
     });
     return most > 1 ? B * most * 2 * n * 4 : 0;
 }
