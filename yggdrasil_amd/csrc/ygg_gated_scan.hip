@@ -180,8 +180,10 @@ template <bool kBack, int kV> __device__ __forceinline__ void join_waves(const M
     }
 }
 // carry: what the first segment begins with, then what the one after the `count` of these maps does. The maps lie `hop` values apart; each
-// part takes its share of them, side by side, and the parts are joined as those of a chunk (one after the other those of 131072 x 256 took 5 us longer)
-template <int kV> __device__ __forceinline__ void join_segments(const float *maps, int64_t hop, int n, int count, Maps<kV> &lds_a, Maps<kV> &lds_h, float *carry) {
+// part takes its share of them, side by side, and the parts are joined as those of a chunk (one after the other those of 131072 x 256
+// took 5 us longer)
+template <int kV>
+__device__ __forceinline__ void join_segments(const float *maps, int64_t hop, int n, int count, Maps<kV> &lds_a, Maps<kV> &lds_h, float *carry) {
     if (count == 0) return;
     const int per = (count + kParts - 1) / kParts, first = threadIdx.x / kCols * per, end = min(first + per, count);
     float A[kV], H[kV], in[kV];
@@ -550,8 +552,10 @@ Cut cut_of(int64_t B, int64_t T, int n, int wide, int chunk, int want) {
     Cut c;
     c.slabs = (n + wide - 1) / wide;
     const int64_t columns = B * c.slabs, chunks = std::max<int64_t>((T + chunk - 1) / chunk, 1);
-    // a segment is of two chunks or more
-    int64_t segments = columns >= 256 ? 1 : std::min<int64_t>(std::min<int64_t>((want + columns - 1) / columns, kMostSegments), chunks / 2);
+    // a segment is of two chunks or more; one alone from 160 slabs on, which keep the memory busy by themselves (forward and backward of
+    // sequences of 4096 x 2048 bf16 with one segment and with as many as fill the chip: 128 slabs 126 and 249 us, 111 and 189; 160
+    // 132 and 253, 144 and 239; 192 140 and 255, 193 and 309)
+    int64_t segments = columns >= 160 ? 1 : std::min<int64_t>(std::min<int64_t>((want + columns - 1) / columns, kMostSegments), chunks / 2);
     segments = std::max<int64_t>(segments, 1);
     const int64_t per = (chunks + segments - 1) / segments;
     c.per = per * chunk;

@@ -548,8 +548,8 @@ template <class T, class F> bool with_form(int n, F f) {
     constexpr std::integral_constant<int, 64> l64{};
     constexpr std::integral_constant<int, 256> l256{};
     constexpr std::false_type no{};
-    return is(one, one, std::true_type()) || is(one, one, no) || is(four, one, no) || is(four, two, no) || is(l16, one, no) || is(l16, two, no) || is(l16, four, no) ||
-           is(l64, two, no) || is(l64, three, no) || is(l64, four, no) || is(l256, two, no) || is(l256, three, no) || is(l256, four, no);
+    return is(one, one, std::true_type()) || is(one, one, no) || is(four, one, no) || is(four, two, no) || is(l16, one, no) ||
+           is(l16, two, no) || is(l16, four, no) || is(l64, two, no) || is(l64, three, no) || is(l64, four, no) || is(l256, two, no) || is(l256, three, no) || is(l256, four, no);
 }
 // values of the widest rows that a backward pass's workgroup holds with their columns' sums: f32 in 1024 lanes, 16-bit types in 512
 // (1024 by 3 pieces of those spilled: 20000 bf16 303 us, in two readings 280)
@@ -636,7 +636,9 @@ template <class T> hipError_t go_grad(NormGradArgs a, void *scratch, hipStream_t
 template <class T> int64_t scratch_of(int64_t rows, int n) {
     return grad_groups<T>(rows, n) * 2 * n * 4 + (wide_rows(n) ? rows * waves_of<T>(n) * 8 : 0);
 }
-int64_t norm_grad_scratch(int type, int64_t rows, int n) { return type == kOpF32 ? scratch_of<float>(rows, n) : scratch_of<bf16_t>(rows, n); }
+int64_t norm_grad_scratch(int type, int64_t rows, int n) {
+    return type == kOpF32 ? scratch_of<float>(rows, n) : scratch_of<bf16_t>(rows, n);
+}
 bool norm_grad_wide(int n) { return wide_rows(n); }
 hipError_t launch_norm(int type, const NormArgs &a, hipStream_t st) {
     if (type == kOpF32) return go<float>(a, st);
