@@ -86,7 +86,7 @@ def test_shapes(B, T, n, dtype, gate_type):
 
 
 @pytest.mark.parametrize("dtype, gate_type", TYPES, ids=str)
-@pytest.mark.parametrize("B, T, n", [(1, 5000, 24), (1, 20011, 3), (3, 1030, 130), (2, 2500, 66), (40, 600, 32)])
+@pytest.mark.parametrize("B, T, n", [(1, 5000, 24), (1, 20011, 3), (3, 1030, 130), (2, 2500, 66), (40, 600, 32), (10, 300, 600), (10, 290, 1300)])
 def test_long(B, T, n, dtype, gate_type):
     """Sequences that are cut into segments, the last of them short."""
     check(*make(B, T, n, dtype, gate_type, seed=T))

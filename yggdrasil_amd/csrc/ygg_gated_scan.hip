@@ -3,7 +3,7 @@
 //   dstate = a_0 e_0.
 //
 // A run of steps maps the state before it to the one after it, h -> A h + H with A the product of its gates and H its result from
-// zero; two runs join to (A2 A1, A2 H1 + H2). A workgroup takes a slab of kCols groups of channels, 16 bytes of gates each, and goes
+// zero; two runs join to (A2 A1, A2 H1 + H2). A workgroup takes a slab of kCols groups of channels, 16 or 8 bytes of gates each, and goes
 // through time by chunks of kParts parts: each thread holds a part, kSteps steps, in registers, so that its loads are all in flight
 // together and values are read once; the four parts of a wave are joined by exchanging its rows of lanes, the waves' maps in LDS,
 // and each thread then computes its steps again from the state it begins with. (With all 16 parts' maps in LDS the backward pass of
@@ -546,16 +546,17 @@ __global__ __launch_bounds__(kCols *kParts, 2) void scan_grad_kernel(const ScanG
     }
 }
 
+constexpr int kAlone = 160;          // slabs from which on time is not cut
 constexpr int kMostSegments = 256;   // maps that a workgroup of the second kernel joins
 // want: workgroups that fill the chip
 Cut cut_of(int64_t B, int64_t T, int n, int wide, int chunk, int want) {
     Cut c;
     c.slabs = (n + wide - 1) / wide;
     const int64_t columns = B * c.slabs, chunks = std::max<int64_t>((T + chunk - 1) / chunk, 1);
-    // a segment is of two chunks or more; one alone from 160 slabs on, which keep the memory busy by themselves (forward and backward of
+    // a segment is of two chunks or more; one alone from kAlone slabs on, which keep the memory busy by themselves (forward and backward of
     // sequences of 4096 x 2048 bf16 with one segment and with as many as fill the chip: 128 slabs 126 and 249 us, 111 and 189; 160
     // 132 and 253, 144 and 239; 192 140 and 255, 193 and 309)
-    int64_t segments = columns >= 160 ? 1 : std::min<int64_t>(std::min<int64_t>((want + columns - 1) / columns, kMostSegments), chunks / 2);
+    int64_t segments = columns >= kAlone ? 1 : std::min<int64_t>(std::min<int64_t>((want + columns - 1) / columns, kMostSegments), chunks / 2);
     segments = std::max<int64_t>(segments, 1);
     const int64_t per = (chunks + segments - 1) / segments;
     c.per = per * chunk;
@@ -563,25 +564,32 @@ Cut cut_of(int64_t B, int64_t T, int n, int wide, int chunk, int want) {
     c.segments = (int)((chunks + per - 1) / per);
     return c;
 }
-// values of a thread, by the row's length
-template <class TG, class F> auto with_width(int n, F f) {
+// Channels of a thread: 16 bytes of gates, or 8 where that makes slabs enough of too few (half; forward 4 x 4096 x 2048 f32 106 us with 16
+// bytes and segments, 82 with 8 and none, 20 x 1000 x 300 f32 25 and 17; f32 backward 177 and 145; but of bf16 with f32 gates backward 113
+// and 155, as the joins of a chunk take twice their share, and wide enough slabs are better off with 16: 6 x 4096 x 2048 125 and 144)
+template <class TG, class F> auto with_width(int64_t B, int n, bool half, F f) {
     constexpr std::integral_constant<int, 16 / sizeof(TG)> wide{};
+    constexpr std::integral_constant<int, 8 / sizeof(TG)> narrow{};
     constexpr std::integral_constant<int, 1> one{};
-    return n >= decltype(wide)::value ? f(wide) : f(one);
+    auto slabs = [&](int v) { return B * ((n + kCols * v - 1) / (kCols * v)); };
+    if (n < decltype(wide)::value) return f(one);
+    if (half && slabs(decltype(wide)::value) < kAlone && slabs(decltype(narrow)::value) >= kAlone) return f(narrow);
+    return f(wide);
 }
+template <class TX> constexpr bool half_of(bool back) { return !back || sizeof(TX) == 4; }
 constexpr int steps_of(bool back) { return back ? 4 : 8; }     // of a thread
 // Two workgroups on each CU, by the registers, three of the forward kernel of 16-bit values with gates in f32 (131072 x 256 bf16: 74 us of
 // kernels, 80 with two; the backward kernel of 5 x 1001 x 1003 f32 18 us with two and 20 with three)
 template <class TX, class TG> Cut cut_for(int64_t B, int64_t T, int n, bool back) {
     const int want = !back && sizeof(TX) == 2 && sizeof(TG) == 4 ? 768 : 512;
-    return with_width<TG>(n, [&](auto v) { return cut_of(B, T, n, kCols * decltype(v)::value, kParts * steps_of(back), want); });
+    return with_width<TG>(B, n, half_of<TX>(back), [&](auto v) { return cut_of(B, T, n, kCols * decltype(v)::value, kParts * steps_of(back), want); });
 }
 
 bool writes_past(int64_t B, int64_t T, int n, int size) { return B * T * n * size >= kPastBytes; }
 
 template <class TX, class TG> hipError_t go(ScanArgs a, void *scratch, hipStream_t st) {
     a.past = writes_past(a.B, a.T, a.n, sizeof(TX));
-    return with_width<TG>(a.n, [&](auto v) {
+    return with_width<TG>(a.B, a.n, half_of<TX>(false), [&](auto v) {
         constexpr int kV = decltype(v)::value, kSteps = steps_of(false);
         if (a.T <= 8) {
             const int64_t threads = a.B * ((a.n + kV - 1) / kV);
@@ -604,7 +612,7 @@ template <class TX, class TG> hipError_t go(ScanArgs a, void *scratch, hipStream
 }
 template <class TX, class TG> hipError_t go_grad(ScanGradArgs a, void *scratch, hipStream_t st) {
     a.past = writes_past(a.B, a.T, a.n, sizeof(TX));
-    return with_width<TG>(a.n, [&](auto v) {
+    return with_width<TG>(a.B, a.n, half_of<TX>(true), [&](auto v) {
         constexpr int kV = decltype(v)::value, kSteps = steps_of(true);
         const Cut cut = cut_for<TX, TG>(a.B, a.T, a.n, true);
         const int64_t blocks = a.B * cut.slabs * cut.segments;
