@@ -345,7 +345,8 @@ int ygg_gated_scan_grad(const void *d_gate, int gate_type, int64_t gate_b, int64
    memory of ygg_gated_linear_kept bytes for g and u, which the gradients want (f32, or its upper 24 bits for 16-bit types). */
 int64_t ygg_gated_linear_kept(int type, int M, int N);
 int ygg_gated_linear(const void *d_x, const void *d_w, int type, int act, int M, int N, int K, void *d_y, void *d_gu, void *stream);
-/* The gradients, from dy (M, N): of the rows and of w. NULL: not wanted. */
+/* The gradients, from dy (M, N): of the rows and of w. NULL: not wanted. dy u act'(g) and dy act(g) are rounded to the type before the
+   products' sums, in f16 after powers of two, one for each row or column, that bring the largest to 2^14 or more. */
 int64_t ygg_gated_linear_scratch(int type, int M, int N, int K);
 int ygg_gated_linear_grad(const void *d_x, const void *d_w, const void *d_gu, const void *d_dy, int type, int act, int M, int N, int K,
                           void *d_dx, void *d_dw, void *d_scratch, int64_t scratch_bytes, void *stream);

@@ -10,6 +10,13 @@
 // of operands in tiles of their own; where the tiles are few for the 256 CUs the reduction is cut too, and the parts, in f32, are
 // added in their order.
 //
+// f16 holds 40 powers of two, and dg and du may lie past them though what comes of them does not (u = dy = 300: dg about 90000; a loss in
+// parts of 2^-20: dg 0). So in f16 they are multiplied by powers of two, undone in f32 behind the sums: one for each row, in a copy for
+// dx, whose sums go along a row, and one for each column, in a copy for dw, that bring the largest to 2^14 or more. A kernel before takes
+// the rows' and columns' largest, by maxima, which come out the same in any order. A factor is off by 2^-11 of itself or by 2^-39 of the
+// largest that is summed with it. It costs f16 a second reading of g, u and dy and the second copy (16384 x 2048 x 4096 gelu 200 us of 1740,
+// 1001 x 1000 x 2003 17 us of 112). bf16 reaches as far as f32.
+//
 // The matrix cores bound large products (16384 x 2048 x 4096 bf16 forward 490 us of kernels with g and u kept, 1.1 PFLOP/s at the 1.8 GHz
 // that the card falls to; dg and du 145, by the memory; dx 440 and dw 500), the weights' reading few rows (1 x 4096 x 8192 bf16 24 us,
 // 5.7 TB/s), the launches and the tiles' first loads what lies between.
@@ -251,31 +258,131 @@ __global__ __launch_bounds__(256) void gated_few_kernel(const T *x, const T *w, 
     }
 }
 
-// dg and du lie as g and u do, so that the products' loads are aligned, zeros behind N. A thread: 16 bytes of each
+// of dg and du the powers of two, see above
+template <class T> constexpr bool kScaled = std::is_same_v<T, f16_t>;
+// e with 2^14 <= v / 2^e < 2^15, from v's bits; 0 of no value
+__device__ __forceinline__ int power_of(uint32_t bits) { return bits ? (int)(bits >> 23) - 127 - 14 : 0; }
+__device__ __forceinline__ float times_power(float v, int e) { return __builtin_amdgcn_ldexpf(v, e); }
+
+// 16 bytes of a row's columns from n on: what is kept of them and dy, then dg and du, zeros behind N
+template <class T, int kAct, bool kPast> struct Slope {
+    static constexpr int kE = 16 / sizeof(T);
+    typename Kept<T>::Piece gp, up;
+    u32x4 dp;
+    __device__ __forceinline__ void load(const Kept<T> &gu, const T *dy, int64_t row, int N, int half, int n) {
+        const int64_t at = row * 2 * half + n;
+        gp = gu.template load<kPast>(at);
+        up = gu.template load<kPast>(at + half);
+        dp = N - n >= kE ? load16(dy + row * N + n) : load16(dy + row * N + n, N - n);
+    }
+    __device__ __forceinline__ void values(float *g, float *u, int left) const {
+        float d[kE];
+        Kept<T>::values(gp, g);
+        Kept<T>::values(up, u);
+        unpack(dp, d, T());
+#pragma unroll
+        for (int j = 0; j < kE; j++) {
+            float slope;
+            const float a = act_of<kAct>(g[j], &slope);
+            g[j] = j < left ? d[j] * u[j] * slope : 0.0f;      // what lies behind N may be anything
+            u[j] = j < left ? d[j] * a : 0.0f;
+        }
+    }
+};
+
+// dg and du lie as g and u do, so that the products' loads are aligned, zeros behind N. A thread: 16 bytes of each. by_row, by_col: the copies
+// for dx and dw, NULL where that is not wanted; of other types than f16 the same one
+struct Slopes {
+    void *by_row, *by_col;
+    uint32_t *rows, *cols;      // kScaled: the bits of the rows' and the columns' largest finite magnitudes
+};
 template <class T, int kAct, bool kPast>
-__global__ __launch_bounds__(256) void gated_slope_kernel(Kept<T> gu, const T *dy, int M, int N, T *dgu) {
+__global__ __launch_bounds__(256) void gated_slope_kernel(Kept<T> gu, const T *dy, int M, int N, Slopes to) {
     constexpr int kE = 16 / sizeof(T);
     const int half = half_of(N), per = half / kE;
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / per;
     if (row >= M) return;
-    const int n = (int)(id % per) * kE, left = N - n;
+    const int n = (int)(id % per) * kE;
     const int64_t at = row * 2 * half + n;
-    const typename Kept<T>::Piece gp = gu.template load<kPast>(at), up = gu.template load<kPast>(at + half);
-    const u32x4 dp = left >= kE ? load16(dy + row * N + n) : load16(dy + row * N + n, left);
-    float g[kE], u[kE], d[kE];
-    Kept<T>::values(gp, g);
-    Kept<T>::values(up, u);
-    unpack(dp, d, T());
+    float g[kE], u[kE];
+    Slope<T, kAct, kPast> s;
+    s.load(gu, dy, row, N, half, n);
+    s.values(g, u, N - n);
+    if constexpr (kScaled<T>) {
+        float t[kE];
+        if (to.by_row) {
+            const int e = power_of(to.rows[row]);
+            T *out = (T *)to.by_row + at;
 #pragma unroll
-    for (int j = 0; j < kE; j++) {
-        float slope;
-        const float a = act_of<kAct>(g[j], &slope);
-        g[j] = j < left ? d[j] * u[j] * slope : 0.0f;      // what lies behind N may be anything
-        u[j] = j < left ? d[j] * a : 0.0f;
+            for (int j = 0; j < kE; j++) t[j] = times_power(g[j], -e);
+            store_run<T, kE>(out, t, kE, kPast);
+#pragma unroll
+            for (int j = 0; j < kE; j++) t[j] = times_power(u[j], -e);
+            store_run<T, kE>(out + half, t, kE, kPast);
+        }
+        if (to.by_col) {
+            T *out = (T *)to.by_col + at;
+#pragma unroll
+            for (int j = 0; j < kE; j++) t[j] = times_power(g[j], -power_of(to.cols[n + j]));
+            store_run<T, kE>(out, t, kE, kPast);
+#pragma unroll
+            for (int j = 0; j < kE; j++) t[j] = times_power(u[j], -power_of(to.cols[half + n + j]));
+            store_run<T, kE>(out + half, t, kE, kPast);
+        }
+    } else {
+        T *out = (T *)to.by_row + at;
+        store_run<T, kE>(out, g, kE, kPast);
+        store_run<T, kE>(out + half, u, kE, kPast);
     }
-    T *out = dgu + row * 2 * half + n;
-    store_run<T, kE>(out, g, kE, kPast);
-    store_run<T, kE>(out + half, u, kE, kPast);
+}
+__global__ __launch_bounds__(256) void zero_kernel(uint32_t *p, int64_t count) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < count) p[i] = 0;
+}
+// The largest finite magnitudes of dg and du, of a workgroup's `band` rows and 64 pieces of columns: each of its waves a row at a time. Workgroups of
+// 16 waves, so that the maxima of a band's columns in memory are few (1001 x 2003 13.7 us, with 8 waves 20, with 4 34; 16384 x 4096 177 to 180
+// with either: the activations and the reading)
+constexpr int kReachWaves = 16;
+template <class T, int kAct>
+__global__ __launch_bounds__(64 * kReachWaves)
+void gated_reach_kernel(Kept<T> gu, const T *dy, int M, int N, int band, int slabs, uint32_t *rows, uint32_t *cols) {
+    constexpr int kE = 16 / sizeof(T), kC = 64 * kE;
+    __shared__ uint32_t lds[kReachWaves][2 * kE][65];
+    const int half = half_of(N), lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c0 = (int)(blockIdx.x % slabs) * kC, n = c0 + lane * kE;
+    const int first = (int)(blockIdx.x / slabs) * band, end = min(first + band, M);
+    auto bits = [](float v) {
+        const uint32_t b = __builtin_bit_cast(uint32_t, v) & 0x7fffffffu;
+        return b < 0x7f800000u ? b : 0u;
+    };
+    uint32_t most[2 * kE] = {};
+    for (int row = first + wave; row < end; row += kReachWaves) {
+        uint32_t all = 0;
+        if (n < half) {
+            float g[kE], u[kE];
+            Slope<T, kAct, false> s;
+            s.load(gu, dy, row, N, half, n);
+            s.values(g, u, N - n);
+#pragma unroll
+            for (int j = 0; j < kE; j++) {
+                most[j] = max(most[j], bits(g[j]));
+                most[kE + j] = max(most[kE + j], bits(u[j]));
+                all = max(all, max(bits(g[j]), bits(u[j])));
+            }
+        }
+        all = join<64>(all, [](uint32_t a, uint32_t b) { return max(a, b); });
+        if (lane == 0 && all) atomicMax(rows + row, all);
+    }
+#pragma unroll
+    for (int j = 0; j < 2 * kE; j++) lds[wave][j][lane] = most[j];
+    __syncthreads();
+    // neighbouring lanes take neighbouring columns; most maxima are not new ones
+    for (int i = threadIdx.x; i < 2 * kC; i += 64 * kReachWaves) {
+        const int c = i % kC, j = i / kC * kE + c % kE;
+        if (c0 + c >= half) continue;
+        uint32_t *to = cols + (i < kC ? 0 : half) + c0 + c, all = 0;
+        for (int w = 0; w < kReachWaves; w++) all = max(all, lds[w][j][c / kE]);
+        if (all > *(volatile uint32_t *)to) atomicMax(to, all);
+    }
 }
 
 // ---- the gradients' products: out (I, O) = sum over r of A(i, r) b(r, o), b's rows `pitch` values apart. kRows: A is a (I, 2 half), the r's
@@ -288,6 +395,7 @@ struct Dense {
     void *out;
     float *sums;
     int tiles, cols, per;       // tiles of a part, tiles along O, steps of a part
+    const uint32_t *most;       // kScaled: the largest that A's row i was scaled by
     // the row of w that a column of dg and du belongs to, or -1
     __device__ __forceinline__ int place(int k) const { return k < N ? k : k >= half && k < half + N ? k - half + N : -1; }
 };
@@ -298,6 +406,13 @@ template <class T, bool kRows> struct DenseOut {
         const int row = kRows ? (i0 + i < g.I ? i0 + i : -1) : g.place(i0 + i);
         if (row < 0 || o0 + o >= g.O) return;
         const int64_t at = (int64_t)row * g.O + o0 + o;
+        float t[N::value];
+        if constexpr (kScaled<T>) {
+            const int e = power_of(g.most[i0 + i]);
+#pragma unroll
+            for (int j = 0; j < N::value; j++) t[j] = times_power(v[j], e);
+            v = t;
+        }
         if (g.sums) store_run<float, N::value>(g.sums + (int64_t)part * g.I * g.O + at, v, g.O - o0 - o);
         else store_run<T, N::value>((T *)g.out + at, v, g.O - o0 - o);
     }
@@ -439,17 +554,25 @@ template <class T, int kAct> hipError_t go(const void *x, const void *w, int M, 
     // 1001 x 1000 x 2003, 256 of them, 19.8 and 19.1
     return tiles128 >= 384 ? tiles(four, two, two) : tiles(two, two, two);
 }
-template <class T, int kAct> hipError_t go_slope(const void *gu, const void *dy, int M, int N, void *dgu, hipStream_t st) {
+template <class T, int kAct> hipError_t go_slope(const void *gu, const void *dy, int M, int N, const Slopes &to, hipStream_t st) {
     constexpr int kE = 16 / sizeof(T);
-    const int64_t blocks = ((int64_t)M * (half_of(N) / kE) + 255) / 256;
+    const int half = half_of(N);
+    const int64_t blocks = ((int64_t)M * (half / kE) + 255) / 256;
     if (blocks == 0) return hipSuccess;
     if (blocks > most_blocks(256)) return kTooLarge;
-    const Kept<T> kept = {(char *)gu, (int64_t)M * 2 * half_of(N)};
+    const Kept<T> kept = {(char *)gu, (int64_t)M * 2 * half};
+    if constexpr (kScaled<T>) {
+        const int64_t count = (int64_t)M + 2 * half;      // rows and cols lie one behind the other
+        hipLaunchKernelGGL(zero_kernel, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, st, to.rows, count);
+        const int slabs = (half / kE + 63) / 64, bands = std::max(512 / slabs, 1), band = ((M + bands - 1) / bands + kReachWaves - 1) / kReachWaves * kReachWaves;
+        hipLaunchKernelGGL((gated_reach_kernel<T, kAct>), dim3((unsigned)(slabs * ((M + band - 1) / band))), dim3(64 * kReachWaves), 0, st,
+                           kept, (const T *)dy, M, N, band, slabs, to.rows, to.cols);
+    }
     // 16384 x 4096 bf16: 184 us with the caches, 145 past them
     if (kept.count * Kept<T>::kBytes >= kPastBytes)
-        hipLaunchKernelGGL((gated_slope_kernel<T, kAct, true>), dim3((unsigned)blocks), dim3(256), 0, st, kept, (const T *)dy, M, N, (T *)dgu);
+        hipLaunchKernelGGL((gated_slope_kernel<T, kAct, true>), dim3((unsigned)blocks), dim3(256), 0, st, kept, (const T *)dy, M, N, to);
     else
-        hipLaunchKernelGGL((gated_slope_kernel<T, kAct, false>), dim3((unsigned)blocks), dim3(256), 0, st, kept, (const T *)dy, M, N, (T *)dgu);
+        hipLaunchKernelGGL((gated_slope_kernel<T, kAct, false>), dim3((unsigned)blocks), dim3(256), 0, st, kept, (const T *)dy, M, N, to);
     return hipGetLastError();
 }
 
@@ -493,7 +616,8 @@ int64_t spaced_bytes(const Plan &p, int size, bool rows, int M, int N) {
     return p.spaced ? ((int64_t)(rows ? 2 * N : M) * p.pitch * size + 255) / 256 * 256 : 0;
 }
 int64_t part_bytes(const Plan &p, bool rows, int M, int N, int K) { return p.parts > 1 ? (int64_t)p.parts * (rows ? M : 2 * N) * K * 4 : 0; }
-template <class T, bool kRows> hipError_t go_dense(const void *a, const void *b, int M, int N, int K, void *out, void *scratch, hipStream_t st) {
+template <class T, bool kRows>
+hipError_t go_dense(const void *a, const uint32_t *most, const void *b, int M, int N, int K, void *out, void *scratch, hipStream_t st) {
     const Plan p = plan_of(sizeof(T), kRows, M, N, K, (uintptr_t)b % 16 == 0);
     float *sums = (float *)((char *)scratch + spaced_bytes(p, sizeof(T), kRows, M, N));
     const int64_t blocks = p.tiles * p.parts, I = kRows ? M : 2 * N, count = I * K;
@@ -507,7 +631,7 @@ template <class T, bool kRows> hipError_t go_dense(const void *a, const void *b,
         if (e != hipSuccess) return e;
         b = scratch;
     }
-    const Dense g = {a, b, (int)I, K, M, p.pitch, N, half_of(N), out, p.parts > 1 ? sums : nullptr, (int)p.tiles, p.cols, p.per};
+    const Dense g = {a, b, (int)I, K, M, p.pitch, N, half_of(N), out, p.parts > 1 ? sums : nullptr, (int)p.tiles, p.cols, p.per, most};
     if (p.turn) {
         if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((dense_turn_kernel<T, kRows>), dim3((unsigned)blocks), dim3(512), 0, st, g);
     } else if (p.large) {
@@ -534,8 +658,14 @@ hipError_t launch_gated(int type, int act, const void *x, const void *w, int M, 
     });
 }
 int64_t gated_kept(int type, int M, int N) { return (int64_t)M * 2 * half_of(N) * (type == kOpF32 ? 4 : 3); }
-// dg and du, then what one product at a time takes; whether its operand turns out to be aligned or not
-int64_t dgu_bytes(int type, int M, int N) { return ((int64_t)M * 2 * half_of(N) * op_bytes(type) + 255) / 256 * 256; }
+// dg and du (f16: a copy for each product, then the rows' and columns' largest), then what one product at a time takes; whether its
+// operand turns out to be aligned or not
+int64_t up_to_256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+int64_t dgu_copy(int type, int M, int N) { return up_to_256((int64_t)M * 2 * half_of(N) * op_bytes(type)); }
+int64_t dgu_bytes(int type, int M, int N) {
+    const int64_t copy = dgu_copy(type, M, N);
+    return type == kOpF16 && M ? 2 * copy + up_to_256(((int64_t)M + 2 * half_of(N)) * 4) : copy;
+}
 int64_t gated_grad_scratch(int type, int M, int N, int K) {
     const int size = op_bytes(type);
     int64_t most = 0;
@@ -548,16 +678,24 @@ int64_t gated_grad_scratch(int type, int M, int N, int K) {
 }
 hipError_t launch_gated_grad(int type, int act, const void *x, const void *w, const void *gu, const void *dy, int M, int N, int K,
                              void *dx, void *dw, void *scratch, hipStream_t st) {
-    void *dgu = scratch, *rest = (char *)scratch + dgu_bytes(type, M, N);
+    char *const at = (char *)scratch, *rest = at + dgu_bytes(type, M, N);
+    const int64_t copy = dgu_copy(type, M, N);
+    Slopes to = {at, at, nullptr, nullptr};
+    if (type == kOpF16) {
+        to.by_row = dx ? at : nullptr;
+        to.by_col = dw ? at + copy : nullptr;
+        to.rows = (uint32_t *)(at + 2 * copy);
+        to.cols = to.rows + M;
+    }
     hipError_t e = with_type(type, [&](auto one) {
-        return with_act(act, [&](auto k) { return go_slope<decltype(one), decltype(k)::value>(gu, dy, M, N, dgu, st); });
+        return with_act(act, [&](auto k) { return go_slope<decltype(one), decltype(k)::value>(gu, dy, M, N, to, st); });
     });
     if (e != hipSuccess) return e;
     return with_type(type, [&](auto one) {
         typedef decltype(one) T;
         hipError_t e = hipSuccess;
-        if (dx) e = go_dense<T, true>(dgu, w, M, N, K, dx, rest, st);
-        if (e == hipSuccess && dw) e = go_dense<T, false>(dgu, x, M, N, K, dw, rest, st);
+        if (dx) e = go_dense<T, true>(to.by_row, to.rows, w, M, N, K, dx, rest, st);
+        if (e == hipSuccess && dw) e = go_dense<T, false>(to.by_col, to.cols, x, M, N, K, dw, rest, st);
         return e;
     });
 }

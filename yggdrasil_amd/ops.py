@@ -280,7 +280,9 @@ def gated_linear(x, w, activation: str = "silu") -> torch.Tensor:
     """The gated projections of a feed-forward block in one kernel: x (..., K), w (2, N, K) in x's type ->
     act(x w[0]^T) (x w[1]^T) (..., N) in x's type, act "silu" (g sigmoid(g)), "gelu" (g Phi(g)) or "sigmoid". Sums and
     the product are in f32, rounded once. Differentiable in x and w: for that, both projections are kept (in f32, or its upper 24
-    bits for 16-bit types), and the gradients' products take their factors in x's type."""
+    bits for 16-bit types), and the gradients' products take their factors in x's type: dy u act'(g) and dy act(g) are rounded to it
+    before the sums, in float16 after a power of two for each row (the gradient of x) or column (that of w), so that their range is
+    float32's and what is under 2^-39 of the largest beside it is lost."""
     act = ACTIVATIONS.get(activation) if isinstance(activation, str) else None
     if act is None:
         raise ValueError(f"activation {activation!r}: one of {', '.join(ACTIVATIONS)}")
