@@ -4,7 +4,8 @@
 // A row is held in the registers of 1 to 64 lanes or of a workgroup, 16 bytes a load, so that it is read once: the mean and
 // then the squares about it are joined in f32. A workgroup's waves first take each its own mean and squares M2 and are joined by
 //   m = sum n_i m_i / n,  M2 = sum M2_i + n_i (m_i - m)^2,
-// which takes one barrier instead of two and cancels nothing. The backward pass reads x and dy once, writes dx, and keeps its
+// which takes one barrier instead of two and cancels nothing. z is (x - m) times the inverse deviation, as it stands: with m times that
+// rounded by itself, x rstd + (-m rstd) in one operation, rows far from zero lose half a step of |m| rstd, and rows of one value are not 0. The backward pass reads x and dy once, writes dx, and keeps its
 // columns' sums of dy z and dy in registers over all of a workgroup's rows; the workgroups' sums are added in their order by a
 // second kernel, so that they come out the same every time. Rows wider than the registers hold are read again: past 65536 values of
 // f32, and in the backward pass, which holds the columns' sums too, past 16384.
@@ -200,7 +201,6 @@ __global__ __launch_bounds__(kL > 256 ? kL : 256) void norm_kernel(const NormArg
         if (a.stats && at.lane == 0) ((float2 *)a.stats)[row] = s;
         let_go(x);
         if constexpr (!kAhead || (kL == 1024 && sizeof(T) == 2)) at.anew();
-        const float c = -s.x * s.y;        // z = x / deviation + c: its rounding is one more of the mean's
         T *y = (T *)a.y + row * a.n;
 #pragma unroll
         for (int i = 0; i < kP; i++) {
@@ -214,7 +214,7 @@ __global__ __launch_bounds__(kL > 256 ? kL : 256) void norm_kernel(const NormArg
                 whole_weight<T>(bf, a.bias, a.wide, at.column(i), 0.0f);
             }
 #pragma unroll
-            for (int j = 0; j < kE; j++) f[j] = __builtin_fmaf(__builtin_fmaf(f[j], s.y, c), wf[j], bf[j]);
+            for (int j = 0; j < kE; j++) f[j] = __builtin_fmaf((f[j] - s.x) * s.y, wf[j], bf[j]);
             at.store(y, f, i, a.past);
             if constexpr (kP > 4) __builtin_amdgcn_sched_barrier(0);
         }
@@ -322,7 +322,6 @@ __global__ __launch_bounds__(kL > 256 ? kL : 256, 2) void norm_grad_kernel(const
         s = next_s;
         if constexpr (kWide) at.anew();
         else load(row + hop);
-        const float c = -s.x * s.y;
         float q1 = 0.0f, q2 = 0.0f;
 #pragma unroll
         for (int i = 0; i < kP; i++) {
@@ -337,7 +336,7 @@ __global__ __launch_bounds__(kL > 256 ? kL : 256, 2) void norm_grad_kernel(const
             }
 #pragma unroll
             for (int j = 0; j < kE; j++) {
-                const float z = __builtin_fmaf(f[j], s.y, c), q = wf[j] * d[j];
+                const float z = (f[j] - s.x) * s.y, q = wf[j] * d[j];
                 aw[i][j] = __builtin_fmaf(d[j], z, aw[i][j]);
                 if constexpr (kWide) b.v[i][j / 4][threadIdx.x][j % 4] += d[j];
                 else ab[i][j] += d[j];
@@ -359,8 +358,8 @@ __global__ __launch_bounds__(kL > 256 ? kL : 256, 2) void norm_grad_kernel(const
             }
         }
         if (!a.dx) continue;       // not before the joins: the compiler would hold all the values that they add until then
-        q1 *= -s.y / (float)n;
-        q2 *= -s.y / (float)n;
+        q1 /= (float)n;
+        q2 /= -(float)n;
         let_go(x);
         let_go(dy);
         if constexpr (kWide) at.anew();
@@ -374,8 +373,8 @@ __global__ __launch_bounds__(kL > 256 ? kL : 256, 2) void norm_grad_kernel(const
             else w.get(wf, i, at.lane);
 #pragma unroll
             for (int j = 0; j < kE; j++) {
-                const float z = __builtin_fmaf(f[j], s.y, c);
-                f[j] = __builtin_fmaf(z, q2, __builtin_fmaf(wf[j] * s.y, d[j], q1));
+                const float z = (f[j] - s.x) * s.y;
+                f[j] = __builtin_fmaf(z, q2, wf[j] * d[j] - q1) * s.y;     // the deviation last: equal q cancel wholly
             }
             at.store(dx, f, i, a.past);
             __builtin_amdgcn_sched_barrier(0);
