@@ -429,16 +429,6 @@ std::pair<std::vector<Tensor>, Tensor> clip_grad_norm(std::vector<Tensor> in, do
         out = *to;
         for (const Tensor &t : out)
             if (t.layout() != at::kStrided || !t.is_non_overlapping_and_dense()) throw py::value_error("out must hold dense tensors");
-        std::vector<Range> written = ranges_of(out);
-        std::sort(written.begin(), written.end(), [](const Range &a, const Range &b) { return a.from < b.from; });
-        for (size_t k = 1; k < written.size(); k++)
-            if (written[k].from < written[k - 1].end) throw py::value_error("two tensors that clip_grad_norm writes share memory");
-        for (const Range &r : ranges_of(in)) {
-            // the written ones that end past r's begin: those from here on
-            auto w = std::upper_bound(written.begin(), written.end(), r.from, [](uintptr_t p, const Range &b) { return p < b.end; });
-            for (; w != written.end() && w->from < r.end; ++w)
-                if (w->i != r.i || w->from != r.from) throw py::value_error("clip_grad_norm would write into memory of another of its tensors");
-        }
     }
     std::vector<const void *> from(in.size());
     std::vector<void *> into(in.size());
@@ -455,6 +445,20 @@ std::pair<std::vector<Tensor>, Tensor> clip_grad_norm(std::vector<Tensor> in, do
         from[i] = in[i].data_ptr();
         sizes[i] = in[i].numel();
         types[i] = type_of(in[i]);
+    }
+    if (clip && to) {
+        // of what is read where it lies; the copies made above are nobody else's, and of tensors that are not dense the bytes that they
+        // count are not those that they reach over
+        std::vector<Range> written = ranges_of(out);
+        std::sort(written.begin(), written.end(), [](const Range &a, const Range &b) { return a.from < b.from; });
+        for (size_t k = 1; k < written.size(); k++)
+            if (written[k].from < written[k - 1].end) throw py::value_error("two tensors that clip_grad_norm writes share memory");
+        for (const Range &r : ranges_of(in)) {
+            // the written ones that end past r's begin: those from here on
+            auto w = std::upper_bound(written.begin(), written.end(), r.from, [](uintptr_t p, const Range &b) { return p < b.end; });
+            for (; w != written.end() && w->from < r.end; ++w)
+                if (w->i != r.i || w->from != r.from) throw py::value_error("clip_grad_norm would write into memory of another of its tensors");
+        }
     }
     Tensor norm = empty(first, {}, at::kFloat);
     const int64_t need = api.clip_scratch(sizes.data(), (int)sizes.size());
