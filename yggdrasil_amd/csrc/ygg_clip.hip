@@ -91,6 +91,16 @@ __global__ __launch_bounds__(kThreads) void squares_kernel(const Table tab, doub
     if (threadIdx.x == 0) part[blockIdx.x] = all;
 }
 
+// v for a later rounding to T, so that both together are one: f32 itself, else towards zero with the last bit set where anything is lost
+// (f32 has 13 bits more than f16, and 16 more than bf16, so what is no value of f32 stays on its side of their middles)
+template <class T> __device__ __forceinline__ float to_odd(double v) {
+    const float f = (float)v;
+    if constexpr (sizeof(T) == 4) return f;
+    const double back = (double)f;
+    const uint32_t b = __builtin_bit_cast(uint32_t, f);
+    return back == v ? f : __builtin_bit_cast(float, (b - (__builtin_fabs(back) > __builtin_fabs(v))) | 1u);
+}
+
 // in thread 0: the norm, and what the values are multiplied by. A norm that is no finite number changes nothing.
 struct Norm {
     double norm, by;
@@ -135,7 +145,7 @@ __global__ __launch_bounds__(kThreads) void scale_kernel(const Table tab, const 
             float t[kE];
             unpack(v, t, T());
 #pragma unroll
-            for (int j = 0; j < kE; j++) t[j] = (float)((double)t[j] * f);
+            for (int j = 0; j < kE; j++) t[j] = to_odd<T>((double)t[j] * f);
             store_run<T, kE>(out + c, t, s.count - c, tab.past);
         };
         int c = threadIdx.x * kE;
