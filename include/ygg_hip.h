@@ -352,7 +352,8 @@ int ygg_gated_linear_grad(const void *d_x, const void *d_w, const void *d_gu, co
                           void *d_dx, void *d_dw, void *d_scratch, int64_t scratch_bytes, void *stream);
 
 /* d_norm (1): the root of the sum of the squares of all values of `count` tensors, summed in 64 bits. d_out (NULL: the norm
-   alone): each tensor times min(1, most / norm), each value rounded once; a norm that is no finite number changes nothing. The
+   alone): each tensor times min(1, most / norm), each value rounded once; a norm that is no finite number of 64 bits changes nothing
+   (one past f32's largest is infinite in d_norm, and the values are clipped by it). The
    arrays (of device addresses, sizes and types) are host memory that is read before the call returns; d_out may hold the
    tensors themselves, but no two tensors may overlap otherwise. */
 int64_t ygg_clip_scratch(const int64_t *sizes, int count);

@@ -342,8 +342,8 @@ def _clip(grads, most: float, clip: bool, out=None):
 
 
 def grad_norm(grads) -> torch.Tensor:
-    """The norm of all values of the tensors together (None: left out), the root of the sum of their squares: () f32, squares
-    summed in 64 bits, in the same order every time."""
+    """The norm of all values of the tensors together (None: left out), the root of the sum of their squares: () f32 (infinite past its
+    largest), squares summed in 64 bits, in the same order every time."""
     with torch.no_grad():
         return _clip(grads, 0.0, False)[1]
 
@@ -352,7 +352,8 @@ def clip_grad_norm(grads, max_norm: float, out=None):
     """Gradients (None: there is none) brought to a norm of at most max_norm together: each times min(1, max_norm / norm), rounded
     once -> the list of them, and the norm that they had, () f32. New tensors, or out: tensors of their shapes and types, also
     the gradients themselves (out=grads: in place); no others may share memory with what is written. A norm that is NaN or
-    infinite leaves the values as they are; the caller sees it in the norm. Nothing waits for the GPU."""
+    infinite in 64 bits, in which the squares are summed, leaves the values as they are, and the caller sees it in the norm; one that is
+    only past float32's largest comes back as infinite too, but the values are clipped by it. Nothing waits for the GPU."""
     if not (isinstance(max_norm, (int, float)) and max_norm >= 0):
         raise ValueError(f"max_norm {max_norm!r}: a number of at least 0")
     return _clip(grads, float(max_norm), True, out)
