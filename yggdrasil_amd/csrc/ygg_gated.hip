@@ -31,7 +31,7 @@ namespace {
 // act(g) and, of the backward pass, act'(g)
 template <int kAct> __device__ __forceinline__ float act_of(float g, float *slope = nullptr) {
     if constexpr (kAct == kGelu) {
-        const float phi = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
+        const float phi = 0.5f * erfcf(g * -0.70710678118654752f);      // 1 + erf has no digits left where g is far below 0
         if (slope) *slope = __builtin_fmaf(g, 0.3989422804014327f * expf(-0.5f * g * g), phi);
         return g * phi;
     } else {
