@@ -35,12 +35,12 @@ template <int kAct> __device__ __forceinline__ float act_of(float g, float *slop
         if (slope) *slope = __builtin_fmaf(g, 0.3989422804014327f * expf(-0.5f * g * g), phi);
         return g * phi;
     } else {
-        const float p = 1.0f / (1.0f + expf(-g));
+        const float e = expf(-g), p = 1.0f / (1.0f + e);
         if constexpr (kAct == kSilu) {
             if (slope) *slope = p * __builtin_fmaf(g, 1.0f - p, 1.0f);
             return g * p;
         } else {
-            if (slope) *slope = p * (1.0f - p);
+            if (slope) *slope = p * (g > 0.0f ? e * p : 1.0f - p);      // 1 - p, which has no digits left where p is near 1
             return p;
         }
     }
