@@ -594,6 +594,10 @@ Plan plan_of(int size, bool rows, int M, int N, int K, bool aligned) {
         p.per = (int)std::max<int64_t>((steps + parts - 1) / parts, 1);
         p.parts = std::max((steps + p.per - 1) / p.per, 1);      // without rows there is still the weights' gradient, zero
     };
+    // 256 x 256 tiles where both sides fill most of one, and where tiles and parts come to 96 workgroups or more. Forward and one gradient of bf16
+    // (rows, N, K) by those and by the smaller ones, us: 8192 x 2048 of K = 192 dx 108 and 128, dw 111 and 132, of K = 128 96 and 95, 100
+    // and 95; 128 x 8192 x 4096 dx 96 and 91. 112 of them, 1001 x 2003 x 1000 dx 62 and 68, dw 63 and 67; 64 of them, 1024 x 1024 x 1024 47 and
+    // 39, 49 and 39, 192 x 2048 x 2048 dx 47 and 41; 128, 256 x 4096 x 2048 dx 62 and 57
     p.pitch = half_of(K);
     const int64_t a_bytes = (int64_t)M * 2 * half * size, b_bytes = (int64_t)(rows ? 2 * N : M) * p.pitch * size;
     p.spaced = p.pitch != K;

@@ -553,9 +553,9 @@ Cut cut_of(int64_t B, int64_t T, int n, int wide, int chunk, int want) {
     Cut c;
     c.slabs = (n + wide - 1) / wide;
     const int64_t columns = B * c.slabs, chunks = std::max<int64_t>((T + chunk - 1) / chunk, 1);
-    // a segment is of two chunks or more; one alone from kAlone slabs on, which keep the memory busy by themselves (forward and backward of
-    // sequences of 4096 x 2048 bf16 with one segment and with as many as fill the chip: 128 slabs 126 and 249 us, 111 and 189; 160
-    // 132 and 253, 144 and 239; 192 140 and 255, 193 and 309)
+    // a segment is of two chunks or more; one alone from kAlone slabs on, which keep the memory busy by themselves (sequences of 4096 x 2048 bf16
+    // with one segment and with as many as fill the chip, us: forward of 160 slabs 130 and 141, of 192 143 and 195, of 128 in wide slabs 126 and
+    // 111; backward of 128 235 and 181, of 144 232 and 214, of 160 242 and 244, of 176 245 and 308, of 192 242 and 317)
     int64_t segments = columns >= kAlone ? 1 : std::min<int64_t>(std::min<int64_t>((want + columns - 1) / columns, kMostSegments), chunks / 2);
     segments = std::max<int64_t>(segments, 1);
     const int64_t per = (chunks + segments - 1) / segments;
@@ -591,6 +591,9 @@ template <class TX, class TG> hipError_t go(ScanArgs a, void *scratch, hipStream
     a.past = writes_past(a.B, a.T, a.n, sizeof(TX));
     return with_width<TG>(a.B, a.n, half_of<TX>(false), [&](auto v) {
         constexpr int kV = decltype(v)::value, kSteps = steps_of(false);
+        // by steps as long as the parts of a chunk would have few: 64 x 256 f32 of 8 steps 3.5 us and 4.2 by parts, of 12 4.1 and 4.2, of 16 4.7 and
+        // 4.3; 16 x 2048 f32 3.6 and 5.2, 4.3 and 5.1, 5.0 and 5.1. (Channels enough to fill the chip are faster by steps further on:
+        // 256 x 4096 bf16 of 16 18 us and 82, of 32 32 and 84.)
         if (a.T <= 8) {
             const int64_t threads = a.B * ((a.n + kV - 1) / kV);
             if ((threads + 255) / 256 > most_blocks(256)) return kTooLarge;
