@@ -343,7 +343,7 @@ __global__ __launch_bounds__(256) void zero_kernel(uint32_t *p, int64_t count) {
 // 16 waves, so that the maxima of a band's columns in memory are few (1001 x 2003 13.7 us, with 8 waves 20, with 4 34; 16384 x 4096 177 to 180
 // with either: the activations and the reading)
 constexpr int kReachWaves = 16;
-template <class T, int kAct>
+template <class T, int kAct, bool kPast>
 __global__ __launch_bounds__(64 * kReachWaves)
 void gated_reach_kernel(Kept<T> gu, const T *dy, int M, int N, int band, int slabs, uint32_t *rows, uint32_t *cols) {
     constexpr int kE = 16 / sizeof(T), kC = 64 * kE;
@@ -359,7 +359,7 @@ void gated_reach_kernel(Kept<T> gu, const T *dy, int M, int N, int band, int sla
         uint32_t all = 0;
         if (n < half) {
             float g[kE], u[kE];
-            Slope<T, kAct, false> s;
+            Slope<T, kAct, kPast> s;
             s.load(gu, dy, row, N, half, n);
             s.values(g, u, N - n);
 #pragma unroll
@@ -561,18 +561,21 @@ template <class T, int kAct> hipError_t go_slope(const void *gu, const void *dy,
     if (blocks == 0) return hipSuccess;
     if (blocks > most_blocks(256)) return kTooLarge;
     const Kept<T> kept = {(char *)gu, (int64_t)M * 2 * half};
-    if constexpr (kScaled<T>) {
-        const int64_t count = (int64_t)M + 2 * half;      // rows and cols lie one behind the other
-        hipLaunchKernelGGL(zero_kernel, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, st, to.rows, count);
-        const int slabs = (half / kE + 63) / 64, bands = std::max(512 / slabs, 1), band = ((M + bands - 1) / bands + kReachWaves - 1) / kReachWaves * kReachWaves;
-        hipLaunchKernelGGL((gated_reach_kernel<T, kAct>), dim3((unsigned)(slabs * ((M + band - 1) / band))), dim3(64 * kReachWaves), 0, st,
-                           kept, (const T *)dy, M, N, band, slabs, to.rows, to.cols);
-    }
-    // 16384 x 4096 bf16: 184 us with the caches, 145 past them
-    if (kept.count * Kept<T>::kBytes >= kPastBytes)
-        hipLaunchKernelGGL((gated_slope_kernel<T, kAct, true>), dim3((unsigned)blocks), dim3(256), 0, st, kept, (const T *)dy, M, N, to);
-    else
-        hipLaunchKernelGGL((gated_slope_kernel<T, kAct, false>), dim3((unsigned)blocks), dim3(256), 0, st, kept, (const T *)dy, M, N, to);
+    auto launch = [&](auto past) {
+        constexpr bool kPast = decltype(past)::value;
+        if constexpr (kScaled<T>) {
+            const int64_t count = (int64_t)M + 2 * half;      // rows and cols lie one behind the other
+            hipLaunchKernelGGL(zero_kernel, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, st, to.rows, count);
+            const int slabs = (half / kE + 63) / 64, bands = std::max(512 / slabs, 1);
+            const int band = ((M + bands - 1) / bands + kReachWaves - 1) / kReachWaves * kReachWaves;
+            hipLaunchKernelGGL((gated_reach_kernel<T, kAct, kPast>), dim3((unsigned)(slabs * ((M + band - 1) / band))), dim3(64 * kReachWaves), 0, st,
+                               kept, (const T *)dy, M, N, band, slabs, to.rows, to.cols);
+        }
+        hipLaunchKernelGGL((gated_slope_kernel<T, kAct, kPast>), dim3((unsigned)blocks), dim3(256), 0, st, kept, (const T *)dy, M, N, to);
+    };
+    // 16384 x 4096 bf16: 184 us with the caches, 145 past them; f16's two kernels 177 and 187, 173 and 173
+    if (kept.count * Kept<T>::kBytes >= kPastBytes) launch(std::true_type());
+    else launch(std::false_type());
     return hipGetLastError();
 }
 
