@@ -129,3 +129,50 @@ def test_values_that_are_not_finite(M, N, K, dtype):
         good = torch.ones(len(t), dtype=torch.bool)
         good[bad] = False
         near(t[good.cuda()], ref[good], tol[good], "others")
+
+
+@pytest.mark.parametrize("N, K", [(5, 9), (300, 264), (4096, 777)])
+def test_no_rows(N, K):
+    from yggdrasil_amd import ops
+    x, w = (torch.zeros(s, dtype=torch.float16, device="cuda", requires_grad=True) for s in ((0, K), (2, N, K)))
+    dx, dw = torch.autograd.grad(ops.gated_linear(x, w).sum(), (x, w))
+    assert dx.shape == (0, K) and dw.shape == w.shape and not dw.any()
+
+
+@pytest.mark.parametrize("M, N, K", [(1, 300, 256), (300, 200, 264), (2048, 4096, 64), (500, 1003, 203)])
+def test_streams_and_graphs(M, N, K):
+    """Rows of other sizes in each replay: the largest of the one before must not stay."""
+    from yggdrasil_amd import ops
+
+    def make(seed):
+        g = torch.Generator("cuda").manual_seed(seed)
+        x, w, dy = (torch.randn(s, generator=g, device="cuda") for s in ((M, K), (2, N, K), (M, N)))
+        return x.half(), (w / math.sqrt(K)).half(), (dy * 2.0 ** torch.randint(-12, 9, (M, 1), generator=g, device="cuda")).half()
+
+    def both(leaves, dy):
+        y = ops.gated_linear(*leaves)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+    x, w, dy = make(0)
+    leaves = [t.requires_grad_() for t in (x, w)]
+    want = both(leaves, dy)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = both(leaves, dy)
+    s.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    del want, got
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = both(leaves, dy)
+    for k in range(4):
+        new = make(10 + k)
+        with torch.no_grad():
+            for t, v in zip((x, w, dy), new):
+                t.copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [t.clone() for t in out]
+        want = both([t.requires_grad_() for t in new[:2]], new[2])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(kept, want)), k

@@ -395,7 +395,7 @@ struct Dense {
     void *out;
     float *sums;
     int tiles, cols, per;       // tiles of a part, tiles along O, steps of a part
-    const uint32_t *most;       // kScaled: the largest that A's row i was scaled by
+    const uint32_t *most;       // kScaled: the largest that A's row i was scaled by; NULL without rows
     // the row of w that a column of dg and du belongs to, or -1
     __device__ __forceinline__ int place(int k) const { return k < N ? k : k >= half && k < half + N ? k - half + N : -1; }
 };
@@ -408,7 +408,7 @@ template <class T, bool kRows> struct DenseOut {
         const int64_t at = (int64_t)row * g.O + o0 + o;
         float t[N::value];
         if constexpr (kScaled<T>) {
-            const int e = power_of(g.most[i0 + i]);
+            const int e = g.most ? power_of(g.most[i0 + i]) : 0;
 #pragma unroll
             for (int j = 0; j < N::value; j++) t[j] = times_power(v[j], e);
             v = t;
@@ -688,7 +688,7 @@ hipError_t launch_gated_grad(int type, int act, const void *x, const void *w, co
     char *const at = (char *)scratch, *rest = at + dgu_bytes(type, M, N);
     const int64_t copy = dgu_copy(type, M, N);
     Slopes to = {at, at, nullptr, nullptr};
-    if (type == kOpF16) {
+    if (type == kOpF16 && M) {
         to.by_row = dx ? at : nullptr;
         to.by_col = dw ? at + copy : nullptr;
         to.rows = (uint32_t *)(at + 2 * copy);
