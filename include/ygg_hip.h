@@ -302,7 +302,8 @@ int ygg_int8_linear(const void *d_x, int type, const int8_t *d_w, const float *d
                     void *d_scratch, int64_t scratch_bytes, void *stream);
 
 /* ---- Operators of a recurrent block that is trained and served beside the model (the reference trains with JAX: its scan
-   yggdrasil/scan.py:6-15, its norm yggdrasil/model.py:92-93, its clipping yggdrasil/train.py:64-68). As those above: on the
+   yggdrasil/scan.py:6-15, its clipping yggdrasil/train.py:64-68, and an RMS norm, yggdrasil/model.py:92-93, where this one also takes
+   the mean and adds a bias). As those above: on the
    caller's current device and stream, without a wait or an allocation; types 0 f32, 1 bf16, 2 f16. Scratch is device
    memory of the bytes that the _scratch entry gives, 256-byte aligned, that no other call uses until this one has run. ---- */
 #define YGG_MOST_STEPS (1 << 30)             /* steps of a recurrence */
@@ -346,7 +347,7 @@ int ygg_gated_scan_grad(const void *d_gate, int gate_type, int64_t gate_b, int64
 int64_t ygg_gated_linear_kept(int type, int M, int N);
 int ygg_gated_linear(const void *d_x, const void *d_w, int type, int act, int M, int N, int K, void *d_y, void *d_gu, void *stream);
 /* The gradients, from dy (M, N): of the rows and of w. NULL: not wanted. dy u act'(g) and dy act(g) are rounded to the type before the
-   products' sums, in f16 after powers of two, one for each row or column, that bring the largest to 2^14 or more. */
+   products' sums, in f16 after powers of two of their rows or columns where its range would not hold them. */
 int64_t ygg_gated_linear_scratch(int type, int M, int N, int K);
 int ygg_gated_linear_grad(const void *d_x, const void *d_w, const void *d_gu, const void *d_dy, int type, int act, int M, int N, int K,
                           void *d_dx, void *d_dw, void *d_scratch, int64_t scratch_bytes, void *stream);

@@ -4,7 +4,7 @@ them does not; and where rows or columns of them differ by many powers of two.
 Tolerances, with h half a step of the type: those of g and u (sums of K products in f32, p(K, s) = 2^-22 (8 + 2 sqrt(K)) s with s^2 the
 squares' sum; kept in 24 bits, 2^-16 of themselves, in f32 whole) times dy, the other factor and the activation's slopes (act' at most
 1.13, act'' at most 0.8); dg and du are rounded to the type: h of themselves, or in float16 half a step of its smallest, 2^-25, where the
-row's (for dx) or column's (for dw) largest is brought to 2^14 or more: 2^-39 of that. Then each sum's own p and half a step of the
+row's (for dx) or column's (for dw) largest is 2^-3 or more as it is, or brought to 2^14: 2^-22 of that. Then each sum's own p and half a step of the
 result's type."""
 import math
 
@@ -52,12 +52,12 @@ def gradients(x, w, dy, act):
     rg = dy.abs() * (eu * (slope.abs() + 0.8 * eg) + 0.8 * eg * u.abs() + 16 * U * u.abs()) + 1.01 * h * dg.abs()
     ru = dy.abs() * (1.13 * eg + 16 * U * (1 + g.abs())) + 1.01 * h * du.abs()
     both = torch.cat([dg, du], 1).abs()
-    row = 2.0 ** -39 * both.amax(1, keepdim=True) if half else 0.0
+    row = 2.0 ** -22 * both.amax(1, keepdim=True) if half else 0.0
     dx = dg @ w[0] + du @ w[1]
     tx = (rg + row) @ w[0].abs() + (ru + row) @ w[1].abs() + 1.1 * p(2 * N, dg ** 2 @ w[0] ** 2 + du ** 2 @ w[1] ** 2)
     dw, tw = [], []
     for d, r in ((dg, rg), (du, ru)):
-        column = 2.0 ** -39 * d.abs().amax(0, keepdim=True) if half else 0.0
+        column = 2.0 ** -22 * d.abs().amax(0, keepdim=True) if half else 0.0
         dw.append(d.t() @ x)
         tw.append((r + column).t() @ x.abs() + 1.1 * p(M, (d ** 2).t() @ x ** 2))
     return dg, du, (dx, tx), (torch.stack(dw), torch.stack(tw))

@@ -11,11 +11,12 @@
 // added in their order.
 //
 // f16 holds 40 powers of two, and dg and du may lie past them though what comes of them does not (u = dy = 300: dg about 90000; a loss in
-// parts of 2^-20: dg 0). So in f16 they are multiplied by powers of two, undone in f32 behind the sums: one for each row, in a copy for
-// dx, whose sums go along a row, and one for each column, in a copy for dw, that bring the largest to 2^14 or more. A kernel before takes
-// the rows' and columns' largest, by maxima, which come out the same in any order. A factor is off by 2^-11 of itself or by 2^-39 of the
-// largest that is summed with it. It costs f16 a second reading of g, u and dy and the second copy (16384 x 2048 x 4096 gelu 200 us of 1740,
-// 1001 x 1000 x 2003 17 us of 112). bf16 reaches as far as f32.
+// parts of 2^-20: dg 0). So the kernel that takes them also takes the largest of each row, which dx sums along, and of each column, which
+// dw does, by maxima, which come out the same in any order. Where every one that is not 0 lies in f16 from 2^-3 on, dg and du are right as
+// they are: off by 2^-11 of themselves or by 2^-22 of the largest that is summed with them. Else they are taken once more, into a copy for
+// dx and one for dw, multiplied by powers of two of their rows and columns that bring the largest to 2^14 or more (2^-39 of the largest then),
+// which are undone in f32 behind the sums; the card decides, and the products read which. 16384 x 2048 x 4096 f16, forward and
+// backward, takes 1618 us without all that, 1675 with it and 1900 where the copies are made; 1001 x 1000 x 2003 97, 112 and 126. bf16 reaches as far as f32.
 //
 // The matrix cores bound large products (16384 x 2048 x 4096 bf16 forward 490 us of kernels with g and u kept, 1.1 PFLOP/s at the 1.8 GHz
 // that the card falls to; dg and du 145, by the memory; dx 440 and dw 500), the weights' reading few rows (1 x 4096 x 8192 bf16 24 us,
@@ -258,7 +259,7 @@ __global__ __launch_bounds__(256) void gated_few_kernel(const T *x, const T *w, 
     }
 }
 
-// of dg and du the powers of two, see above
+// dg and du come with the powers of two of their rows or columns, where they want them
 template <class T> constexpr bool kScaled = std::is_same_v<T, f16_t>;
 // e with 2^14 <= v / 2^e < 2^15, from v's bits; 0 of no value
 __device__ __forceinline__ int power_of(uint32_t bits) { return bits ? (int)(bits >> 23) - 127 - 14 : 0; }
@@ -290,62 +291,39 @@ template <class T, int kAct, bool kPast> struct Slope {
     }
 };
 
-// dg and du lie as g and u do, so that the products' loads are aligned, zeros behind N. A thread: 16 bytes of each. by_row, by_col: the copies
-// for dx and dw, NULL where that is not wanted; of other types than f16 the same one
-struct Slopes {
-    void *by_row, *by_col;
-    uint32_t *rows, *cols;      // kScaled: the bits of the rows' and the columns' largest finite magnitudes
-};
+// dg and du lie as g and u do, so that the products' loads are aligned, zeros behind N. A thread: 16 bytes of each
 template <class T, int kAct, bool kPast>
-__global__ __launch_bounds__(256) void gated_slope_kernel(Kept<T> gu, const T *dy, int M, int N, Slopes to) {
+__global__ __launch_bounds__(256) void gated_slope_kernel(Kept<T> gu, const T *dy, int M, int N, T *dgu) {
     constexpr int kE = 16 / sizeof(T);
     const int half = half_of(N), per = half / kE;
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / per;
     if (row >= M) return;
     const int n = (int)(id % per) * kE;
-    const int64_t at = row * 2 * half + n;
     float g[kE], u[kE];
     Slope<T, kAct, kPast> s;
     s.load(gu, dy, row, N, half, n);
     s.values(g, u, N - n);
-    if constexpr (kScaled<T>) {
-        float t[kE];
-        if (to.by_row) {
-            const int e = power_of(to.rows[row]);
-            T *out = (T *)to.by_row + at;
-#pragma unroll
-            for (int j = 0; j < kE; j++) t[j] = times_power(g[j], -e);
-            store_run<T, kE>(out, t, kE, kPast);
-#pragma unroll
-            for (int j = 0; j < kE; j++) t[j] = times_power(u[j], -e);
-            store_run<T, kE>(out + half, t, kE, kPast);
-        }
-        if (to.by_col) {
-            T *out = (T *)to.by_col + at;
-#pragma unroll
-            for (int j = 0; j < kE; j++) t[j] = times_power(g[j], -power_of(to.cols[n + j]));
-            store_run<T, kE>(out, t, kE, kPast);
-#pragma unroll
-            for (int j = 0; j < kE; j++) t[j] = times_power(u[j], -power_of(to.cols[half + n + j]));
-            store_run<T, kE>(out + half, t, kE, kPast);
-        }
-    } else {
-        T *out = (T *)to.by_row + at;
-        store_run<T, kE>(out, g, kE, kPast);
-        store_run<T, kE>(out + half, u, kE, kPast);
-    }
+    T *out = dgu + row * 2 * half + n;
+    store_run<T, kE>(out, g, kE, kPast);
+    store_run<T, kE>(out + half, u, kE, kPast);
 }
+
+// f16: dg and du as they are, and the bits of the largest finite magnitudes of the rows and columns; `range` is 1 where those do not let
+// them be. by_col: room for dw's copy then
+struct Reach {
+    uint32_t *rows, *cols, *range;
+    void *by_col;
+};
 __global__ __launch_bounds__(256) void zero_kernel(uint32_t *p, int64_t count) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i < count) p[i] = 0;
 }
-// The largest finite magnitudes of dg and du, of a workgroup's `band` rows and 64 pieces of columns: each of its waves a row at a time. Workgroups of
-// 16 waves, so that the maxima of a band's columns in memory are few (1001 x 2003 13.7 us, with 8 waves 20, with 4 34; 16384 x 4096 177 to 180
-// with either: the activations and the reading)
+// A workgroup: `band` rows of 64 pieces of columns, each of its waves a row at a time. Workgroups of 16 waves, so that the maxima of a band's
+// columns in memory are few (1001 x 2003 16.4 us, with 8 waves 25; 16384 x 4096 190 with either: the activations and the reading)
 constexpr int kReachWaves = 16;
 template <class T, int kAct, bool kPast>
 __global__ __launch_bounds__(64 * kReachWaves)
-void gated_reach_kernel(Kept<T> gu, const T *dy, int M, int N, int band, int slabs, uint32_t *rows, uint32_t *cols) {
+void gated_reach_kernel(Kept<T> gu, const T *dy, int M, int N, int band, int slabs, T *dgu, Reach to) {
     constexpr int kE = 16 / sizeof(T), kC = 64 * kE;
     __shared__ uint32_t lds[kReachWaves][2 * kE][65];
     const int half = half_of(N), lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c0 = (int)(blockIdx.x % slabs) * kC, n = c0 + lane * kE;
@@ -362,6 +340,9 @@ void gated_reach_kernel(Kept<T> gu, const T *dy, int M, int N, int band, int sla
             Slope<T, kAct, kPast> s;
             s.load(gu, dy, row, N, half, n);
             s.values(g, u, N - n);
+            T *out = dgu + (int64_t)row * 2 * half + n;
+            store_run<T, kE>(out, g, kE, kPast);
+            store_run<T, kE>(out + half, u, kE, kPast);
 #pragma unroll
             for (int j = 0; j < kE; j++) {
                 most[j] = max(most[j], bits(g[j]));
@@ -370,7 +351,7 @@ void gated_reach_kernel(Kept<T> gu, const T *dy, int M, int N, int band, int sla
             }
         }
         all = join<64>(all, [](uint32_t a, uint32_t b) { return max(a, b); });
-        if (lane == 0 && all) atomicMax(rows + row, all);
+        if (lane == 0 && all) atomicMax(to.rows + row, all);
     }
 #pragma unroll
     for (int j = 0; j < 2 * kE; j++) lds[wave][j][lane] = most[j];
@@ -379,9 +360,46 @@ void gated_reach_kernel(Kept<T> gu, const T *dy, int M, int N, int band, int sla
     for (int i = threadIdx.x; i < 2 * kC; i += 64 * kReachWaves) {
         const int c = i % kC, j = i / kC * kE + c % kE;
         if (c0 + c >= half) continue;
-        uint32_t *to = cols + (i < kC ? 0 : half) + c0 + c, all = 0;
+        uint32_t *at = to.cols + (i < kC ? 0 : half) + c0 + c, all = 0;
         for (int w = 0; w < kReachWaves; w++) all = max(all, lds[w][j][c / kE]);
-        if (all > *(volatile uint32_t *)to) atomicMax(to, all);
+        if (all > *(volatile uint32_t *)at) atomicMax(at, all);
+    }
+}
+// the rows' and columns' largest lie one behind the other, `count` in all
+__global__ __launch_bounds__(256) void gated_range_kernel(const uint32_t *most, int64_t count, uint32_t *range) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const uint32_t v = i < count ? most[i] : 0;
+    if (v && (v < 0x3e000000u || v > 0x477fe000u)) *range = 1;      // 2^-3, 65504
+}
+// Where they are out of range: the two copies, by rows into dgu and by columns
+template <class T, int kAct, bool kPast>
+__global__ __launch_bounds__(256) void gated_rescale_kernel(Kept<T> gu, const T *dy, int M, int N, T *dgu, Reach to) {
+    if (!*to.range) return;
+    constexpr int kE = 16 / sizeof(T);
+    const int half = half_of(N), per = half / kE;
+    const int64_t all = (int64_t)M * per, hop = (int64_t)gridDim.x * 256;
+    for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < all; id += hop) {
+        const int64_t row = id / per;
+        const int n = (int)(id % per) * kE, e = power_of(to.rows[row]);
+        const int64_t at = row * 2 * half + n;
+        float g[kE], u[kE], t[kE];
+        Slope<T, kAct, kPast> s;
+        s.load(gu, dy, row, N, half, n);
+        s.values(g, u, N - n);
+#pragma unroll
+        for (int j = 0; j < kE; j++) t[j] = times_power(g[j], -e);
+        store_run<T, kE>(dgu + at, t, kE, kPast);
+#pragma unroll
+        for (int j = 0; j < kE; j++) t[j] = times_power(u[j], -e);
+        store_run<T, kE>(dgu + at + half, t, kE, kPast);
+        if (!to.by_col) continue;
+        T *out = (T *)to.by_col + at;
+#pragma unroll
+        for (int j = 0; j < kE; j++) t[j] = times_power(g[j], -power_of(to.cols[n + j]));
+        store_run<T, kE>(out, t, kE, kPast);
+#pragma unroll
+        for (int j = 0; j < kE; j++) t[j] = times_power(u[j], -power_of(to.cols[half + n + j]));
+        store_run<T, kE>(out + half, t, kE, kPast);
     }
 }
 
@@ -395,20 +413,24 @@ struct Dense {
     void *out;
     float *sums;
     int tiles, cols, per;       // tiles of a part, tiles along O, steps of a part
-    const uint32_t *most;       // kScaled: the largest that A's row i was scaled by; NULL without rows
+    // kScaled, NULL without rows: where *range, A is `scaled` instead, its row i by the power of two of most[i]
+    const uint32_t *range, *most;
+    const void *scaled;
+    __device__ __forceinline__ bool is_scaled() const { return range && *range; }
     // the row of w that a column of dg and du belongs to, or -1
     __device__ __forceinline__ int place(int k) const { return k < N ? k : k >= half && k < half + N ? k - half + N : -1; }
 };
 template <class T, bool kRows> struct DenseOut {
     const Dense &g;
     int part, i0, o0;
+    bool scaled;
     template <class N> __device__ __forceinline__ void operator()(int i, int o, const float *v, N) const {
         const int row = kRows ? (i0 + i < g.I ? i0 + i : -1) : g.place(i0 + i);
         if (row < 0 || o0 + o >= g.O) return;
         const int64_t at = (int64_t)row * g.O + o0 + o;
         float t[N::value];
         if constexpr (kScaled<T>) {
-            const int e = g.most ? power_of(g.most[i0 + i]) : 0;
+            const int e = scaled ? power_of(g.most[i0 + i]) : 0;
 #pragma unroll
             for (int j = 0; j < N::value; j++) t[j] = times_power(v[j], e);
             v = t;
@@ -427,11 +449,13 @@ __global__ __launch_bounds__(64 * WI * WO) void dense_kernel(const Dense g) {
     const int part = blockIdx.x / g.tiles, wide = 2 * g.half, R = kRows ? wide : g.R;
     const Place t = place_of(tile_of(blockIdx.x % g.tiles, g.tiles), g.tiles / g.cols, g.cols, kBand);
     const int i0 = t.row * kI, o0 = t.col * kO, steps = (R + A::kStep - 1) / A::kStep, first = part * g.per;
+    const bool scaled = kScaled<T> && g.is_scaled();
+    const void *const from = scaled ? g.scaled : g.a;
     Tl tile;
     A a;
     B b;
-    if constexpr (kRows) a.begin([&](int i) { return (const T *)g.a + (int64_t)min(i0 + i, g.I - 1) * wide; });
-    else a.begin((const T *)g.a, i0, wide);
+    if constexpr (kRows) a.begin([&](int i) { return (const T *)from + (int64_t)min(i0 + i, g.I - 1) * wide; });
+    else a.begin((const T *)from, i0, wide);
     b.begin((const T *)g.b, o0, g.O);
     tile.run(a, b, lds, min(g.per, steps - first), [&](int s) {
         const int r0 = (first + s) * A::kStep;
@@ -446,7 +470,7 @@ __global__ __launch_bounds__(64 * WI * WO) void dense_kernel(const Dense g) {
             b.load([&](int i) { return r0 + B::r_of(i) < R ? (int64_t)(r0 + B::r_of(i)) * g.pitch : -1; });
         }
     });
-    const DenseOut<T, kRows> put = {g, part, i0, o0};
+    const DenseOut<T, kRows> put = {g, part, i0, o0, scaled};
     tile.template each<false>([&](int i, int o, const typename Tl::Acc *v, auto n) { put(i, o, (const float *)v, n); });
 }
 template <class T, bool kRows> __global__ __launch_bounds__(512) void dense_turn_kernel(const Dense g) {
@@ -459,11 +483,13 @@ template <class T, bool kRows> __global__ __launch_bounds__(512) void dense_turn
     const Place t = place_of(tile_of(blockIdx.x % g.tiles, g.tiles), g.tiles / g.cols, g.cols, kBand);
     const int i0 = t.row * 256, o0 = t.col * 256, steps = (R + B::kStep - 1) / B::kStep, first = part * g.per;
     const uint32_t a_row = wide * kSize, b_row = g.pitch * kSize;
+    const bool scaled = kScaled<T> && g.is_scaled();
+    const void *const from = scaled ? g.scaled : g.a;
     Tl tile;
     A a;
     B b;
-    if constexpr (kRows) a.begin(g.a, g.I * a_row, a_row, [&](int i) { return i0 + i < g.I ? (uint32_t)(i0 + i) * a_row : kFar; });
-    else a.begin(g.a, g.R * a_row, i0 * kSize, (wide - i0) * kSize);
+    if constexpr (kRows) a.begin(from, g.I * a_row, a_row, [&](int i) { return i0 + i < g.I ? (uint32_t)(i0 + i) * a_row : kFar; });
+    else a.begin(from, g.R * a_row, i0 * kSize, (wide - i0) * kSize);
     b.begin(g.b, (kRows ? 2 * g.N : g.R) * b_row, o0 * kSize, (g.O - o0) * kSize);
     tile.clear();
     auto row = [&](int r, uint32_t bytes) { return r >= 0 && r < R ? (uint32_t)r * bytes : kFar; };
@@ -479,7 +505,7 @@ template <class T, bool kRows> __global__ __launch_bounds__(512) void dense_turn
                  });
              },
              [](int) {}, kRows ? min(g.I - i0, 256) : 256);
-    const DenseOut<T, kRows> put = {g, part, i0, o0};
+    const DenseOut<T, kRows> put = {g, part, i0, o0, scaled};
     tile.template each<false>([&](int i, int o, const typename Tl::Acc *v, auto n) { put(i, o, (const float *)v, n); });
 }
 // rows of n values, `pitch` of whole 16 bytes apart
@@ -554,7 +580,7 @@ template <class T, int kAct> hipError_t go(const void *x, const void *w, int M, 
     // 1001 x 1000 x 2003, 256 of them, 19.8 and 19.1
     return tiles128 >= 384 ? tiles(four, two, two) : tiles(two, two, two);
 }
-template <class T, int kAct> hipError_t go_slope(const void *gu, const void *dy, int M, int N, const Slopes &to, hipStream_t st) {
+template <class T, int kAct> hipError_t go_slope(const void *gu, const void *dy, int M, int N, void *dgu, const Reach &to, hipStream_t st) {
     constexpr int kE = 16 / sizeof(T);
     const int half = half_of(N);
     const int64_t blocks = ((int64_t)M * (half / kE) + 255) / 256;
@@ -564,16 +590,21 @@ template <class T, int kAct> hipError_t go_slope(const void *gu, const void *dy,
     auto launch = [&](auto past) {
         constexpr bool kPast = decltype(past)::value;
         if constexpr (kScaled<T>) {
-            const int64_t count = (int64_t)M + 2 * half;      // rows and cols lie one behind the other
-            hipLaunchKernelGGL(zero_kernel, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, st, to.rows, count);
+            const int64_t count = (int64_t)M + 2 * half;      // rows, cols and range lie one behind the other
             const int slabs = (half / kE + 63) / 64, bands = std::max(512 / slabs, 1);
             const int band = ((M + bands - 1) / bands + kReachWaves - 1) / kReachWaves * kReachWaves;
+            hipLaunchKernelGGL(zero_kernel, dim3((unsigned)((count + 256) / 256)), dim3(256), 0, st, to.rows, count + 1);
             hipLaunchKernelGGL((gated_reach_kernel<T, kAct, kPast>), dim3((unsigned)(slabs * ((M + band - 1) / band))), dim3(64 * kReachWaves), 0, st,
-                               kept, (const T *)dy, M, N, band, slabs, to.rows, to.cols);
+                               kept, (const T *)dy, M, N, band, slabs, (T *)dgu, to);
+            hipLaunchKernelGGL(gated_range_kernel, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, st, to.rows, count, to.range);
+            // 2048: as many as the chip holds, so that they are soon gone where there is nothing to do
+            hipLaunchKernelGGL((gated_rescale_kernel<T, kAct, kPast>), dim3((unsigned)std::min<int64_t>(blocks, 2048)), dim3(256), 0, st, kept,
+                               (const T *)dy, M, N, (T *)dgu, to);
+        } else {
+            hipLaunchKernelGGL((gated_slope_kernel<T, kAct, kPast>), dim3((unsigned)blocks), dim3(256), 0, st, kept, (const T *)dy, M, N, (T *)dgu);
         }
-        hipLaunchKernelGGL((gated_slope_kernel<T, kAct, kPast>), dim3((unsigned)blocks), dim3(256), 0, st, kept, (const T *)dy, M, N, to);
     };
-    // 16384 x 4096 bf16: 184 us with the caches, 145 past them; f16's two kernels 177 and 187, 173 and 173
+    // 16384 x 4096 bf16: 184 us with the caches, 145 past them
     if (kept.count * Kept<T>::kBytes >= kPastBytes) launch(std::true_type());
     else launch(std::false_type());
     return hipGetLastError();
@@ -624,7 +655,7 @@ int64_t spaced_bytes(const Plan &p, int size, bool rows, int M, int N) {
 }
 int64_t part_bytes(const Plan &p, bool rows, int M, int N, int K) { return p.parts > 1 ? (int64_t)p.parts * (rows ? M : 2 * N) * K * 4 : 0; }
 template <class T, bool kRows>
-hipError_t go_dense(const void *a, const uint32_t *most, const void *b, int M, int N, int K, void *out, void *scratch, hipStream_t st) {
+hipError_t go_dense(const void *a, const Reach &to, const void *b, int M, int N, int K, void *out, void *scratch, hipStream_t st) {
     const Plan p = plan_of(sizeof(T), kRows, M, N, K, (uintptr_t)b % 16 == 0);
     float *sums = (float *)((char *)scratch + spaced_bytes(p, sizeof(T), kRows, M, N));
     const int64_t blocks = p.tiles * p.parts, I = kRows ? M : 2 * N, count = I * K;
@@ -638,7 +669,8 @@ hipError_t go_dense(const void *a, const uint32_t *most, const void *b, int M, i
         if (e != hipSuccess) return e;
         b = scratch;
     }
-    const Dense g = {a, b, (int)I, K, M, p.pitch, N, half_of(N), out, p.parts > 1 ? sums : nullptr, (int)p.tiles, p.cols, p.per, most};
+    const Dense g = {a, b, (int)I, K, M, p.pitch, N, half_of(N), out, p.parts > 1 ? sums : nullptr, (int)p.tiles, p.cols, p.per,
+                     to.range, kRows ? to.rows : to.cols, kRows ? a : to.by_col};
     if (p.turn) {
         if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((dense_turn_kernel<T, kRows>), dim3((unsigned)blocks), dim3(512), 0, st, g);
     } else if (p.large) {
@@ -665,13 +697,13 @@ hipError_t launch_gated(int type, int act, const void *x, const void *w, int M, 
     });
 }
 int64_t gated_kept(int type, int M, int N) { return (int64_t)M * 2 * half_of(N) * (type == kOpF32 ? 4 : 3); }
-// dg and du (f16: a copy for each product, then the rows' and columns' largest), then what one product at a time takes; whether its
-// operand turns out to be aligned or not
+// dg and du (f16: a copy for each product, the rows' and columns' largest and what is made of them), then what one product at a time takes;
+// whether its operand turns out to be aligned or not
 int64_t up_to_256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 int64_t dgu_copy(int type, int M, int N) { return up_to_256((int64_t)M * 2 * half_of(N) * op_bytes(type)); }
 int64_t dgu_bytes(int type, int M, int N) {
     const int64_t copy = dgu_copy(type, M, N);
-    return type == kOpF16 && M ? 2 * copy + up_to_256(((int64_t)M + 2 * half_of(N)) * 4) : copy;
+    return type == kOpF16 && M ? 2 * copy + up_to_256(((int64_t)M + 2 * half_of(N) + 1) * 4) : copy;
 }
 int64_t gated_grad_scratch(int type, int M, int N, int K) {
     const int size = op_bytes(type);
@@ -687,22 +719,22 @@ hipError_t launch_gated_grad(int type, int act, const void *x, const void *w, co
                              void *dx, void *dw, void *scratch, hipStream_t st) {
     char *const at = (char *)scratch, *rest = at + dgu_bytes(type, M, N);
     const int64_t copy = dgu_copy(type, M, N);
-    Slopes to = {at, at, nullptr, nullptr};
+    Reach to = {};
     if (type == kOpF16 && M) {
-        to.by_row = dx ? at : nullptr;
-        to.by_col = dw ? at + copy : nullptr;
         to.rows = (uint32_t *)(at + 2 * copy);
         to.cols = to.rows + M;
+        to.range = to.cols + 2 * half_of(N);
+        to.by_col = dw ? at + copy : nullptr;
     }
     hipError_t e = with_type(type, [&](auto one) {
-        return with_act(act, [&](auto k) { return go_slope<decltype(one), decltype(k)::value>(gu, dy, M, N, to, st); });
+        return with_act(act, [&](auto k) { return go_slope<decltype(one), decltype(k)::value>(gu, dy, M, N, at, to, st); });
     });
     if (e != hipSuccess) return e;
     return with_type(type, [&](auto one) {
         typedef decltype(one) T;
         hipError_t e = hipSuccess;
-        if (dx) e = go_dense<T, true>(to.by_row, to.rows, w, M, N, K, dx, rest, st);
-        if (e == hipSuccess && dw) e = go_dense<T, false>(to.by_col, to.cols, x, M, N, K, dw, rest, st);
+        if (dx) e = go_dense<T, true>(at, to, w, M, N, K, dx, rest, st);
+        if (e == hipSuccess && dw) e = go_dense<T, false>(at, to, x, M, N, K, dw, rest, st);
         return e;
     });
 }

@@ -281,8 +281,8 @@ def gated_linear(x, w, activation: str = "silu") -> torch.Tensor:
     act(x w[0]^T) (x w[1]^T) (..., N) in x's type, act "silu" (g sigmoid(g)), "gelu" (g Phi(g)) or "sigmoid". Sums and
     the product are in f32, rounded once. Differentiable in x and w: for that, both projections are kept (in f32, or its upper 24
     bits for 16-bit types), and the gradients' products take their factors in x's type: dy u act'(g) and dy act(g) are rounded to it
-    before the sums, in float16 after a power of two for each row (the gradient of x) or column (that of w), so that their range is
-    float32's and what is under 2^-39 of the largest beside it is lost."""
+    before the sums. In float16 that is with a power of two for each row (for the gradient of x) and column (for that of w) where its
+    range would not do, so that they reach as far as float32's, and what is under 2^-22 of the largest beside it may be lost."""
     act = ACTIVATIONS.get(activation) if isinstance(activation, str) else None
     if act is None:
         raise ValueError(f"activation {activation!r}: one of {', '.join(ACTIVATIONS)}")
