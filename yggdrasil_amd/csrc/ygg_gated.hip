@@ -16,7 +16,8 @@
 // they are: off by 2^-11 of themselves or by 2^-22 of the largest that is summed with them. Else they are taken once more, into a copy for
 // dx and one for dw, multiplied by powers of two of their rows and columns that bring the largest to 2^14 or more (2^-39 of the largest then),
 // which are undone in f32 behind the sums; the card decides, and the products read which. 16384 x 2048 x 4096 f16, forward and
-// backward, takes 1618 us without all that, 1675 with it and 1900 where the copies are made; 1001 x 1000 x 2003 97, 112 and 126. bf16 reaches as far as f32.
+// backward, takes 1618 us without all that, 1675 with it and 1900 where the copies are made; 1001 x 1000 x 2003 97, 112 and 126. bf16
+// reaches as far as f32.
 //
 // The matrix cores bound large products (16384 x 2048 x 4096 bf16 forward 490 us of kernels with g and u kept, 1.1 PFLOP/s at the 1.8 GHz
 // that the card falls to; dg and du 145, by the memory; dx 440 and dw 500), the weights' reading few rows (1 x 4096 x 8192 bf16 24 us,
